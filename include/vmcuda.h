@@ -270,6 +270,152 @@ VM_API int64_t vm_launch_count(const vm_engine* engine);
 VM_API vm_status vm_host_alloc(void** ptr, size_t bytes);
 VM_API void vm_host_free(void* ptr);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Operators on what a network answered (no counterpart in the reference's engines): how sure it was of every row, and what a
+ * sequence of frames adds. All pointers are DEVICE pointers of the caller, on `device` (< 0: the current device; the device that was
+ * current is current again when the call returns). The calls enqueue their kernels on `stream` (a cudaStream_t, NULL: the default
+ * stream) and return: they neither wait, allocate nor keep anything, so they may be captured into a CUDA graph, from any number of
+ * threads. Outputs overlap neither inputs nor one another. What an engine left on the device (VM_RESULTS_ON_DEVICE) is complete when
+ * its call returns; let `stream` finish before the engine's next call writes there again.
+ * ------------------------------------------------------------------------------------------------------------------ */
+
+/* element types; sums, logarithms and states are 32-bit floats whatever the type */
+enum { VM_F32 = 0, VM_F16 = 1, VM_BF16 = 2 };
+
+enum {
+    VM_PROBABILITIES = 1, /* rows hold probabilities (what a softmax layer wrote) instead of logits: v_j = log x_j, else v_j = x_j */
+    VM_LABELS_64     = 2  /* labels are int64_t, else int32_t */
+};
+#define VM_MAX_TOP 32
+
+/* For every row of `classes` values, row_stride elements after the row before it: log_sum = log sum_j exp v_j, with
+ * log p_j = v_j - log_sum the log probability of the row's label, entropy = -sum_j p_j log p_j (natural logarithms) and the `top`
+ * largest values in descending order with their indices, the lowest index first among equals (top_log_prob and top_index: rows x top).
+ * Any output may be NULL; top <= min(classes, VM_MAX_TOP), and top > 0 needs both of its outputs, log_prob needs labels.
+ * Label -1: none, log_prob is 0. Any other label outside 0..classes-1: log_prob is NaN.
+ * v_j = -infinity (a probability of 0) masks a class: it adds nothing to sum and entropy and its log probability is -infinity. A row
+ * with nothing else has log_sum -infinity and entropy 0. A row with NaN or +infinity (or a negative probability) has no
+ * distribution: its log_sum, entropy and log probabilities are NaN; in the order of the top values NaN comes before +infinity. */
+VM_API vm_status vm_scores(int device,
+                           const void* x,
+                           int32_t type,
+                           int64_t rows,
+                           int32_t classes,
+                           int64_t row_stride,
+                           uint32_t flags,
+                           const void* labels,
+                           int32_t top,
+                           float* log_prob,
+                           float* entropy,
+                           float* log_sum,
+                           float* top_log_prob,
+                           int32_t* top_index,
+                           void* stream);
+
+/* The gradient of x (rows dx_row_stride apart, type as x) from those of log_prob, entropy and log_sum (each NULL: zero), with x, labels,
+ * flags, entropy and log_sum as vm_scores had and wrote them (labels and d_log_prob come together; entropy is needed with d_entropy):
+ *   logits         dx_j = p_j (d_log_sum - d_log_prob - d_entropy (log p_j + entropy)) + d_log_prob [j = label]
+ *   probabilities  dx_j = (the same bracket) / sum_j x_j + d_log_prob [j = label] / x_j
+ * A masked class gets the gradient 0, also where it is the label; label -1 counts as d_log_prob 0; the gradient of a row with another
+ * label outside 0..classes-1, or without a distribution, is NaN but for its masked classes. */
+VM_API vm_status vm_scores_backward(int device,
+                                    const void* x,
+                                    int32_t type,
+                                    int64_t rows,
+                                    int32_t classes,
+                                    int64_t row_stride,
+                                    uint32_t flags,
+                                    const void* labels,
+                                    const float* entropy,
+                                    const float* log_sum,
+                                    const float* d_log_prob,
+                                    const float* d_entropy,
+                                    const float* d_log_sum,
+                                    void* dx,
+                                    int64_t dx_row_stride,
+                                    void* stream);
+
+/* Element (b, t, c) of a sequence is data[b * batch_stride + t * step_stride + c * channel_stride] (in elements, >= 0; 0 repeats an
+ * input along that dimension, outputs have an element of their own for every index). */
+typedef struct vm_sequence {
+    void* data;
+    int64_t batch_stride;
+    int64_t step_stride;
+    int64_t channel_stride;
+} vm_sequence;
+
+/* Steps between two states that vm_gated_scan keeps for its backward pass. */
+#define VM_GATED_KEEP 64
+
+/* A gated linear recurrence over `steps` of batch x channels sequences: with f = 1 / (1 + exp(-gate)),
+ *   h_t = f_t h_(t-1) + (1 - f_t) x_t,   y_t = h_t,   h_(-1) = h0 (NULL: zero),   last = h after the last step.
+ * gate = -infinity drops what was before (the sequence begins anew), +infinity drops x_t (nothing was seen), whatever they hold, NaN
+ * and infinities included. lengths (NULL: all `steps`): sequence b has lengths[b] steps (clamped to 0..steps); y is 0 behind them and
+ * last is h after the last of them. x, gate and y have `type`; h0, last and states are 32-bit, batch x channels without gaps.
+ * states (may be NULL): batch x ceil(steps / VM_GATED_KEEP) x channels, h before steps 0, 64, 128, ...: what the backward pass starts from.
+ * y and last may be NULL. workspace: at least vm_gated_workspace(batch, steps, channels) bytes, aligned to 16, that no other call uses
+ * until this one's kernels are done (NULL when that is 0). steps, batch or channels may be 0. */
+VM_API vm_status vm_gated_scan(int device,
+                               int32_t type,
+                               int64_t batch,
+                               int64_t steps,
+                               int64_t channels,
+                               const vm_sequence* x,
+                               const vm_sequence* gate,
+                               const float* h0,
+                               const int32_t* lengths,
+                               const vm_sequence* y,
+                               float* last,
+                               float* states,
+                               void* workspace,
+                               size_t workspace_bytes,
+                               void* stream);
+
+/* The gradients of x, gate and h0 (each may be NULL) from those of y and last (each NULL: zero), with x, gate and lengths as
+ * vm_gated_scan had them and the states that it kept. An input that a stride of 0 repeats gets a gradient for every place it was
+ * used at: what belongs to the one value is their sum. Behind a sequence's length the gradients of x and gate are 0. Workspace as above. */
+VM_API vm_status vm_gated_scan_backward(int device,
+                                        int32_t type,
+                                        int64_t batch,
+                                        int64_t steps,
+                                        int64_t channels,
+                                        const vm_sequence* x,
+                                        const vm_sequence* gate,
+                                        const float* states,
+                                        const int32_t* lengths,
+                                        const vm_sequence* dy,
+                                        const float* d_last,
+                                        const vm_sequence* dx,
+                                        const vm_sequence* d_gate,
+                                        float* d_h0,
+                                        void* workspace,
+                                        size_t workspace_bytes,
+                                        void* stream);
+
+/* Bytes of workspace that either of the two needs at these sizes (0 for sizes that they refuse). */
+VM_API size_t vm_gated_workspace(int64_t batch, int64_t steps, int64_t channels);
+
+/* One step of the recurrence for rows whose states stand in a table of `slots` rows of `channels` 32-bit floats (state_stride elements
+ * apart), updated in place: h = f h + (1 - f) x for the slot index[row] (NULL: slot = row, rows <= slots), y[row] = h.
+ * x, gate and y have rows x channels elements of `type`, row and channel strides in batch_stride (step_stride is not used) and
+ * channel_stride. A row whose index is outside 0..slots-1, or whose slot an earlier row of the call names too, changes no state and its
+ * y is 0. y may be NULL. workspace: at least vm_gated_step_workspace(rows, slots) bytes when index is given, aligned to 16. */
+VM_API vm_status vm_gated_step(int device,
+                               int32_t type,
+                               int64_t rows,
+                               int64_t slots,
+                               int64_t channels,
+                               float* state,
+                               int64_t state_stride,
+                               const vm_sequence* x,
+                               const vm_sequence* gate,
+                               const int32_t* index,
+                               const vm_sequence* y,
+                               void* workspace,
+                               size_t workspace_bytes,
+                               void* stream);
+VM_API size_t vm_gated_step_workspace(int64_t rows, int64_t slots);
+
 /* Message of the last failing call on this thread. */
 VM_API const char* vm_last_error(void);
 

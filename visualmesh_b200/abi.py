@@ -18,6 +18,12 @@ VM_ERR_NO_BSP = 8
 VM_RESULTS_ON_DEVICE = 1
 VM_TIME_STAGES = 2
 
+VM_F32, VM_F16, VM_BF16 = 0, 1, 2
+VM_PROBABILITIES = 1
+VM_LABELS_64 = 2
+VM_MAX_TOP = 32
+VM_GATED_KEEP = 64
+
 
 class vm_lens(C.Structure):
     _fields_ = [
@@ -67,6 +73,15 @@ class vm_batch_result(C.Structure):
     ]
 
 
+class vm_sequence(C.Structure):
+    _fields_ = [
+        ("data", C.c_void_p),
+        ("batch_stride", C.c_int64),
+        ("step_stride", C.c_int64),
+        ("channel_stride", C.c_int64),
+    ]
+
+
 # every symbol the header declares: name -> (restype, argtypes)
 SYMBOLS = {
     "vm_engine_create": (C.c_int, [C.c_int, C.POINTER(vm_layer), C.POINTER(C.c_int32), C.c_int32, C.POINTER(C.c_void_p)]),
@@ -95,6 +110,19 @@ SYMBOLS = {
     "vm_launch_count": (C.c_int64, [C.c_void_p]),
     "vm_host_alloc": (C.c_int, [C.POINTER(C.c_void_p), C.c_size_t]),
     "vm_host_free": (None, [C.c_void_p]),
+    "vm_scores": (C.c_int, [C.c_int, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_uint32, C.c_void_p, C.c_int32]
+                  + [C.c_void_p] * 6),
+    "vm_scores_backward": (C.c_int, [C.c_int, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_uint32] + [C.c_void_p] * 7
+                           + [C.c_int64, C.c_void_p]),
+    "vm_gated_scan": (C.c_int, [C.c_int, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.POINTER(vm_sequence), C.POINTER(vm_sequence), C.c_void_p, C.c_void_p,
+                                C.POINTER(vm_sequence), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "vm_gated_scan_backward": (C.c_int, [C.c_int, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.POINTER(vm_sequence), C.POINTER(vm_sequence), C.c_void_p,
+                                         C.c_void_p, C.POINTER(vm_sequence), C.c_void_p, C.POINTER(vm_sequence), C.POINTER(vm_sequence), C.c_void_p,
+                                         C.c_void_p, C.c_size_t, C.c_void_p]),
+    "vm_gated_workspace": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64]),
+    "vm_gated_step": (C.c_int, [C.c_int, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.POINTER(vm_sequence), C.POINTER(vm_sequence),
+                                C.c_void_p, C.POINTER(vm_sequence), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "vm_gated_step_workspace": (C.c_size_t, [C.c_int64, C.c_int64]),
     "vm_last_error": (C.c_char_p, []),
     "vm_hostmesh_create": (C.c_int, [C.c_char_p, C.c_char_p, C.c_float, C.c_float, C.c_float, C.c_float, C.c_float,
                                      C.POINTER(C.c_void_p)]),

@@ -27,6 +27,7 @@
 #include "host_math.hpp"
 #include "kernels.cuh"
 #include "conv_dispatch.hpp"
+#include "device_call.hpp"
 #include "upload.hpp"
 #include "libm_tables.hpp"
 
@@ -34,7 +35,7 @@ namespace vm {
 
 static thread_local std::string g_error;
 
-static vm_status fail(vm_status s, const std::string& msg) {
+vm_status fail(vm_status s, const std::string& msg) {
     g_error = msg;
     return s;
 }
@@ -44,7 +45,7 @@ static vm_status fail(vm_status s, const std::string& msg) {
 struct UnsupportedLens {};
 
 // The status of the exception in flight: nothing leaves a C entry point as an exception. Called inside a handler.
-static vm_status status_of_exception() {
+vm_status status_of_exception() {
     cudaGetLastError();
     try {
         throw;

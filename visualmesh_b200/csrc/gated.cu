@@ -1,0 +1,176 @@
+// vm_gated_scan, vm_gated_scan_backward and vm_gated_step: checks and launches of the kernels in gated.cuh.
+#include "device_call.hpp"
+#include "gated.cuh"
+
+namespace {
+
+using namespace vm;
+using namespace vm::answers;
+
+constexpr int64_t MOST = INT64_MAX >> 4;  // no offset in bytes comes near the end of 64 bits
+
+bool sizes_fit(int64_t batch, int64_t steps, int64_t channels) {
+    if (batch < 0 || steps < 0 || channels < 0 || batch > INT32_MAX || steps > INT32_MAX || channels > INT32_MAX) return false;
+    return batch * channels <= (int64_t(1) << 38);
+}
+
+// An output needs a place of its own for every index: strides that nest, in the order that their sizes give.
+bool nests(const vm_sequence& s, const int64_t (&sizes)[3]) {
+    int64_t stride[3] = {s.batch_stride, s.step_stride, s.channel_stride}, size[3] = {sizes[0], sizes[1], sizes[2]};
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if (stride[j] < stride[i]) {
+                std::swap(stride[i], stride[j]);
+                std::swap(size[i], size[j]);
+            }
+    int64_t reach = 1;
+    for (int i = 0; i < 3; ++i) {
+        if (size[i] <= 1) continue;
+        if (stride[i] < reach) return false;
+        reach = stride[i] * (size[i] - 1) + reach;
+    }
+    return true;
+}
+
+// Whether s (NULL: absent, where that is allowed) can be addressed; throws the message otherwise.
+void check_sequence(const vm_sequence* s, const char* name, int32_t type, const int64_t (&sizes)[3], bool needed, bool output) {
+    if (s == nullptr || s->data == nullptr) {
+        if (needed) throw std::string("null ") + name;
+        return;
+    }
+    if (!aligned(s->data, element_size(type))) throw std::string(name) + " is not aligned to its elements";
+    const int64_t stride[3] = {s->batch_stride, s->step_stride, s->channel_stride};
+    int64_t reach = 0;
+    for (int i = 0; i < 3; ++i) {
+        if (stride[i] < 0) throw std::string(name) + ": strides must not be negative";
+        if (sizes[i] > 1 && stride[i] > MOST / sizes[i]) throw std::string(name) + ": stride out of range";
+        reach += sizes[i] > 1 ? stride[i] * (sizes[i] - 1) : 0;
+        if (reach > MOST) throw std::string(name) + ": strides out of range";
+    }
+    if (output && !nests(*s, sizes)) throw std::string(name) + ": elements of an output share a place";
+}
+
+Sequence sequence(const vm_sequence* s) {
+    if (s == nullptr) return Sequence{nullptr, 0, 0, 0};
+    return Sequence{s->data, s->batch_stride, s->step_stride, s->channel_stride};
+}
+
+unsigned blocks_of(int64_t threads) {
+    const int64_t n = (threads + 255) / 256;
+    if (n > INT32_MAX) throw std::string("too many elements for one call");
+    return static_cast<unsigned>(n);
+}
+
+void check_sizes(int32_t type, int64_t batch, int64_t steps, int64_t channels) {
+    if (!known_type(type)) throw std::string("unknown element type");
+    if (!sizes_fit(batch, steps, channels)) throw std::string("batch, steps and channels must be 0..2^31-1 (batch * channels at most 2^38)");
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t vm_gated_workspace(int64_t batch, int64_t steps, int64_t channels) {
+    (void)batch, (void)steps, (void)channels;
+    return 0;
+}
+
+vm_status vm_gated_scan(int device, int32_t type, int64_t batch, int64_t steps, int64_t channels, const vm_sequence* x, const vm_sequence* gate, const float* h0,
+                        const int32_t* lengths, const vm_sequence* y, float* last, float* states, void* workspace, size_t workspace_bytes, void* stream) {
+    try {
+        check_sizes(type, batch, steps, channels);
+        if (batch == 0 || channels == 0) return VM_OK;
+        const int64_t sizes[3] = {batch, steps, channels};
+        check_sequence(x, "x", type, sizes, steps > 0, false);
+        check_sequence(gate, "gate", type, sizes, steps > 0, false);
+        check_sequence(y, "y", type, sizes, false, true);
+        if (workspace_bytes < vm_gated_workspace(batch, steps, channels)) throw std::string("the workspace is too small");
+        (void)workspace;
+        const OnDevice on(device);
+        GatedArgs a{};
+        a.batch = batch, a.steps = steps, a.channels = channels;
+        a.x = sequence(x), a.gate = sequence(gate), a.y = sequence(y);
+        a.h0 = h0, a.lengths = lengths, a.last = last, a.states = states;
+        const unsigned grid = blocks_of(batch * channels);
+        with_type(type, [&](auto kind) { launch_kernel(k_gated_scan<decltype(kind)>, dim3(grid), 256, 0, static_cast<cudaStream_t>(stream), false, a); });
+    }
+    catch (const std::string& refused) {
+        return fail(VM_ERR_INVALID_ARGUMENT, refused);
+    }
+    catch (...) {
+        return status_of_exception();
+    }
+    return VM_OK;
+}
+
+vm_status vm_gated_scan_backward(int device, int32_t type, int64_t batch, int64_t steps, int64_t channels, const vm_sequence* x, const vm_sequence* gate, const float* states,
+                                 const int32_t* lengths, const vm_sequence* dy, const float* d_last, const vm_sequence* dx, const vm_sequence* d_gate, float* d_h0,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+    try {
+        check_sizes(type, batch, steps, channels);
+        if (batch == 0 || channels == 0) return VM_OK;
+        const int64_t sizes[3] = {batch, steps, channels};
+        check_sequence(x, "x", type, sizes, steps > 0, false);
+        check_sequence(gate, "gate", type, sizes, steps > 0, false);
+        check_sequence(dy, "dy", type, sizes, false, false);
+        check_sequence(dx, "dx", type, sizes, false, true);
+        check_sequence(d_gate, "d_gate", type, sizes, false, true);
+        if (steps > 0 && states == nullptr) throw std::string("null states");
+        if (workspace_bytes < vm_gated_workspace(batch, steps, channels)) throw std::string("the workspace is too small");
+        (void)workspace;
+        const OnDevice on(device);
+        GatedArgs a{};
+        a.batch = batch, a.steps = steps, a.channels = channels;
+        a.x = sequence(x), a.gate = sequence(gate), a.y = sequence(dy);
+        a.lengths = lengths, a.states = const_cast<float*>(states), a.d_last = d_last;
+        a.dx = sequence(dx), a.d_gate = sequence(d_gate), a.d_h0 = d_h0;
+        const unsigned grid = blocks_of(batch * channels);
+        with_type(type, [&](auto kind) { launch_kernel(k_gated_scan_grad<decltype(kind)>, dim3(grid), 256, 0, static_cast<cudaStream_t>(stream), false, a); });
+    }
+    catch (const std::string& refused) {
+        return fail(VM_ERR_INVALID_ARGUMENT, refused);
+    }
+    catch (...) {
+        return status_of_exception();
+    }
+    return VM_OK;
+}
+
+size_t vm_gated_step_workspace(int64_t rows, int64_t slots) {
+    return rows > 0 && slots > 0 ? static_cast<size_t>(slots) * sizeof(uint32_t) : 0;
+}
+
+vm_status vm_gated_step(int device, int32_t type, int64_t rows, int64_t slots, int64_t channels, float* state, int64_t state_stride, const vm_sequence* x,
+                        const vm_sequence* gate, const int32_t* index, const vm_sequence* y, void* workspace, size_t workspace_bytes, void* stream) {
+    try {
+        check_sizes(type, rows, 1, channels);
+        if (slots < 0 || slots > INT32_MAX) throw std::string("slots must be 0..2^31-1");
+        if (index == nullptr && rows > slots) throw std::string("more rows than slots, and no index");
+        if (rows == 0 || channels == 0) return VM_OK;
+        const int64_t sizes[3] = {rows, 1, channels};
+        check_sequence(x, "x", type, sizes, true, false);
+        check_sequence(gate, "gate", type, sizes, true, false);
+        check_sequence(y, "y", type, sizes, false, true);
+        if (slots > 0 && state == nullptr) throw std::string("null state");
+        if (state_stride < (slots > 1 ? channels : 0) || state_stride > MOST / (slots > 0 ? slots : 1)) throw std::string("the states of slots overlap");
+        if (index != nullptr && (workspace_bytes < vm_gated_step_workspace(rows, slots) || (slots > 0 && workspace == nullptr))) throw std::string("the workspace is too small");
+        const OnDevice on(device);
+        const auto q = static_cast<cudaStream_t>(stream);
+        StepArgs a{rows, slots, channels, state, state_stride, sequence(x), sequence(gate), sequence(y), index, static_cast<uint32_t*>(workspace)};
+        if (index != nullptr && slots > 0) {
+            VM_CUDA(cudaMemsetAsync(workspace, 0xFF, static_cast<size_t>(slots) * sizeof(uint32_t), q));
+            launch_kernel(k_first_rows, dim3(blocks_of(rows)), 256, 0, q, false, a);
+        }
+        const unsigned grid = blocks_of(rows * channels);
+        with_type(type, [&](auto kind) { launch_kernel(k_gated_step<decltype(kind)>, dim3(grid), 256, 0, q, false, a); });
+    }
+    catch (const std::string& refused) {
+        return fail(VM_ERR_INVALID_ARGUMENT, refused);
+    }
+    catch (...) {
+        return status_of_exception();
+    }
+    return VM_OK;
+}
+
+}  // extern "C"

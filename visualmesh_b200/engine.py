@@ -175,6 +175,13 @@ class FrameInput:
     image_on_device: bool = False
 
 
+class _DeviceArray:
+    """Device memory of the engine, for torch.as_tensor."""
+
+    def __init__(self, pointer, shape, kind):
+        self.__cuda_array_interface__ = {"data": (C.cast(pointer, C.c_void_p).value, False), "shape": shape, "typestr": kind, "version": 3}
+
+
 class BatchResult:
     """Results of Engine.run_batch: per-frame views into the engine's pinned buffers (valid until its next call),
     or device pointers when the batch was run with results_on_device."""
@@ -205,6 +212,65 @@ class BatchResult:
         if self._cls is None:
             return ProjectedMesh(cp(self._px[p0:p1]), cp(self._nb[r0:r1]), cp(self._gi[p0:p1]))
         return ClassifiedMesh(cp(self._px[p0:p1]), cp(self._nb[r0:r1]), cp(self._gi[p0:p1]), cp(self._cls[r0:r1]))
+
+    def tensors(self):
+        """The arrays of results that were left on the device as torch tensors, frames one after another: pixel_coordinates [points, 2],
+        global_indices [points], neighbourhood and classifications [points + n_frames, ...] (each frame's last row is its off-screen
+        row; classifications is None after a projection). They are the engine's memory: valid until its next call, which does not wait
+        for what other streams still read there."""
+        import torch
+        if not self.on_device:
+            raise VisualMeshError(abi.VM_ERR_INVALID_ARGUMENT, "results were copied to the host")
+        points, rows = self.total_points, self.total_points + self.n_frames
+
+        def tensor(pointer, shape, kind, dtype):
+            if 0 in shape:
+                return torch.empty(shape, dtype=dtype, device="cuda")
+            return torch.as_tensor(_DeviceArray(pointer, shape, kind), device="cuda")
+
+        return {"pixel_coordinates": tensor(self.raw.pixel_coordinates, (points, 2), "<f4", torch.float32),
+                "global_indices": tensor(self.raw.global_indices, (points,), "<i4", torch.int32),
+                "neighbourhood": tensor(self.raw.neighbourhood, (rows, self.n_neighbours), "<i4", torch.int32),
+                "classifications": tensor(self.raw.classifications, (rows, self.n_classes), "<f4", torch.float32) if self.n_classes else None}
+
+    def _classifications(self):
+        got = self.tensors()
+        if got["classifications"] is None:
+            raise VisualMeshError(abi.VM_ERR_NETWORK_SHAPE, "these results are projections only")
+        return got["classifications"], got["global_indices"]
+
+    def scores(self, labels=None, top=1):
+        """answers.scores of the classifications of a network that ends in a softmax: how probable its label ([points + n_frames], -1: none)
+        is for every row, its entropy, and its best classes."""
+        from . import answers
+        return answers.scores(self._classifications()[0], labels, top, probabilities=True)
+
+    def advance(self, state, gate):
+        """Filters the classifications over time, node by node: answers.gated_step for frame after frame, with the state of every node of
+        the mesh in state [n_nodes, n_classes] (float32, updated in place; nodes off the screen keep theirs). All frames are of one
+        mesh. gate: what broadcasts to [points + n_frames, n_classes] float32, a row for every row of the classifications. Returns the
+        filtered classifications, 0 in the off-screen rows."""
+        import torch
+        from . import answers
+        x, nodes = self._classifications()
+        gate, y = gate.expand(x.shape), torch.zeros_like(x)
+        for f in range(self.n_frames):
+            p0, p1 = int(self.offsets[f]), int(self.offsets[f + 1])
+            at = slice(p0 + f, p1 + f)
+            answers.gated_step(state, x[at], gate[at], nodes[p0:p1], out=y[at])
+        return y
+
+    def filtered(self, gate, h0=None, keep=False):
+        """answers.gated_scan over the frames of a camera that stands still over one mesh: every frame shows the same nodes (anything else is
+        refused), so that row r of all frames is one sequence. gate: what broadcasts to [n_frames, rows, n_classes] float32; h0: [rows,
+        n_classes]. y, last and states have the rows' classes side by side."""
+        from . import answers
+        x, nodes = self._classifications()
+        n = self.total_points // max(self.n_frames, 1)
+        if any(int(self.offsets[f]) != f * n for f in range(self.n_frames + 1)) or not bool((nodes.view(self.n_frames, n) == nodes[:n]).all()):
+            raise VisualMeshError(abi.VM_ERR_INVALID_ARGUMENT, "the frames show different nodes")
+        gate = gate.expand(self.n_frames, n + 1, self.n_classes).reshape(1, self.n_frames, -1)
+        return answers.gated_scan(x.view(gate.shape), gate, None if h0 is None else h0.reshape(1, -1), keep=keep)
 
 
 def _mesh_at(mesh, Hoc) -> Mesh:
