@@ -1,4 +1,8 @@
 // vm_gated_scan, vm_gated_scan_backward and vm_gated_step: checks and launches of the kernels in gated.cuh.
+#include <algorithm>
+#include <type_traits>
+#include <utility>
+
 #include "device_call.hpp"
 #include "gated.cuh"
 
@@ -66,13 +70,90 @@ void check_sizes(int32_t type, int64_t batch, int64_t steps, int64_t channels) {
     if (!sizes_fit(batch, steps, channels)) throw std::string("batch, steps and channels must be 0..2^31-1 (batch * channels at most 2^38)");
 }
 
+// ---- how a scan is laid out ----------------------------------------------------------------------------------------------
+constexpr int SMS = 148;
+
+struct Plan {
+    int tx;        // threads along the channels
+    int64_t run;   // steps of a part
+    int64_t parts;
+};
+
+// `vector` elements and `length` steps a thread.
+Plan plan_of(int64_t all, int64_t steps, int vector, int length) {
+    Plan p{32, steps, 1};
+    if (vector > 1 && steps > THREADS / 32 * length) p.tx = 8;
+    const int64_t tile = THREADS / p.tx * length, tiles = (steps + tile - 1) / tile;
+    const int64_t blocks = (all + p.tx * vector - 1) / (p.tx * vector);
+    if (blocks < SMS && tiles > 1) {
+        const int64_t wanted = std::min(tiles, (4 * SMS + blocks - 1) / blocks);
+        p.run                = (tiles + wanted - 1) / wanted * tile;
+        p.parts              = (steps + p.run - 1) / p.run;
+    }
+    return p;
+}
+// of the forward and of the backward pass: steps of a thread where it takes vectors and where it takes single elements
+constexpr int FORWARD = 8, BACKWARD = 4, SINGLE = 16;
+
+// Whether `vector` neighbouring channels of s lie side by side at a place that one load or store can take.
+bool takes(const vm_sequence* s, int32_t type, int vector, const int64_t (&sizes)[3]) {
+    if (s == nullptr || s->data == nullptr) return true;
+    const size_t size = element_size(type);
+    return s->channel_stride == 1 && aligned(s->data, vector * size) && (sizes[0] <= 1 || s->batch_stride % vector == 0) && (sizes[1] <= 1 || s->step_stride % vector == 0);
+}
+
+// f(a value of the element type, how many of them a thread takes, threads along the channels), as constants
+template <typename F>
+void with_layout(int32_t type, int vector, int tx, F f) {
+    using One = std::integral_constant<int, 1>;
+    using Four = std::integral_constant<int, 4>;
+    with_type(type, [&](auto kind) {
+        if (vector == 1) f(kind, One{}, std::integral_constant<int, 32>{});
+        else if (tx == 32) f(kind, Four{}, std::integral_constant<int, 32>{});
+        else f(kind, Four{}, std::integral_constant<int, 8>{});
+    });
+}
+
+// Launches one kernel, which is told once for a device that it may take more shared memory than every kernel may.
+template <auto KERNEL>
+void launch_tiles(dim3 grid, int shared, cudaStream_t q, const GatedArgs& a, const Split& s) {
+    static LaunchPlans plans;
+    if (shared > 0) {
+        plans.get([&](int) {
+            VM_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, shared));
+            return LaunchPlan{};
+        });
+    }
+    launch_kernel(KERNEL, grid, THREADS, shared, q, false, a, s);
+}
+
+Split split_of(const Plan& p, void* workspace) {
+    return Split{p.run, static_cast<int32_t>(p.parts), static_cast<float2*>(workspace)};
+}
+
+void check_workspace(int64_t batch, int64_t steps, int64_t channels, const void* workspace, size_t bytes) {
+    const size_t needed = vm_gated_workspace(batch, steps, channels);
+    if (bytes < needed) throw std::string("the workspace is too small");
+    if (needed > 0 && (workspace == nullptr || !aligned(workspace, 16))) throw std::string("the workspace is null or not aligned to 16 bytes");
+}
+
+dim3 grid_of(int64_t all, const Plan& p, int vector) {
+    const int64_t blocks = (all + p.tx * vector - 1) / (p.tx * vector);
+    if (blocks > INT32_MAX) throw std::string("too many sequences for one call");
+    return dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(p.parts));
+}
+
 }  // namespace
 
 extern "C" {
 
 size_t vm_gated_workspace(int64_t batch, int64_t steps, int64_t channels) {
-    (void)batch, (void)steps, (void)channels;
-    return 0;
+    if (!sizes_fit(batch, steps, channels) || batch == 0 || channels == 0) return 0;
+    const int64_t all = batch * channels;
+    int64_t parts     = 1;
+    for (const int length : {FORWARD, BACKWARD}) parts = std::max(parts, plan_of(all, steps, 4, length).parts);
+    parts = std::max(parts, plan_of(all, steps, 1, SINGLE).parts);
+    return parts > 1 ? static_cast<size_t>(parts * all) * sizeof(float2) : 0;
 }
 
 vm_status vm_gated_scan(int device, int32_t type, int64_t batch, int64_t steps, int64_t channels, const vm_sequence* x, const vm_sequence* gate, const float* h0,
@@ -84,15 +165,26 @@ vm_status vm_gated_scan(int device, int32_t type, int64_t batch, int64_t steps, 
         check_sequence(x, "x", type, sizes, steps > 0, false);
         check_sequence(gate, "gate", type, sizes, steps > 0, false);
         check_sequence(y, "y", type, sizes, false, true);
-        if (workspace_bytes < vm_gated_workspace(batch, steps, channels)) throw std::string("the workspace is too small");
-        (void)workspace;
+        check_workspace(batch, steps, channels, workspace, workspace_bytes);
         const OnDevice on(device);
         GatedArgs a{};
         a.batch = batch, a.steps = steps, a.channels = channels;
         a.x = sequence(x), a.gate = sequence(gate), a.y = sequence(y);
         a.h0 = h0, a.lengths = lengths, a.last = last, a.states = states;
-        const unsigned grid = blocks_of(batch * channels);
-        with_type(type, [&](auto kind) { launch_kernel(k_gated_scan<decltype(kind)>, dim3(grid), 256, 0, static_cast<cudaStream_t>(stream), false, a); });
+        const bool vectors = channels % 4 == 0 && takes(x, type, 4, sizes) && takes(gate, type, 4, sizes) && takes(y, type, 4, sizes) && aligned(h0, 16) && aligned(last, 16)
+                             && aligned(states, 16);
+        const int vector = vectors ? 4 : 1;
+        const Plan p     = plan_of(batch * channels, steps, vector, vectors ? FORWARD : SINGLE);
+        const Split s    = split_of(p, workspace);
+        const dim3 grid  = grid_of(batch * channels, p, vector);
+        const auto q     = static_cast<cudaStream_t>(stream);
+        with_layout(type, vector, p.tx, [&](auto kind, auto v, auto tx) {
+            using T = decltype(kind);
+            constexpr int V = decltype(v)::value, TX = decltype(tx)::value, L = V == 1 ? SINGLE : FORWARD, STAGES = V == 1 ? 0 : sizeof(T) == 2 ? 3 : 2;
+            constexpr int shared = Tiles<T, V, L, 2, STAGES>::BYTES;
+            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, TX, L, STAGES, false>>(grid, shared, q, a, s);
+            launch_tiles<k_gated_scan<T, V, TX, L, STAGES>>(grid, shared, q, a, s);
+        });
     }
     catch (const std::string& refused) {
         return fail(VM_ERR_INVALID_ARGUMENT, refused);
@@ -116,16 +208,26 @@ vm_status vm_gated_scan_backward(int device, int32_t type, int64_t batch, int64_
         check_sequence(dx, "dx", type, sizes, false, true);
         check_sequence(d_gate, "d_gate", type, sizes, false, true);
         if (steps > 0 && states == nullptr) throw std::string("null states");
-        if (workspace_bytes < vm_gated_workspace(batch, steps, channels)) throw std::string("the workspace is too small");
-        (void)workspace;
+        check_workspace(batch, steps, channels, workspace, workspace_bytes);
         const OnDevice on(device);
         GatedArgs a{};
         a.batch = batch, a.steps = steps, a.channels = channels;
         a.x = sequence(x), a.gate = sequence(gate), a.y = sequence(dy);
         a.lengths = lengths, a.states = const_cast<float*>(states), a.d_last = d_last;
         a.dx = sequence(dx), a.d_gate = sequence(d_gate), a.d_h0 = d_h0;
-        const unsigned grid = blocks_of(batch * channels);
-        with_type(type, [&](auto kind) { launch_kernel(k_gated_scan_grad<decltype(kind)>, dim3(grid), 256, 0, static_cast<cudaStream_t>(stream), false, a); });
+        const bool vectors = channels % 4 == 0 && takes(x, type, 4, sizes) && takes(gate, type, 4, sizes) && takes(dy, type, 4, sizes) && takes(dx, type, 4, sizes)
+                             && takes(d_gate, type, 4, sizes) && aligned(states, 16) && aligned(d_last, 16) && aligned(d_h0, 16);
+        const int vector = vectors ? 4 : 1;
+        const Plan p     = plan_of(batch * channels, steps, vector, vectors ? BACKWARD : SINGLE);
+        const Split s    = split_of(p, workspace);
+        const dim3 grid  = grid_of(batch * channels, p, vector);
+        const auto q     = static_cast<cudaStream_t>(stream);
+        with_layout(type, vector, p.tx, [&](auto kind, auto v, auto tx) {
+            using T = decltype(kind);
+            constexpr int V = decltype(v)::value, TX = decltype(tx)::value, L = V == 1 ? SINGLE : BACKWARD, STAGES = V == 1 ? 0 : sizeof(T) == 2 ? 3 : 2;
+            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, TX, L, STAGES, true>>(grid, Tiles<T, V, L, 2, STAGES>::BYTES, q, a, s);
+            launch_tiles<k_gated_scan_grad<T, V, TX, L, STAGES>>(grid, Tiles<T, V, L, 3, STAGES>::BYTES, q, a, s);
+        });
     }
     catch (const std::string& refused) {
         return fail(VM_ERR_INVALID_ARGUMENT, refused);

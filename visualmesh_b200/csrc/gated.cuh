@@ -10,6 +10,8 @@
 #pragma once
 
 #include <cstdint>
+#include <cstring>
+#include <type_traits>
 
 #include "../../include/vmcuda.h"
 #include "element.cuh"
@@ -50,12 +52,23 @@ struct Factors {
     float f, u;
 };
 __device__ __forceinline__ Factors factors_of(float g) {
-    const float e = __expf(-fabsf(g)), r = 1.0f / (1.0f + e), s = e * r;  // e <= 1: nothing overflows
+    const float e = __expf(-fabsf(g)), r = __fdividef(1.0f, 1.0f + e), s = e * r;  // e <= 1: nothing overflows
     return g >= 0.0f ? Factors{r, s} : Factors{s, r};
 }
 // a * b, where a of 0 drops b
 __device__ __forceinline__ float gated(float a, float b) {
     return a == 0.0f ? 0.0f : a * b;
+}
+
+// a * b + c, where a of 0 drops b
+__device__ __forceinline__ float gated(float a, float b, float c) {
+    return a == 0.0f ? c : fmaf(a, b, c);
+}
+// The factor of two runs of steps. It is 0 only where a step's is: what 32 bits cannot hold becomes their smallest normal number, so that an
+// infinity or NaN goes on through a long run as it does step by step.
+__device__ __forceinline__ float product(float a, float b) {
+    const float r = a * b;
+    return a == 0.0f || b == 0.0f ? 0.0f : r == 0.0f ? 1.17549435e-38f : r;
 }
 
 __device__ __forceinline__ int64_t length_of(const GatedArgs& a, int64_t b) {
@@ -64,67 +77,561 @@ __device__ __forceinline__ int64_t length_of(const GatedArgs& a, int64_t b) {
     return n < 0 ? 0 : n > a.steps ? a.steps : n;
 }
 
-// A thread per sequence of one channel.
-template <typename T>
-__global__ void __launch_bounds__(256) k_gated_scan(const GatedArgs a) {
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (at >= a.batch * a.channels) return;
-    const int64_t b = at / a.channels, c = at % a.channels;
-    const T* x = static_cast<const T*>(a.x.data) + b * a.x.b + c * a.x.c;
-    const T* g = static_cast<const T*>(a.gate.data) + b * a.gate.b + c * a.gate.c;
-    T* y       = a.y.data != nullptr ? static_cast<T*>(a.y.data) + b * a.y.b + c * a.y.c : nullptr;
-    float h    = a.h0 != nullptr ? a.h0[at] : 0.0f;
-    const int64_t n = length_of(a, b), kept = (a.steps + KEEP - 1) / KEEP;
-    for (int64_t t = 0; t < a.steps; ++t) {
-        if (a.states != nullptr && t % KEEP == 0) a.states[(b * kept + t / KEEP) * a.channels + c] = h;
-        if (t < n) {
-            const Factors k = factors_of(to_float(g[t * a.gate.t]));
-            h = gated(k.f, h) + gated(k.u, to_float(x[t * a.x.t]));
+// ---- tiles -------------------------------------------------------------------------------------------------------------------
+// A block owns TX * V neighbouring channels and walks over time, a tile of WARPS * 32 / TX * L steps at a time: a thread holds V channels of
+// L consecutive steps, TX threads lie along the channels, the others along time. A step h -> f h + v is an affine map, and so is every run
+// of steps (A, H): h -> A h + H. A tile is three things: the maps of the threads' own steps, a scan of the maps over the threads along time
+// (shuffles inside a warp, shared memory between the warps, one barrier), and the states of the own steps from the one that the scan gives.
+// Every element is read once and written once. Vectors come through a ring of tiles in shared memory, where every thread has its
+// own places, filled by asynchronous copies a few tiles ahead: they hold no registers and need no barrier.
+//
+// Whether a factor of 0 meets an infinity or NaN is not asked step by step: a factor of 0 leaves A = 0, an infinity or NaN leaves H without
+// a finite value (0 times it is NaN), and only then the thread goes over its steps again, with the rule.
+constexpr int THREADS = 128;
+constexpr int WARPS   = THREADS / 32;
+
+template <int BYTES>
+struct RawOf;
+template <>
+struct RawOf<2> {
+    using type = uint16_t;
+};
+template <>
+struct RawOf<4> {
+    using type = uint32_t;
+};
+template <>
+struct RawOf<8> {
+    using type = uint2;
+};
+template <>
+struct RawOf<16> {
+    using type = uint4;
+};
+template <typename T, int V>
+using Raw = typename RawOf<V * sizeof(T)>::type;
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Raw<T, V>& raw, float (&to)[V]) {
+    T e[V];
+    memcpy(e, &raw, sizeof(raw));
+#pragma unroll
+    for (int k = 0; k < V; ++k) to[k] = to_float(e[k]);
+}
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> pack(const float (&from)[V]) {
+    T e[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) e[k] = from_float<T>(from[k]);
+    Raw<T, V> raw;
+    memcpy(&raw, e, sizeof(raw));
+    return raw;
+}
+template <int V>
+__device__ __forceinline__ void load_floats(const float* from, float (&to)[V]) {
+    if constexpr (V % 4 == 0) {
+#pragma unroll
+        for (int k = 0; k < V; k += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(from + k);
+            to[k] = q.x, to[k + 1] = q.y, to[k + 2] = q.z, to[k + 3] = q.w;
         }
-        if (y != nullptr) y[t * a.y.t] = from_float<T>(t < n ? h : 0.0f);
     }
-    if (a.last != nullptr) a.last[at] = h;
+    else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) to[k] = from[k];
+    }
+}
+template <int V>
+__device__ __forceinline__ void store_floats(float* to, const float (&from)[V]) {
+    if constexpr (V % 4 == 0) {
+#pragma unroll
+        for (int k = 0; k < V; k += 4) *reinterpret_cast<float4*>(to + k) = make_float4(from[k], from[k + 1], from[k + 2], from[k + 3]);
+    }
+    else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) to[k] = from[k];
+    }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) k_gated_scan_grad(const GatedArgs a) {
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (at >= a.batch * a.channels) return;
-    const int64_t b = at / a.channels, c = at % a.channels;
-    const T* x  = static_cast<const T*>(a.x.data) + b * a.x.b + c * a.x.c;
-    const T* g  = static_cast<const T*>(a.gate.data) + b * a.gate.b + c * a.gate.c;
-    const T* dy = a.y.data != nullptr ? static_cast<const T*>(a.y.data) + b * a.y.b + c * a.y.c : nullptr;
-    T* dx       = a.dx.data != nullptr ? static_cast<T*>(a.dx.data) + b * a.dx.b + c * a.dx.c : nullptr;
-    T* dg       = a.d_gate.data != nullptr ? static_cast<T*>(a.d_gate.data) + b * a.d_gate.b + c * a.d_gate.c : nullptr;
-    float carry = a.d_last != nullptr ? a.d_last[at] : 0.0f;
-    const int64_t n = length_of(a, b), kept = (a.steps + KEEP - 1) / KEEP;
-    float before[KEEP];
-    for (int64_t k = kept - 1; k >= 0; --k) {
-        const int64_t first = k * KEEP;
-        const int count     = static_cast<int>(a.steps - first < KEEP ? a.steps - first : KEEP);
-        float h             = a.states[(b * kept + k) * a.channels + c];
-        for (int i = 0; i < count; ++i) {
-            before[i] = h;
-            if (first + i < n) {
-                const Factors q = factors_of(to_float(g[(first + i) * a.gate.t]));
-                h = gated(q.f, h) + gated(q.u, to_float(x[(first + i) * a.x.t]));
-            }
+template <int V, int TX>
+struct Place {
+    static constexpr int SEGMENTS = 32 / TX;  // of a warp
+    int warp, lane, tx, ty;
+    int64_t at, b, c;  // first of the thread's channels: of all, its batch, within that
+    bool there;
+    __device__ __forceinline__ Place(const GatedArgs& a) {
+        warp  = threadIdx.x / 32;
+        lane  = threadIdx.x % 32;
+        tx    = lane % TX;
+        ty    = warp * SEGMENTS + lane / TX;
+        at    = (static_cast<int64_t>(blockIdx.x) * TX + tx) * V;
+        there = at < a.batch * a.channels;
+        b     = there ? at / a.channels : 0;
+        c     = there ? at - b * a.channels : 0;
+    }
+};
+
+// (A, H) after (pa, ph): h -> A (pa h + ph) + H
+template <int V>
+__device__ __forceinline__ void compose(float (&A)[V], float (&H)[V], const float (&pa)[V], const float (&ph)[V]) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        H[k] = gated(A[k], ph[k], H[k]);
+        A[k] = product(A[k], pa[k]);
+    }
+}
+
+// Scan over the threads along time, in their order or (REVERSE) against it. In: every thread's map (A, H). Out: the map of all threads
+// before it in its own warp (A, H), and in `totals` (shared memory, [WARPS][TX * V]) the maps of the whole warps.
+template <int V, int TX, bool REVERSE>
+__device__ __forceinline__ void scan_warp(const Place<V, TX>& at, float (&A)[V], float (&H)[V], float2* totals) {
+#pragma unroll
+    for (int d = TX; d < 32; d *= 2) {
+        float pa[V], ph[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            pa[k] = REVERSE ? __shfl_down_sync(~0u, A[k], d) : __shfl_up_sync(~0u, A[k], d);
+            ph[k] = REVERSE ? __shfl_down_sync(~0u, H[k], d) : __shfl_up_sync(~0u, H[k], d);
         }
-        for (int i = count - 1; i >= 0; --i) {
-            const int64_t t = first + i;
-            float to_x = 0.0f, to_g = 0.0f;
-            if (t < n) {
-                const Factors q   = factors_of(to_float(g[t * a.gate.t]));
-                const float total = (dy != nullptr ? to_float(dy[t * a.y.t]) : 0.0f) + carry;
-                to_x  = gated(q.u, total);
-                to_g  = gated(q.f * q.u, (before[i] - to_float(x[t * a.x.t])) * total);
-                carry = gated(q.f, total);
-            }
-            if (dx != nullptr) dx[t * a.dx.t] = from_float<T>(to_x);
-            if (dg != nullptr) dg[t * a.d_gate.t] = from_float<T>(to_g);
+        if (REVERSE ? at.lane + d < 32 : at.lane >= d) compose<V>(A, H, pa, ph);
+    }
+    if (REVERSE ? at.lane < TX : at.lane >= 32 - TX) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) totals[at.warp * TX * V + at.tx * V + k] = make_float2(A[k], H[k]);
+    }
+    if constexpr (TX < 32) {
+        const bool first = REVERSE ? at.lane >= 32 - TX : at.lane < TX;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float pa = REVERSE ? __shfl_down_sync(~0u, A[k], TX) : __shfl_up_sync(~0u, A[k], TX);
+            const float ph = REVERSE ? __shfl_down_sync(~0u, H[k], TX) : __shfl_up_sync(~0u, H[k], TX);
+            A[k] = first ? 1.0f : pa;
+            H[k] = first ? 0.0f : ph;
         }
     }
-    if (a.d_h0 != nullptr) a.d_h0[at] = carry;
+    else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) A[k] = 1.0f, H[k] = 0.0f;
+    }
+}
+// After a barrier: the state in front of the thread's own steps, from the one in front of all threads (carry), which becomes the one
+// behind them.
+template <int V, int TX, bool REVERSE>
+__device__ __forceinline__ void scan_block(const Place<V, TX>& at, const float (&A)[V], const float (&H)[V], const float2* totals, float (&carry)[V], float (&mine)[V]) {
+#pragma unroll 1
+    for (int i = 0; i < WARPS; ++i) {
+        const int w = REVERSE ? WARPS - 1 - i : i;
+        if (w == at.warp) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) mine[k] = gated(A[k], carry[k], H[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float2 q = totals[w * TX * V + at.tx * V + k];
+            carry[k]       = gated(q.x, carry[k], q.y);
+        }
+    }
+}
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+    static_assert(BYTES == 4 || BYTES == 8 || BYTES == 16, "sizes of an asynchronous copy");
+    const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
+}
+
+// The tiles of N sequences on their way: the steps of a thread that come before `stop`, of tile after tile, read by that thread alone.
+// STAGES == 0: read when they are asked for.
+template <typename T, int V, int L, int N, int STAGES>
+struct Tiles {
+    using R = Raw<T, V>;
+    static constexpr int BYTES = STAGES * N * L * THREADS * sizeof(R);
+    R* ring;
+    const T* from[N];   // the thread's first step of the tile to be asked for next (STAGES == 0: of the present one)
+    int64_t stride[N];  // from step to step
+    int64_t next, left; // that step's number, and how many tiles are to be asked for
+    int put, at;
+
+    __device__ __forceinline__ R* place(int stage, int n, int i) const {
+        return ring + ((stage * N + n) * L + i) * THREADS + threadIdx.x;
+    }
+    // by: steps from tile to tile; stop: behind the last step that is read
+    __device__ __forceinline__ void ask(int64_t by, const int64_t (&stop)[N]) {
+        if (left-- > 0) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const T* p = from[n];
+#pragma unroll
+                for (int i = 0; i < L; ++i) {
+                    if (next + i < stop[n]) copy_async<sizeof(R)>(place(put, n, i), p);
+                    p += stride[n];
+                }
+                from[n] += by * stride[n];
+            }
+        }
+        next += by;
+        put = put + 1 == STAGES ? 0 : put + 1;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    __device__ __forceinline__ void begin(void* shared, int64_t first, int64_t by, int64_t tiles, const int64_t (&stop)[N]) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) from[n] += first * stride[n];
+        ring = static_cast<R*>(shared), next = first, left = tiles, put = 0, at = STAGES - 1;
+        if constexpr (STAGES > 0) {
+#pragma unroll
+            for (int s = 0; s + 1 < STAGES; ++s) ask(by, stop);
+        }
+        else {
+#pragma unroll
+            for (int n = 0; n < N; ++n) from[n] -= by * stride[n];
+        }
+    }
+    // on to the next tile
+    __device__ __forceinline__ void advance(int64_t by, const int64_t (&stop)[N]) {
+        if constexpr (STAGES > 0) {
+            ask(by, stop);
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+            at = at + 1 == STAGES ? 0 : at + 1;
+        }
+        else {
+#pragma unroll
+            for (int n = 0; n < N; ++n) from[n] += by * stride[n];
+        }
+    }
+    // step number i of the thread's in sequence n; 0 where it is not `on`
+    __device__ __forceinline__ void get(int n, int i, bool on, float (&to)[V]) const {
+        R raw{};
+        if (on) raw = STAGES > 0 ? *place(at, n, i) : *reinterpret_cast<const R*>(from[n] + i * stride[n]);
+        unpack<T, V>(raw, to);
+    }
+};
+
+// The part of time that a block of a split launch has: whole tiles of `run` steps, the last as long as there are steps.
+struct Split {
+    int64_t run;      // steps of a part, a multiple of a tile's; all of them where nothing is split
+    int32_t parts;
+    float2* summary;  // [parts][batch * channels]: the map of every part
+};
+
+// whether a run of steps met nothing that needs care: no factor of 0 (nor a product that came to it), no value that is not finite
+template <int V>
+__device__ __forceinline__ bool plain(const float (&A)[V], const float (&H)[V]) {
+    bool ok = true;
+#pragma unroll
+    for (int k = 0; k < V; ++k) ok = ok && A[k] > 0.0f && fabsf(H[k]) < INFINITY;
+    return ok;
+}
+template <int V>
+__device__ __forceinline__ bool finite(const float (&v)[V]) {
+    float zero = 0.0f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) zero = fmaf(v[k], 0.0f, zero);
+    return zero == 0.0f;
+}
+
+// The state in front of part `part` of a split sequence (or, REVERSE, behind it), from the one at the sequence's end: a thread along
+// time for every part on that side.
+template <int V, int TX, bool REVERSE>
+__device__ __forceinline__ void join_parts(const GatedArgs& a, const Split& s, const Place<V, TX>& at, int part, float (&carry)[V], float2 (*totals)[WARPS * TX * V]) {
+    constexpr int TY  = THREADS / TX;
+    const int64_t all = a.batch * a.channels;
+    const int begin = REVERSE ? part + 1 : 0, end = REVERSE ? s.parts : part;
+    const int rounds = (end - begin + TY - 1) / TY;
+    for (int r = 0; r < rounds; ++r) {
+        const int j = begin + (REVERSE ? rounds - 1 - r : r) * TY + at.ty;
+        float A[V], H[V], ignored[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            A[k] = 1.0f, H[k] = 0.0f;
+            if (j < end && at.there) {
+                const float2 q = s.summary[j * all + at.at + k];
+                A[k] = q.x, H[k] = q.y;
+            }
+        }
+        scan_warp<V, TX, REVERSE>(at, A, H, totals[r & 1]);
+        __syncthreads();
+        scan_block<V, TX, REVERSE>(at, A, H, totals[r & 1], carry, ignored);
+    }
+    if (rounds > 0) __syncthreads();  // the walk over the tiles begins with the first of the two buffers again
+}
+
+// Maps of the parts of a split sequence, of the recurrence or (REVERSE) of its gradient.
+template <typename T, int V, int TX, int L, int STAGES, bool REVERSE>
+__global__ void __launch_bounds__(THREADS) k_gated_summary(const GatedArgs a, const Split s) {
+    constexpr int TILE = THREADS / TX * L;
+    extern __shared__ uint4 ring[];
+    __shared__ float2 totals[2][WARPS * TX * V];
+    const Place<V, TX> at(a);
+    const int64_t n     = at.there ? length_of(a, at.b) : 0;
+    const int64_t begin = blockIdx.y * s.run, end = begin + s.run < a.steps ? begin + s.run : a.steps;
+    const int64_t tiles = (end - begin + TILE - 1) / TILE, stop = end < n ? end : n;
+    const Sequence& in  = REVERSE ? a.y : a.x;
+    Tiles<T, V, L, 2, STAGES> io;
+    const int64_t stops[2] = {in.data != nullptr ? stop : 0, stop};
+    io.from[0] = static_cast<const T*>(in.data) + at.b * in.b + at.c * in.c, io.stride[0] = in.t;
+    io.from[1] = static_cast<const T*>(a.gate.data) + at.b * a.gate.b + at.c * a.gate.c, io.stride[1] = a.gate.t;
+    constexpr int BY = REVERSE ? -TILE : TILE;
+    int64_t t        = begin + (REVERSE ? tiles - 1 : 0) * TILE + at.ty * L;
+    io.begin(ring, t, BY, tiles, stops);
+    float carry[V], whole[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) carry[k] = 0.0f, whole[k] = 1.0f;
+    for (int64_t tile = 0; tile < tiles; ++tile, t += BY) {
+        io.advance(BY, stops);
+        float A[V], H[V], mine[V];
+        const auto pass = [&](auto careful) {
+            constexpr bool CAREFUL = decltype(careful)::value;
+#pragma unroll
+            for (int k = 0; k < V; ++k) A[k] = 1.0f, H[k] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                const int step = REVERSE ? L - 1 - i : i;
+                float x[V], g[V];
+                io.get(0, step, t + step < stops[0], x);
+                io.get(1, step, t + step < stop, g);
+                if (t + step < stop) {
+#pragma unroll
+                    for (int k = 0; k < V; ++k) {
+                        const Factors w = factors_of(g[k]);
+                        if constexpr (CAREFUL) {
+                            H[k] = REVERSE ? gated(w.f, x[k] + H[k]) : gated(w.f, H[k], gated(w.u, x[k]));
+                            A[k] = product(w.f, A[k]);
+                        }
+                        else {
+                            H[k] = REVERSE ? w.f * (x[k] + H[k]) : fmaf(w.f, H[k], w.u * x[k]);
+                            A[k] = w.f * A[k];
+                        }
+                    }
+                }
+            }
+        };
+        pass(std::false_type{});
+        if (!plain<V>(A, H)) pass(std::true_type{});
+        scan_warp<V, TX, REVERSE>(at, A, H, totals[tile & 1]);
+        __syncthreads();
+        scan_block<V, TX, REVERSE>(at, A, H, totals[tile & 1], carry, mine);
+#pragma unroll 1
+        for (int i = 0; i < WARPS; ++i) {
+            const int w = REVERSE ? WARPS - 1 - i : i;
+#pragma unroll
+            for (int k = 0; k < V; ++k) whole[k] = product(totals[tile & 1][w * TX * V + at.tx * V + k].x, whole[k]);
+        }
+    }
+    if (at.there && at.ty == 0) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) s.summary[blockIdx.y * (a.batch * a.channels) + at.at + k] = make_float2(whole[k], carry[k]);
+    }
+}
+
+template <typename T, int V, int TX, int L, int STAGES>
+__global__ void __launch_bounds__(THREADS, 4) k_gated_scan(const GatedArgs a, const Split s) {
+    constexpr int TILE = THREADS / TX * L;
+    extern __shared__ uint4 ring[];
+    __shared__ float2 totals[2][WARPS * TX * V];
+    const Place<V, TX> at(a);
+    const int64_t n     = at.there ? length_of(a, at.b) : 0, kept = (a.steps + KEEP - 1) / KEEP;
+    const int64_t begin = blockIdx.y * s.run, end = begin + s.run < a.steps ? begin + s.run : a.steps;
+    const int64_t tiles = (end - begin + TILE - 1) / TILE, stop = end < n ? end : n;
+    Tiles<T, V, L, 2, STAGES> io;
+    const int64_t stops[2] = {stop, stop};
+    io.from[0] = static_cast<const T*>(a.x.data) + at.b * a.x.b + at.c * a.x.c, io.stride[0] = a.x.t;
+    io.from[1] = static_cast<const T*>(a.gate.data) + at.b * a.gate.b + at.c * a.gate.c, io.stride[1] = a.gate.t;
+    int64_t t = begin + at.ty * L;
+    io.begin(ring, t, TILE, tiles, stops);
+    T* y              = static_cast<T*>(a.y.data) + at.b * a.y.b + at.c * a.y.c;
+    const bool writes = at.there && a.y.data != nullptr;
+    float carry[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) carry[k] = 0.0f;
+    if (at.there && a.h0 != nullptr) load_floats<V>(a.h0 + at.at, carry);
+    if (s.parts > 1) join_parts<V, TX, false>(a, s, at, blockIdx.y, carry, totals);
+    for (int64_t tile = 0; tile < tiles; ++tile, t += TILE) {
+        io.advance(TILE, stops);
+        float f[L][V], v[L][V], A[V], H[V], h[V];
+        const auto pass = [&](auto careful) {
+            constexpr bool CAREFUL = decltype(careful)::value;
+#pragma unroll
+            for (int k = 0; k < V; ++k) A[k] = 1.0f, H[k] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                const bool on = t + i < stop;
+                io.get(0, i, on, v[i]);
+                io.get(1, i, on, f[i]);
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const Factors q = factors_of(f[i][k]);
+                    f[i][k] = on ? q.f : 1.0f;
+                    v[i][k] = CAREFUL ? gated(q.u, v[i][k]) : q.u * v[i][k];  // behind the end v is 0, and so is this
+                    H[k]    = CAREFUL ? gated(f[i][k], H[k], v[i][k]) : fmaf(f[i][k], H[k], v[i][k]);
+                    A[k]    = CAREFUL ? product(f[i][k], A[k]) : f[i][k] * A[k];
+                }
+            }
+        };
+        pass(std::false_type{});
+        bool careful = !plain<V>(A, H);
+        if (careful) pass(std::true_type{});
+        scan_warp<V, TX, false>(at, A, H, totals[tile & 1]);
+        __syncthreads();
+        scan_block<V, TX, false>(at, A, H, totals[tile & 1], carry, h);
+        if (a.states != nullptr && at.there && t < end && t % KEEP == 0) store_floats<V>(a.states + (at.b * kept + t / KEEP) * a.channels + at.c, h);
+        careful = careful || !finite<V>(h);
+        if (careful) {
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[i][k] = h[k] = gated(f[i][k], h[k], v[i][k]);
+            }
+        }
+        else {
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[i][k] = h[k] = fmaf(f[i][k], h[k], v[i][k]);
+            }
+        }
+        T* to = y + t * a.y.t;
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            if (writes && t + i < end) *reinterpret_cast<Raw<T, V>*>(to) = t + i < stop ? pack<T, V>(v[i]) : Raw<T, V>{};
+            to += a.y.t;
+        }
+    }
+    if (a.last != nullptr && at.there && at.ty == 0 && blockIdx.y + 1 == gridDim.y) store_floats<V>(a.last + at.at, carry);
+}
+
+template <typename T, int V, int TX, int L, int STAGES>
+__global__ void __launch_bounds__(THREADS, 4) k_gated_scan_grad(const GatedArgs a, const Split s) {
+    constexpr int TILE = THREADS / TX * L;
+    extern __shared__ uint4 ring[];
+    __shared__ float2 totals[2][WARPS * TX * V], totals_back[2][WARPS * TX * V];
+    const Place<V, TX> at(a);
+    const int64_t n     = at.there ? length_of(a, at.b) : 0, kept = (a.steps + KEEP - 1) / KEEP;
+    const int64_t begin = blockIdx.y * s.run, end = begin + s.run < a.steps ? begin + s.run : a.steps;
+    const int64_t tiles = (end - begin + TILE - 1) / TILE, stop = end < n ? end : n;
+    Tiles<T, V, L, 3, STAGES> io;
+    const int64_t stops[3] = {stop, stop, a.y.data != nullptr ? stop : 0};
+    io.from[0] = static_cast<const T*>(a.x.data) + at.b * a.x.b + at.c * a.x.c, io.stride[0] = a.x.t;
+    io.from[1] = static_cast<const T*>(a.gate.data) + at.b * a.gate.b + at.c * a.gate.c, io.stride[1] = a.gate.t;
+    io.from[2] = static_cast<const T*>(a.y.data) + at.b * a.y.b + at.c * a.y.c, io.stride[2] = a.y.t;
+    int64_t t0 = begin + (tiles > 0 ? tiles - 1 : 0) * TILE;  // the last tile comes first
+    io.begin(ring, t0 + at.ty * L, -TILE, tiles, stops);
+    T* dx = static_cast<T*>(a.dx.data) + at.b * a.dx.b + at.c * a.dx.c;
+    T* dg = static_cast<T*>(a.d_gate.data) + at.b * a.d_gate.b + at.c * a.d_gate.c;
+    const bool writes_x = at.there && a.dx.data != nullptr, writes_g = at.there && a.d_gate.data != nullptr;
+    const float* states = a.states + at.b * kept * a.channels + at.c;
+    float back[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) back[k] = 0.0f;
+    if (at.there && a.d_last != nullptr) load_floats<V>(a.d_last + at.at, back);
+    if (s.parts > 1) join_parts<V, TX, true>(a, s, at, blockIdx.y, back, totals_back);
+    for (int64_t tile = 0; tile < tiles; ++tile, t0 -= TILE) {
+        const int64_t t = t0 + at.ty * L;
+        float carry[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) carry[k] = 0.0f;
+        if (at.there) load_floats<V>(states + t0 / KEEP * a.channels, carry);
+        io.advance(-TILE, stops);
+        float f[L][V], u[L][V], w[L][V], d[L][V], A[V], H[V], AR[V], R[V], h[V], c[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) A[k] = 1.0f, H[k] = 0.0f, R[k] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            const bool on = t + i < stop;
+            io.get(0, i, on, w[i]);
+            io.get(1, i, on, f[i]);
+            io.get(2, i, t + i < stops[2], d[i]);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const Factors q = factors_of(f[i][k]);
+                f[i][k] = on ? q.f : 1.0f;
+                u[i][k] = on ? q.u : 0.0f;
+                H[k]    = fmaf(f[i][k], H[k], u[i][k] * w[i][k]);
+                A[k]    = f[i][k] * A[k];
+            }
+        }
+#pragma unroll
+        for (int i = L - 1; i >= 0; --i) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) R[k] = f[i][k] * (d[i][k] + R[k]);
+        }
+        bool careful = !plain<V>(A, H) || !finite<V>(R);
+        if (careful) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) A[k] = 1.0f, H[k] = 0.0f, R[k] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    H[k] = gated(f[i][k], H[k], gated(u[i][k], w[i][k]));
+                    A[k] = product(f[i][k], A[k]);
+                    R[k] = gated(f[L - 1 - i][k], d[L - 1 - i][k] + R[k]);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) AR[k] = A[k];
+        scan_warp<V, TX, false>(at, A, H, totals[tile & 1]);
+        scan_warp<V, TX, true>(at, AR, R, totals_back[tile & 1]);
+        __syncthreads();
+        scan_block<V, TX, false>(at, A, H, totals[tile & 1], carry, h);
+        scan_block<V, TX, true>(at, AR, R, totals_back[tile & 1], back, c);
+        careful = careful || !finite<V>(h) || !finite<V>(c);
+        // w: from x to h_(t-1) - x; then u to the gradient of x and w to that of the gate
+        if (careful) {
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const float here = w[i][k];
+                    w[i][k] = h[k] - here;
+                    h[k]    = gated(f[i][k], h[k], gated(u[i][k], here));
+                }
+            }
+#pragma unroll
+            for (int i = L - 1; i >= 0; --i) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const float total = d[i][k] + c[k];
+                    w[i][k] = gated(f[i][k] * u[i][k], w[i][k] * total);
+                    u[i][k] = gated(u[i][k], total);
+                    c[k]    = gated(f[i][k], total);
+                }
+            }
+        }
+        else {
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const float here = w[i][k];
+                    w[i][k] = h[k] - here;
+                    h[k]    = fmaf(f[i][k], h[k], u[i][k] * here);
+                }
+            }
+#pragma unroll
+            for (int i = L - 1; i >= 0; --i) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const float total = d[i][k] + c[k];
+                    u[i][k] = u[i][k] * total;
+                    c[k]    = f[i][k] * total;
+                    w[i][k] = f[i][k] * u[i][k] * w[i][k];
+                }
+            }
+        }
+        T* to_x = dx + t * a.dx.t;
+        T* to_g = dg + t * a.d_gate.t;
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+            if (t + i < end) {
+                if (writes_x) *reinterpret_cast<Raw<T, V>*>(to_x) = pack<T, V>(u[i]);
+                if (writes_g) *reinterpret_cast<Raw<T, V>*>(to_g) = pack<T, V>(w[i]);
+            }
+            to_x += a.dx.t, to_g += a.d_gate.t;
+        }
+    }
+    if (a.d_h0 != nullptr && at.there && at.ty == 0 && blockIdx.y == 0) store_floats<V>(a.d_h0 + at.at, back);
 }
 
 __global__ void __launch_bounds__(256) k_first_rows(const StepArgs a) {
@@ -148,7 +655,7 @@ __global__ void __launch_bounds__(256) k_gated_step(const StepArgs a) {
     if (slot >= 0) {
         const Factors k = factors_of(to_float(static_cast<const T*>(a.gate.data)[row * a.gate.b + c * a.gate.c]));
         float* state    = a.state + slot * a.state_stride + c;
-        h = gated(k.f, *state) + gated(k.u, to_float(static_cast<const T*>(a.x.data)[row * a.x.b + c * a.x.c]));
+        h = gated(k.f, *state, gated(k.u, to_float(static_cast<const T*>(a.x.data)[row * a.x.b + c * a.x.c])));
         *state = h;
     }
     if (a.y.data != nullptr) static_cast<T*>(a.y.data)[row * a.y.b + c * a.y.c] = from_float<T>(h);
