@@ -1,4 +1,6 @@
 // vm_scores and vm_scores_backward: checks and launches of the kernels in scores.cuh.
+#include <type_traits>
+
 #include "device_call.hpp"
 #include "scores.cuh"
 
@@ -17,6 +19,61 @@ vm_status check_rows(const void* x, int32_t type, int64_t rows, int32_t classes,
     return VM_OK;
 }
 
+constexpr int SMS          = 148;
+constexpr int MOST_IN_ROWS = 1024;  // classes that a row's lanes hold in registers
+
+// f(lanes of a row, values of a lane), as constants
+template <typename F>
+void with_lanes(int classes, F f) {
+    using std::integral_constant;
+    if (classes <= 2) f(integral_constant<int, 1>{}, integral_constant<int, 2>{});
+    else if (classes <= 4) f(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+    else if (classes <= 8) f(integral_constant<int, 1>{}, integral_constant<int, 8>{});
+    else if (classes <= 16) f(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+    else if (classes <= 32) f(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+    else if (classes <= 128) f(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+    else if (classes <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+    else if (classes <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+    else f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+}
+template <typename F>
+void with_values(int32_t type, uint32_t flags, F f) {
+    with_type(type, [&](auto kind) {
+        if ((flags & VM_PROBABILITIES) != 0) f(kind, std::true_type{});
+        else f(kind, std::false_type{});
+    });
+}
+
+dim3 grid_of(int64_t blocks) {
+    if (blocks > INT32_MAX) throw std::string("too many rows for one call");
+    return dim3(static_cast<unsigned>(blocks));
+}
+bool starts_on_16(const void* p, int64_t stride, int32_t type) {
+    return aligned(p, 16) && stride * static_cast<int64_t>(element_size(type)) % 16 == 0;
+}
+
+// Blocks of a cluster for one row: as many as keep the SMs busy with all rows' blocks, each with at least two pieces of 16 bytes a thread.
+int blocks_of_row(int64_t rows, int64_t classes, int32_t type) {
+    int n = 1;
+    while (n < MOST_BLOCKS && rows * n * 2 <= 4 * SMS && classes * static_cast<int64_t>(element_size(type)) / 16 / (n * 2) >= 2 * STREAM_BLOCK) n *= 2;
+    return n;
+}
+
+template <typename Kernel>
+void launch_cluster(Kernel kernel, dim3 grid, int blocks, cudaStream_t q, const ScoresArgs& a) {
+    cudaLaunchAttribute attribute{};
+    attribute.id               = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = blocks;
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim  = grid;
+    config.blockDim = dim3(STREAM_BLOCK);
+    config.stream   = q;
+    config.attrs    = &attribute;
+    config.numAttrs = 1;
+    VM_CUDA(cudaLaunchKernelEx(&config, kernel, a, blocks));
+}
+
 }  // namespace
 
 extern "C" {
@@ -33,12 +90,23 @@ vm_status vm_scores(int device, const void* x, int32_t type, int64_t rows, int32
         const OnDevice on(device);
         const ScoresArgs a{x, rows, classes, row_stride, labels, (flags & VM_LABELS_64) != 0, top, log_prob, entropy, log_sum, top_log_prob, top_index};
         const auto q       = static_cast<cudaStream_t>(stream);
-        const int64_t grid = (rows + 7) / 8;
-        with_type(type, [&](auto kind) {
+        with_values(type, flags, [&](auto kind, auto probabilities) {
             using T = decltype(kind);
-            if ((flags & VM_PROBABILITIES) != 0) launch_kernel(k_scores<T, true>, dim3(grid), 256, 0, q, false, a);
-            else launch_kernel(k_scores<T, false>, dim3(grid), 256, 0, q, false, a);
+            constexpr bool P = decltype(probabilities)::value;
+            if (classes <= MOST_IN_ROWS) {
+                with_lanes(classes, [&](auto lanes, auto values) {
+                    constexpr int G = decltype(lanes)::value, E = decltype(values)::value;
+                    launch_kernel(k_scores_rows<T, P, G, E>, grid_of((rows * G + ROW_BLOCK - 1) / ROW_BLOCK), ROW_BLOCK, 0, q, false, a, starts_on_16(x, row_stride, type));
+                });
+                return;
+            }
+            const int blocks = blocks_of_row(rows, classes, type);
+            if (blocks > 1) launch_cluster(k_scores_stream<T, P, true>, grid_of(rows * blocks), blocks, q, a);
+            else launch_kernel(k_scores_stream<T, P, false>, grid_of(rows), STREAM_BLOCK, 0, q, false, a, 1);
         });
+    }
+    catch (const std::string& refused) {
+        return fail(VM_ERR_INVALID_ARGUMENT, refused);
     }
     catch (...) {
         return status_of_exception();
@@ -61,12 +129,26 @@ vm_status vm_scores_backward(int device, const void* x, int32_t type, int64_t ro
         const OnDevice on(device);
         const ScoresGradArgs a{x, rows, classes, row_stride, labels, (flags & VM_LABELS_64) != 0, entropy, log_sum, d_log_prob, d_entropy, d_log_sum, dx, dx_row_stride};
         const auto q       = static_cast<cudaStream_t>(stream);
-        const int64_t grid = (rows + 7) / 8;
-        with_type(type, [&](auto kind) {
+        with_values(type, flags, [&](auto kind, auto probabilities) {
             using T = decltype(kind);
-            if ((flags & VM_PROBABILITIES) != 0) launch_kernel(k_scores_grad<T, true>, dim3(grid), 256, 0, q, false, a);
-            else launch_kernel(k_scores_grad<T, false>, dim3(grid), 256, 0, q, false, a);
+            constexpr bool P = decltype(probabilities)::value;
+            if (classes <= MOST_IN_ROWS) {
+                const bool wide  = starts_on_16(x, row_stride, type) && starts_on_16(dx, dx_row_stride, type);
+                const bool dense = dx_row_stride == classes && aligned(dx, 16);
+                with_lanes(classes, [&](auto lanes, auto values) {
+                    constexpr int G = decltype(lanes)::value, E = decltype(values)::value;
+                    launch_kernel(k_scores_grad_rows<T, P, G, E>, grid_of((rows * G + ROW_BLOCK - 1) / ROW_BLOCK), ROW_BLOCK, 0, q, false, a, wide, dense);
+                });
+                return;
+            }
+            constexpr int PIECES = STREAM_BLOCK * STREAM_AHEAD;
+            const int64_t pieces = classes / (16 / static_cast<int64_t>(sizeof(T))) + 2;  // one more where a row begins inside a piece
+            const int64_t blocks = (pieces + PIECES - 1) / PIECES;
+            launch_kernel(k_scores_grad_stream<T, P>, grid_of(rows * blocks), STREAM_BLOCK, 0, q, false, a, static_cast<int>(blocks));
         });
+    }
+    catch (const std::string& refused) {
+        return fail(VM_ERR_INVALID_ARGUMENT, refused);
     }
     catch (...) {
         return status_of_exception();

@@ -2,11 +2,16 @@
 //
 // With m = max_j v_j, t_j = v_j - m and e_j = exp t_j:
 //   log_sum = m + log sum e_j,   entropy = log sum e_j - (sum e_j t_j) / (sum e_j),   log p_j = v_j - log_sum
-// All of it in 32 bits: t_j <= 0, so no e_j overflows, and the largest is 1, so the sum is at least 1.
+// All of it in 32 bits: t_j <= 0, so no e_j overflows, and the largest is 1, so the sum is at least 1. Probabilities need no maximum and
+// no exponential: with s = sum x_j, log p_j = log x_j - log s and entropy = log s - (sum x_j log x_j) / s.
 #pragma once
 
-#include <cstdint>
+#include <cooperative_groups.h>
 
+#include <cstdint>
+#include <cstring>
+
+#include "../../include/vmcuda.h"
 #include "element.cuh"
 
 namespace vm {
@@ -56,127 +61,537 @@ __device__ __forceinline__ float value_of(float x) {
 
 // An order of all floats in which larger values have larger keys, equal ones (0 and -0 too) the lower index the larger key, and NaN
 // the largest: 32 bits of value above 32 bits of index. No key is 0 or has all bits set.
+__device__ __forceinline__ uint32_t order_of(float x) {
+    const uint32_t bits = __float_as_uint(x + 0.0f);
+    return x != x ? 0xFFFFFFFEu : (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ float value_of_order(uint32_t order) {
+    return order == 0xFFFFFFFEu ? NAN : __uint_as_float((order & 0x80000000u) ? order ^ 0x80000000u : ~order);
+}
 __device__ __forceinline__ uint64_t key_of(float x, int32_t index) {
-    const uint32_t bits  = __float_as_uint(x + 0.0f);
-    const uint32_t order = x != x ? 0xFFFFFFFEu : (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
-    return static_cast<uint64_t>(order) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(index));
+    return static_cast<uint64_t>(order_of(x)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(index));
 }
 __device__ __forceinline__ int32_t index_of_key(uint64_t key) {
     return static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(key));
 }
 
-// log p = (v - m) - log sum e: from the difference, not from log_sum, whose rounding grows with m. A class that is masked (-infinity)
-// stays that, whatever the rest of the row.
-__device__ __forceinline__ float log_prob_of(float v, float m, float log_of_sum) {
-    return v == -INFINITY && m < INFINITY ? -INFINITY : (v - m) - log_of_sum;
+// What a row's values come to. Logits: m their maximum, s = sum e^t and w = sum e^t t with t = v - m. Probabilities: m = 0, s = sum x,
+// w = SCALE sum x log x (a product with a number below the normal ones would lose its digits). A value that makes the row no distribution leaves NaN in s or w.
+struct Sums {
+    float m, s, w;
+};
+constexpr float SCALE       = 16777216.0f;  // 2^24
+constexpr float NO_EXPONENT = -1000.0f;  // e^t is 0 there, and 0 times -infinity would not be
+__device__ __forceinline__ float bounded(float t) {
+    return fmaxf(t, NO_EXPONENT);
+}
+__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
+    const float m = fmaxf(a.m, b.m), da = bounded(a.m - m), db = bounded(b.m - m), fa = __expf(da), fb = __expf(db);
+    return Sums{m, fmaf(a.s, fa, b.s * fb), fmaf(fmaf(a.s, da, a.w), fa, fmaf(b.s, db, b.w) * fb)};
+}
+template <bool PROBABILITIES>
+__device__ __forceinline__ Sums joined_of(const Sums& a, const Sums& b) {
+    return PROBABILITIES ? Sums{0.0f, a.s + b.s, a.w + b.w} : joined(a, b);
 }
 
-__device__ __forceinline__ float warp_max(float v) {
-    for (int d = WARP / 2; d > 0; d /= 2) {
-        const float o = __shfl_xor_sync(~0u, v, d);
-        v = (o > v || o != o) ? o : v;
+// The results of a row from its sums; log p of one of its values.
+struct Row {
+    float m, l, log_sum, entropy;
+};
+template <bool PROBABILITIES>
+__device__ __forceinline__ Row row_of(const Sums& q) {
+    Row r{q.m, 0.0f, -INFINITY, 0.0f};
+    if (!(q.s < INFINITY) || q.w != q.w) r.m = r.l = r.log_sum = r.entropy = NAN;
+    else if (q.s > 0.0f) {
+        r.l       = logf(q.s);
+        r.log_sum = q.m + r.l;
+        r.entropy = r.l - q.w / (PROBABILITIES ? SCALE * q.s : q.s);
     }
-    return v;
+    return r;
 }
-__device__ __forceinline__ float warp_sum(float v) {
-    for (int d = WARP / 2; d > 0; d /= 2) v += __shfl_xor_sync(~0u, v, d);
-    return v;
+// log p = (v - m) - log s: from the difference, not from log_sum, whose rounding grows with m. A class that is masked (-infinity) stays
+// that in a row that has a distribution.
+template <bool PROBABILITIES>
+__device__ __forceinline__ float log_prob_of(float x, const Row& r) {
+    const float v = value_of<PROBABILITIES>(x);
+    return v == -INFINITY && r.l == r.l ? -INFINITY : (v - r.m) - r.l;
 }
-
-// A warp per row.
 template <typename T, bool PROBABILITIES>
-__global__ void __launch_bounds__(256) k_scores(const ScoresArgs a) {
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / WARP) + threadIdx.x / WARP;
-    if (row >= a.rows) return;
-    const int lane = threadIdx.x % WARP;
-    const T* x     = static_cast<const T*>(a.x) + row * a.row_stride;
+__device__ __forceinline__ void write_row(const ScoresArgs& a, int64_t row, const T* x, const Row& r) {
+    if (a.log_sum != nullptr) a.log_sum[row] = r.log_sum;
+    if (a.entropy != nullptr) a.entropy[row] = r.entropy;
+    if (a.log_prob != nullptr) {
+        const int64_t label = label_of(a.labels, a.labels_64, row);
+        float lp = 0.0f;
+        if (label != -1) lp = label < 0 || label >= a.classes ? NAN : log_prob_of<PROBABILITIES>(to_float(x[label]), r);
+        a.log_prob[row] = lp;
+    }
+}
+template <bool PROBABILITIES>
+__device__ __forceinline__ void write_top(const ScoresArgs& a, int64_t row, int k, uint32_t order, int32_t index, const Row& r) {
+    a.top_index[row * a.top + k]    = index;
+    a.top_log_prob[row * a.top + k] = log_prob_of<PROBABILITIES>(value_of_order(order), r);
+}
 
-    float m = -INFINITY;
-    for (int32_t j = lane; j < a.classes; j += WARP) {
-        const float v = value_of<PROBABILITIES>(to_float(x[j]));
-        m = (v > m || v != v) ? v : m;
-        if (m != m) break;
+// ---- up to 1024 classes: G lanes per row, E values a lane in registers ---------------------------------------------------------
+// Lane l of a row has the values l, l + G, l + 2 G, ..., or (WIDE, G = 32, rows that begin on 16 bytes) the same with pieces of 16 bytes.
+constexpr int ROW_BLOCK = 256;
+
+template <typename T, int G, int E>
+struct RowLoad {
+    static constexpr int PIECE = 16 / sizeof(T);
+    static constexpr bool MAY  = G == 32 && E % PIECE == 0;
+    __device__ static __forceinline__ int index(bool wide, int lane, int i) {
+        return MAY && wide ? (i / PIECE * G + lane) * PIECE + i % PIECE : i * G + lane;
     }
-    m = warp_max(m);
-    float sum = 0.0f, weighted = 0.0f;
-    if (m > -INFINITY && m < INFINITY) {
-        for (int32_t j = lane; j < a.classes; j += WARP) {
-            const float v = value_of<PROBABILITIES>(to_float(x[j]));
-            if (v == -INFINITY) continue;
-            const float t = fmaxf(v - m, -1000.0f), e = __expf(t);  // e is 0 there, and 0 * -infinity would not be
-            sum += e;
-            weighted = fmaf(e, t, weighted);
+    __device__ static __forceinline__ void load(const T* x, int classes, bool wide, int lane, float (&to)[E]) {
+        if constexpr (MAY) {
+            if (wide) {
+#pragma unroll
+                for (int i = 0; i < E; i += PIECE) {
+                    const int j = index(true, lane, i);
+                    T e[PIECE];
+                    if (j + PIECE <= classes) {
+                        const uint4 raw = *reinterpret_cast<const uint4*>(x + j);
+                        memcpy(e, &raw, 16);
+#pragma unroll
+                        for (int k = 0; k < PIECE; ++k) to[i + k] = to_float(e[k]);
+                    }
+                    else {
+#pragma unroll
+                        for (int k = 0; k < PIECE; ++k) to[i + k] = j + k < classes ? to_float(x[j + k]) : 0.0f;
+                    }
+                }
+                return;
+            }
         }
-        sum      = warp_sum(sum);
-        weighted = warp_sum(weighted);
+#pragma unroll
+        for (int i = 0; i < E; ++i) to[i] = i * G + lane < classes ? to_float(x[i * G + lane]) : 0.0f;
     }
-    float l = 0.0f, log_sum = -INFINITY, entropy = 0.0f;
-    if (!(m < INFINITY)) l = log_sum = entropy = NAN;
-    else if (m > -INFINITY) {
-        l       = logf(sum);
-        log_sum = m + l;
-        entropy = l - weighted / sum;
-    }
-    if (lane == 0) {
-        if (a.log_sum != nullptr) a.log_sum[row] = log_sum;
-        if (a.entropy != nullptr) a.entropy[row] = entropy;
-        if (a.log_prob != nullptr) {
-            const int64_t label = label_of(a.labels, a.labels_64, row);
-            float lp = 0.0f;
-            if (label != -1) lp = label < 0 || label >= a.classes ? NAN : log_prob_of(value_of<PROBABILITIES>(to_float(x[label])), m, l);
-            a.log_prob[row] = lp;
+};
+
+template <int G, typename F>
+__device__ __forceinline__ void over_lanes(F f) {
+#pragma unroll
+    for (int d = G / 2; d > 0; d /= 2) f(d);
+}
+
+template <typename T, bool PROBABILITIES, int G, int E>
+__global__ void __launch_bounds__(ROW_BLOCK) k_scores_rows(const ScoresArgs a, bool wide) {
+    const int64_t row = (static_cast<int64_t>(blockIdx.x) * ROW_BLOCK + threadIdx.x) / G;
+    const int lane    = threadIdx.x % G;
+    const bool there  = row < a.rows;
+    const int classes = there ? a.classes : 0;
+    const T* x        = static_cast<const T*>(a.x) + (there ? row : 0) * a.row_stride;
+    using Load        = RowLoad<T, G, E>;
+    float v[E];
+    Load::load(x, classes, wide, lane, v);
+
+    Sums q{0.0f, 0.0f, 0.0f};
+    if constexpr (PROBABILITIES) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            if (Load::index(wide, lane, i) < classes) {
+                q.s += v[i];
+                q.w += v[i] == 0.0f ? 0.0f : SCALE * v[i] * logf(v[i]);
+            }
         }
     }
-    uint64_t below = ~0ull;
-    for (int k = 0; k < a.top; ++k) {
-        uint64_t best = 0;
-        for (int32_t j = lane; j < a.classes; j += WARP) {
-            const uint64_t key = key_of(to_float(x[j]), j);
-            if (key < below && key > best) best = key;
+    else {
+        q.m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (Load::index(wide, lane, i) < classes) q.m = fmaxf(q.m, v[i]);
+        over_lanes<G>([&](int d) { q.m = fmaxf(q.m, __shfl_xor_sync(~0u, q.m, d)); });
+        if (q.m == -INFINITY) q.m = 0.0f;  // then nothing is left, or only NaN
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            if (Load::index(wide, lane, i) < classes) {
+                const float t = v[i] - q.m, e = __expf(t);
+                q.s += e;
+                q.w = fmaf(e, bounded(t), q.w);
+            }
         }
-        for (int d = WARP / 2; d > 0; d /= 2) {
-            const uint64_t o = __shfl_xor_sync(~0u, best, d);
-            best = o > best ? o : best;
-        }
-        below = best;
-        if (lane == 0) {
-            const int32_t j = index_of_key(best);
-            a.top_index[row * a.top + k]    = j;
-            a.top_log_prob[row * a.top + k] = log_prob_of(value_of<PROBABILITIES>(to_float(x[j])), m, l);
+    }
+    over_lanes<G>([&](int d) {
+        q.s += __shfl_xor_sync(~0u, q.s, d);
+        q.w += __shfl_xor_sync(~0u, q.w, d);
+    });
+    const Row r = row_of<PROBABILITIES>(q);
+    if (there && lane == 0) write_row<T, PROBABILITIES>(a, row, x, r);
+
+    if (a.top > 0) {
+        uint32_t order[E];  // 0: not there, or taken
+#pragma unroll
+        for (int i = 0; i < E; ++i) order[i] = Load::index(wide, lane, i) < classes ? order_of(v[i]) : 0;
+        for (int k = 0; k < a.top; ++k) {
+            uint32_t best = 0;
+            int at        = 0;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {  // a lane's indices rise with i: the first of equals stays
+                if (order[i] > best) best = order[i], at = Load::index(wide, lane, i);
+            }
+            const uint32_t mine = best;
+            const int mine_at   = at;
+            if constexpr (G == 32) {
+                best = __reduce_max_sync(~0u, mine);
+                at   = __reduce_min_sync(~0u, mine == best ? mine_at : INT32_MAX);
+            }
+            else {
+                over_lanes<G>([&](int d) {
+                    const uint32_t o = __shfl_xor_sync(~0u, best, d);
+                    const int o_at   = __shfl_xor_sync(~0u, at, d);
+                    if (o > best || (o == best && o_at < at)) best = o, at = o_at;
+                });
+            }
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if (Load::index(wide, lane, i) == at) order[i] = 0;
+            if (there && lane == 0) write_top<PROBABILITIES>(a, row, k, best, at, r);
         }
     }
 }
 
-// The gradient is one pass over the elements once the row's sums are known.
-template <typename T, bool PROBABILITIES>
-__global__ void __launch_bounds__(256) k_scores_grad(const ScoresGradArgs a) {
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / WARP) + threadIdx.x / WARP;
-    if (row >= a.rows) return;
-    const int lane = threadIdx.x % WARP;
-    const T* x     = static_cast<const T*>(a.x) + row * a.row_stride;
-    T* dx          = static_cast<T*>(a.dx) + row * a.dx_row_stride;
+// ---- more classes: blocks per row ----------------------------------------------------------------------------------------------
+// One pass over the row in pieces of 16 bytes (the row's first and last may be shorter): a thread keeps its running maximum with the sums
+// below it, and which of its pieces held the maximum. The `top` largest then need no second pass: with the threads' maxima in order (by
+// value, then by place), every one of the row's `top` largest values lies in a thread whose maximum is among the first `top`, and is at
+// least the last of those. So `top` threads' pieces are read again (by a warp each, from the cache), what is that large is
+// collected and the largest of it taken. Where that is more than there is room for (many of the largest in one thread's pieces) or the row holds
+// NaN, the row is searched `top` times instead.
+// Few rows: a cluster of blocks shares a row, and the first of them joins their results through its shared memory.
+constexpr int STREAM_BLOCK = 256;
+constexpr int STREAM_AHEAD = 4;    // pieces that a thread has under way
+constexpr int CANDIDATES   = 256;  // top * (values of a piece) at least: that many can tie
+constexpr int MOST_BLOCKS  = 8;    // of a cluster
+static_assert(VM_MAX_TOP * 8 <= CANDIDATES && VM_MAX_TOP * MOST_BLOCKS <= CANDIDATES, "room for ties within pieces, and for every block's best");
 
-    const float log_sum = a.log_sum[row];
-    float d_label = 0.0f;
-    int64_t label = -1;
-    if (a.d_log_prob != nullptr) {
-        label = label_of(a.labels, a.labels_64, row);
-        if (label != -1) d_label = label < 0 || label >= a.classes ? NAN : a.d_log_prob[row];
+template <typename T>
+struct Pieces {
+    static constexpr int N = 16 / sizeof(T);
+    const T* x;     // the row
+    int classes;
+    int before;     // values of piece 0 that lie in front of the row
+    int64_t count;  // pieces that hold values of the row
+    __device__ __forceinline__ Pieces(const T* row, int n) : x(row), classes(n) {
+        before = static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T));
+        count  = (static_cast<int64_t>(before) + n + N - 1) / N;
     }
-    const float d_entropy = a.d_entropy != nullptr ? a.d_entropy[row] : 0.0f;
-    const float entropy   = a.d_entropy != nullptr ? a.entropy[row] : 0.0f;
-    const float constant  = log_sum != log_sum ? NAN : (a.d_log_sum != nullptr ? a.d_log_sum[row] : 0.0f) - d_label;
-    const float one_over  = PROBABILITIES ? 1.0f / __expf(log_sum) : 0.0f;
-    for (int32_t j = lane; j < a.classes; j += WARP) {
-        const float p = to_float(x[j]);
-        const float v = value_of<PROBABILITIES>(p);
-        float d = 0.0f;
-        if (v != -INFINITY) {
-            const float lp = fmaxf(v - log_sum, -1000.0f);  // p is 0 there, and 0 * -infinity would not be
-            d = (constant - d_entropy * (lp + entropy)) * (PROBABILITIES ? one_over : __expf(lp));
-            if (j == label) d += PROBABILITIES ? d_label / p : d_label;
+    // index of the first value of a piece in the row; those outside 0..classes-1 are not the row's
+    __device__ __forceinline__ int64_t first(int64_t piece) const {
+        return piece * N - before;
+    }
+    __device__ __forceinline__ uint4 load(int64_t piece, T outside) const {
+        const int64_t j = first(piece);
+        if (j >= 0 && j + N <= classes) return *reinterpret_cast<const uint4*>(x + j);
+        T e[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) e[k] = j + k >= 0 && j + k < classes ? x[j + k] : outside;
+        uint4 raw;
+        memcpy(&raw, e, 16);
+        return raw;
+    }
+};
+template <typename T>
+__device__ __forceinline__ void values_of(const uint4& raw, float (&to)[16 / sizeof(T)]) {
+    T e[16 / sizeof(T)];
+    memcpy(e, &raw, 16);
+#pragma unroll
+    for (int k = 0; k < 16 / static_cast<int>(sizeof(T)); ++k) to[k] = to_float(e[k]);
+}
+
+// The `top` largest of `n` different keys (0: none) in shared memory, in order, by one warp.
+__device__ __forceinline__ void largest_keys(const uint64_t* keys, int n, int top, uint64_t* into) {
+    const int lane = threadIdx.x % WARP;
+    uint64_t held[CANDIDATES / WARP];
+#pragma unroll
+    for (int i = 0; i < CANDIDATES / WARP; ++i) held[i] = i * WARP + lane < n ? keys[i * WARP + lane] : 0;
+    for (int k = 0; k < top; ++k) {
+        uint64_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < CANDIDATES / WARP; ++i) mine = held[i] > mine ? held[i] : mine;
+        const uint32_t high = __reduce_max_sync(~0u, static_cast<uint32_t>(mine >> 32));
+        const uint32_t low  = __reduce_max_sync(~0u, static_cast<uint32_t>(mine >> 32) == high ? static_cast<uint32_t>(mine) : 0);
+        const uint64_t best = static_cast<uint64_t>(high) << 32 | low;
+#pragma unroll
+        for (int i = 0; i < CANDIDATES / WARP; ++i)
+            if (held[i] == best) held[i] = 0;
+        if (lane == 0) into[k] = best;
+    }
+}
+
+struct StreamShared {
+    Sums warps[STREAM_BLOCK / WARP];
+    uint64_t keys[CANDIDATES];      // the threads' maxima, then what may be among the largest
+    uint64_t best[VM_MAX_TOP];      // of this block
+    uint64_t searched[STREAM_BLOCK / WARP];
+    int found;
+    // of the cluster, in its first block
+    Sums sums[MOST_BLOCKS];
+    uint64_t bests[MOST_BLOCKS * VM_MAX_TOP];
+};
+static_assert(STREAM_BLOCK <= CANDIDATES, "the threads' maxima are chosen from as candidates are");
+
+template <typename T, bool PROBABILITIES, bool CLUSTER>
+__global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs a, int blocks) {
+    namespace cg = cooperative_groups;
+    __shared__ StreamShared shared;
+    const int rank    = CLUSTER ? blockIdx.x % blocks : 0;
+    const int64_t row = CLUSTER ? blockIdx.x / blocks : blockIdx.x;
+    const int lane = threadIdx.x % WARP, warp = threadIdx.x / WARP;
+    const T* x = static_cast<const T*>(a.x) + row * a.row_stride;
+    const Pieces<T> pieces(x, a.classes);
+    constexpr int N     = Pieces<T>::N;
+    const int64_t share = CLUSTER ? (pieces.count + blocks - 1) / blocks : pieces.count;
+    const int64_t begin = rank * share, end = begin + share < pieces.count ? begin + share : pieces.count;
+    const T outside     = from_float<T>(PROBABILITIES ? 0.0f : -INFINITY);
+
+    Sums q{PROBABILITIES ? 0.0f : -3.402823466e38f, 0.0f, 0.0f};  // a finite maximum, below or at every value that counts
+    float best   = PROBABILITIES ? -1.0f : -INFINITY;
+    int64_t held = begin + threadIdx.x;  // the piece with the maximum
+    for (int64_t p = begin + threadIdx.x; p < end; p += STREAM_BLOCK * STREAM_AHEAD) {
+        uint4 raw[STREAM_AHEAD];
+#pragma unroll
+        for (int u = 0; u < STREAM_AHEAD; ++u)
+            if (p + u * STREAM_BLOCK < end) raw[u] = pieces.load(p + u * STREAM_BLOCK, outside);
+#pragma unroll
+        for (int u = 0; u < STREAM_AHEAD; ++u) {
+            if (p + u * STREAM_BLOCK >= end) break;
+            float v[N];
+            values_of<T>(raw[u], v);
+            float top = v[0];
+#pragma unroll
+            for (int k = 1; k < N; ++k) top = fmaxf(top, v[k]);
+            if (top > best) best = top, held = p + u * STREAM_BLOCK;
+            if constexpr (PROBABILITIES) {
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    q.s += v[k];
+                    q.w += v[k] == 0.0f ? 0.0f : SCALE * v[k] * logf(v[k]);
+                }
+            }
+            else {
+                const float m = fmaxf(q.m, top), d = bounded(q.m - m), f = __expf(d);
+                q.w = fmaf(q.s, d, q.w) * f;
+                q.s *= f;
+                q.m = m;
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const float t = v[k] - m, e = __expf(t);
+                    q.s += e;
+                    q.w = fmaf(e, bounded(t), q.w);
+                }
+            }
         }
-        dx[j] = from_float<T>(d);
+    }
+    over_lanes<WARP>([&](int d) {
+        const Sums o{__shfl_xor_sync(~0u, q.m, d), __shfl_xor_sync(~0u, q.s, d), __shfl_xor_sync(~0u, q.w, d)};
+        q = joined_of<PROBABILITIES>(q, o);
+    });
+    if (lane == 0) shared.warps[warp] = q;
+    if (threadIdx.x == 0) shared.found = 0;
+    if (a.top > 0) shared.keys[threadIdx.x] = begin + threadIdx.x < end ? static_cast<uint64_t>(order_of(best)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(held)) : 0;
+    __syncthreads();
+    q = shared.warps[0];
+#pragma unroll
+    for (int w = 1; w < STREAM_BLOCK / WARP; ++w) q = joined_of<PROBABILITIES>(q, shared.warps[w]);
+
+    if (a.top > 0) {
+        if (warp == 0) largest_keys(shared.keys, STREAM_BLOCK, a.top, shared.best);
+        __syncthreads();
+        const uint64_t least = shared.best[a.top - 1];
+        bool search          = q.s != q.s || q.w != q.w;
+        if (!search) {
+            const uint32_t least_order  = static_cast<uint32_t>(least >> 32);
+            const int64_t least_piece   = 0xFFFFFFFFu - static_cast<uint32_t>(least);
+            for (int i = warp; i < a.top; i += STREAM_BLOCK / WARP) {
+                const int64_t piece = 0xFFFFFFFFu - static_cast<uint32_t>(shared.best[i]);
+                const int64_t first = begin + (piece - begin) % STREAM_BLOCK;
+                for (int64_t p = first + lane * STREAM_BLOCK; p < end; p += WARP * STREAM_BLOCK) {
+                    float v[N];
+                    values_of<T>(pieces.load(p, outside), v);
+#pragma unroll
+                    for (int k = 0; k < N; ++k) {
+                        const int64_t j      = pieces.first(p) + k;
+                        const uint32_t order = order_of(v[k]);
+                        if (j < 0 || j >= a.classes || order < least_order || (order == least_order && p > least_piece)) continue;
+                        const int at = atomicAdd(&shared.found, 1);
+                        if (at < CANDIDATES) shared.keys[at] = key_of(v[k], static_cast<int32_t>(j));
+                    }
+                }
+            }
+            __syncthreads();
+            search = shared.found > CANDIDATES;
+            if (!search && warp == 0) largest_keys(shared.keys, shared.found, a.top, shared.best);
+        }
+        if (search) {
+            uint64_t below = ~0ull;
+            for (int k = 0; k < a.top; ++k) {
+                uint64_t most = 0;
+                for (int64_t p = begin + threadIdx.x; p < end; p += STREAM_BLOCK) {
+                    float v[N];
+                    values_of<T>(pieces.load(p, outside), v);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const int64_t j    = pieces.first(p) + i;
+                        const uint64_t key = j >= 0 && j < a.classes ? key_of(v[i], static_cast<int32_t>(j)) : 0;
+                        if (key < below && key > most) most = key;
+                    }
+                }
+                over_lanes<WARP>([&](int d) {
+                    const uint64_t o = __shfl_xor_sync(~0u, most, d);
+                    most = o > most ? o : most;
+                });
+                __syncthreads();
+                if (lane == 0) shared.searched[warp] = most;
+                __syncthreads();
+                below = shared.searched[0];
+                for (int w = 1; w < STREAM_BLOCK / WARP; ++w) below = shared.searched[w] > below ? shared.searched[w] : below;
+                if (threadIdx.x == 0) shared.best[k] = below;
+            }
+        }
+        __syncthreads();
+    }
+
+    if constexpr (CLUSTER) {
+        const cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();  // the first block runs
+        StreamShared* first = cluster.map_shared_rank(&shared, 0);
+        if (threadIdx.x == 0) first->sums[rank] = q;
+        if (threadIdx.x < a.top) first->bests[rank * a.top + threadIdx.x] = shared.best[threadIdx.x];
+        cluster.sync();
+        if (rank != 0) return;
+        q = shared.sums[0];
+        for (int b = 1; b < blocks; ++b) q = joined_of<PROBABILITIES>(q, shared.sums[b]);
+        if (a.top > 0 && warp == 0) largest_keys(shared.bests, blocks * a.top, a.top, shared.best);
+    }
+    if (warp != 0) return;
+    __syncwarp();
+    const Row r = row_of<PROBABILITIES>(q);
+    if (lane == 0) write_row<T, PROBABILITIES>(a, row, x, r);
+    if (lane < a.top) write_top<PROBABILITIES>(a, row, lane, static_cast<uint32_t>(shared.best[lane] >> 32), index_of_key(shared.best[lane]), r);
+}
+
+// ---- gradients -----------------------------------------------------------------------------------------------------------------
+// One pass over the elements once the row's sums are known.
+template <bool PROBABILITIES>
+struct RowGrad {
+    float log_sum, d_label, d_entropy, offset, one_over;
+    int64_t label;
+    __device__ __forceinline__ RowGrad(const ScoresGradArgs& a, int64_t row) : log_sum(a.log_sum[row]), d_label(0.0f), label(-1) {
+        if (a.d_log_prob != nullptr) {
+            label = label_of(a.labels, a.labels_64, row);
+            if (label != -1) d_label = label < 0 || label >= a.classes ? NAN : a.d_log_prob[row];
+        }
+        d_entropy = a.d_entropy != nullptr ? a.d_entropy[row] : 0.0f;
+        offset    = (a.d_log_sum != nullptr ? a.d_log_sum[row] : 0.0f) - d_label - (a.d_entropy != nullptr ? d_entropy * a.entropy[row] : 0.0f);
+        if (log_sum != log_sum) offset = NAN;
+        one_over = PROBABILITIES ? __expf(-log_sum) : 0.0f;
+    }
+    __device__ __forceinline__ float of(float x, int64_t j) const {
+        const float v = value_of<PROBABILITIES>(x);
+        if (v == -INFINITY) return 0.0f;
+        const float lp = bounded(v - log_sum);
+        const float d  = fmaf(-d_entropy, lp, offset) * (PROBABILITIES ? one_over : __expf(lp));
+        return j == label ? d + (PROBABILITIES ? d_label / x : d_label) : d;
+    }
+};
+
+// Rows of up to 1024 classes as above. Where a thread has a whole row, its results go through shared memory, so that a block writes
+// its rows, which lie side by side, in one piece.
+template <typename T, bool PROBABILITIES, int G, int E>
+__global__ void __launch_bounds__(ROW_BLOCK) k_scores_grad_rows(const ScoresGradArgs a, bool wide, bool dense) {
+    __shared__ alignas(16) unsigned char staged[G == 1 ? ROW_BLOCK * E * sizeof(T) : 16];
+    const int64_t row = (static_cast<int64_t>(blockIdx.x) * ROW_BLOCK + threadIdx.x) / G;
+    const int lane    = threadIdx.x % G;
+    if (G > 1 && row >= a.rows) return;
+    if (row < a.rows) {
+        const T* x = static_cast<const T*>(a.x) + row * a.row_stride;
+        T* dx      = static_cast<T*>(a.dx) + row * a.dx_row_stride;
+        using Load = RowLoad<T, G, E>;
+        float v[E];
+        Load::load(x, a.classes, wide, lane, v);
+        const RowGrad<PROBABILITIES> grad(a, row);
+        if constexpr (Load::MAY) {
+            if (wide) {
+#pragma unroll
+                for (int i = 0; i < E; i += Load::PIECE) {
+                    const int j = Load::index(true, lane, i);
+                    T e[Load::PIECE];
+#pragma unroll
+                    for (int k = 0; k < Load::PIECE; ++k) e[k] = from_float<T>(grad.of(v[i + k], j + k));
+                    if (j + Load::PIECE <= a.classes) {
+                        uint4 raw;
+                        memcpy(&raw, e, 16);
+                        *reinterpret_cast<uint4*>(dx + j) = raw;
+                    }
+                    else {
+#pragma unroll
+                        for (int k = 0; k < Load::PIECE; ++k)
+                            if (j + k < a.classes) dx[j + k] = e[k];
+                    }
+                }
+                return;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int j = i * G + lane;
+            if (j < a.classes) {
+                const T d = from_float<T>(grad.of(v[i], j));
+                if (G == 1 && dense) reinterpret_cast<T*>(staged)[threadIdx.x * a.classes + j] = d;
+                else dx[j] = d;
+            }
+        }
+    }
+    if (G == 1 && dense) {
+        __syncthreads();
+        const int64_t first = static_cast<int64_t>(blockIdx.x) * ROW_BLOCK;
+        const int values    = static_cast<int>(a.rows - first < ROW_BLOCK ? a.rows - first : ROW_BLOCK) * a.classes;
+        T* to               = static_cast<T*>(a.dx) + first * a.classes;
+        constexpr int PIECE = 16 / sizeof(T);
+        for (int i = threadIdx.x; i < values / PIECE; i += ROW_BLOCK) reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(staged)[i];
+        for (int i = values / PIECE * PIECE + threadIdx.x; i < values; i += ROW_BLOCK) to[i] = reinterpret_cast<const T*>(staged)[i];
+    }
+}
+
+// Longer rows: a block for STREAM_BLOCK * STREAM_AHEAD pieces of a row. The last rows come first: they are what the cache still holds of
+// the pass that made the sums.
+template <typename T, bool PROBABILITIES>
+__global__ void __launch_bounds__(STREAM_BLOCK) k_scores_grad_stream(const ScoresGradArgs a, int blocks) {
+    const int64_t row = a.rows - 1 - blockIdx.x / blocks;
+    const T* x        = static_cast<const T*>(a.x) + row * a.row_stride;
+    T* dx             = static_cast<T*>(a.dx) + row * a.dx_row_stride;
+    const Pieces<T> pieces(x, a.classes);
+    constexpr int N      = Pieces<T>::N;
+    const bool together  = reinterpret_cast<uintptr_t>(dx) % 16 == reinterpret_cast<uintptr_t>(x) % 16;
+    const int64_t begin  = static_cast<int64_t>(blockIdx.x % blocks) * (STREAM_BLOCK * STREAM_AHEAD) + threadIdx.x;
+    const T outside      = from_float<T>(0.0f);
+    uint4 raw[STREAM_AHEAD];
+#pragma unroll
+    for (int u = 0; u < STREAM_AHEAD; ++u)
+        if (begin + u * STREAM_BLOCK < pieces.count) raw[u] = pieces.load(begin + u * STREAM_BLOCK, outside);
+    const RowGrad<PROBABILITIES> grad(a, row);
+#pragma unroll
+    for (int u = 0; u < STREAM_AHEAD; ++u) {
+        const int64_t p = begin + u * STREAM_BLOCK;
+        if (p >= pieces.count) break;
+        const int64_t j = pieces.first(p);
+        float v[N];
+        T e[N];
+        values_of<T>(raw[u], v);
+#pragma unroll
+        for (int k = 0; k < N; ++k) e[k] = from_float<T>(grad.of(v[k], j + k));
+        if (together && j >= 0 && j + N <= a.classes) {
+            uint4 out;
+            memcpy(&out, e, 16);
+            *reinterpret_cast<uint4*>(dx + j) = out;
+        }
+        else {
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (j + k >= 0 && j + k < a.classes) dx[j + k] = e[k];
+        }
     }
 }
 
