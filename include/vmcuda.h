@@ -399,7 +399,7 @@ VM_API size_t vm_gated_workspace(int64_t batch, int64_t steps, int64_t channels)
  * apart), updated in place: h = f h + (1 - f) x for the slot index[row] (NULL: slot = row, rows <= slots), y[row] = h.
  * x, gate and y have rows x channels elements of `type`, row and channel strides in batch_stride (step_stride is not used) and
  * channel_stride. A row whose index is outside 0..slots-1, or whose slot an earlier row of the call names too, changes no state and its
- * y is 0. y may be NULL. workspace: at least vm_gated_step_workspace(rows, slots) bytes when index is given, aligned to 16. */
+ * y is 0. y may be NULL. workspace: as above, at least vm_gated_step_workspace(rows, slots) bytes when index is given. */
 VM_API vm_status vm_gated_step(int device,
                                int32_t type,
                                int64_t rows,

@@ -74,7 +74,7 @@ def test_scan_backward_refuses(bad):
 
 @pytest.mark.parametrize("bad", [
     dict(type=3), dict(rows=-1), dict(slots=-1), dict(slots=2**31), dict(channels=-1), dict(state=None), dict(stride=6), dict(stride=2**61), dict(x=None), dict(gate=None),
-    dict(x=(P + 2, 7, 0, 1)), dict(y=(P, 6, 0, 1)), dict(y=(P, 0, 0, 1)), dict(index=None, rows=10), dict(workspace=None), dict(size=8),
+    dict(x=(P + 2, 7, 0, 1)), dict(y=(P, 6, 0, 1)), dict(y=(P, 0, 0, 1)), dict(index=None, rows=10), dict(rows=4000, workspace=None), dict(rows=4000, workspace=P + 4), dict(rows=4000, size=8),
 ])
 def test_step_refuses(bad):
     assert step(**bad) == REFUSED

@@ -1,5 +1,5 @@
-"""Builds libvmcuda.so (the CUDA engine and its C ABI) in-tree for sm_100a with nvcc, and the extension module _native (marshalling
-for engine.py) against it with g++.
+"""Builds libvmcuda.so (the CUDA engine and its C ABI) in-tree for sm_100a with nvcc, and against it with g++ the extension modules
+_native (marshalling for engine.py) and _answers (tensors for answers.py).
 
     python -m visualmesh_b200.build            # rebuild what is older than its sources
     python -m visualmesh_b200.build --force [-v]
@@ -19,7 +19,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "_build")
 LIB = os.path.join(HERE, "libvmcuda.so")
-NATIVE = os.path.join(HERE, "_native" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+SUFFIX = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
+NATIVE = os.path.join(HERE, "_native" + SUFFIX)
+ANSWERS = os.path.join(HERE, "_answers" + SUFFIX)
 ABI_HEADER = os.path.join("..", "..", "include", "vmcuda.h")
 FFMA_HEADERS = ["conv_ffma_launch.cuh", "conv_ffma.cuh", "conv_common.cuh", "conv_dispatch.hpp", "conv_args.hpp", ABI_HEADER]
 # translation unit -> headers it includes (directly or not)
@@ -36,7 +38,8 @@ UNITS = {
     "gated.cu": ["gated.cuh", "element.cuh", "device_call.hpp", "conv_dispatch.hpp", "conv_args.hpp", ABI_HEADER],
     "hostmesh.cpp": ["host_math.hpp", ABI_HEADER],
 }
-NATIVE_SOURCES = ["native.cpp", ABI_HEADER]
+# extension module -> its sources
+MODULES = {NATIVE: ["native.cpp", ABI_HEADER], ANSWERS: ["answers.cpp", ABI_HEADER]}
 
 
 def _nvcc():
@@ -61,7 +64,7 @@ def _stale(unit):
 
 def needs_build():
     """The library is missing or older than one of its sources (object files may be absent: they do not travel)."""
-    return _library_stale() or _native_stale()
+    return _library_stale() or any(_module_stale(m) for m in MODULES)
 
 
 def _library_stale():
@@ -72,21 +75,28 @@ def _library_stale():
     return any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in files if os.path.exists(os.path.join(CSRC, f)))
 
 
-def _native_stale():
-    if not os.path.exists(NATIVE):
+def _module_stale(module):
+    if not os.path.exists(module):
         return True
-    t = os.path.getmtime(NATIVE)
-    return any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in NATIVE_SOURCES if os.path.exists(os.path.join(CSRC, f)))
+    t = os.path.getmtime(module)
+    return any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in MODULES[module] if os.path.exists(os.path.join(CSRC, f)))
+
+
+def _build_module(module, more):
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-I", sysconfig.get_paths()["include"],
+                    os.path.join(CSRC, MODULES[module][0]), "-o", module, LIB, "-Wl,-rpath,$ORIGIN"] + more, check=True, cwd=CSRC)
 
 
 def build(force=False, verbose=False):
     if force or _library_stale():
         _build_library(force, verbose)
-    if force or _native_stale():
+    if force or _module_stale(NATIVE):
         import numpy
-        subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-I", sysconfig.get_paths()["include"],
-                        "-I", numpy.get_include(), os.path.join(CSRC, "native.cpp"), "-o", NATIVE, LIB, "-Wl,-rpath,$ORIGIN"],
-                       check=True, cwd=CSRC)
+        _build_module(NATIVE, ["-I", numpy.get_include()])
+    if force or _module_stale(ANSWERS):
+        from torch.utils import cpp_extension  # torch's own libraries are loaded before the module is
+        _build_module(ANSWERS, [f"-isystem{p}" for p in cpp_extension.include_paths("cuda")] + [f"-L{cpp_extension.library_paths()[0]}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+                                                                                                "-ltorch", "-ltorch_python"])
     return LIB
 
 

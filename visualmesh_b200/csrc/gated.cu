@@ -59,8 +59,11 @@ Sequence sequence(const vm_sequence* s) {
     return Sequence{s->data, s->batch_stride, s->step_stride, s->channel_stride};
 }
 
+// Rows of a step among which every block looks for those that name a slot before it does.
+constexpr int64_t MOST_LOOKED_THROUGH = 1024;
+
 unsigned blocks_of(int64_t threads) {
-    const int64_t n = (threads + 255) / 256;
+    const int64_t n = (threads + STEP_BLOCK - 1) / STEP_BLOCK;
     if (n > INT32_MAX) throw std::string("too many elements for one call");
     return static_cast<unsigned>(n);
 }
@@ -239,7 +242,7 @@ vm_status vm_gated_scan_backward(int device, int32_t type, int64_t batch, int64_
 }
 
 size_t vm_gated_step_workspace(int64_t rows, int64_t slots) {
-    return rows > 0 && slots > 0 ? static_cast<size_t>(slots) * sizeof(uint32_t) : 0;
+    return rows > MOST_LOOKED_THROUGH && slots > 0 ? static_cast<size_t>(slots) * sizeof(uint32_t) : 0;
 }
 
 vm_status vm_gated_step(int device, int32_t type, int64_t rows, int64_t slots, int64_t channels, float* state, int64_t state_stride, const vm_sequence* x,
@@ -255,16 +258,28 @@ vm_status vm_gated_step(int device, int32_t type, int64_t rows, int64_t slots, i
         check_sequence(y, "y", type, sizes, false, true);
         if (slots > 0 && state == nullptr) throw std::string("null state");
         if (state_stride < (slots > 1 ? channels : 0) || state_stride > MOST / (slots > 0 ? slots : 1)) throw std::string("the states of slots overlap");
-        if (index != nullptr && (workspace_bytes < vm_gated_step_workspace(rows, slots) || (slots > 0 && workspace == nullptr))) throw std::string("the workspace is too small");
+        const size_t needed = index != nullptr ? vm_gated_step_workspace(rows, slots) : 0;
+        if (workspace_bytes < needed || (needed > 0 && (workspace == nullptr || !aligned(workspace, 16)))) throw std::string("the workspace is too small, null or not aligned");
         const OnDevice on(device);
         const auto q = static_cast<cudaStream_t>(stream);
-        StepArgs a{rows, slots, channels, state, state_stride, sequence(x), sequence(gate), sequence(y), index, static_cast<uint32_t*>(workspace)};
-        if (index != nullptr && slots > 0) {
-            VM_CUDA(cudaMemsetAsync(workspace, 0xFF, static_cast<size_t>(slots) * sizeof(uint32_t), q));
-            launch_kernel(k_first_rows, dim3(blocks_of(rows)), 256, 0, q, false, a);
+        const StepArgs a{rows, slots, channels, state, state_stride, sequence(x), sequence(gate), sequence(y), index, static_cast<uint32_t*>(workspace)};
+        if (needed > 0) {
+            VM_CUDA(cudaMemsetAsync(workspace, 0xFF, needed, q));
+            launch_kernel(k_first_rows, dim3(blocks_of(rows)), STEP_BLOCK, 0, q, false, a);
         }
-        const unsigned grid = blocks_of(rows * channels);
-        with_type(type, [&](auto kind) { launch_kernel(k_gated_step<decltype(kind)>, dim3(grid), 256, 0, q, false, a); });
+        const bool vectors = channels % 4 == 0 && takes(x, type, 4, sizes) && takes(gate, type, 4, sizes) && takes(y, type, 4, sizes) && aligned(state, 16) && state_stride % 4 == 0;
+        with_type(type, [&](auto kind) {
+            using T = decltype(kind);
+            const auto launch = [&](auto v) {
+                constexpr int V     = decltype(v)::value;
+                const unsigned grid = blocks_of(rows * (channels / V));
+                if (index == nullptr) launch_kernel(k_gated_step<T, V, ROW_IS_SLOT>, dim3(grid), STEP_BLOCK, 0, q, false, a);
+                else if (needed == 0) launch_kernel(k_gated_step<T, V, LOOK_THROUGH>, dim3(grid), STEP_BLOCK, 0, q, false, a);
+                else launch_kernel(k_gated_step<T, V, TABLE>, dim3(grid), STEP_BLOCK, 0, q, false, a);
+            };
+            if (vectors) launch(std::integral_constant<int, 4>{});
+            else launch(std::integral_constant<int, 1>{});
+        });
     }
     catch (const std::string& refused) {
         return fail(VM_ERR_INVALID_ARGUMENT, refused);
