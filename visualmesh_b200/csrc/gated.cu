@@ -62,6 +62,7 @@ Sequence sequence(const vm_sequence* s) {
 // Rows of a step among which every block looks for those that name a slot before it does.
 constexpr int64_t MOST_LOOKED_THROUGH = 1024;
 
+static_assert(STEP_BLOCK == SERIAL_BLOCK, "blocks_of counts blocks of either");
 unsigned blocks_of(int64_t threads) {
     const int64_t n = (threads + STEP_BLOCK - 1) / STEP_BLOCK;
     if (n > INT32_MAX) throw std::string("too many elements for one call");
@@ -89,14 +90,20 @@ Plan plan_of(int64_t all, int64_t steps, int vector, int length) {
     const int64_t tile = THREADS / p.tx * length, tiles = (steps + tile - 1) / tile;
     const int64_t blocks = (all + p.tx * vector - 1) / (p.tx * vector);
     if (blocks < SMS && tiles > 1) {
-        const int64_t wanted = std::min(tiles, (4 * SMS + blocks - 1) / blocks);
+        const int64_t wanted = std::min(tiles, (2 * SMS + blocks - 1) / blocks);
         p.run                = (tiles + wanted - 1) / wanted * tile;
         p.parts              = (steps + p.run - 1) / p.run;
     }
     return p;
 }
-// of the forward and of the backward pass: steps of a thread where it takes vectors and where it takes single elements
-constexpr int FORWARD = 8, BACKWARD = 4, SINGLE = 16;
+// Steps of a thread in the forward and in the backward pass, where it takes vectors and where it takes single elements: what its registers
+// hold, and 24 to 32 KB for a tile of the ring.
+constexpr int forward_steps(bool wide_type) {
+    return wide_type ? 4 : 8;
+}
+constexpr int BACKWARD = 4, SINGLE = 8;
+// Sequences of single elements from which on each has a thread: two blocks an SM.
+constexpr int64_t SERIAL_FROM = 2 * SMS * SERIAL_BLOCK;
 
 // Whether `vector` neighbouring channels of s lie side by side at a place that one load or store can take.
 bool takes(const vm_sequence* s, int32_t type, int vector, const int64_t (&sizes)[3]) {
@@ -154,7 +161,7 @@ size_t vm_gated_workspace(int64_t batch, int64_t steps, int64_t channels) {
     if (!sizes_fit(batch, steps, channels) || batch == 0 || channels == 0) return 0;
     const int64_t all = batch * channels;
     int64_t parts     = 1;
-    for (const int length : {FORWARD, BACKWARD}) parts = std::max(parts, plan_of(all, steps, 4, length).parts);
+    for (const int length : {4, 8}) parts = std::max(parts, plan_of(all, steps, 4, length).parts);
     parts = std::max(parts, plan_of(all, steps, 1, SINGLE).parts);
     return parts > 1 ? static_cast<size_t>(parts * all) * sizeof(float2) : 0;
 }
@@ -177,13 +184,18 @@ vm_status vm_gated_scan(int device, int32_t type, int64_t batch, int64_t steps, 
         const bool vectors = channels % 4 == 0 && takes(x, type, 4, sizes) && takes(gate, type, 4, sizes) && takes(y, type, 4, sizes) && aligned(h0, 16) && aligned(last, 16)
                              && aligned(states, 16);
         const int vector = vectors ? 4 : 1;
-        const Plan p     = plan_of(batch * channels, steps, vector, vectors ? FORWARD : SINGLE);
+        if (!vectors && batch * channels >= SERIAL_FROM) {
+            const dim3 grid(blocks_of(batch * channels));
+            with_type(type, [&](auto kind) { launch_kernel(k_gated_serial<decltype(kind)>, grid, SERIAL_BLOCK, 0, static_cast<cudaStream_t>(stream), false, a); });
+            return VM_OK;
+        }
+        const Plan p     = plan_of(batch * channels, steps, vector, vectors ? forward_steps(type == VM_F32) : SINGLE);
         const Split s    = split_of(p, workspace);
         const dim3 grid  = grid_of(batch * channels, p, vector);
         const auto q     = static_cast<cudaStream_t>(stream);
         with_layout(type, vector, p.tx, [&](auto kind, auto v, auto tx) {
             using T = decltype(kind);
-            constexpr int V = decltype(v)::value, TX = decltype(tx)::value, L = V == 1 ? SINGLE : FORWARD, STAGES = V == 1 ? 0 : sizeof(T) == 2 ? 3 : 2;
+            constexpr int V = decltype(v)::value, TX = decltype(tx)::value, L = V == 1 ? SINGLE : forward_steps(sizeof(T) == 4), STAGES = V == 1 ? 0 : sizeof(T) == 2 ? 3 : 2;
             constexpr int shared = Tiles<T, V, L, 2, STAGES>::BYTES;
             if (p.parts > 1) launch_tiles<k_gated_summary<T, V, TX, L, STAGES, false>>(grid, shared, q, a, s);
             launch_tiles<k_gated_scan<T, V, TX, L, STAGES>>(grid, shared, q, a, s);

@@ -52,7 +52,7 @@ struct Factors {
     float f, u;
 };
 __device__ __forceinline__ Factors factors_of(float g) {
-    const float e = __expf(-fabsf(g)), r = __fdividef(1.0f, 1.0f + e), s = e * r;  // e <= 1: nothing overflows
+    const float e = exp_of(-fabsf(g)), r = one_over(1.0f + e), s = e * r;  // e <= 1: nothing overflows
     return g >= 0.0f ? Factors{r, s} : Factors{s, r};
 }
 // a * b, where a of 0 drops b
@@ -87,8 +87,8 @@ __device__ __forceinline__ int64_t length_of(const GatedArgs& a, int64_t b) {
 //
 // Whether a factor of 0 meets an infinity or NaN is not asked step by step: a factor of 0 leaves A = 0, an infinity or NaN leaves H without
 // a finite value (0 times it is NaN), and only then the thread goes over its steps again, with the rule.
-constexpr int THREADS = 128;
-constexpr int WARPS   = THREADS / 32;
+constexpr int WARPS   = 8;
+constexpr int THREADS = 32 * WARPS;
 
 template <int BYTES>
 struct RawOf;
@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(THREADS) k_gated_summary(const GatedArgs a, co
 }
 
 template <typename T, int V, int TX, int L, int STAGES>
-__global__ void __launch_bounds__(THREADS, 4) k_gated_scan(const GatedArgs a, const Split s) {
+__global__ void __launch_bounds__(THREADS, 2) k_gated_scan(const GatedArgs a, const Split s) {
     constexpr int TILE = THREADS / TX * L;
     extern __shared__ uint4 ring[];
     __shared__ float2 totals[2][WARPS * TX * V];
@@ -500,8 +500,51 @@ __global__ void __launch_bounds__(THREADS, 4) k_gated_scan(const GatedArgs a, co
     if (a.last != nullptr && at.there && at.ty == 0 && blockIdx.y + 1 == gridDim.y) store_floats<V>(a.last + at.at, carry);
 }
 
+// Many sequences of single elements: a thread for each walks along time alone, AHEAD steps' loads in front of itself.
+constexpr int SERIAL_BLOCK = 256, AHEAD = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(SERIAL_BLOCK) k_gated_serial(const GatedArgs a) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * SERIAL_BLOCK + threadIdx.x;
+    if (at >= a.batch * a.channels) return;
+    const int64_t b = at / a.channels, c = at - b * a.channels;
+    const int64_t n = length_of(a, b), kept = (a.steps + KEEP - 1) / KEEP;
+    const T* x = static_cast<const T*>(a.x.data) + b * a.x.b + c * a.x.c;
+    const T* g = static_cast<const T*>(a.gate.data) + b * a.gate.b + c * a.gate.c;
+    T* y       = static_cast<T*>(a.y.data) + b * a.y.b + c * a.y.c;
+    T rx[AHEAD], rg[AHEAD];
+    const auto load = [&](int64_t t) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (t + i < n) rx[i] = *x, rg[i] = *g;
+            x += a.x.t, g += a.gate.t;
+        }
+    };
+    float h = a.h0 != nullptr ? a.h0[at] : 0.0f;
+    load(0);
+    for (int64_t t = 0; t < a.steps; t += AHEAD) {
+        float f[AHEAD], v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const bool on   = t + i < n;
+            const Factors q = factors_of(on ? to_float(rg[i]) : 0.0f);
+            f[i] = on ? q.f : 1.0f;
+            v[i] = on ? gated(q.u, to_float(rx[i])) : 0.0f;
+        }
+        load(t + AHEAD);
+        if (a.states != nullptr && t % KEEP == 0) a.states[(b * kept + t / KEEP) * a.channels + c] = h;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            h = gated(f[i], h, v[i]);
+            if (a.y.data != nullptr && t + i < a.steps) *y = from_float<T>(t + i < n ? h : 0.0f);
+            y += a.y.t;
+        }
+    }
+    if (a.last != nullptr) a.last[at] = h;
+}
+
 template <typename T, int V, int TX, int L, int STAGES>
-__global__ void __launch_bounds__(THREADS, 4) k_gated_scan_grad(const GatedArgs a, const Split s) {
+__global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs a, const Split s) {
     constexpr int TILE = THREADS / TX * L;
     extern __shared__ uint4 ring[];
     __shared__ float2 totals[2][WARPS * TX * V], totals_back[2][WARPS * TX * V];

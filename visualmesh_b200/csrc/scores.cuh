@@ -58,6 +58,12 @@ template <bool PROBABILITIES>
 __device__ __forceinline__ float value_of(float x) {
     return PROBABILITIES ? logf(x) : x;
 }
+// SCALE x log x for the sum of an entropy: the fast logarithm is off by 2^-21.4 near 1 and by two units in the last place elsewhere, which times
+// a probability is what rounding the entropy would be. (Log probabilities themselves need all of their digits near 1.)
+constexpr float SCALE = 16777216.0f;  // 2^24: a product with a number below the normal ones would lose its digits
+__device__ __forceinline__ float times_log(float x) {
+    return x == 0.0f ? 0.0f : SCALE * x * __logf(x);
+}
 
 // An order of all floats in which larger values have larger keys, equal ones (0 and -0 too) the lower index the larger key, and NaN
 // the largest: 32 bits of value above 32 bits of index. No key is 0 or has all bits set.
@@ -76,17 +82,16 @@ __device__ __forceinline__ int32_t index_of_key(uint64_t key) {
 }
 
 // What a row's values come to. Logits: m their maximum, s = sum e^t and w = sum e^t t with t = v - m. Probabilities: m = 0, s = sum x,
-// w = SCALE sum x log x (a product with a number below the normal ones would lose its digits). A value that makes the row no distribution leaves NaN in s or w.
+// w = SCALE sum x log x. A value that makes the row no distribution leaves NaN in s or w.
 struct Sums {
     float m, s, w;
 };
-constexpr float SCALE       = 16777216.0f;  // 2^24
 constexpr float NO_EXPONENT = -1000.0f;  // e^t is 0 there, and 0 times -infinity would not be
 __device__ __forceinline__ float bounded(float t) {
     return fmaxf(t, NO_EXPONENT);
 }
 __device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
-    const float m = fmaxf(a.m, b.m), da = bounded(a.m - m), db = bounded(b.m - m), fa = __expf(da), fb = __expf(db);
+    const float m = fmaxf(a.m, b.m), da = bounded(a.m - m), db = bounded(b.m - m), fa = exp_of(da), fb = exp_of(db);
     return Sums{m, fmaf(a.s, fa, b.s * fb), fmaf(fmaf(a.s, da, a.w), fa, fmaf(b.s, db, b.w) * fb)};
 }
 template <bool PROBABILITIES>
@@ -105,7 +110,7 @@ __device__ __forceinline__ Row row_of(const Sums& q) {
     else if (q.s > 0.0f) {
         r.l       = logf(q.s);
         r.log_sum = q.m + r.l;
-        r.entropy = r.l - q.w / (PROBABILITIES ? SCALE * q.s : q.s);
+        r.entropy = r.l - __fdividef(q.w, PROBABILITIES ? SCALE * q.s : q.s);
     }
     return r;
 }
@@ -193,7 +198,7 @@ __global__ void __launch_bounds__(ROW_BLOCK) k_scores_rows(const ScoresArgs a, b
         for (int i = 0; i < E; ++i) {
             if (Load::index(wide, lane, i) < classes) {
                 q.s += v[i];
-                q.w += v[i] == 0.0f ? 0.0f : SCALE * v[i] * logf(v[i]);
+                q.w += times_log(v[i]);
             }
         }
     }
@@ -207,7 +212,7 @@ __global__ void __launch_bounds__(ROW_BLOCK) k_scores_rows(const ScoresArgs a, b
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             if (Load::index(wide, lane, i) < classes) {
-                const float t = v[i] - q.m, e = __expf(t);
+                const float t = v[i] - q.m, e = exp_of(t);
                 q.s += e;
                 q.w = fmaf(e, bounded(t), q.w);
             }
@@ -367,17 +372,17 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs
 #pragma unroll
                 for (int k = 0; k < N; ++k) {
                     q.s += v[k];
-                    q.w += v[k] == 0.0f ? 0.0f : SCALE * v[k] * logf(v[k]);
+                    q.w += times_log(v[k]);
                 }
             }
             else {
-                const float m = fmaxf(q.m, top), d = bounded(q.m - m), f = __expf(d);
+                const float m = fmaxf(q.m, top), d = bounded(q.m - m), f = exp_of(d);
                 q.w = fmaf(q.s, d, q.w) * f;
                 q.s *= f;
                 q.m = m;
 #pragma unroll
                 for (int k = 0; k < N; ++k) {
-                    const float t = v[k] - m, e = __expf(t);
+                    const float t = v[k] - m, e = exp_of(t);
                     q.s += e;
                     q.w = fmaf(e, bounded(t), q.w);
                 }
@@ -476,7 +481,7 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs
 // One pass over the elements once the row's sums are known.
 template <bool PROBABILITIES>
 struct RowGrad {
-    float log_sum, d_label, d_entropy, offset, one_over;
+    float log_sum, d_label, d_entropy, offset, one_over_sum;
     int64_t label;
     __device__ __forceinline__ RowGrad(const ScoresGradArgs& a, int64_t row) : log_sum(a.log_sum[row]), d_label(0.0f), label(-1) {
         if (a.d_log_prob != nullptr) {
@@ -486,14 +491,25 @@ struct RowGrad {
         d_entropy = a.d_entropy != nullptr ? a.d_entropy[row] : 0.0f;
         offset    = (a.d_log_sum != nullptr ? a.d_log_sum[row] : 0.0f) - d_label - (a.d_entropy != nullptr ? d_entropy * a.entropy[row] : 0.0f);
         if (log_sum != log_sum) offset = NAN;
-        one_over = PROBABILITIES ? __expf(-log_sum) : 0.0f;
+        one_over_sum = PROBABILITIES ? exp_of(-log_sum) : 0.0f;
     }
-    __device__ __forceinline__ float of(float x, int64_t j) const {
-        const float v = value_of<PROBABILITIES>(x);
-        if (v == -INFINITY) return 0.0f;
-        const float lp = bounded(v - log_sum);
-        const float d  = fmaf(-d_entropy, lp, offset) * (PROBABILITIES ? one_over : __expf(lp));
-        return j == label ? d + (PROBABILITIES ? d_label / x : d_label) : d;
+    // of N neighbouring classes, the first of them number j
+    template <int N>
+    __device__ __forceinline__ void of(const float (&x)[N], int64_t j, float (&to)[N]) const {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const float v  = value_of<PROBABILITIES>(x[k]);
+            const float lp = bounded(v - log_sum);  // a masked class: p is 0, and so is its gradient
+            const float d  = fmaf(-d_entropy, lp, offset);
+            to[k]          = PROBABILITIES ? (v == -INFINITY ? 0.0f : d * one_over_sum) : d * exp_of(lp);
+        }
+        if (offset != offset || (label >= j && label < j + N)) {  // the row's label is one of these, or the row has no distribution
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                if (j + k == label) to[k] += PROBABILITIES ? d_label / x[k] : d_label;
+                if (x[k] == (PROBABILITIES ? 0.0f : -INFINITY)) to[k] = 0.0f;
+            }
+        }
     }
 };
 
@@ -506,20 +522,24 @@ __global__ void __launch_bounds__(ROW_BLOCK) k_scores_grad_rows(const ScoresGrad
     const int lane    = threadIdx.x % G;
     if (G > 1 && row >= a.rows) return;
     if (row < a.rows) {
-        const T* x = static_cast<const T*>(a.x) + row * a.row_stride;
-        T* dx      = static_cast<T*>(a.dx) + row * a.dx_row_stride;
+        const T* from = static_cast<const T*>(a.x) + row * a.row_stride;
+        T* dx         = static_cast<T*>(a.dx) + row * a.dx_row_stride;
         using Load = RowLoad<T, G, E>;
         float v[E];
-        Load::load(x, a.classes, wide, lane, v);
+        Load::load(from, a.classes, wide, lane, v);
         const RowGrad<PROBABILITIES> grad(a, row);
         if constexpr (Load::MAY) {
             if (wide) {
 #pragma unroll
                 for (int i = 0; i < E; i += Load::PIECE) {
                     const int j = Load::index(true, lane, i);
+                    float x[Load::PIECE], d[Load::PIECE];
                     T e[Load::PIECE];
 #pragma unroll
-                    for (int k = 0; k < Load::PIECE; ++k) e[k] = from_float<T>(grad.of(v[i + k], j + k));
+                    for (int k = 0; k < Load::PIECE; ++k) x[k] = v[i + k];
+                    grad.of(x, j, d);
+#pragma unroll
+                    for (int k = 0; k < Load::PIECE; ++k) e[k] = from_float<T>(d[k]);
                     if (j + Load::PIECE <= a.classes) {
                         uint4 raw;
                         memcpy(&raw, e, 16);
@@ -538,9 +558,11 @@ __global__ void __launch_bounds__(ROW_BLOCK) k_scores_grad_rows(const ScoresGrad
         for (int i = 0; i < E; ++i) {
             const int j = i * G + lane;
             if (j < a.classes) {
-                const T d = from_float<T>(grad.of(v[i], j));
-                if (G == 1 && dense) reinterpret_cast<T*>(staged)[threadIdx.x * a.classes + j] = d;
-                else dx[j] = d;
+                const float x[1] = {v[i]};
+                float d[1];
+                grad.of(x, j, d);
+                if (G == 1 && dense) reinterpret_cast<T*>(staged)[threadIdx.x * a.classes + j] = from_float<T>(d[0]);
+                else dx[j] = from_float<T>(d[0]);
             }
         }
     }
@@ -577,11 +599,12 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_grad_stream(const Score
         const int64_t p = begin + u * STREAM_BLOCK;
         if (p >= pieces.count) break;
         const int64_t j = pieces.first(p);
-        float v[N];
+        float v[N], d[N];
         T e[N];
         values_of<T>(raw[u], v);
+        grad.of(v, j, d);
 #pragma unroll
-        for (int k = 0; k < N; ++k) e[k] = from_float<T>(grad.of(v[k], j + k));
+        for (int k = 0; k < N; ++k) e[k] = from_float<T>(d[k]);
         if (together && j >= 0 && j + N <= a.classes) {
             uint4 out;
             memcpy(&out, e, 16);
