@@ -77,33 +77,39 @@ void check_sizes(int32_t type, int64_t batch, int64_t steps, int64_t channels) {
 // ---- how a scan is laid out ----------------------------------------------------------------------------------------------
 constexpr int SMS = 148;
 
+// A thread takes pairs of channels where they lie side by side, else single ones; a block 32 channels either way.
+constexpr int lanes_of(int vector) {
+    return 32 / vector;
+}
+// Steps of a thread in the forward and in the backward pass: what its registers hold, and 24 to 48 KB for a tile of the ring.
+constexpr int forward_steps(int vector, bool wide_type) {
+    return vector == 2 && !wide_type ? 16 : 8;
+}
+constexpr int BACKWARD = 8;
+// Tiles of the ring by the bytes of a thread's piece (an asynchronous copy takes 4 at least).
+constexpr int stages_of(int bytes) {
+    return bytes == 2 ? 0 : bytes == 8 ? 2 : 3;
+}
+// Sequences of single elements from which on each has a thread: two blocks an SM.
+constexpr int64_t SERIAL_FROM = 2 * SMS * SERIAL_BLOCK;
+
 struct Plan {
-    int tx;        // threads along the channels
-    int64_t run;   // steps of a part
+    int64_t blocks;  // along the channels
+    int64_t run;     // steps of a part
     int64_t parts;
 };
 
 // `vector` elements and `length` steps a thread.
 Plan plan_of(int64_t all, int64_t steps, int vector, int length) {
-    Plan p{32, steps, 1};
-    if (vector > 1 && steps > THREADS / 32 * length) p.tx = 8;
-    const int64_t tile = THREADS / p.tx * length, tiles = (steps + tile - 1) / tile;
-    const int64_t blocks = (all + p.tx * vector - 1) / (p.tx * vector);
-    if (blocks < SMS && tiles > 1) {
-        const int64_t wanted = std::min(tiles, (2 * SMS + blocks - 1) / blocks);
+    Plan p{(all + 31) / 32, steps, 1};
+    const int64_t tile = THREADS / lanes_of(vector) * length, tiles = (steps + tile - 1) / tile;
+    if (p.blocks < SMS && tiles > 1) {
+        const int64_t wanted = std::min(tiles, (2 * SMS + p.blocks - 1) / p.blocks);
         p.run                = (tiles + wanted - 1) / wanted * tile;
         p.parts              = (steps + p.run - 1) / p.run;
     }
     return p;
 }
-// Steps of a thread in the forward and in the backward pass, where it takes vectors and where it takes single elements: what its registers
-// hold, and 24 to 32 KB for a tile of the ring.
-constexpr int forward_steps(bool wide_type) {
-    return wide_type ? 4 : 8;
-}
-constexpr int BACKWARD = 4, SINGLE = 8;
-// Sequences of single elements from which on each has a thread: two blocks an SM.
-constexpr int64_t SERIAL_FROM = 2 * SMS * SERIAL_BLOCK;
 
 // Whether `vector` neighbouring channels of s lie side by side at a place that one load or store can take.
 bool takes(const vm_sequence* s, int32_t type, int vector, const int64_t (&sizes)[3]) {
@@ -112,15 +118,12 @@ bool takes(const vm_sequence* s, int32_t type, int vector, const int64_t (&sizes
     return s->channel_stride == 1 && aligned(s->data, vector * size) && (sizes[0] <= 1 || s->batch_stride % vector == 0) && (sizes[1] <= 1 || s->step_stride % vector == 0);
 }
 
-// f(a value of the element type, how many of them a thread takes, threads along the channels), as constants
+// f(a value of the element type, how many of them a thread takes), as constants
 template <typename F>
-void with_layout(int32_t type, int vector, int tx, F f) {
-    using One = std::integral_constant<int, 1>;
-    using Four = std::integral_constant<int, 4>;
+void with_layout(int32_t type, int vector, F f) {
     with_type(type, [&](auto kind) {
-        if (vector == 1) f(kind, One{}, std::integral_constant<int, 32>{});
-        else if (tx == 32) f(kind, Four{}, std::integral_constant<int, 32>{});
-        else f(kind, Four{}, std::integral_constant<int, 8>{});
+        if (vector == 1) f(kind, std::integral_constant<int, 1>{});
+        else f(kind, std::integral_constant<int, 2>{});
     });
 }
 
@@ -147,10 +150,9 @@ void check_workspace(int64_t batch, int64_t steps, int64_t channels, const void*
     if (needed > 0 && (workspace == nullptr || !aligned(workspace, 16))) throw std::string("the workspace is null or not aligned to 16 bytes");
 }
 
-dim3 grid_of(int64_t all, const Plan& p, int vector) {
-    const int64_t blocks = (all + p.tx * vector - 1) / (p.tx * vector);
-    if (blocks > INT32_MAX) throw std::string("too many sequences for one call");
-    return dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(p.parts));
+dim3 grid_of(const Plan& p) {
+    if (p.blocks > INT32_MAX) throw std::string("too many sequences for one call");
+    return dim3(static_cast<unsigned>(p.blocks), static_cast<unsigned>(p.parts));
 }
 
 }  // namespace
@@ -161,8 +163,8 @@ size_t vm_gated_workspace(int64_t batch, int64_t steps, int64_t channels) {
     if (!sizes_fit(batch, steps, channels) || batch == 0 || channels == 0) return 0;
     const int64_t all = batch * channels;
     int64_t parts     = 1;
-    for (const int length : {4, 8}) parts = std::max(parts, plan_of(all, steps, 4, length).parts);
-    parts = std::max(parts, plan_of(all, steps, 1, SINGLE).parts);
+    for (const int vector : {1, 2})
+        for (const int length : {8, 16}) parts = std::max(parts, plan_of(all, steps, vector, length).parts);
     return parts > 1 ? static_cast<size_t>(parts * all) * sizeof(float2) : 0;
 }
 
@@ -181,21 +183,20 @@ vm_status vm_gated_scan(int device, int32_t type, int64_t batch, int64_t steps, 
         a.batch = batch, a.steps = steps, a.channels = channels;
         a.x = sequence(x), a.gate = sequence(gate), a.y = sequence(y);
         a.h0 = h0, a.lengths = lengths, a.last = last, a.states = states;
-        const bool vectors = channels % 4 == 0 && takes(x, type, 4, sizes) && takes(gate, type, 4, sizes) && takes(y, type, 4, sizes) && aligned(h0, 16) && aligned(last, 16)
-                             && aligned(states, 16);
-        const int vector = vectors ? 4 : 1;
-        if (!vectors && batch * channels >= SERIAL_FROM) {
+        const auto q       = static_cast<cudaStream_t>(stream);
+        const bool pairs   = channels % 2 == 0 && takes(x, type, 2, sizes) && takes(gate, type, 2, sizes) && takes(y, type, 2, sizes) && aligned(states, 8);
+        const int vector   = pairs ? 2 : 1;
+        if (!pairs && batch * channels >= SERIAL_FROM) {
             const dim3 grid(blocks_of(batch * channels));
-            with_type(type, [&](auto kind) { launch_kernel(k_gated_serial<decltype(kind)>, grid, SERIAL_BLOCK, 0, static_cast<cudaStream_t>(stream), false, a); });
+            with_type(type, [&](auto kind) { launch_kernel(k_gated_serial<decltype(kind)>, grid, SERIAL_BLOCK, 0, q, false, a); });
             return VM_OK;
         }
-        const Plan p     = plan_of(batch * channels, steps, vector, vectors ? forward_steps(type == VM_F32) : SINGLE);
-        const Split s    = split_of(p, workspace);
-        const dim3 grid  = grid_of(batch * channels, p, vector);
-        const auto q     = static_cast<cudaStream_t>(stream);
-        with_layout(type, vector, p.tx, [&](auto kind, auto v, auto tx) {
+        const Plan p    = plan_of(batch * channels, steps, vector, forward_steps(vector, type == VM_F32));
+        const Split s   = split_of(p, workspace);
+        const dim3 grid = grid_of(p);
+        with_layout(type, vector, [&](auto kind, auto v) {
             using T = decltype(kind);
-            constexpr int V = decltype(v)::value, TX = decltype(tx)::value, L = V == 1 ? SINGLE : forward_steps(sizeof(T) == 4), STAGES = V == 1 ? 0 : sizeof(T) == 2 ? 3 : 2;
+            constexpr int V = decltype(v)::value, TX = lanes_of(V), L = forward_steps(V, sizeof(T) == 4), STAGES = stages_of(V * sizeof(T));
             constexpr int shared = Tiles<T, V, L, 2, STAGES>::BYTES;
             if (p.parts > 1) launch_tiles<k_gated_summary<T, V, TX, L, STAGES, false>>(grid, shared, q, a, s);
             launch_tiles<k_gated_scan<T, V, TX, L, STAGES>>(grid, shared, q, a, s);
@@ -230,16 +231,15 @@ vm_status vm_gated_scan_backward(int device, int32_t type, int64_t batch, int64_
         a.x = sequence(x), a.gate = sequence(gate), a.y = sequence(dy);
         a.lengths = lengths, a.states = const_cast<float*>(states), a.d_last = d_last;
         a.dx = sequence(dx), a.d_gate = sequence(d_gate), a.d_h0 = d_h0;
-        const bool vectors = channels % 4 == 0 && takes(x, type, 4, sizes) && takes(gate, type, 4, sizes) && takes(dy, type, 4, sizes) && takes(dx, type, 4, sizes)
-                             && takes(d_gate, type, 4, sizes) && aligned(states, 16) && aligned(d_last, 16) && aligned(d_h0, 16);
-        const int vector = vectors ? 4 : 1;
-        const Plan p     = plan_of(batch * channels, steps, vector, vectors ? BACKWARD : SINGLE);
-        const Split s    = split_of(p, workspace);
-        const dim3 grid  = grid_of(batch * channels, p, vector);
         const auto q     = static_cast<cudaStream_t>(stream);
-        with_layout(type, vector, p.tx, [&](auto kind, auto v, auto tx) {
+        const bool pairs = channels % 2 == 0 && takes(x, type, 2, sizes) && takes(gate, type, 2, sizes) && takes(dy, type, 2, sizes) && takes(dx, type, 2, sizes) && takes(d_gate, type, 2, sizes);
+        const int vector = pairs ? 2 : 1;
+        const Plan p     = plan_of(batch * channels, steps, vector, BACKWARD);
+        const Split s    = split_of(p, workspace);
+        const dim3 grid  = grid_of(p);
+        with_layout(type, vector, [&](auto kind, auto v) {
             using T = decltype(kind);
-            constexpr int V = decltype(v)::value, TX = decltype(tx)::value, L = V == 1 ? SINGLE : BACKWARD, STAGES = V == 1 ? 0 : sizeof(T) == 2 ? 3 : 2;
+            constexpr int V = decltype(v)::value, TX = lanes_of(V), L = BACKWARD, STAGES = stages_of(V * sizeof(T));
             if (p.parts > 1) launch_tiles<k_gated_summary<T, V, TX, L, STAGES, true>>(grid, Tiles<T, V, L, 2, STAGES>::BYTES, q, a, s);
             launch_tiles<k_gated_scan_grad<T, V, TX, L, STAGES>>(grid, Tiles<T, V, L, 3, STAGES>::BYTES, q, a, s);
         });

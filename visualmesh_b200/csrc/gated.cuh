@@ -66,9 +66,10 @@ __device__ __forceinline__ float gated(float a, float b, float c) {
 }
 // The factor of two runs of steps. It is 0 only where a step's is: what 32 bits cannot hold becomes their smallest normal number, so that an
 // infinity or NaN goes on through a long run as it does step by step.
+constexpr float SMALLEST = 1.17549435e-38f;
 __device__ __forceinline__ float product(float a, float b) {
     const float r = a * b;
-    return a == 0.0f || b == 0.0f ? 0.0f : r == 0.0f ? 1.17549435e-38f : r;
+    return a == 0.0f || b == 0.0f ? 0.0f : r < SMALLEST ? SMALLEST : r;
 }
 
 __device__ __forceinline__ int64_t length_of(const GatedArgs& a, int64_t b) {
@@ -127,35 +128,23 @@ __device__ __forceinline__ Raw<T, V> pack(const float (&from)[V]) {
     memcpy(&raw, e, sizeof(raw));
     return raw;
 }
+// V neighbouring 32-bit floats at a place that is aligned to all of them
 template <int V>
 __device__ __forceinline__ void load_floats(const float* from, float (&to)[V]) {
-    if constexpr (V % 4 == 0) {
-#pragma unroll
-        for (int k = 0; k < V; k += 4) {
-            const float4 q = *reinterpret_cast<const float4*>(from + k);
-            to[k] = q.x, to[k + 1] = q.y, to[k + 2] = q.z, to[k + 3] = q.w;
-        }
-    }
-    else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) to[k] = from[k];
-    }
+    const Raw<float, V> raw = *reinterpret_cast<const Raw<float, V>*>(from);
+    memcpy(to, &raw, sizeof(raw));
 }
 template <int V>
 __device__ __forceinline__ void store_floats(float* to, const float (&from)[V]) {
-    if constexpr (V % 4 == 0) {
-#pragma unroll
-        for (int k = 0; k < V; k += 4) *reinterpret_cast<float4*>(to + k) = make_float4(from[k], from[k + 1], from[k + 2], from[k + 3]);
-    }
-    else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) to[k] = from[k];
-    }
+    Raw<float, V> raw;
+    memcpy(&raw, from, sizeof(raw));
+    *reinterpret_cast<Raw<float, V>*>(to) = raw;
 }
 
 template <int V, int TX>
 struct Place {
     static constexpr int SEGMENTS = 32 / TX;  // of a warp
+    static constexpr int CHANNELS = TX * V;   // of the block
     int warp, lane, tx, ty;
     int64_t at, b, c;  // first of the thread's channels: of all, its batch, within that
     bool there;
@@ -171,66 +160,90 @@ struct Place {
     }
 };
 
-// (A, H) after (pa, ph): h -> A (pa h + ph) + H
+// Maps of the warps of a block, and the states in front of them.
+template <int V, int TX>
+struct alignas(16) Between {
+    float before[WARPS][TX * V];
+    float2 totals[WARPS][TX * V];
+};
+
+// Whether a run of steps met nothing that needs care: no factor of 0 (nor a product that came to it), no value that is not finite.
 template <int V>
-__device__ __forceinline__ void compose(float (&A)[V], float (&H)[V], const float (&pa)[V], const float (&ph)[V]) {
+__device__ __forceinline__ bool plain(const float (&A)[V], const float (&H)[V]) {
+    bool ok = true;
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        H[k] = gated(A[k], ph[k], H[k]);
-        A[k] = product(A[k], pa[k]);
-    }
+    for (int k = 0; k < V; ++k) ok = ok && A[k] > 0.0f && fabsf(H[k]) < INFINITY;
+    return ok;
+}
+template <int V>
+__device__ __forceinline__ bool finite(const float (&v)[V]) {
+    bool ok = true;
+#pragma unroll
+    for (int k = 0; k < V; ++k) ok = ok && fabsf(v[k]) < INFINITY;
+    return ok;
 }
 
-// Scan over the threads along time, in their order or (REVERSE) against it. In: every thread's map (A, H). Out: the map of all threads
-// before it in its own warp (A, H), and in `totals` (shared memory, [WARPS][TX * V]) the maps of the whole warps.
+// Scan over the lanes along time, in their order or (REVERSE) against it. In: every thread's map (A, H). Out: the map of all threads
+// before it in its own warp, and that of the whole warp in `totals`. careful: in one of the lanes a factor is 0 or a value not finite.
 template <int V, int TX, bool REVERSE>
-__device__ __forceinline__ void scan_warp(const Place<V, TX>& at, float (&A)[V], float (&H)[V], float2* totals) {
+__device__ __forceinline__ void scan_warp(const Place<V, TX>& at, float (&A)[V], float (&H)[V], bool careful, float2 (*totals)[TX * V]) {
+    const auto from = [](float v, int d) { return REVERSE ? __shfl_down_sync(~0u, v, d) : __shfl_up_sync(~0u, v, d); };
+    const auto scan = [&](auto care) {
 #pragma unroll
-    for (int d = TX; d < 32; d *= 2) {
-        float pa[V], ph[V];
+        for (int d = TX; d < 32; d *= 2) {
+            const bool has = REVERSE ? at.lane + d < 32 : at.lane >= d;
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            pa[k] = REVERSE ? __shfl_down_sync(~0u, A[k], d) : __shfl_up_sync(~0u, A[k], d);
-            ph[k] = REVERSE ? __shfl_down_sync(~0u, H[k], d) : __shfl_up_sync(~0u, H[k], d);
+            for (int k = 0; k < V; ++k) {
+                const float pa = from(A[k], d), ph = from(H[k], d);
+                if (has) {
+                    if constexpr (decltype(care)::value) {
+                        H[k] = gated(A[k], ph, H[k]);
+                        A[k] = product(A[k], pa);
+                    }
+                    else {
+                        H[k] = fmaf(A[k], ph, H[k]);
+                        A[k] = fmaxf(A[k] * pa, SMALLEST);
+                    }
+                }
+            }
         }
-        if (REVERSE ? at.lane + d < 32 : at.lane >= d) compose<V>(A, H, pa, ph);
-    }
+    };
+    if (__any_sync(~0u, careful)) scan(std::true_type{});
+    else scan(std::false_type{});
     if (REVERSE ? at.lane < TX : at.lane >= 32 - TX) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) totals[at.warp * TX * V + at.tx * V + k] = make_float2(A[k], H[k]);
+        for (int k = 0; k < V; ++k) totals[at.warp][at.tx * V + k] = make_float2(A[k], H[k]);
     }
-    if constexpr (TX < 32) {
-        const bool first = REVERSE ? at.lane >= 32 - TX : at.lane < TX;
+    const bool first = REVERSE ? at.lane >= 32 - TX : at.lane < TX;
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const float pa = REVERSE ? __shfl_down_sync(~0u, A[k], TX) : __shfl_up_sync(~0u, A[k], TX);
-            const float ph = REVERSE ? __shfl_down_sync(~0u, H[k], TX) : __shfl_up_sync(~0u, H[k], TX);
+    for (int k = 0; k < V; ++k) {
+        if constexpr (TX < 32) {
+            const float pa = from(A[k], TX), ph = from(H[k], TX);
             A[k] = first ? 1.0f : pa;
             H[k] = first ? 0.0f : ph;
         }
-    }
-    else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) A[k] = 1.0f, H[k] = 0.0f;
+        else A[k] = 1.0f, H[k] = 0.0f;
     }
 }
-// After a barrier: the state in front of the thread's own steps, from the one in front of all threads (carry), which becomes the one
-// behind them.
+// One thread for a channel, between two barriers: the states in front of every warp, from the one in front of the block (carry), which
+// becomes the one behind it.
 template <int V, int TX, bool REVERSE>
-__device__ __forceinline__ void scan_block(const Place<V, TX>& at, const float (&A)[V], const float (&H)[V], const float2* totals, float (&carry)[V], float (&mine)[V]) {
-#pragma unroll 1
+__device__ __forceinline__ void fold_warps(Between<V, TX>& shared, int channel, float& carry) {
+#pragma unroll
     for (int i = 0; i < WARPS; ++i) {
-        const int w = REVERSE ? WARPS - 1 - i : i;
-        if (w == at.warp) {
-#pragma unroll
-            for (int k = 0; k < V; ++k) mine[k] = gated(A[k], carry[k], H[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const float2 q = totals[w * TX * V + at.tx * V + k];
-            carry[k]       = gated(q.x, carry[k], q.y);
-        }
+        const int w              = REVERSE ? WARPS - 1 - i : i;
+        const float2 q           = shared.totals[w][channel];
+        shared.before[w][channel] = carry;
+        carry                    = gated(q.x, carry, q.y);
     }
+}
+// The state in front of the thread's own steps.
+template <int V, int TX>
+__device__ __forceinline__ void state_before(const Place<V, TX>& at, const Between<V, TX>& shared, const float (&A)[V], const float (&H)[V], float (&h)[V]) {
+    float before[V];
+    load_floats<V>(&shared.before[at.warp][at.tx * V], before);
+#pragma unroll
+    for (int k = 0; k < V; ++k) h[k] = gated(A[k], before[k], H[k]);
 }
 
 template <int BYTES>
@@ -299,9 +312,9 @@ struct Tiles {
             for (int n = 0; n < N; ++n) from[n] += by * stride[n];
         }
     }
-    // step number i of the thread's in sequence n; 0 where it is not `on`
-    __device__ __forceinline__ void get(int n, int i, bool on, float (&to)[V]) const {
-        R raw{};
+    // step number i of the thread's in sequence n; `otherwise` where it is not `on`
+    __device__ __forceinline__ void get(int n, int i, bool on, R otherwise, float (&to)[V]) const {
+        R raw = otherwise;
         if (on) raw = STAGES > 0 ? *place(at, n, i) : *reinterpret_cast<const R*>(from[n] + i * stride[n]);
         unpack<T, V>(raw, to);
     }
@@ -314,33 +327,31 @@ struct Split {
     float2* summary;  // [parts][batch * channels]: the map of every part
 };
 
-// whether a run of steps met nothing that needs care: no factor of 0 (nor a product that came to it), no value that is not finite
-template <int V>
-__device__ __forceinline__ bool plain(const float (&A)[V], const float (&H)[V]) {
-    bool ok = true;
-#pragma unroll
-    for (int k = 0; k < V; ++k) ok = ok && A[k] > 0.0f && fabsf(H[k]) < INFINITY;
-    return ok;
+// How many of a thread's L steps from t on come before `stop`.
+template <int L>
+__device__ __forceinline__ int steps_before(int64_t stop, int64_t t) {
+    return stop - t >= L ? L : stop > t ? static_cast<int>(stop - t) : 0;
 }
-template <int V>
-__device__ __forceinline__ bool finite(const float (&v)[V]) {
-    float zero = 0.0f;
+// A gate that keeps the state, and values of nothing: steps that are not there.
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> kept_gate() {
+    float v[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) zero = fmaf(v[k], 0.0f, zero);
-    return zero == 0.0f;
+    for (int k = 0; k < V; ++k) v[k] = INFINITY;
+    return pack<T, V>(v);
 }
 
 // The state in front of part `part` of a split sequence (or, REVERSE, behind it), from the one at the sequence's end: a thread along
-// time for every part on that side.
+// time for every part on that side. channel: the one whose state the thread carries, or -1.
 template <int V, int TX, bool REVERSE>
-__device__ __forceinline__ void join_parts(const GatedArgs& a, const Split& s, const Place<V, TX>& at, int part, float (&carry)[V], float2 (*totals)[WARPS * TX * V]) {
+__device__ __forceinline__ void join_parts(const GatedArgs& a, const Split& s, const Place<V, TX>& at, int part, int channel, float& carry, Between<V, TX>& shared) {
     constexpr int TY  = THREADS / TX;
     const int64_t all = a.batch * a.channels;
     const int begin = REVERSE ? part + 1 : 0, end = REVERSE ? s.parts : part;
     const int rounds = (end - begin + TY - 1) / TY;
     for (int r = 0; r < rounds; ++r) {
         const int j = begin + (REVERSE ? rounds - 1 - r : r) * TY + at.ty;
-        float A[V], H[V], ignored[V];
+        float A[V], H[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             A[k] = 1.0f, H[k] = 0.0f;
@@ -349,11 +360,11 @@ __device__ __forceinline__ void join_parts(const GatedArgs& a, const Split& s, c
                 A[k] = q.x, H[k] = q.y;
             }
         }
-        scan_warp<V, TX, REVERSE>(at, A, H, totals[r & 1]);
+        scan_warp<V, TX, REVERSE>(at, A, H, !plain<V>(A, H), shared.totals);
         __syncthreads();
-        scan_block<V, TX, REVERSE>(at, A, H, totals[r & 1], carry, ignored);
+        if (channel >= 0) fold_warps<V, TX, REVERSE>(shared, channel, carry);
+        __syncthreads();
     }
-    if (rounds > 0) __syncthreads();  // the walk over the tiles begins with the first of the two buffers again
 }
 
 // Maps of the parts of a split sequence, of the recurrence or (REVERSE) of its gradient.
@@ -361,7 +372,7 @@ template <typename T, int V, int TX, int L, int STAGES, bool REVERSE>
 __global__ void __launch_bounds__(THREADS) k_gated_summary(const GatedArgs a, const Split s) {
     constexpr int TILE = THREADS / TX * L;
     extern __shared__ uint4 ring[];
-    __shared__ float2 totals[2][WARPS * TX * V];
+    __shared__ Between<V, TX> shared;
     const Place<V, TX> at(a);
     const int64_t n     = at.there ? length_of(a, at.b) : 0;
     const int64_t begin = blockIdx.y * s.run, end = begin + s.run < a.steps ? begin + s.run : a.steps;
@@ -374,12 +385,12 @@ __global__ void __launch_bounds__(THREADS) k_gated_summary(const GatedArgs a, co
     constexpr int BY = REVERSE ? -TILE : TILE;
     int64_t t        = begin + (REVERSE ? tiles - 1 : 0) * TILE + at.ty * L;
     io.begin(ring, t, BY, tiles, stops);
-    float carry[V], whole[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) carry[k] = 0.0f, whole[k] = 1.0f;
+    const int channel = threadIdx.x < at.CHANNELS ? threadIdx.x : -1;
+    float carry = 0.0f, whole = 1.0f;
     for (int64_t tile = 0; tile < tiles; ++tile, t += BY) {
         io.advance(BY, stops);
-        float A[V], H[V], mine[V];
+        const int in_left = steps_before<L>(stops[0], t), left = steps_before<L>(stop, t);
+        float A[V], H[V];
         const auto pass = [&](auto careful) {
             constexpr bool CAREFUL = decltype(careful)::value;
 #pragma unroll
@@ -388,47 +399,43 @@ __global__ void __launch_bounds__(THREADS) k_gated_summary(const GatedArgs a, co
             for (int i = 0; i < L; ++i) {
                 const int step = REVERSE ? L - 1 - i : i;
                 float x[V], g[V];
-                io.get(0, step, t + step < stops[0], x);
-                io.get(1, step, t + step < stop, g);
-                if (t + step < stop) {
+                io.get(0, step, step < in_left, Raw<T, V>{}, x);
+                io.get(1, step, step < left, kept_gate<T, V>(), g);
 #pragma unroll
-                    for (int k = 0; k < V; ++k) {
-                        const Factors w = factors_of(g[k]);
-                        if constexpr (CAREFUL) {
-                            H[k] = REVERSE ? gated(w.f, x[k] + H[k]) : gated(w.f, H[k], gated(w.u, x[k]));
-                            A[k] = product(w.f, A[k]);
-                        }
-                        else {
-                            H[k] = REVERSE ? w.f * (x[k] + H[k]) : fmaf(w.f, H[k], w.u * x[k]);
-                            A[k] = w.f * A[k];
-                        }
+                for (int k = 0; k < V; ++k) {
+                    const Factors w = factors_of(g[k]);
+                    if constexpr (CAREFUL) {
+                        H[k] = REVERSE ? gated(w.f, x[k] + H[k]) : gated(w.f, H[k], gated(w.u, x[k]));
+                        A[k] = product(w.f, A[k]);
+                    }
+                    else {
+                        H[k] = REVERSE ? w.f * (x[k] + H[k]) : fmaf(w.f, H[k], w.u * x[k]);
+                        A[k] = w.f * A[k];
                     }
                 }
             }
         };
         pass(std::false_type{});
-        if (!plain<V>(A, H)) pass(std::true_type{});
-        scan_warp<V, TX, REVERSE>(at, A, H, totals[tile & 1]);
+        const bool careful = !plain<V>(A, H);
+        if (careful) pass(std::true_type{});
+        scan_warp<V, TX, REVERSE>(at, A, H, careful, shared.totals);
         __syncthreads();
-        scan_block<V, TX, REVERSE>(at, A, H, totals[tile & 1], carry, mine);
-#pragma unroll 1
-        for (int i = 0; i < WARPS; ++i) {
-            const int w = REVERSE ? WARPS - 1 - i : i;
+        if (channel >= 0) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) whole[k] = product(totals[tile & 1][w * TX * V + at.tx * V + k].x, whole[k]);
+            for (int w = 0; w < WARPS; ++w) whole = product(shared.totals[w][channel].x, whole);
+            fold_warps<V, TX, REVERSE>(shared, channel, carry);
         }
+        __syncthreads();
     }
-    if (at.there && at.ty == 0) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) s.summary[blockIdx.y * (a.batch * a.channels) + at.at + k] = make_float2(whole[k], carry[k]);
-    }
+    const int64_t of_channel = static_cast<int64_t>(blockIdx.x) * at.CHANNELS + channel, all = a.batch * a.channels;
+    if (channel >= 0 && of_channel < all) s.summary[blockIdx.y * all + of_channel] = make_float2(whole, carry);
 }
 
 template <typename T, int V, int TX, int L, int STAGES>
 __global__ void __launch_bounds__(THREADS, 2) k_gated_scan(const GatedArgs a, const Split s) {
     constexpr int TILE = THREADS / TX * L;
     extern __shared__ uint4 ring[];
-    __shared__ float2 totals[2][WARPS * TX * V];
+    __shared__ Between<V, TX> shared;
     const Place<V, TX> at(a);
     const int64_t n     = at.there ? length_of(a, at.b) : 0, kept = (a.steps + KEEP - 1) / KEEP;
     const int64_t begin = blockIdx.y * s.run, end = begin + s.run < a.steps ? begin + s.run : a.steps;
@@ -439,15 +446,16 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan(const GatedArgs a, co
     io.from[1] = static_cast<const T*>(a.gate.data) + at.b * a.gate.b + at.c * a.gate.c, io.stride[1] = a.gate.t;
     int64_t t = begin + at.ty * L;
     io.begin(ring, t, TILE, tiles, stops);
-    T* y              = static_cast<T*>(a.y.data) + at.b * a.y.b + at.c * a.y.c;
+    T* y              = static_cast<T*>(a.y.data) + at.b * a.y.b + at.c * a.y.c + t * a.y.t;
     const bool writes = at.there && a.y.data != nullptr;
-    float carry[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) carry[k] = 0.0f;
-    if (at.there && a.h0 != nullptr) load_floats<V>(a.h0 + at.at, carry);
-    if (s.parts > 1) join_parts<V, TX, false>(a, s, at, blockIdx.y, carry, totals);
-    for (int64_t tile = 0; tile < tiles; ++tile, t += TILE) {
+    const int64_t of_channel = static_cast<int64_t>(blockIdx.x) * at.CHANNELS + threadIdx.x;
+    const int channel        = threadIdx.x < at.CHANNELS ? threadIdx.x : -1;
+    const bool carries       = channel >= 0 && of_channel < a.batch * a.channels;
+    float carry              = carries && a.h0 != nullptr ? a.h0[of_channel] : 0.0f;
+    if (s.parts > 1) join_parts<V, TX, false>(a, s, at, blockIdx.y, channel, carry, shared);
+    for (int64_t tile = 0; tile < tiles; ++tile, t += TILE, y += TILE * a.y.t) {
         io.advance(TILE, stops);
+        const int left = steps_before<L>(stop, t), room = steps_before<L>(end, t);
         float f[L][V], v[L][V], A[V], H[V], h[V];
         const auto pass = [&](auto careful) {
             constexpr bool CAREFUL = decltype(careful)::value;
@@ -455,26 +463,27 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan(const GatedArgs a, co
             for (int k = 0; k < V; ++k) A[k] = 1.0f, H[k] = 0.0f;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
-                const bool on = t + i < stop;
-                io.get(0, i, on, v[i]);
-                io.get(1, i, on, f[i]);
+                io.get(0, i, i < left, Raw<T, V>{}, v[i]);
+                io.get(1, i, i < left, kept_gate<T, V>(), f[i]);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     const Factors q = factors_of(f[i][k]);
-                    f[i][k] = on ? q.f : 1.0f;
-                    v[i][k] = CAREFUL ? gated(q.u, v[i][k]) : q.u * v[i][k];  // behind the end v is 0, and so is this
-                    H[k]    = CAREFUL ? gated(f[i][k], H[k], v[i][k]) : fmaf(f[i][k], H[k], v[i][k]);
-                    A[k]    = CAREFUL ? product(f[i][k], A[k]) : f[i][k] * A[k];
+                    f[i][k] = q.f;
+                    v[i][k] = CAREFUL ? gated(q.u, v[i][k]) : q.u * v[i][k];
+                    H[k]    = CAREFUL ? gated(q.f, H[k], v[i][k]) : fmaf(q.f, H[k], v[i][k]);
+                    A[k]    = CAREFUL ? product(q.f, A[k]) : q.f * A[k];
                 }
             }
         };
         pass(std::false_type{});
         bool careful = !plain<V>(A, H);
         if (careful) pass(std::true_type{});
-        scan_warp<V, TX, false>(at, A, H, totals[tile & 1]);
+        scan_warp<V, TX, false>(at, A, H, careful, shared.totals);
         __syncthreads();
-        scan_block<V, TX, false>(at, A, H, totals[tile & 1], carry, h);
-        if (a.states != nullptr && at.there && t < end && t % KEEP == 0) store_floats<V>(a.states + (at.b * kept + t / KEEP) * a.channels + at.c, h);
+        if (channel >= 0) fold_warps<V, TX, false>(shared, channel, carry);
+        __syncthreads();
+        state_before<V, TX>(at, shared, A, H, h);
+        if (a.states != nullptr && at.there && room > 0 && t % KEEP == 0) store_floats<V>(a.states + (at.b * kept + t / KEEP) * a.channels + at.c, h);
         careful = careful || !finite<V>(h);
         if (careful) {
 #pragma unroll
@@ -490,14 +499,14 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan(const GatedArgs a, co
                 for (int k = 0; k < V; ++k) v[i][k] = h[k] = fmaf(f[i][k], h[k], v[i][k]);
             }
         }
-        T* to = y + t * a.y.t;
+        T* to = y;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            if (writes && t + i < end) *reinterpret_cast<Raw<T, V>*>(to) = t + i < stop ? pack<T, V>(v[i]) : Raw<T, V>{};
+            if (writes && i < room) *reinterpret_cast<Raw<T, V>*>(to) = i < left ? pack<T, V>(v[i]) : Raw<T, V>{};
             to += a.y.t;
         }
     }
-    if (a.last != nullptr && at.there && at.ty == 0 && blockIdx.y + 1 == gridDim.y) store_floats<V>(a.last + at.at, carry);
+    if (a.last != nullptr && carries && blockIdx.y + 1 == gridDim.y) a.last[of_channel] = carry;
 }
 
 // Many sequences of single elements: a thread for each walks along time alone, AHEAD steps' loads in front of itself.
@@ -543,11 +552,13 @@ __global__ void __launch_bounds__(SERIAL_BLOCK) k_gated_serial(const GatedArgs a
     if (a.last != nullptr) a.last[at] = h;
 }
 
+// The gradient's walk goes from the last tile to the first. Its own scan runs against time beside the recurrence's, which starts in every
+// tile from a kept state.
 template <typename T, int V, int TX, int L, int STAGES>
 __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs a, const Split s) {
     constexpr int TILE = THREADS / TX * L;
     extern __shared__ uint4 ring[];
-    __shared__ float2 totals[2][WARPS * TX * V], totals_back[2][WARPS * TX * V];
+    __shared__ Between<V, TX> shared, shared_back;
     const Place<V, TX> at(a);
     const int64_t n     = at.there ? length_of(a, at.b) : 0, kept = (a.steps + KEEP - 1) / KEEP;
     const int64_t begin = blockIdx.y * s.run, end = begin + s.run < a.steps ? begin + s.run : a.steps;
@@ -557,124 +568,108 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
     io.from[0] = static_cast<const T*>(a.x.data) + at.b * a.x.b + at.c * a.x.c, io.stride[0] = a.x.t;
     io.from[1] = static_cast<const T*>(a.gate.data) + at.b * a.gate.b + at.c * a.gate.c, io.stride[1] = a.gate.t;
     io.from[2] = static_cast<const T*>(a.y.data) + at.b * a.y.b + at.c * a.y.c, io.stride[2] = a.y.t;
-    int64_t t0 = begin + (tiles > 0 ? tiles - 1 : 0) * TILE;  // the last tile comes first
-    io.begin(ring, t0 + at.ty * L, -TILE, tiles, stops);
-    T* dx = static_cast<T*>(a.dx.data) + at.b * a.dx.b + at.c * a.dx.c;
-    T* dg = static_cast<T*>(a.d_gate.data) + at.b * a.d_gate.b + at.c * a.d_gate.c;
+    int64_t t0 = begin + (tiles > 0 ? tiles - 1 : 0) * TILE, t = t0 + at.ty * L;
+    io.begin(ring, t, -TILE, tiles, stops);
+    T* dx = static_cast<T*>(a.dx.data) + at.b * a.dx.b + at.c * a.dx.c + t * a.dx.t;
+    T* dg = static_cast<T*>(a.d_gate.data) + at.b * a.d_gate.b + at.c * a.d_gate.c + t * a.d_gate.t;
     const bool writes_x = at.there && a.dx.data != nullptr, writes_g = at.there && a.d_gate.data != nullptr;
-    const float* states = a.states + at.b * kept * a.channels + at.c;
-    float back[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) back[k] = 0.0f;
-    if (at.there && a.d_last != nullptr) load_floats<V>(a.d_last + at.at, back);
-    if (s.parts > 1) join_parts<V, TX, true>(a, s, at, blockIdx.y, back, totals_back);
-    for (int64_t tile = 0; tile < tiles; ++tile, t0 -= TILE) {
-        const int64_t t = t0 + at.ty * L;
-        float carry[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) carry[k] = 0.0f;
-        if (at.there) load_floats<V>(states + t0 / KEEP * a.channels, carry);
+    // the first threads carry the recurrence's states, the last ones the gradient's
+    static_assert(2 * Place<V, TX>::CHANNELS <= THREADS, "a thread carries one state");
+    const int channel = threadIdx.x < at.CHANNELS ? threadIdx.x : -1, channel_back = static_cast<int>(threadIdx.x) - (THREADS - at.CHANNELS);
+    const int64_t of_channel = static_cast<int64_t>(blockIdx.x) * at.CHANNELS + (channel >= 0 ? channel : channel_back), all = a.batch * a.channels;
+    const bool carries = channel >= 0 && of_channel < all, carries_back = channel_back >= 0 && of_channel < all;
+    const float* states = a.states;
+    if (carries) states += of_channel / a.channels * kept * a.channels + of_channel % a.channels;
+    float next = carries && tiles > 0 ? states[t0 / KEEP * a.channels] : 0.0f;  // the state in front of the tile to come
+    float back = carries_back && a.d_last != nullptr ? a.d_last[of_channel] : 0.0f;
+    if (s.parts > 1) join_parts<V, TX, true>(a, s, at, blockIdx.y, channel_back, back, shared_back);
+    for (int64_t tile = 0; tile < tiles; ++tile, t0 -= TILE, t -= TILE, dx -= TILE * a.dx.t, dg -= TILE * a.d_gate.t) {
+        float carry = next;
+        if (carries && tile + 1 < tiles) next = states[(t0 - TILE) / KEEP * a.channels];
         io.advance(-TILE, stops);
-        float f[L][V], u[L][V], w[L][V], d[L][V], A[V], H[V], AR[V], R[V], h[V], c[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) A[k] = 1.0f, H[k] = 0.0f, R[k] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < L; ++i) {
-            const bool on = t + i < stop;
-            io.get(0, i, on, w[i]);
-            io.get(1, i, on, f[i]);
-            io.get(2, i, t + i < stops[2], d[i]);
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const Factors q = factors_of(f[i][k]);
-                f[i][k] = on ? q.f : 1.0f;
-                u[i][k] = on ? q.u : 0.0f;
-                H[k]    = fmaf(f[i][k], H[k], u[i][k] * w[i][k]);
-                A[k]    = f[i][k] * A[k];
-            }
-        }
-#pragma unroll
-        for (int i = L - 1; i >= 0; --i) {
-#pragma unroll
-            for (int k = 0; k < V; ++k) R[k] = f[i][k] * (d[i][k] + R[k]);
-        }
-        bool careful = !plain<V>(A, H) || !finite<V>(R);
-        if (careful) {
+        const int left = steps_before<L>(stop, t), d_left = steps_before<L>(stops[2], t), room = steps_before<L>(end, t);
+        float f[L][V], u[L][V], w[L][V], A[V], H[V], AR[V], R[V], h[V], c[V];
+        // x and dy are read from the ring twice, here and behind the scan, instead of being held
+        const auto pass = [&](auto careful) {
+            constexpr bool CAREFUL = decltype(careful)::value;
 #pragma unroll
             for (int k = 0; k < V; ++k) A[k] = 1.0f, H[k] = 0.0f, R[k] = 0.0f;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
+                float x[V], d[V], g[V];
+                io.get(0, i, i < left, Raw<T, V>{}, x);
+                io.get(1, i, i < left, kept_gate<T, V>(), g);
+                io.get(2, i, i < d_left, Raw<T, V>{}, d);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
-                    H[k] = gated(f[i][k], H[k], gated(u[i][k], w[i][k]));
-                    A[k] = product(f[i][k], A[k]);
-                    R[k] = gated(f[L - 1 - i][k], d[L - 1 - i][k] + R[k]);
+                    const Factors q = factors_of(g[k]);
+                    f[i][k] = q.f;
+                    u[i][k] = q.u;
+                    H[k]    = CAREFUL ? gated(q.f, H[k], gated(q.u, x[k])) : fmaf(q.f, H[k], q.u * x[k]);
+                    A[k]    = CAREFUL ? product(q.f, A[k]) : q.f * A[k];
+                    R[k]    = CAREFUL ? gated(A[k], d[k], R[k]) : fmaf(A[k], d[k], R[k]);
                 }
             }
-        }
+        };
+        pass(std::false_type{});
+        bool careful = !plain<V>(A, H) || !finite<V>(R);
+        if (careful) pass(std::true_type{});
 #pragma unroll
         for (int k = 0; k < V; ++k) AR[k] = A[k];
-        scan_warp<V, TX, false>(at, A, H, totals[tile & 1]);
-        scan_warp<V, TX, true>(at, AR, R, totals_back[tile & 1]);
+        scan_warp<V, TX, false>(at, A, H, careful, shared.totals);
+        scan_warp<V, TX, true>(at, AR, R, careful, shared_back.totals);
         __syncthreads();
-        scan_block<V, TX, false>(at, A, H, totals[tile & 1], carry, h);
-        scan_block<V, TX, true>(at, AR, R, totals_back[tile & 1], back, c);
+        if (channel >= 0) fold_warps<V, TX, false>(shared, channel, carry);
+        if (channel_back >= 0) fold_warps<V, TX, true>(shared_back, channel_back, back);
+        __syncthreads();
+        state_before<V, TX>(at, shared, A, H, h);
+        state_before<V, TX>(at, shared_back, AR, R, c);
         careful = careful || !finite<V>(h) || !finite<V>(c);
-        // w: from x to h_(t-1) - x; then u to the gradient of x and w to that of the gate
-        if (careful) {
+        // w: h_(t-1) - x, then the gradient of the gate; u: to the gradient of x
+        const auto grads = [&](auto care) {
+            constexpr bool CAREFUL = decltype(care)::value;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
+                float x[V];
+                io.get(0, i, i < left, Raw<T, V>{}, x);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
-                    const float here = w[i][k];
-                    w[i][k] = h[k] - here;
-                    h[k]    = gated(f[i][k], h[k], gated(u[i][k], here));
+                    w[i][k] = h[k] - x[k];
+                    h[k]    = CAREFUL ? gated(f[i][k], h[k], gated(u[i][k], x[k])) : fmaf(f[i][k], h[k], u[i][k] * x[k]);
                 }
             }
 #pragma unroll
             for (int i = L - 1; i >= 0; --i) {
+                float d[V];
+                io.get(2, i, i < d_left, Raw<T, V>{}, d);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
-                    const float total = d[i][k] + c[k];
-                    w[i][k] = gated(f[i][k] * u[i][k], w[i][k] * total);
-                    u[i][k] = gated(u[i][k], total);
-                    c[k]    = gated(f[i][k], total);
+                    const float total = d[k] + c[k];
+                    if constexpr (CAREFUL) {
+                        w[i][k] = gated(f[i][k] * u[i][k], w[i][k] * total);
+                        c[k]    = gated(f[i][k], total);
+                        u[i][k] = gated(u[i][k], total);
+                    }
+                    else {
+                        c[k]    = f[i][k] * total;
+                        w[i][k] = u[i][k] * (w[i][k] * c[k]);
+                        u[i][k] = u[i][k] * total;
+                    }
                 }
             }
-        }
-        else {
-#pragma unroll
-            for (int i = 0; i < L; ++i) {
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const float here = w[i][k];
-                    w[i][k] = h[k] - here;
-                    h[k]    = fmaf(f[i][k], h[k], u[i][k] * here);
-                }
-            }
-#pragma unroll
-            for (int i = L - 1; i >= 0; --i) {
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const float total = d[i][k] + c[k];
-                    u[i][k] = u[i][k] * total;
-                    c[k]    = f[i][k] * total;
-                    w[i][k] = f[i][k] * u[i][k] * w[i][k];
-                }
-            }
-        }
-        T* to_x = dx + t * a.dx.t;
-        T* to_g = dg + t * a.d_gate.t;
+        };
+        if (careful) grads(std::true_type{});
+        else grads(std::false_type{});
+        T* to_x = dx;
+        T* to_g = dg;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            if (t + i < end) {
-                if (writes_x) *reinterpret_cast<Raw<T, V>*>(to_x) = pack<T, V>(u[i]);
-                if (writes_g) *reinterpret_cast<Raw<T, V>*>(to_g) = pack<T, V>(w[i]);
-            }
+            if (writes_x && i < room) *reinterpret_cast<Raw<T, V>*>(to_x) = pack<T, V>(u[i]);
+            if (writes_g && i < room) *reinterpret_cast<Raw<T, V>*>(to_g) = pack<T, V>(w[i]);
             to_x += a.dx.t, to_g += a.d_gate.t;
         }
     }
-    if (a.d_h0 != nullptr && at.there && at.ty == 0 && blockIdx.y == 0) store_floats<V>(a.d_h0 + at.at, back);
+    if (a.d_h0 != nullptr && carries_back && blockIdx.y == 0) a.d_h0[of_channel] = back;
 }
 
 // ---- single steps ------------------------------------------------------------------------------------------------------------
