@@ -1,5 +1,6 @@
 // vm_gated_scan, vm_gated_scan_backward and vm_gated_step: checks and launches of the kernels in gated.cuh.
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 #include <utility>
 
@@ -77,19 +78,15 @@ void check_sizes(int32_t type, int64_t batch, int64_t steps, int64_t channels) {
 // ---- how a scan is laid out ----------------------------------------------------------------------------------------------
 constexpr int SMS = 148;
 
-// A thread takes pairs of channels where they lie side by side, else single ones; a block 32 channels either way.
-constexpr int lanes_of(int vector) {
-    return 32 / vector;
-}
-// Steps of a thread in the forward and in the backward pass: what its registers hold, and 24 to 48 KB for a tile of the ring.
+// A thread takes pairs of channels where they lie side by side, else single ones; a block 32 channels either way. Steps of a thread in the
+// forward and in the backward pass: what its registers hold, with 24 to 34 KB for a tile of the ring, of which there are three.
 constexpr int forward_steps(int vector, bool wide_type) {
     return vector == 2 && !wide_type ? 16 : 8;
 }
-constexpr int BACKWARD = 8;
-// Tiles of the ring by the bytes of a thread's piece (an asynchronous copy takes 4 at least).
-constexpr int stages_of(int bytes) {
-    return bytes == 2 ? 0 : bytes == 8 ? 2 : 3;
+constexpr int backward_steps(int vector, bool wide_type) {
+    return vector == 2 && wide_type ? 4 : 8;
 }
+constexpr int STAGES = 3;
 // Sequences of single elements from which on each has a thread: two blocks an SM.
 constexpr int64_t SERIAL_FROM = 2 * SMS * SERIAL_BLOCK;
 
@@ -102,7 +99,7 @@ struct Plan {
 // `vector` elements and `length` steps a thread.
 Plan plan_of(int64_t all, int64_t steps, int vector, int length) {
     Plan p{(all + 31) / 32, steps, 1};
-    const int64_t tile = THREADS / lanes_of(vector) * length, tiles = (steps + tile - 1) / tile;
+    const int64_t tile = THREADS / (32 / vector) * length, tiles = (steps + tile - 1) / tile;
     if (p.blocks < SMS && tiles > 1) {
         const int64_t wanted = std::min(tiles, (2 * SMS + p.blocks - 1) / p.blocks);
         p.run                = (tiles + wanted - 1) / wanted * tile;
@@ -118,13 +115,27 @@ bool takes(const vm_sequence* s, int32_t type, int vector, const int64_t (&sizes
     return s->channel_stride == 1 && aligned(s->data, vector * size) && (sizes[0] <= 1 || s->batch_stride % vector == 0) && (sizes[1] <= 1 || s->step_stride % vector == 0);
 }
 
-// f(a value of the element type, how many of them a thread takes), as constants
+// How a thread takes elements (vector) and copies them (piece, in bytes; 0: not through the ring).
+struct Access {
+    int vector, piece;
+};
+// f(a value of the element type, elements of a thread, bytes of a copy), as constants
 template <typename F>
-void with_layout(int32_t type, int vector, F f) {
+void with_access(int32_t type, const Access& access, F f) {
+    using std::integral_constant;
     with_type(type, [&](auto kind) {
-        if (vector == 1) f(kind, std::integral_constant<int, 1>{});
-        else f(kind, std::integral_constant<int, 2>{});
+        constexpr int SIZE = sizeof(kind);
+        if (access.piece == 16) f(kind, integral_constant<int, 2>{}, integral_constant<int, 16>{});
+        else if (access.vector == 2) f(kind, integral_constant<int, 2>{}, integral_constant<int, 2 * SIZE>{});
+        else f(kind, integral_constant<int, 1>{}, integral_constant<int, SIZE == 4 ? 4 : 0>{});
     });
+}
+// inputs are read through the ring in pieces, outputs are written by a thread's vectors
+Access access_of(int32_t type, int64_t channels, const int64_t (&sizes)[3], std::initializer_list<const vm_sequence*> inputs, std::initializer_list<const vm_sequence*> outputs, const float* states) {
+    const int size = static_cast<int>(element_size(type)), wide = 16 / size;
+    const auto all = [&](std::initializer_list<const vm_sequence*> list, int n) { return std::all_of(list.begin(), list.end(), [&](const vm_sequence* s) { return takes(s, type, n, sizes); }); };
+    if (channels % 2 != 0 || !all(inputs, 2) || !all(outputs, 2) || !aligned(states, 8)) return {1, size == 4 ? 4 : 0};
+    return {2, channels % wide == 0 && all(inputs, wide) ? 16 : 2 * size};
 }
 
 // Launches one kernel, which is told once for a device that it may take more shared memory than every kernel may.
@@ -164,7 +175,7 @@ size_t vm_gated_workspace(int64_t batch, int64_t steps, int64_t channels) {
     const int64_t all = batch * channels;
     int64_t parts     = 1;
     for (const int vector : {1, 2})
-        for (const int length : {8, 16}) parts = std::max(parts, plan_of(all, steps, vector, length).parts);
+        for (const int length : {4, 8, 16}) parts = std::max(parts, plan_of(all, steps, vector, length).parts);
     return parts > 1 ? static_cast<size_t>(parts * all) * sizeof(float2) : 0;
 }
 
@@ -184,22 +195,20 @@ vm_status vm_gated_scan(int device, int32_t type, int64_t batch, int64_t steps, 
         a.x = sequence(x), a.gate = sequence(gate), a.y = sequence(y);
         a.h0 = h0, a.lengths = lengths, a.last = last, a.states = states;
         const auto q       = static_cast<cudaStream_t>(stream);
-        const bool pairs   = channels % 2 == 0 && takes(x, type, 2, sizes) && takes(gate, type, 2, sizes) && takes(y, type, 2, sizes) && aligned(states, 8);
-        const int vector   = pairs ? 2 : 1;
-        if (!pairs && batch * channels >= SERIAL_FROM) {
+        const Access access = access_of(type, channels, sizes, {x, gate}, {y}, states);
+        if (access.vector == 1 && batch * channels >= SERIAL_FROM) {
             const dim3 grid(blocks_of(batch * channels));
             with_type(type, [&](auto kind) { launch_kernel(k_gated_serial<decltype(kind)>, grid, SERIAL_BLOCK, 0, q, false, a); });
             return VM_OK;
         }
-        const Plan p    = plan_of(batch * channels, steps, vector, forward_steps(vector, type == VM_F32));
+        const Plan p    = plan_of(batch * channels, steps, access.vector, forward_steps(access.vector, type == VM_F32));
         const Split s   = split_of(p, workspace);
         const dim3 grid = grid_of(p);
-        with_layout(type, vector, [&](auto kind, auto v) {
+        with_access(type, access, [&](auto kind, auto v, auto piece) {
             using T = decltype(kind);
-            constexpr int V = decltype(v)::value, TX = lanes_of(V), L = forward_steps(V, sizeof(T) == 4), STAGES = stages_of(V * sizeof(T));
-            constexpr int shared = Tiles<T, V, L, 2, STAGES>::BYTES;
-            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, TX, L, STAGES, false>>(grid, shared, q, a, s);
-            launch_tiles<k_gated_scan<T, V, TX, L, STAGES>>(grid, shared, q, a, s);
+            constexpr int V = decltype(v)::value, PIECE = decltype(piece)::value, L = forward_steps(V, sizeof(T) == 4), SHARED = Tiles<T, V, L, 2, PIECE, STAGES>::SHARED;
+            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, L, PIECE, STAGES, false>>(grid, SHARED, q, a, s);
+            launch_tiles<k_gated_scan<T, V, L, PIECE, STAGES>>(grid, SHARED, q, a, s);
         });
     }
     catch (const std::string& refused) {
@@ -232,16 +241,15 @@ vm_status vm_gated_scan_backward(int device, int32_t type, int64_t batch, int64_
         a.lengths = lengths, a.states = const_cast<float*>(states), a.d_last = d_last;
         a.dx = sequence(dx), a.d_gate = sequence(d_gate), a.d_h0 = d_h0;
         const auto q     = static_cast<cudaStream_t>(stream);
-        const bool pairs = channels % 2 == 0 && takes(x, type, 2, sizes) && takes(gate, type, 2, sizes) && takes(dy, type, 2, sizes) && takes(dx, type, 2, sizes) && takes(d_gate, type, 2, sizes);
-        const int vector = pairs ? 2 : 1;
-        const Plan p     = plan_of(batch * channels, steps, vector, BACKWARD);
+        const Access access = access_of(type, channels, sizes, {x, gate, dy}, {dx, d_gate}, nullptr);
+        const Plan p     = plan_of(batch * channels, steps, access.vector, backward_steps(access.vector, type == VM_F32));
         const Split s    = split_of(p, workspace);
         const dim3 grid  = grid_of(p);
-        with_layout(type, vector, [&](auto kind, auto v) {
+        with_access(type, access, [&](auto kind, auto v, auto piece) {
             using T = decltype(kind);
-            constexpr int V = decltype(v)::value, TX = lanes_of(V), L = BACKWARD, STAGES = stages_of(V * sizeof(T));
-            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, TX, L, STAGES, true>>(grid, Tiles<T, V, L, 2, STAGES>::BYTES, q, a, s);
-            launch_tiles<k_gated_scan_grad<T, V, TX, L, STAGES>>(grid, Tiles<T, V, L, 3, STAGES>::BYTES, q, a, s);
+            constexpr int V = decltype(v)::value, PIECE = decltype(piece)::value, L = backward_steps(V, sizeof(T) == 4);
+            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, L, PIECE, STAGES, true>>(grid, Tiles<T, V, L, 2, PIECE, STAGES>::SHARED, q, a, s);
+            launch_tiles<k_gated_scan_grad<T, V, L, PIECE, STAGES>>(grid, Tiles<T, V, L, 3, PIECE, STAGES>::SHARED, q, a, s);
         });
     }
     catch (const std::string& refused) {

@@ -254,69 +254,107 @@ __device__ __forceinline__ void copy_async(void* to, const void* from) {
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
 }
 
-// The tiles of N sequences on their way: the steps of a thread that come before `stop`, of tile after tile, read by that thread alone.
-// STAGES == 0: read when they are asked for.
-template <typename T, int V, int L, int N, int STAGES>
+// A gate that keeps the state: what stands for steps that are not there (with a value of 0).
+template <typename T>
+__device__ __forceinline__ T kept_gate() {
+    return from_float<T>(INFINITY);
+}
+enum { X = 0, GATE = 1, DY = 2 };  // which of the sequences of a kernel
+template <typename T, int PIECE>
+__device__ __forceinline__ typename RawOf<PIECE>::type filled(bool gate) {
+    T e[PIECE / sizeof(T)];
+#pragma unroll
+    for (int i = 0; i < PIECE / static_cast<int>(sizeof(T)); ++i) e[i] = gate ? kept_gate<T>() : from_float<T>(0.0f);
+    typename RawOf<PIECE>::type raw;
+    memcpy(&raw, e, PIECE);
+    return raw;
+}
+
+// The tiles of N sequences on their way through a ring in shared memory, a row of the block's 32 channels for a step. A thread copies
+// pieces of PIECE bytes (16 where the sequences' places allow it) for channels of its own, and after a barrier every thread reads what it works
+// on. Rows at and behind a sequence's stop are filled instead. A row of 16-bit elements is half as wide as the banks, so that the rows of
+// every other thread along time begin in their other half (a gap behind every L rows).
+// PIECE == 0: no ring, every thread reads its own elements when it needs them (single elements of 16 bits).
+template <typename T, int V, int L, int N, int PIECE, int STAGES>
 struct Tiles {
-    using R = Raw<T, V>;
-    static constexpr int BYTES = STAGES * N * L * THREADS * sizeof(R);
-    R* ring;
-    const T* from[N];   // the thread's first step of the tile to be asked for next (STAGES == 0: of the present one)
-    int64_t stride[N];  // from step to step
-    int64_t next, left; // that step's number, and how many tiles are to be asked for
+    static constexpr int CHANNELS = 32, TX = CHANNELS / V, TILE = THREADS / TX * L;
+    static constexpr int ROW   = CHANNELS * sizeof(T), GAP = ROW < 128 ? ROW : 0;
+    static constexpr int BYTES = TILE * ROW + TILE / L * GAP;  // of a tile of one sequence
+    static constexpr int SHARED = PIECE > 0 ? STAGES * N * BYTES : 0;
+    static constexpr int ACROSS = PIECE > 0 ? ROW / (PIECE > 0 ? PIECE : 1) : 1, ROWS = THREADS / ACROSS;  // pieces of a row; rows copied side by side
+    static_assert(PIECE == 0 || THREADS % ACROSS == 0, "a thread's channels are the same in every row");
+
+    unsigned char* ring;
+    const T* from[N];
+    int64_t stride[N];
+    int64_t next, left;  // the step that the next tile begins with, and how many tiles are still to be asked for
     int put, at;
 
-    __device__ __forceinline__ R* place(int stage, int n, int i) const {
-        return ring + ((stage * N + n) * L + i) * THREADS + threadIdx.x;
+    __device__ __forceinline__ static int offset(int row) {
+        return row * ROW + row / L * GAP;
     }
-    // by: steps from tile to tile; stop: behind the last step that is read
-    __device__ __forceinline__ void ask(int64_t by, const int64_t (&stop)[N]) {
+    // by: steps from tile to tile
+    template <int BY>
+    __device__ __forceinline__ void ask(const int64_t (&stop)[N]) {
         if (left-- > 0) {
+            const int first = threadIdx.x / ACROSS;
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                const T* p = from[n];
+                const int64_t rows = stop[n] - next;  // of the tile that are there (or more)
+                const T* p         = from[n];
+                unsigned char* to  = ring + (put * N + n) * BYTES + threadIdx.x % ACROSS * PIECE;
 #pragma unroll
-                for (int i = 0; i < L; ++i) {
-                    if (next + i < stop[n]) copy_async<sizeof(R)>(place(put, n, i), p);
-                    p += stride[n];
+                for (int k = 0; k < TILE / ROWS; ++k) {
+                    const int row = first + k * ROWS;
+                    if (row < rows) copy_async<PIECE>(to + offset(row), p);
+                    else *reinterpret_cast<typename RawOf<PIECE>::type*>(to + offset(row)) = filled<T, PIECE>(n == GATE);
+                    p += ROWS * stride[n];
                 }
-                from[n] += by * stride[n];
+                from[n] += BY * stride[n];
             }
         }
-        next += by;
+        next += BY;
         put = put + 1 == STAGES ? 0 : put + 1;
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    __device__ __forceinline__ void begin(void* shared, int64_t first, int64_t by, int64_t tiles, const int64_t (&stop)[N]) {
+    // The first tiles; `from` are the first elements of the first tile that the thread copies (PIECE == 0: that it works on, in that tile).
+    template <int BY>
+    __device__ __forceinline__ void begin(void* shared, int64_t first, int64_t tiles, const int64_t (&stop)[N]) {
+        at = 0;
+        if constexpr (PIECE > 0) {
+            ring = static_cast<unsigned char*>(shared), next = first, left = tiles, put = 0;
 #pragma unroll
-        for (int n = 0; n < N; ++n) from[n] += first * stride[n];
-        ring = static_cast<R*>(shared), next = first, left = tiles, put = 0, at = STAGES - 1;
-        if constexpr (STAGES > 0) {
-#pragma unroll
-            for (int s = 0; s + 1 < STAGES; ++s) ask(by, stop);
-        }
-        else {
-#pragma unroll
-            for (int n = 0; n < N; ++n) from[n] -= by * stride[n];
+            for (int s = 0; s + 1 < STAGES; ++s) ask<BY>(stop);
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         }
     }
-    // on to the next tile
-    __device__ __forceinline__ void advance(int64_t by, const int64_t (&stop)[N]) {
-        if constexpr (STAGES > 0) {
-            ask(by, stop);
-            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-            at = at + 1 == STAGES ? 0 : at + 1;
-        }
-        else {
-#pragma unroll
-            for (int n = 0; n < N; ++n) from[n] += by * stride[n];
+    // In a tile, between two barriers that all threads come to with what they read of the tile before it: the tile behind it is there after
+    // the second of them.
+    template <int BY>
+    __device__ __forceinline__ void ahead(const int64_t (&stop)[N]) {
+        if constexpr (PIECE > 0) {
+            ask<BY>(stop);
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         }
     }
-    // step number i of the thread's in sequence n; `otherwise` where it is not `on`
-    __device__ __forceinline__ void get(int n, int i, bool on, R otherwise, float (&to)[V]) const {
-        R raw = otherwise;
-        if (on) raw = STAGES > 0 ? *place(at, n, i) : *reinterpret_cast<const R*>(from[n] + i * stride[n]);
-        unpack<T, V>(raw, to);
+    template <int BY>
+    __device__ __forceinline__ void advance() {
+        if constexpr (PIECE > 0) at = at + 1 == STAGES ? 0 : at + 1;
+        else {
+#pragma unroll
+            for (int n = 0; n < N; ++n) from[n] += BY * stride[n];
+        }
+    }
+    // step number i of the thread's (ty along time, tx along the channels) in sequence n, of which `there` come before its stop
+    __device__ __forceinline__ void get(int n, int i, int tx, int ty, int there, float (&to)[V]) const {
+        T e[V];
+        if constexpr (PIECE > 0) {
+            const Raw<T, V> raw = *reinterpret_cast<const Raw<T, V>*>(ring + (at * N + n) * BYTES + offset(ty * L) + i * ROW + tx * V * sizeof(T));
+            memcpy(e, &raw, sizeof(raw));
+        }
+        else e[0] = i < there ? from[n][i * stride[n]] : n == GATE ? kept_gate<T>() : from_float<T>(0.0f);
+#pragma unroll
+        for (int k = 0; k < V; ++k) to[k] = to_float(e[k]);
     }
 };
 
@@ -332,13 +370,18 @@ template <int L>
 __device__ __forceinline__ int steps_before(int64_t stop, int64_t t) {
     return stop - t >= L ? L : stop > t ? static_cast<int>(stop - t) : 0;
 }
-// A gate that keeps the state, and values of nothing: steps that are not there.
-template <typename T, int V>
-__device__ __forceinline__ Raw<T, V> kept_gate() {
-    float v[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = INFINITY;
-    return pack<T, V>(v);
+// Sequence number n of a kernel, from step `first` on: where the thread's copies begin, and (returned) behind which step of first..end-1 there
+// is nothing. What a thread copies belongs to other channels than what it works on, maybe of another batch.
+template <typename T, int V, int L, int N, int PIECE, int STAGES>
+__device__ __forceinline__ int64_t set_up(Tiles<T, V, L, N, PIECE, STAGES>& io, int n, const Sequence& q, const GatedArgs& a, const Place<V, 32 / V>& at, int64_t first, int64_t end) {
+    using IO             = Tiles<T, V, L, N, PIECE, STAGES>;
+    const int64_t copied = PIECE > 0 ? blockIdx.x * int64_t(IO::CHANNELS) + threadIdx.x % IO::ACROSS * (PIECE / int(sizeof(T))) : at.at;
+    io.stride[n]         = q.t;
+    io.from[n]           = nullptr;
+    if (copied >= a.batch * a.channels || q.data == nullptr) return 0;
+    const int64_t b = copied / a.channels, length = length_of(a, b);
+    io.from[n] = static_cast<const T*>(q.data) + b * q.b + (copied - b * a.channels) * q.c + (first + (PIECE > 0 ? threadIdx.x / IO::ACROSS : at.ty * L)) * q.t;
+    return end < length ? end : length;
 }
 
 // The state in front of part `part` of a split sequence (or, REVERSE, behind it), from the one at the sequence's end: a thread along
@@ -368,28 +411,25 @@ __device__ __forceinline__ void join_parts(const GatedArgs& a, const Split& s, c
 }
 
 // Maps of the parts of a split sequence, of the recurrence or (REVERSE) of its gradient.
-template <typename T, int V, int TX, int L, int STAGES, bool REVERSE>
+template <typename T, int V, int L, int PIECE, int STAGES, bool REVERSE>
 __global__ void __launch_bounds__(THREADS) k_gated_summary(const GatedArgs a, const Split s) {
-    constexpr int TILE = THREADS / TX * L;
+    using IO = Tiles<T, V, L, 2, PIECE, STAGES>;
+    constexpr int TX = IO::TX, TILE = IO::TILE, BY = REVERSE ? -TILE : TILE;
     extern __shared__ uint4 ring[];
     __shared__ Between<V, TX> shared;
     const Place<V, TX> at(a);
     const int64_t n     = at.there ? length_of(a, at.b) : 0;
     const int64_t begin = blockIdx.y * s.run, end = begin + s.run < a.steps ? begin + s.run : a.steps;
-    const int64_t tiles = (end - begin + TILE - 1) / TILE, stop = end < n ? end : n;
-    const Sequence& in  = REVERSE ? a.y : a.x;
-    Tiles<T, V, L, 2, STAGES> io;
-    const int64_t stops[2] = {in.data != nullptr ? stop : 0, stop};
-    io.from[0] = static_cast<const T*>(in.data) + at.b * in.b + at.c * in.c, io.stride[0] = in.t;
-    io.from[1] = static_cast<const T*>(a.gate.data) + at.b * a.gate.b + at.c * a.gate.c, io.stride[1] = a.gate.t;
-    constexpr int BY = REVERSE ? -TILE : TILE;
-    int64_t t        = begin + (REVERSE ? tiles - 1 : 0) * TILE + at.ty * L;
-    io.begin(ring, t, BY, tiles, stops);
+    const int64_t tiles = (end - begin + TILE - 1) / TILE, stop = end < n ? end : n, first = begin + (REVERSE ? tiles - 1 : 0) * TILE;
+    IO io;
+    const int64_t stops[2] = {set_up(io, X, REVERSE ? a.y : a.x, a, at, first, end), set_up(io, GATE, a.gate, a, at, first, end)};
+    io.template begin<BY>(ring, first, tiles, stops);
     const int channel = threadIdx.x < at.CHANNELS ? threadIdx.x : -1;
     float carry = 0.0f, whole = 1.0f;
+    int64_t t = first + at.ty * L;
+    __syncthreads();
     for (int64_t tile = 0; tile < tiles; ++tile, t += BY) {
-        io.advance(BY, stops);
-        const int in_left = steps_before<L>(stops[0], t), left = steps_before<L>(stop, t);
+        const int left = steps_before<L>(stop, t), in_left = REVERSE && a.y.data == nullptr ? 0 : left;
         float A[V], H[V];
         const auto pass = [&](auto careful) {
             constexpr bool CAREFUL = decltype(careful)::value;
@@ -397,21 +437,15 @@ __global__ void __launch_bounds__(THREADS) k_gated_summary(const GatedArgs a, co
             for (int k = 0; k < V; ++k) A[k] = 1.0f, H[k] = 0.0f;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
-                const int step = REVERSE ? L - 1 - i : i;
                 float x[V], g[V];
-                io.get(0, step, step < in_left, Raw<T, V>{}, x);
-                io.get(1, step, step < left, kept_gate<T, V>(), g);
+                io.get(X, i, at.tx, at.ty, in_left, x);
+                io.get(GATE, i, at.tx, at.ty, left, g);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     const Factors w = factors_of(g[k]);
-                    if constexpr (CAREFUL) {
-                        H[k] = REVERSE ? gated(w.f, x[k] + H[k]) : gated(w.f, H[k], gated(w.u, x[k]));
-                        A[k] = product(w.f, A[k]);
-                    }
-                    else {
-                        H[k] = REVERSE ? w.f * (x[k] + H[k]) : fmaf(w.f, H[k], w.u * x[k]);
-                        A[k] = w.f * A[k];
-                    }
+                    if constexpr (!REVERSE) H[k] = CAREFUL ? gated(w.f, H[k], gated(w.u, x[k])) : fmaf(w.f, H[k], w.u * x[k]);
+                    A[k] = CAREFUL ? product(w.f, A[k]) : w.f * A[k];
+                    if constexpr (REVERSE) H[k] = CAREFUL ? gated(A[k], x[k], H[k]) : fmaf(A[k], x[k], H[k]);
                 }
             }
         };
@@ -420,32 +454,33 @@ __global__ void __launch_bounds__(THREADS) k_gated_summary(const GatedArgs a, co
         if (careful) pass(std::true_type{});
         scan_warp<V, TX, REVERSE>(at, A, H, careful, shared.totals);
         __syncthreads();
+        io.template ahead<BY>(stops);
         if (channel >= 0) {
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) whole = product(shared.totals[w][channel].x, whole);
             fold_warps<V, TX, REVERSE>(shared, channel, carry);
         }
         __syncthreads();
+        io.template advance<BY>();
     }
     const int64_t of_channel = static_cast<int64_t>(blockIdx.x) * at.CHANNELS + channel, all = a.batch * a.channels;
     if (channel >= 0 && of_channel < all) s.summary[blockIdx.y * all + of_channel] = make_float2(whole, carry);
 }
 
-template <typename T, int V, int TX, int L, int STAGES>
+template <typename T, int V, int L, int PIECE, int STAGES>
 __global__ void __launch_bounds__(THREADS, 2) k_gated_scan(const GatedArgs a, const Split s) {
-    constexpr int TILE = THREADS / TX * L;
+    using IO = Tiles<T, V, L, 2, PIECE, STAGES>;
+    constexpr int TX = IO::TX, TILE = IO::TILE;
     extern __shared__ uint4 ring[];
     __shared__ Between<V, TX> shared;
     const Place<V, TX> at(a);
     const int64_t n     = at.there ? length_of(a, at.b) : 0, kept = (a.steps + KEEP - 1) / KEEP;
     const int64_t begin = blockIdx.y * s.run, end = begin + s.run < a.steps ? begin + s.run : a.steps;
     const int64_t tiles = (end - begin + TILE - 1) / TILE, stop = end < n ? end : n;
-    Tiles<T, V, L, 2, STAGES> io;
-    const int64_t stops[2] = {stop, stop};
-    io.from[0] = static_cast<const T*>(a.x.data) + at.b * a.x.b + at.c * a.x.c, io.stride[0] = a.x.t;
-    io.from[1] = static_cast<const T*>(a.gate.data) + at.b * a.gate.b + at.c * a.gate.c, io.stride[1] = a.gate.t;
-    int64_t t = begin + at.ty * L;
-    io.begin(ring, t, TILE, tiles, stops);
+    IO io;
+    const int64_t stops[2] = {set_up(io, X, a.x, a, at, begin, end), set_up(io, GATE, a.gate, a, at, begin, end)};
+    io.template begin<TILE>(ring, begin, tiles, stops);
+    int64_t t         = begin + at.ty * L;
     T* y              = static_cast<T*>(a.y.data) + at.b * a.y.b + at.c * a.y.c + t * a.y.t;
     const bool writes = at.there && a.y.data != nullptr;
     const int64_t of_channel = static_cast<int64_t>(blockIdx.x) * at.CHANNELS + threadIdx.x;
@@ -453,8 +488,8 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan(const GatedArgs a, co
     const bool carries       = channel >= 0 && of_channel < a.batch * a.channels;
     float carry              = carries && a.h0 != nullptr ? a.h0[of_channel] : 0.0f;
     if (s.parts > 1) join_parts<V, TX, false>(a, s, at, blockIdx.y, channel, carry, shared);
+    __syncthreads();
     for (int64_t tile = 0; tile < tiles; ++tile, t += TILE, y += TILE * a.y.t) {
-        io.advance(TILE, stops);
         const int left = steps_before<L>(stop, t), room = steps_before<L>(end, t);
         float f[L][V], v[L][V], A[V], H[V], h[V];
         const auto pass = [&](auto careful) {
@@ -463,8 +498,8 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan(const GatedArgs a, co
             for (int k = 0; k < V; ++k) A[k] = 1.0f, H[k] = 0.0f;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
-                io.get(0, i, i < left, Raw<T, V>{}, v[i]);
-                io.get(1, i, i < left, kept_gate<T, V>(), f[i]);
+                io.get(X, i, at.tx, at.ty, left, v[i]);
+                io.get(GATE, i, at.tx, at.ty, left, f[i]);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     const Factors q = factors_of(f[i][k]);
@@ -480,12 +515,13 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan(const GatedArgs a, co
         if (careful) pass(std::true_type{});
         scan_warp<V, TX, false>(at, A, H, careful, shared.totals);
         __syncthreads();
+        io.template ahead<TILE>(stops);
         if (channel >= 0) fold_warps<V, TX, false>(shared, channel, carry);
         __syncthreads();
+        io.template advance<TILE>();
         state_before<V, TX>(at, shared, A, H, h);
         if (a.states != nullptr && at.there && room > 0 && t % KEEP == 0) store_floats<V>(a.states + (at.b * kept + t / KEEP) * a.channels + at.c, h);
-        careful = careful || !finite<V>(h);
-        if (careful) {
+        if (careful || !finite<V>(h)) {
 #pragma unroll
             for (int i = 0; i < L; ++i) {
 #pragma unroll
@@ -500,10 +536,14 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan(const GatedArgs a, co
             }
         }
         T* to = y;
+        if (writes && left == L) {
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            if (writes && i < room) *reinterpret_cast<Raw<T, V>*>(to) = i < left ? pack<T, V>(v[i]) : Raw<T, V>{};
-            to += a.y.t;
+            for (int i = 0; i < L; ++i, to += a.y.t) *reinterpret_cast<Raw<T, V>*>(to) = pack<T, V>(v[i]);
+        }
+        else if (writes) {
+#pragma unroll
+            for (int i = 0; i < L; ++i, to += a.y.t)
+                if (i < room) *reinterpret_cast<Raw<T, V>*>(to) = i < left ? pack<T, V>(v[i]) : Raw<T, V>{};
         }
     }
     if (a.last != nullptr && carries && blockIdx.y + 1 == gridDim.y) a.last[of_channel] = carry;
@@ -554,22 +594,20 @@ __global__ void __launch_bounds__(SERIAL_BLOCK) k_gated_serial(const GatedArgs a
 
 // The gradient's walk goes from the last tile to the first. Its own scan runs against time beside the recurrence's, which starts in every
 // tile from a kept state.
-template <typename T, int V, int TX, int L, int STAGES>
+template <typename T, int V, int L, int PIECE, int STAGES>
 __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs a, const Split s) {
-    constexpr int TILE = THREADS / TX * L;
+    using IO = Tiles<T, V, L, 3, PIECE, STAGES>;
+    constexpr int TX = IO::TX, TILE = IO::TILE;
     extern __shared__ uint4 ring[];
     __shared__ Between<V, TX> shared, shared_back;
     const Place<V, TX> at(a);
     const int64_t n     = at.there ? length_of(a, at.b) : 0, kept = (a.steps + KEEP - 1) / KEEP;
     const int64_t begin = blockIdx.y * s.run, end = begin + s.run < a.steps ? begin + s.run : a.steps;
     const int64_t tiles = (end - begin + TILE - 1) / TILE, stop = end < n ? end : n;
-    Tiles<T, V, L, 3, STAGES> io;
-    const int64_t stops[3] = {stop, stop, a.y.data != nullptr ? stop : 0};
-    io.from[0] = static_cast<const T*>(a.x.data) + at.b * a.x.b + at.c * a.x.c, io.stride[0] = a.x.t;
-    io.from[1] = static_cast<const T*>(a.gate.data) + at.b * a.gate.b + at.c * a.gate.c, io.stride[1] = a.gate.t;
-    io.from[2] = static_cast<const T*>(a.y.data) + at.b * a.y.b + at.c * a.y.c, io.stride[2] = a.y.t;
     int64_t t0 = begin + (tiles > 0 ? tiles - 1 : 0) * TILE, t = t0 + at.ty * L;
-    io.begin(ring, t, -TILE, tiles, stops);
+    IO io;
+    const int64_t stops[3] = {set_up(io, X, a.x, a, at, t0, end), set_up(io, GATE, a.gate, a, at, t0, end), set_up(io, DY, a.y, a, at, t0, end)};
+    io.template begin<-TILE>(ring, t0, tiles, stops);
     T* dx = static_cast<T*>(a.dx.data) + at.b * a.dx.b + at.c * a.dx.c + t * a.dx.t;
     T* dg = static_cast<T*>(a.d_gate.data) + at.b * a.d_gate.b + at.c * a.d_gate.c + t * a.d_gate.t;
     const bool writes_x = at.there && a.dx.data != nullptr, writes_g = at.there && a.d_gate.data != nullptr;
@@ -583,11 +621,11 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
     float next = carries && tiles > 0 ? states[t0 / KEEP * a.channels] : 0.0f;  // the state in front of the tile to come
     float back = carries_back && a.d_last != nullptr ? a.d_last[of_channel] : 0.0f;
     if (s.parts > 1) join_parts<V, TX, true>(a, s, at, blockIdx.y, channel_back, back, shared_back);
+    __syncthreads();
     for (int64_t tile = 0; tile < tiles; ++tile, t0 -= TILE, t -= TILE, dx -= TILE * a.dx.t, dg -= TILE * a.d_gate.t) {
         float carry = next;
         if (carries && tile + 1 < tiles) next = states[(t0 - TILE) / KEEP * a.channels];
-        io.advance(-TILE, stops);
-        const int left = steps_before<L>(stop, t), d_left = steps_before<L>(stops[2], t), room = steps_before<L>(end, t);
+        const int left = steps_before<L>(stop, t), d_left = a.y.data == nullptr ? 0 : left, room = steps_before<L>(end, t);
         float f[L][V], u[L][V], w[L][V], A[V], H[V], AR[V], R[V], h[V], c[V];
         // x and dy are read from the ring twice, here and behind the scan, instead of being held
         const auto pass = [&](auto careful) {
@@ -597,9 +635,9 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 float x[V], d[V], g[V];
-                io.get(0, i, i < left, Raw<T, V>{}, x);
-                io.get(1, i, i < left, kept_gate<T, V>(), g);
-                io.get(2, i, i < d_left, Raw<T, V>{}, d);
+                io.get(X, i, at.tx, at.ty, left, x);
+                io.get(GATE, i, at.tx, at.ty, left, g);
+                io.get(DY, i, at.tx, at.ty, d_left, d);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     const Factors q = factors_of(g[k]);
@@ -619,6 +657,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
         scan_warp<V, TX, false>(at, A, H, careful, shared.totals);
         scan_warp<V, TX, true>(at, AR, R, careful, shared_back.totals);
         __syncthreads();
+        io.template ahead<-TILE>(stops);
         if (channel >= 0) fold_warps<V, TX, false>(shared, channel, carry);
         if (channel_back >= 0) fold_warps<V, TX, true>(shared_back, channel_back, back);
         __syncthreads();
@@ -631,7 +670,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 float x[V];
-                io.get(0, i, i < left, Raw<T, V>{}, x);
+                io.get(X, i, at.tx, at.ty, left, x);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     w[i][k] = h[k] - x[k];
@@ -641,7 +680,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
 #pragma unroll
             for (int i = L - 1; i >= 0; --i) {
                 float d[V];
-                io.get(2, i, i < d_left, Raw<T, V>{}, d);
+                io.get(DY, i, at.tx, at.ty, d_left, d);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     const float total = d[k] + c[k];
@@ -660,6 +699,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
         };
         if (careful) grads(std::true_type{});
         else grads(std::false_type{});
+        io.template advance<-TILE>();
         T* to_x = dx;
         T* to_g = dg;
 #pragma unroll
