@@ -20,16 +20,29 @@ vm_status check_rows(const void* x, int32_t type, int64_t rows, int32_t classes,
 }
 
 constexpr int SMS          = 148;
-constexpr int MOST_IN_ROWS = 1024;  // classes that a row's lanes hold in registers
+constexpr int MOST_OF_THREAD = 8;     // classes that a thread holds in registers
+constexpr int MOST_IN_ROWS   = 1024;  // and several lanes of a warp
 
+// f(classes), as a constant
+template <typename F>
+void with_classes(int classes, F f) {
+    using std::integral_constant;
+    switch (classes) {
+        case 1: return f(integral_constant<int, 1>{});
+        case 2: return f(integral_constant<int, 2>{});
+        case 3: return f(integral_constant<int, 3>{});
+        case 4: return f(integral_constant<int, 4>{});
+        case 5: return f(integral_constant<int, 5>{});
+        case 6: return f(integral_constant<int, 6>{});
+        case 7: return f(integral_constant<int, 7>{});
+        default: return f(integral_constant<int, 8>{});
+    }
+}
 // f(lanes of a row, values of a lane), as constants
 template <typename F>
 void with_lanes(int classes, F f) {
     using std::integral_constant;
-    if (classes <= 2) f(integral_constant<int, 1>{}, integral_constant<int, 2>{});
-    else if (classes <= 4) f(integral_constant<int, 1>{}, integral_constant<int, 4>{});
-    else if (classes <= 8) f(integral_constant<int, 1>{}, integral_constant<int, 8>{});
-    else if (classes <= 16) f(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+    if (classes <= 16) f(integral_constant<int, 4>{}, integral_constant<int, 4>{});
     else if (classes <= 32) f(integral_constant<int, 8>{}, integral_constant<int, 4>{});
     else if (classes <= 128) f(integral_constant<int, 32>{}, integral_constant<int, 4>{});
     else if (classes <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
@@ -50,6 +63,11 @@ dim3 grid_of(int64_t blocks) {
 }
 bool starts_on_16(const void* p, int64_t stride, int32_t type) {
     return aligned(p, 16) && stride * static_cast<int64_t>(element_size(type)) % 16 == 0;
+}
+// whether loads of 8 or 16 bytes fit every row of a few classes
+bool starts_on_row(const void* x, int64_t stride, int classes, int32_t type) {
+    const int64_t size = static_cast<int64_t>(element_size(type)), to = classes * size == 8 ? 8 : 16;
+    return aligned(x, to) && stride * size % to == 0;
 }
 
 // Blocks of a cluster for one row: as many as keep the SMs busy with all rows' blocks, each with at least two pieces of 16 bytes a thread.
@@ -93,6 +111,12 @@ vm_status vm_scores(int device, const void* x, int32_t type, int64_t rows, int32
         with_values(type, flags, [&](auto kind, auto probabilities) {
             using T = decltype(kind);
             constexpr bool P = decltype(probabilities)::value;
+            if (classes <= MOST_OF_THREAD) {
+                with_classes(classes, [&](auto c) {
+                    launch_kernel(k_scores_own_row<T, P, decltype(c)::value>, grid_of((rows + ROW_BLOCK - 1) / ROW_BLOCK), ROW_BLOCK, 0, q, false, a, starts_on_row(x, row_stride, classes, type));
+                });
+                return;
+            }
             if (classes <= MOST_IN_ROWS) {
                 with_lanes(classes, [&](auto lanes, auto values) {
                     constexpr int G = decltype(lanes)::value, E = decltype(values)::value;
@@ -101,8 +125,13 @@ vm_status vm_scores(int device, const void* x, int32_t type, int64_t rows, int32
                 return;
             }
             const int blocks = blocks_of_row(rows, classes, type);
-            if (blocks > 1) launch_cluster(k_scores_stream<T, P, true>, grid_of(rows * blocks), blocks, q, a);
-            else launch_kernel(k_scores_stream<T, P, false>, grid_of(rows), STREAM_BLOCK, 0, q, false, a, 1);
+            const auto launch = [&](auto best) {
+                constexpr bool TOP = decltype(best)::value;
+                if (blocks > 1) launch_cluster(k_scores_stream<T, P, TOP, true>, grid_of(rows * blocks), blocks, q, a);
+                else launch_kernel(k_scores_stream<T, P, TOP, false>, grid_of(rows), STREAM_BLOCK, 0, q, false, a, 1);
+            };
+            if (top > 0) launch(std::true_type{});
+            else launch(std::false_type{});
         });
     }
     catch (const std::string& refused) {
@@ -132,12 +161,19 @@ vm_status vm_scores_backward(int device, const void* x, int32_t type, int64_t ro
         with_values(type, flags, [&](auto kind, auto probabilities) {
             using T = decltype(kind);
             constexpr bool P = decltype(probabilities)::value;
-            if (classes <= MOST_IN_ROWS) {
-                const bool wide  = starts_on_16(x, row_stride, type) && starts_on_16(dx, dx_row_stride, type);
+            if (classes <= MOST_OF_THREAD) {
                 const bool dense = dx_row_stride == classes && aligned(dx, 16);
+                with_classes(classes, [&](auto c) {
+                    launch_kernel(k_scores_grad_own_row<T, P, decltype(c)::value>, grid_of((rows + ROW_BLOCK - 1) / ROW_BLOCK), ROW_BLOCK, 0, q, false, a,
+                                  starts_on_row(x, row_stride, classes, type), dense);
+                });
+                return;
+            }
+            if (classes <= MOST_IN_ROWS) {
+                const bool wide = starts_on_16(x, row_stride, type) && starts_on_16(dx, dx_row_stride, type);
                 with_lanes(classes, [&](auto lanes, auto values) {
                     constexpr int G = decltype(lanes)::value, E = decltype(values)::value;
-                    launch_kernel(k_scores_grad_rows<T, P, G, E>, grid_of((rows * G + ROW_BLOCK - 1) / ROW_BLOCK), ROW_BLOCK, 0, q, false, a, wide, dense);
+                    launch_kernel(k_scores_grad_rows<T, P, G, E>, grid_of((rows * G + ROW_BLOCK - 1) / ROW_BLOCK), ROW_BLOCK, 0, q, false, a, wide);
                 });
                 return;
             }

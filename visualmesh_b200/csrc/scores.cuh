@@ -90,15 +90,6 @@ constexpr float NO_EXPONENT = -1000.0f;  // e^t is 0 there, and 0 times -infinit
 __device__ __forceinline__ float bounded(float t) {
     return fmaxf(t, NO_EXPONENT);
 }
-__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
-    const float m = fmaxf(a.m, b.m), da = bounded(a.m - m), db = bounded(b.m - m), fa = exp_of(da), fb = exp_of(db);
-    return Sums{m, fmaf(a.s, fa, b.s * fb), fmaf(fmaf(a.s, da, a.w), fa, fmaf(b.s, db, b.w) * fb)};
-}
-template <bool PROBABILITIES>
-__device__ __forceinline__ Sums joined_of(const Sums& a, const Sums& b) {
-    return PROBABILITIES ? Sums{0.0f, a.s + b.s, a.w + b.w} : joined(a, b);
-}
-
 // The results of a row from its sums; log p of one of its values.
 struct Row {
     float m, l, log_sum, entropy;
@@ -116,9 +107,7 @@ __device__ __forceinline__ Row row_of(const Sums& q) {
 }
 // log p = (v - m) - log s: from the difference, not from log_sum, whose rounding grows with m. A class that is masked (-infinity) stays
 // that in a row that has a distribution.
-template <bool PROBABILITIES>
-__device__ __forceinline__ float log_prob_of(float x, const Row& r) {
-    const float v = value_of<PROBABILITIES>(x);
+__device__ __forceinline__ float log_prob_of(float v, const Row& r) {
     return v == -INFINITY && r.l == r.l ? -INFINITY : (v - r.m) - r.l;
 }
 template <typename T, bool PROBABILITIES>
@@ -128,20 +117,113 @@ __device__ __forceinline__ void write_row(const ScoresArgs& a, int64_t row, cons
     if (a.log_prob != nullptr) {
         const int64_t label = label_of(a.labels, a.labels_64, row);
         float lp = 0.0f;
-        if (label != -1) lp = label < 0 || label >= a.classes ? NAN : log_prob_of<PROBABILITIES>(to_float(x[label]), r);
+        if (label != -1) lp = label < 0 || label >= a.classes ? NAN : log_prob_of(value_of<PROBABILITIES>(to_float(x[label])), r);
         a.log_prob[row] = lp;
     }
 }
 template <bool PROBABILITIES>
 __device__ __forceinline__ void write_top(const ScoresArgs& a, int64_t row, int k, uint32_t order, int32_t index, const Row& r) {
     a.top_index[row * a.top + k]    = index;
-    a.top_log_prob[row * a.top + k] = log_prob_of<PROBABILITIES>(value_of_order(order), r);
+    a.top_log_prob[row * a.top + k] = log_prob_of(value_of<PROBABILITIES>(value_of_order(order)), r);
+}
+
+constexpr int ROW_BLOCK = 256;
+
+// ---- up to 8 classes: a thread per row -----------------------------------------------------------------------------------------
+// C values in registers, every loop over them unrolled. Bound by instructions rather than bytes (48 bytes a row of three classes with
+// their two best are 2.1 cycles of an SM's share of the memory, 270 instructions of its lanes), so each logarithm is taken once, for the sum, the
+// label and the best classes alike.
+template <typename T, int C>
+__device__ __forceinline__ void load_row(const T* x, bool wide, float (&to)[C]) {
+    T e[C];
+    constexpr int BYTES = C * sizeof(T);
+    if constexpr (BYTES == 8 || BYTES % 16 == 0) {
+        if (wide) {
+            if constexpr (BYTES == 8) {
+                const uint2 raw = *reinterpret_cast<const uint2*>(x);
+                memcpy(e, &raw, 8);
+            }
+            else {
+#pragma unroll
+                for (int i = 0; i < BYTES / 16; ++i) {
+                    const uint4 raw = reinterpret_cast<const uint4*>(x)[i];
+                    memcpy(reinterpret_cast<unsigned char*>(e) + 16 * i, &raw, 16);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < C; ++k) to[k] = to_float(e[k]);
+            return;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < C; ++k) to[k] = to_float(x[k]);
+}
+
+template <typename T, bool PROBABILITIES, int C>
+__global__ void __launch_bounds__(ROW_BLOCK) k_scores_own_row(const ScoresArgs a, bool wide) {
+    const int row = blockIdx.x * ROW_BLOCK + threadIdx.x;  // rows < 2^31, and so are those of the last block
+    if (row >= a.rows) return;
+    float x[C], v[C];
+    load_row<T, C>(static_cast<const T*>(a.x) + row * a.row_stride, wide, x);
+    const int64_t label = a.log_prob != nullptr ? label_of(a.labels, a.labels_64, row) : -1;
+
+    Sums q{0.0f, 0.0f, 0.0f};
+    if constexpr (PROBABILITIES) {
+#pragma unroll
+        for (int k = 0; k < C; ++k) {
+            v[k] = logf(x[k]);
+            q.s += x[k];
+            q.w += x[k] == 0.0f ? 0.0f : SCALE * x[k] * v[k];
+        }
+    }
+    else {
+        q.m = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < C; ++k) v[k] = x[k], q.m = fmaxf(q.m, v[k]);
+        if (q.m == -INFINITY) q.m = 0.0f;  // then nothing is left, or only NaN
+#pragma unroll
+        for (int k = 0; k < C; ++k) {
+            const float t = v[k] - q.m, e = exp_of(t);
+            q.s += e;
+            q.w = fmaf(e, bounded(t), q.w);
+        }
+    }
+    const Row r = row_of<PROBABILITIES>(q);
+    if (a.log_sum != nullptr) a.log_sum[row] = r.log_sum;
+    if (a.entropy != nullptr) a.entropy[row] = r.entropy;
+#pragma unroll
+    for (int k = 0; k < C; ++k) v[k] = log_prob_of(v[k], r);
+    if (a.log_prob != nullptr) {
+        float lp = label == -1 ? 0.0f : NAN;
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+            if (label == k) lp = v[k];
+        a.log_prob[row] = lp;
+    }
+    if (a.top > 0) {
+        uint32_t order[C];  // 0: taken
+#pragma unroll
+        for (int k = 0; k < C; ++k) order[k] = order_of(x[k]);
+        float* const values = a.top_log_prob + static_cast<int64_t>(row) * a.top;
+        int32_t* const at   = a.top_index + static_cast<int64_t>(row) * a.top;
+        for (int n = 0; n < a.top; ++n) {
+            uint32_t best = order[0];
+            float lp      = v[0];
+            int index     = 0;
+#pragma unroll
+            for (int k = 1; k < C; ++k)
+                if (order[k] > best) best = order[k], lp = v[k], index = k;
+#pragma unroll
+            for (int k = 0; k < C; ++k)
+                if (index == k) order[k] = 0;
+            values[n] = lp;
+            at[n]     = index;
+        }
+    }
 }
 
 // ---- up to 1024 classes: G lanes per row, E values a lane in registers ---------------------------------------------------------
 // Lane l of a row has the values l, l + G, l + 2 G, ..., or (WIDE, G = 32, rows that begin on 16 bytes) the same with pieces of 16 bytes.
-constexpr int ROW_BLOCK = 256;
-
 template <typename T, int G, int E>
 struct RowLoad {
     static constexpr int PIECE = 16 / sizeof(T);
@@ -305,24 +387,38 @@ __device__ __forceinline__ void values_of(const uint4& raw, float (&to)[16 / siz
     for (int k = 0; k < 16 / static_cast<int>(sizeof(T)); ++k) to[k] = to_float(e[k]);
 }
 
-// The `top` largest of `n` different keys (0: none) in shared memory, in order, by one warp.
-__device__ __forceinline__ void largest_keys(const uint64_t* keys, int n, int top, uint64_t* into) {
+// The `top` largest of `n` different keys (0: none) in shared memory, in order, by one warp: every lane sorts its own, and the largest of their
+// first is taken away `top` times.
+template <int K>
+__device__ __forceinline__ void largest_of_lanes(const uint64_t* keys, int n, int top, uint64_t* into) {
     const int lane = threadIdx.x % WARP;
-    uint64_t held[CANDIDATES / WARP];
+    uint64_t held[K];
 #pragma unroll
-    for (int i = 0; i < CANDIDATES / WARP; ++i) held[i] = i * WARP + lane < n ? keys[i * WARP + lane] : 0;
-    for (int k = 0; k < top; ++k) {
-        uint64_t mine = 0;
+    for (int i = 0; i < K; ++i) held[i] = i * WARP + lane < n ? keys[i * WARP + lane] : 0;
 #pragma unroll
-        for (int i = 0; i < CANDIDATES / WARP; ++i) mine = held[i] > mine ? held[i] : mine;
-        const uint32_t high = __reduce_max_sync(~0u, static_cast<uint32_t>(mine >> 32));
-        const uint32_t low  = __reduce_max_sync(~0u, static_cast<uint32_t>(mine >> 32) == high ? static_cast<uint32_t>(mine) : 0);
-        const uint64_t best = static_cast<uint64_t>(high) << 32 | low;
+    for (int round = 0; round < K; ++round) {  // odd-even transposition
 #pragma unroll
-        for (int i = 0; i < CANDIDATES / WARP; ++i)
-            if (held[i] == best) held[i] = 0;
-        if (lane == 0) into[k] = best;
+        for (int i = round % 2; i + 1 < K; i += 2) {
+            const uint64_t x = held[i], y = held[i + 1];
+            held[i]     = x > y ? x : y;
+            held[i + 1] = x > y ? y : x;
+        }
     }
+    for (int k = 0; k < top; ++k) {
+        const uint32_t high = __reduce_max_sync(~0u, static_cast<uint32_t>(held[0] >> 32));
+        const bool equal    = static_cast<uint32_t>(held[0] >> 32) == high;
+        const uint32_t low  = __reduce_max_sync(~0u, equal ? static_cast<uint32_t>(held[0]) : 0);
+        if (equal && static_cast<uint32_t>(held[0]) == low) {
+            into[k] = held[0];
+#pragma unroll
+            for (int i = 0; i + 1 < K; ++i) held[i] = held[i + 1];
+            held[K - 1] = 0;
+        }
+    }
+}
+__device__ __forceinline__ void largest_keys(const uint64_t* keys, int n, int top, uint64_t* into) {
+    if (n <= WARP) largest_of_lanes<1>(keys, n, top, into);
+    else largest_of_lanes<CANDIDATES / WARP>(keys, n, top, into);
 }
 
 struct StreamShared {
@@ -337,7 +433,70 @@ struct StreamShared {
 };
 static_assert(STREAM_BLOCK <= CANDIDATES, "the threads' maxima are chosen from as candidates are");
 
-template <typename T, bool PROBABILITIES, bool CLUSTER>
+// The sums of long rows of logits are kept in powers of two, for pairs of values: with M = m L, L = log2 e in 32 bits, t_j = x_j L - M (one rounding
+// for a pair), s = sum 2^t_j and w = sum 2^t_j t_j. What rounding m L to M moved, rho = m L - M, is put right in the row's results:
+// log sum e^(x_j - m) = log s - rho log 2. Values are not let below LOW, where 2^t is 0 in every row but one whose maximum is not ABOVE it;
+// START is where maxima begin. Such a row (all masked by infinities or by the type's lowest value) and one beyond BELOW are summed again in the way of the short rows.
+constexpr float LOG2_E = 1.44269504f, LOG_2 = 0.693147181f;
+template <typename T>
+struct Range {
+    static constexpr float LOW = -1e38f, START = -7e37f, ABOVE = -1e37f, BELOW = 1e37f;
+};
+template <>
+struct Range<__half> {
+    static constexpr float LOW = -65504.0f, START = LOW, ABOVE = -64000.0f, BELOW = 1e37f;
+};
+__device__ __forceinline__ Sums joined_by_two(const Sums& a, const Sums& b) {
+    const float m = fmaxf(a.m, b.m), da = a.m * LOG2_E - m * LOG2_E, db = b.m * LOG2_E - m * LOG2_E, fa = exp2_of(da), fb = exp2_of(db);
+    return Sums{m, fmaf(a.s, fa, b.s * fb), fmaf(fmaf(a.s, da, a.w), fa, fmaf(b.s, db, b.w) * fb)};
+}
+template <bool PROBABILITIES>
+__device__ __forceinline__ Sums joined_stream(const Sums& a, const Sums& b) {
+    return PROBABILITIES ? Sums{0.0f, a.s + b.s, a.w + b.w} : joined_by_two(a, b);
+}
+__device__ __forceinline__ Row row_by_two(const Sums& q) {
+    if (!(q.s < INFINITY) || q.w != q.w) return Row{NAN, NAN, NAN, NAN};
+    const float rho = fmaf(q.m, LOG2_E, -(q.m * LOG2_E)), l = logf(q.s) - rho * LOG_2;
+    return Row{q.m, l, q.m + l, l - (__fdividef(q.w, q.s) - rho) * LOG_2};
+}
+
+// Sums of a block's threads, for all of them. Between two uses of `warps` comes a barrier.
+template <typename Join>
+__device__ __forceinline__ Sums joined_block(Sums q, Sums* warps, Join join) {
+    over_lanes<WARP>([&](int d) { q = join(q, Sums{__shfl_xor_sync(~0u, q.m, d), __shfl_xor_sync(~0u, q.s, d), __shfl_xor_sync(~0u, q.w, d)}); });
+    if (threadIdx.x % WARP == 0) warps[threadIdx.x / WARP] = q;
+    __syncthreads();
+    q = warps[0];
+#pragma unroll
+    for (int w = 1; w < STREAM_BLOCK / WARP; ++w) q = join(q, warps[w]);
+    return q;
+}
+
+// A row of logits in the way of the short rows: first its maximum, then its sums.
+template <typename T>
+__device__ __noinline__ Row row_again(const Pieces<T>& pieces, Sums* warps) {
+    constexpr int N = Pieces<T>::N;
+    const auto over = [&](auto f) {
+        for (int64_t p = threadIdx.x; p < pieces.count; p += STREAM_BLOCK) {
+            float v[N];
+            values_of<T>(pieces.load(p, from_float<T>(-INFINITY)), v);
+            for (int k = 0; k < N; ++k) f(v[k]);
+        }
+        __syncthreads();
+    };
+    float m = -INFINITY;
+    over([&](float v) { m = fmaxf(m, v); });
+    m = joined_block(Sums{m, 0.0f, 0.0f}, warps, [](const Sums& a, const Sums& b) { return Sums{fmaxf(a.m, b.m), 0.0f, 0.0f}; }).m;
+    Sums q{m == -INFINITY ? 0.0f : m, 0.0f, 0.0f};  // nothing is left: any number will do
+    over([&](float v) {
+        const float t = v - q.m, e = exp_of(t);
+        q.s += e;
+        q.w = fmaf(e, bounded(t), q.w);
+    });
+    return row_of<false>(joined_block(q, warps, [](const Sums& a, const Sums& b) { return Sums{a.m, a.s + b.s, a.w + b.w}; }));
+}
+
+template <typename T, bool PROBABILITIES, bool TOP, bool CLUSTER>
 __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs a, int blocks) {
     namespace cg = cooperative_groups;
     __shared__ StreamShared shared;
@@ -351,57 +510,71 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs
     const int64_t begin = rank * share, end = begin + share < pieces.count ? begin + share : pieces.count;
     const T outside     = from_float<T>(PROBABILITIES ? 0.0f : -INFINITY);
 
-    Sums q{PROBABILITIES ? 0.0f : -3.402823466e38f, 0.0f, 0.0f};  // a finite maximum, below or at every value that counts
-    float best   = PROBABILITIES ? -1.0f : -INFINITY;
-    int64_t held = begin + threadIdx.x;  // the piece with the maximum
+    Sums q{PROBABILITIES ? 0.0f : Range<T>::START, 0.0f, 0.0f};
+    float best = PROBABILITIES ? -1.0f : -INFINITY;
+    int held   = static_cast<int>(begin) + threadIdx.x;  // the piece with the maximum
+    float2 s2 = make_float2(0.0f, 0.0f), w2 = s2;
     for (int64_t p = begin + threadIdx.x; p < end; p += STREAM_BLOCK * STREAM_AHEAD) {
-        uint4 raw[STREAM_AHEAD];
-#pragma unroll
-        for (int u = 0; u < STREAM_AHEAD; ++u)
-            if (p + u * STREAM_BLOCK < end) raw[u] = pieces.load(p + u * STREAM_BLOCK, outside);
+        using P2 = Pair<T>;
+        typename P2::type v[STREAM_AHEAD][N / 2];
 #pragma unroll
         for (int u = 0; u < STREAM_AHEAD; ++u) {
-            if (p + u * STREAM_BLOCK >= end) break;
-            float v[N];
-            values_of<T>(raw[u], v);
-            float top = v[0];
+            uint4 raw;
+            if (p + u * STREAM_BLOCK < end) raw = pieces.load(p + u * STREAM_BLOCK, outside);
+            else {
+                T e[N];
 #pragma unroll
-            for (int k = 1; k < N; ++k) top = fmaxf(top, v[k]);
-            if (top > best) best = top, held = p + u * STREAM_BLOCK;
-            if constexpr (PROBABILITIES) {
+                for (int k = 0; k < N; ++k) e[k] = outside;
+                memcpy(&raw, e, 16);
+            }
+            memcpy(v[u], &raw, 16);
+        }
+        float most = -INFINITY;
 #pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    q.s += v[k];
-                    q.w += times_log(v[k]);
+        for (int u = 0; u < STREAM_AHEAD; ++u) {
+            typename P2::type larger = v[u][0];
+#pragma unroll
+            for (int k = 1; k < N / 2; ++k) larger = P2::larger(larger, v[u][k]);
+            const float2 f  = P2::floats(larger);
+            const float top = fmaxf(f.x, f.y);
+            if (TOP && top > best) best = top, held = static_cast<int>(p) + u * STREAM_BLOCK;
+            most = fmaxf(most, top);
+        }
+        if constexpr (PROBABILITIES) {
+#pragma unroll
+            for (int u = 0; u < STREAM_AHEAD; ++u) {
+#pragma unroll
+                for (int k = 0; k < N / 2; ++k) {
+                    const float2 f = P2::floats(v[u][k]);
+                    q.s += f.x + f.y;
+                    q.w += times_log(f.x) + times_log(f.y);
                 }
             }
-            else {
-                const float m = fmaxf(q.m, top), d = bounded(q.m - m), f = exp_of(d);
-                q.w = fmaf(q.s, d, q.w) * f;
-                q.s *= f;
-                q.m = m;
+        }
+        else {
+            const float m = fmaxf(q.m, most), M = m * LOG2_E, d = q.m * LOG2_E - M, f = exp2_of(d);
+            w2  = mul2(fma2(s2, make_float2(d, d), w2), make_float2(f, f));
+            s2  = mul2(s2, make_float2(f, f));
+            q.m = m;
+            const auto low = P2::both(Range<T>::LOW);
 #pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    const float t = v[k] - m, e = exp_of(t);
-                    q.s += e;
-                    q.w = fmaf(e, bounded(t), q.w);
+            for (int u = 0; u < STREAM_AHEAD; ++u) {
+#pragma unroll
+                for (int k = 0; k < N / 2; ++k) {
+                    const float2 t = fma2(P2::floats(P2::bounded(v[u][k], low)), make_float2(LOG2_E, LOG2_E), make_float2(-M, -M));
+                    const float2 e = make_float2(exp2_of(t.x), exp2_of(t.y));
+                    s2 = add2(s2, e);
+                    w2 = fma2(e, t, w2);
                 }
             }
         }
     }
-    over_lanes<WARP>([&](int d) {
-        const Sums o{__shfl_xor_sync(~0u, q.m, d), __shfl_xor_sync(~0u, q.s, d), __shfl_xor_sync(~0u, q.w, d)};
-        q = joined_of<PROBABILITIES>(q, o);
-    });
-    if (lane == 0) shared.warps[warp] = q;
+    if constexpr (!PROBABILITIES) q.s = s2.x + s2.y, q.w = w2.x + w2.y;
     if (threadIdx.x == 0) shared.found = 0;
-    if (a.top > 0) shared.keys[threadIdx.x] = begin + threadIdx.x < end ? static_cast<uint64_t>(order_of(best)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(held)) : 0;
-    __syncthreads();
-    q = shared.warps[0];
-#pragma unroll
-    for (int w = 1; w < STREAM_BLOCK / WARP; ++w) q = joined_of<PROBABILITIES>(q, shared.warps[w]);
+    if (TOP) shared.keys[threadIdx.x] = begin + threadIdx.x < end ? static_cast<uint64_t>(order_of(best)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(held)) : 0;
+    q = joined_block(q, shared.warps, joined_stream<PROBABILITIES>);
 
-    if (a.top > 0) {
+    if constexpr (TOP) {
         if (warp == 0) largest_keys(shared.keys, STREAM_BLOCK, a.top, shared.best);
         __syncthreads();
         const uint64_t least = shared.best[a.top - 1];
@@ -463,18 +636,20 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs
         cluster.sync();  // the first block runs
         StreamShared* first = cluster.map_shared_rank(&shared, 0);
         if (threadIdx.x == 0) first->sums[rank] = q;
-        if (threadIdx.x < a.top) first->bests[rank * a.top + threadIdx.x] = shared.best[threadIdx.x];
+        if (TOP && threadIdx.x < a.top) first->bests[rank * a.top + threadIdx.x] = shared.best[threadIdx.x];
         cluster.sync();
         if (rank != 0) return;
         q = shared.sums[0];
-        for (int b = 1; b < blocks; ++b) q = joined_of<PROBABILITIES>(q, shared.sums[b]);
-        if (a.top > 0 && warp == 0) largest_keys(shared.bests, blocks * a.top, a.top, shared.best);
+        for (int b = 1; b < blocks; ++b) q = joined_stream<PROBABILITIES>(q, shared.sums[b]);
+        if (TOP && warp == 0) largest_keys(shared.bests, blocks * a.top, a.top, shared.best);
     }
+    Row r;
+    if constexpr (PROBABILITIES) r = row_of<true>(q);
+    else r = !(q.m > Range<T>::ABOVE && q.m < Range<T>::BELOW) ? row_again<T>(pieces, shared.warps) : row_by_two(q);
     if (warp != 0) return;
     __syncwarp();
-    const Row r = row_of<PROBABILITIES>(q);
     if (lane == 0) write_row<T, PROBABILITIES>(a, row, x, r);
-    if (lane < a.top) write_top<PROBABILITIES>(a, row, lane, static_cast<uint32_t>(shared.best[lane] >> 32), index_of_key(shared.best[lane]), r);
+    if (TOP && lane < a.top) write_top<PROBABILITIES>(a, row, lane, static_cast<uint32_t>(shared.best[lane] >> 32), index_of_key(shared.best[lane]), r);
 }
 
 // ---- gradients -----------------------------------------------------------------------------------------------------------------
@@ -482,11 +657,13 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs
 template <bool PROBABILITIES>
 struct RowGrad {
     float log_sum, d_label, d_entropy, offset, one_over_sum;
-    int64_t label;
-    __device__ __forceinline__ RowGrad(const ScoresGradArgs& a, int64_t row) : log_sum(a.log_sum[row]), d_label(0.0f), label(-1) {
+    int label_at;  // -1: nowhere
+    __device__ __forceinline__ RowGrad(const ScoresGradArgs& a, int64_t row) : log_sum(a.log_sum[row]), d_label(0.0f), label_at(-1) {
         if (a.d_log_prob != nullptr) {
-            label = label_of(a.labels, a.labels_64, row);
-            if (label != -1) d_label = label < 0 || label >= a.classes ? NAN : a.d_log_prob[row];
+            const int64_t label = label_of(a.labels, a.labels_64, row);
+            const bool inside   = label >= 0 && label < a.classes;
+            if (inside) label_at = static_cast<int>(label);
+            if (label != -1) d_label = inside ? a.d_log_prob[row] : NAN;
         }
         d_entropy = a.d_entropy != nullptr ? a.d_entropy[row] : 0.0f;
         offset    = (a.d_log_sum != nullptr ? a.d_log_sum[row] : 0.0f) - d_label - (a.d_entropy != nullptr ? d_entropy * a.entropy[row] : 0.0f);
@@ -503,77 +680,90 @@ struct RowGrad {
             const float d  = fmaf(-d_entropy, lp, offset);
             to[k]          = PROBABILITIES ? (v == -INFINITY ? 0.0f : d * one_over_sum) : d * exp_of(lp);
         }
-        if (offset != offset || (label >= j && label < j + N)) {  // the row's label is one of these, or the row has no distribution
+        if (!(fabsf(offset) < INFINITY) || (label_at >= j && label_at < j + N)) {  // the row's label is one of these, or the row has no distribution
 #pragma unroll
             for (int k = 0; k < N; ++k) {
-                if (j + k == label) to[k] += PROBABILITIES ? d_label / x[k] : d_label;
+                if (j + k == label_at) to[k] += label_gradient(x[k]);
                 if (x[k] == (PROBABILITIES ? 0.0f : -INFINITY)) to[k] = 0.0f;
             }
         }
     }
+    // what the label's own class gets besides
+    __device__ __forceinline__ float label_gradient(float x) const {
+        return PROBABILITIES ? d_label / x : x == -INFINITY ? 0.0f : d_label;
+    }
 };
 
-// Rows of up to 1024 classes as above. Where a thread has a whole row, its results go through shared memory, so that a block writes
-// its rows, which lie side by side, in one piece.
-template <typename T, bool PROBABILITIES, int G, int E>
-__global__ void __launch_bounds__(ROW_BLOCK) k_scores_grad_rows(const ScoresGradArgs a, bool wide, bool dense) {
-    __shared__ alignas(16) unsigned char staged[G == 1 ? ROW_BLOCK * E * sizeof(T) : 16];
-    const int64_t row = (static_cast<int64_t>(blockIdx.x) * ROW_BLOCK + threadIdx.x) / G;
-    const int lane    = threadIdx.x % G;
-    if (G > 1 && row >= a.rows) return;
+// Up to 8 classes: a thread per row. The results go through shared memory, so that a block writes its rows, which lie side by side (dense),
+// in one piece.
+template <typename T, bool PROBABILITIES, int C>
+__global__ void __launch_bounds__(ROW_BLOCK) k_scores_grad_own_row(const ScoresGradArgs a, bool wide, bool dense) {
+    __shared__ alignas(16) T staged[ROW_BLOCK * C];
+    const int first = blockIdx.x * ROW_BLOCK, row = first + threadIdx.x;
     if (row < a.rows) {
-        const T* from = static_cast<const T*>(a.x) + row * a.row_stride;
-        T* dx         = static_cast<T*>(a.dx) + row * a.dx_row_stride;
-        using Load = RowLoad<T, G, E>;
-        float v[E];
-        Load::load(from, a.classes, wide, lane, v);
-        const RowGrad<PROBABILITIES> grad(a, row);
-        if constexpr (Load::MAY) {
-            if (wide) {
+        float x[C], d[C];
+        load_row<T, C>(static_cast<const T*>(a.x) + row * a.row_stride, wide, x);
+        RowGrad<PROBABILITIES>(a, row).of(x, 0, d);
+        T* const dx = dense ? staged + threadIdx.x * C : static_cast<T*>(a.dx) + row * a.dx_row_stride;
 #pragma unroll
-                for (int i = 0; i < E; i += Load::PIECE) {
-                    const int j = Load::index(true, lane, i);
-                    float x[Load::PIECE], d[Load::PIECE];
-                    T e[Load::PIECE];
-#pragma unroll
-                    for (int k = 0; k < Load::PIECE; ++k) x[k] = v[i + k];
-                    grad.of(x, j, d);
-#pragma unroll
-                    for (int k = 0; k < Load::PIECE; ++k) e[k] = from_float<T>(d[k]);
-                    if (j + Load::PIECE <= a.classes) {
-                        uint4 raw;
-                        memcpy(&raw, e, 16);
-                        *reinterpret_cast<uint4*>(dx + j) = raw;
-                    }
-                    else {
-#pragma unroll
-                        for (int k = 0; k < Load::PIECE; ++k)
-                            if (j + k < a.classes) dx[j + k] = e[k];
-                    }
-                }
-                return;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int j = i * G + lane;
-            if (j < a.classes) {
-                const float x[1] = {v[i]};
-                float d[1];
-                grad.of(x, j, d);
-                if (G == 1 && dense) reinterpret_cast<T*>(staged)[threadIdx.x * a.classes + j] = from_float<T>(d[0]);
-                else dx[j] = from_float<T>(d[0]);
-            }
-        }
+        for (int k = 0; k < C; ++k) dx[k] = from_float<T>(d[k]);
     }
-    if (G == 1 && dense) {
+    if (dense) {
         __syncthreads();
-        const int64_t first = static_cast<int64_t>(blockIdx.x) * ROW_BLOCK;
-        const int values    = static_cast<int>(a.rows - first < ROW_BLOCK ? a.rows - first : ROW_BLOCK) * a.classes;
-        T* to               = static_cast<T*>(a.dx) + first * a.classes;
+        const int values    = static_cast<int>(a.rows - first < ROW_BLOCK ? a.rows - first : ROW_BLOCK) * C;
+        T* const to         = static_cast<T*>(a.dx) + static_cast<int64_t>(first) * C;
         constexpr int PIECE = 16 / sizeof(T);
         for (int i = threadIdx.x; i < values / PIECE; i += ROW_BLOCK) reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(staged)[i];
-        for (int i = values / PIECE * PIECE + threadIdx.x; i < values; i += ROW_BLOCK) to[i] = reinterpret_cast<const T*>(staged)[i];
+        for (int i = values / PIECE * PIECE + threadIdx.x; i < values; i += ROW_BLOCK) to[i] = staged[i];
+    }
+}
+
+// Up to 1024 classes, G lanes per row as above.
+template <typename T, bool PROBABILITIES, int G, int E>
+__global__ void __launch_bounds__(ROW_BLOCK) k_scores_grad_rows(const ScoresGradArgs a, bool wide) {
+    const int64_t row = (static_cast<int64_t>(blockIdx.x) * ROW_BLOCK + threadIdx.x) / G;
+    const int lane    = threadIdx.x % G;
+    if (row >= a.rows) return;
+    T* dx      = static_cast<T*>(a.dx) + row * a.dx_row_stride;
+    using Load = RowLoad<T, G, E>;
+    float v[E];
+    Load::load(static_cast<const T*>(a.x) + row * a.row_stride, a.classes, wide, lane, v);
+    const RowGrad<PROBABILITIES> grad(a, row);
+    if constexpr (Load::MAY) {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < E; i += Load::PIECE) {
+                const int j = Load::index(true, lane, i);
+                float x[Load::PIECE], d[Load::PIECE];
+                T e[Load::PIECE];
+#pragma unroll
+                for (int k = 0; k < Load::PIECE; ++k) x[k] = v[i + k];
+                grad.of(x, j, d);
+#pragma unroll
+                for (int k = 0; k < Load::PIECE; ++k) e[k] = from_float<T>(d[k]);
+                if (j + Load::PIECE <= a.classes) {
+                    uint4 raw;
+                    memcpy(&raw, e, 16);
+                    *reinterpret_cast<uint4*>(dx + j) = raw;
+                }
+                else {
+#pragma unroll
+                    for (int k = 0; k < Load::PIECE; ++k)
+                        if (j + k < a.classes) dx[j + k] = e[k];
+                }
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int j = i * G + lane;
+        if (j < a.classes) {
+            const float x[1] = {v[i]};
+            float d[1];
+            grad.of(x, j, d);
+            dx[j] = from_float<T>(d[0]);
+        }
     }
 }
 
@@ -594,17 +784,38 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_grad_stream(const Score
     for (int u = 0; u < STREAM_AHEAD; ++u)
         if (begin + u * STREAM_BLOCK < pieces.count) raw[u] = pieces.load(begin + u * STREAM_BLOCK, outside);
     const RowGrad<PROBABILITIES> grad(a, row);
+    // Logits, in powers of two and by pairs as above: with t = x L - S, S = log_sum L and rho = log_sum L - S, p = 2^(t + rho), so that the factor 2^rho
+    // joins those of the row. Values are not let below log_sum - 1000 (p is 0 there), which has to be a number of the type.
+    const float S = grad.log_sum * LOG2_E, back = exp2_of(-fmaf(grad.log_sum, LOG2_E, -S));
+    const float slope = -grad.d_entropy * LOG_2 * back, level = grad.offset * back;
+    const bool quick  = !PROBABILITIES && grad.log_sum > Range<T>::ABOVE + 2000.0f && grad.log_sum < Range<T>::BELOW && fabsf(grad.offset) < INFINITY;
+    const auto low    = Pair<T>::both(grad.log_sum - 1000.0f);
 #pragma unroll
     for (int u = 0; u < STREAM_AHEAD; ++u) {
         const int64_t p = begin + u * STREAM_BLOCK;
         if (p >= pieces.count) break;
         const int64_t j = pieces.first(p);
-        float v[N], d[N];
         T e[N];
-        values_of<T>(raw[u], v);
-        grad.of(v, j, d);
+        if (quick) {
+            typename Pair<T>::type v[N / 2];
+            memcpy(v, &raw[u], 16);
 #pragma unroll
-        for (int k = 0; k < N; ++k) e[k] = from_float<T>(d[k]);
+            for (int k = 0; k < N / 2; ++k) {
+                const float2 t = fma2(Pair<T>::floats(Pair<T>::bounded(v[k], low)), make_float2(LOG2_E, LOG2_E), make_float2(-S, -S));
+                float2 d       = mul2(fma2(t, make_float2(slope, slope), make_float2(level, level)), make_float2(exp2_of(t.x), exp2_of(t.y)));
+                const int i    = grad.label_at - static_cast<int>(j) - 2 * k;
+                if (i == 0) d.x += grad.label_gradient(to_float(v[k].x));
+                if (i == 1) d.y += grad.label_gradient(to_float(v[k].y));
+                e[2 * k] = from_float<T>(d.x), e[2 * k + 1] = from_float<T>(d.y);
+            }
+        }
+        else {
+            float v[N], d[N];
+            values_of<T>(raw[u], v);
+            grad.of(v, j, d);
+#pragma unroll
+            for (int k = 0; k < N; ++k) e[k] = from_float<T>(d[k]);
+        }
         if (together && j >= 0 && j + N <= a.classes) {
             uint4 out;
             memcpy(&out, e, 16);
