@@ -90,6 +90,11 @@ constexpr float NO_EXPONENT = -1000.0f;  // e^t is 0 there, and 0 times -infinit
 __device__ __forceinline__ float bounded(float t) {
     return fmaxf(t, NO_EXPONENT);
 }
+__device__ __forceinline__ float bounded_or_nan(float t) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(t), "f"(NO_EXPONENT));
+    return r;
+}
 // The results of a row from its sums; log p of one of its values.
 struct Row {
     float m, l, log_sum, entropy;
@@ -105,10 +110,10 @@ __device__ __forceinline__ Row row_of(const Sums& q) {
     }
     return r;
 }
-// log p = (v - m) - log s: from the difference, not from log_sum, whose rounding grows with m. A class that is masked (-infinity) stays
-// that in a row that has a distribution.
+// log p = (v - m) - log s: from the difference, not from log_sum, whose rounding grows with m. m is finite in a row that has a distribution,
+// so a class that is masked (-infinity) stays that.
 __device__ __forceinline__ float log_prob_of(float v, const Row& r) {
-    return v == -INFINITY && r.l == r.l ? -INFINITY : (v - r.m) - r.l;
+    return (v - r.m) - r.l;
 }
 template <typename T, bool PROBABILITIES>
 __device__ __forceinline__ void write_row(const ScoresArgs& a, int64_t row, const T* x, const Row& r) {
@@ -166,6 +171,7 @@ __global__ void __launch_bounds__(ROW_BLOCK) k_scores_own_row(const ScoresArgs a
     float x[C], v[C];
     load_row<T, C>(static_cast<const T*>(a.x) + row * a.row_stride, wide, x);
     const int64_t label = a.log_prob != nullptr ? label_of(a.labels, a.labels_64, row) : -1;
+    const int labelled  = label >= 0 && label < C ? static_cast<int>(label) : label == -1 ? -1 : -2;
 
     Sums q{0.0f, 0.0f, 0.0f};
     if constexpr (PROBABILITIES) {
@@ -173,7 +179,7 @@ __global__ void __launch_bounds__(ROW_BLOCK) k_scores_own_row(const ScoresArgs a
         for (int k = 0; k < C; ++k) {
             v[k] = logf(x[k]);
             q.s += x[k];
-            q.w += x[k] == 0.0f ? 0.0f : SCALE * x[k] * v[k];
+            q.w = fmaf(SCALE * x[k], bounded_or_nan(v[k]), q.w);
         }
     }
     else {
@@ -194,16 +200,22 @@ __global__ void __launch_bounds__(ROW_BLOCK) k_scores_own_row(const ScoresArgs a
 #pragma unroll
     for (int k = 0; k < C; ++k) v[k] = log_prob_of(v[k], r);
     if (a.log_prob != nullptr) {
-        float lp = label == -1 ? 0.0f : NAN;
+        float lp = labelled == -1 ? 0.0f : NAN;
 #pragma unroll
         for (int k = 0; k < C; ++k)
-            if (label == k) lp = v[k];
+            if (labelled == k) lp = v[k];
         a.log_prob[row] = lp;
     }
     if (a.top > 0) {
         uint32_t order[C];  // 0: taken
+        if (PROBABILITIES && r.l == r.l) {
 #pragma unroll
-        for (int k = 0; k < C; ++k) order[k] = order_of(x[k]);
+            for (int k = 0; k < C; ++k) order[k] = __float_as_uint(x[k] + 0.0f) + 1;  // no negative ones in a row that has a distribution
+        }
+        else {
+#pragma unroll
+            for (int k = 0; k < C; ++k) order[k] = order_of(x[k]);
+        }
         float* const values = a.top_log_prob + static_cast<int64_t>(row) * a.top;
         int32_t* const at   = a.top_index + static_cast<int64_t>(row) * a.top;
         for (int n = 0; n < a.top; ++n) {
@@ -395,13 +407,14 @@ __device__ __forceinline__ void largest_of_lanes(const uint64_t* keys, int n, in
     uint64_t held[K];
 #pragma unroll
     for (int i = 0; i < K; ++i) held[i] = i * WARP + lane < n ? keys[i * WARP + lane] : 0;
+    if constexpr (K > 1) {  // Batcher's merge sort of eight
+        static_assert(K == 8, "the pairs below sort eight");
+        constexpr int PAIRS[19][2] = {{0, 1}, {2, 3}, {4, 5}, {6, 7}, {0, 2}, {1, 3}, {4, 6}, {5, 7}, {1, 2}, {5, 6}, {0, 4}, {1, 5}, {2, 6}, {3, 7}, {2, 4}, {3, 5}, {1, 2}, {3, 4}, {5, 6}};
 #pragma unroll
-    for (int round = 0; round < K; ++round) {  // odd-even transposition
-#pragma unroll
-        for (int i = round % 2; i + 1 < K; i += 2) {
-            const uint64_t x = held[i], y = held[i + 1];
-            held[i]     = x > y ? x : y;
-            held[i + 1] = x > y ? y : x;
+        for (int i = 0; i < 19; ++i) {
+            const uint64_t x = held[PAIRS[i][0]], y = held[PAIRS[i][1]];
+            held[PAIRS[i][0]] = x > y ? x : y;
+            held[PAIRS[i][1]] = x > y ? y : x;
         }
     }
     for (int k = 0; k < top; ++k) {
@@ -460,40 +473,34 @@ __device__ __forceinline__ Row row_by_two(const Sums& q) {
     return Row{q.m, l, q.m + l, l - (__fdividef(q.w, q.s) - rho) * LOG_2};
 }
 
-// Sums of a block's threads, for all of them. Between two uses of `warps` comes a barrier.
-template <typename Join>
-__device__ __forceinline__ Sums joined_block(Sums q, Sums* warps, Join join) {
-    over_lanes<WARP>([&](int d) { q = join(q, Sums{__shfl_xor_sync(~0u, q.m, d), __shfl_xor_sync(~0u, q.s, d), __shfl_xor_sync(~0u, q.w, d)}); });
-    if (threadIdx.x % WARP == 0) warps[threadIdx.x / WARP] = q;
-    __syncthreads();
-    q = warps[0];
-#pragma unroll
-    for (int w = 1; w < STREAM_BLOCK / WARP; ++w) q = join(q, warps[w]);
+// Of a warp's lanes, for all of them.
+template <int LANES, typename Join>
+__device__ __forceinline__ Sums joined_lanes(Sums q, Join join) {
+    over_lanes<LANES>([&](int d) { q = join(q, Sums{__shfl_xor_sync(~0u, q.m, d), __shfl_xor_sync(~0u, q.s, d), __shfl_xor_sync(~0u, q.w, d)}); });
     return q;
 }
 
-// A row of logits in the way of the short rows: first its maximum, then its sums.
+// A row of logits in the way of the short rows, by one warp: first its maximum, then its sums.
 template <typename T>
-__device__ __noinline__ Row row_again(const Pieces<T>& pieces, Sums* warps) {
+__device__ __noinline__ Row row_again(const Pieces<T>& pieces) {
     constexpr int N = Pieces<T>::N;
     const auto over = [&](auto f) {
-        for (int64_t p = threadIdx.x; p < pieces.count; p += STREAM_BLOCK) {
+        for (int64_t p = threadIdx.x % WARP; p < pieces.count; p += WARP) {
             float v[N];
             values_of<T>(pieces.load(p, from_float<T>(-INFINITY)), v);
             for (int k = 0; k < N; ++k) f(v[k]);
         }
-        __syncthreads();
     };
     float m = -INFINITY;
     over([&](float v) { m = fmaxf(m, v); });
-    m = joined_block(Sums{m, 0.0f, 0.0f}, warps, [](const Sums& a, const Sums& b) { return Sums{fmaxf(a.m, b.m), 0.0f, 0.0f}; }).m;
+    m = joined_lanes<WARP>(Sums{m, 0.0f, 0.0f}, [](const Sums& a, const Sums& b) { return Sums{fmaxf(a.m, b.m), 0.0f, 0.0f}; }).m;
     Sums q{m == -INFINITY ? 0.0f : m, 0.0f, 0.0f};  // nothing is left: any number will do
     over([&](float v) {
         const float t = v - q.m, e = exp_of(t);
         q.s += e;
         q.w = fmaf(e, bounded(t), q.w);
     });
-    return row_of<false>(joined_block(q, warps, [](const Sums& a, const Sums& b) { return Sums{a.m, a.s + b.s, a.w + b.w}; }));
+    return row_of<false>(joined_lanes<WARP>(q, [](const Sums& a, const Sums& b) { return Sums{a.m, a.s + b.s, a.w + b.w}; }));
 }
 
 template <typename T, bool PROBABILITIES, bool TOP, bool CLUSTER>
@@ -570,15 +577,18 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs
         }
     }
     if constexpr (!PROBABILITIES) q.s = s2.x + s2.y, q.w = w2.x + w2.y;
-    if (threadIdx.x == 0) shared.found = 0;
+    if (TOP && threadIdx.x == 0) shared.found = 0;
     if (TOP) shared.keys[threadIdx.x] = begin + threadIdx.x < end ? static_cast<uint64_t>(order_of(best)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(held)) : 0;
-    q = joined_block(q, shared.warps, joined_stream<PROBABILITIES>);
+    q = joined_lanes<WARP>(q, joined_stream<PROBABILITIES>);
+    if (lane == 0) shared.warps[warp] = q;
+    bool search = __syncthreads_or(q.s != q.s || q.w != q.w);  // NaN, or an infinity: its maxima were no maxima
+    if (!TOP && !CLUSTER && warp != 0) return;
+    q = joined_lanes<STREAM_BLOCK / WARP>(shared.warps[lane % (STREAM_BLOCK / WARP)], joined_stream<PROBABILITIES>);
 
     if constexpr (TOP) {
         if (warp == 0) largest_keys(shared.keys, STREAM_BLOCK, a.top, shared.best);
         __syncthreads();
         const uint64_t least = shared.best[a.top - 1];
-        bool search          = q.s != q.s || q.w != q.w;
         if (!search) {
             const uint32_t least_order  = static_cast<uint32_t>(least >> 32);
             const int64_t least_piece   = 0xFFFFFFFFu - static_cast<uint32_t>(least);
@@ -643,11 +653,11 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs
         for (int b = 1; b < blocks; ++b) q = joined_stream<PROBABILITIES>(q, shared.sums[b]);
         if (TOP && warp == 0) largest_keys(shared.bests, blocks * a.top, a.top, shared.best);
     }
-    Row r;
-    if constexpr (PROBABILITIES) r = row_of<true>(q);
-    else r = !(q.m > Range<T>::ABOVE && q.m < Range<T>::BELOW) ? row_again<T>(pieces, shared.warps) : row_by_two(q);
     if (warp != 0) return;
     __syncwarp();
+    Row r;
+    if constexpr (PROBABILITIES) r = row_of<true>(q);
+    else r = !(q.m > Range<T>::ABOVE && q.m < Range<T>::BELOW) ? row_again<T>(pieces) : row_by_two(q);
     if (lane == 0) write_row<T, PROBABILITIES>(a, row, x, r);
     if (TOP && lane < a.top) write_top<PROBABILITIES>(a, row, lane, static_cast<uint32_t>(shared.best[lane] >> 32), index_of_key(shared.best[lane]), r);
 }
@@ -802,11 +812,15 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_grad_stream(const Score
 #pragma unroll
             for (int k = 0; k < N / 2; ++k) {
                 const float2 t = fma2(Pair<T>::floats(Pair<T>::bounded(v[k], low)), make_float2(LOG2_E, LOG2_E), make_float2(-S, -S));
-                float2 d       = mul2(fma2(t, make_float2(slope, slope), make_float2(level, level)), make_float2(exp2_of(t.x), exp2_of(t.y)));
-                const int i    = grad.label_at - static_cast<int>(j) - 2 * k;
-                if (i == 0) d.x += grad.label_gradient(to_float(v[k].x));
-                if (i == 1) d.y += grad.label_gradient(to_float(v[k].y));
+                const float2 d = mul2(fma2(t, make_float2(slope, slope), make_float2(level, level)), make_float2(exp2_of(t.x), exp2_of(t.y)));
                 e[2 * k] = from_float<T>(d.x), e[2 * k + 1] = from_float<T>(d.y);
+            }
+            if (static_cast<unsigned>(grad.label_at - static_cast<int>(j)) < N) {  // the row's label is one of these
+                float x[N], d[N];
+                values_of<T>(raw[u], x);
+                grad.of(x, j, d);
+#pragma unroll
+                for (int k = 0; k < N; ++k) e[k] = from_float<T>(d[k]);
             }
         }
         else {
