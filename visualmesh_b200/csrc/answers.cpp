@@ -86,6 +86,17 @@ Maybe like(PyObject* o, const char* name, at::IntArrayRef shape, at::ScalarType 
 Tensor make(at::IntArrayRef shape, at::ScalarType type, const at::Device& device) {
     return at::empty(shape, at::TensorOptions().dtype(type).device(device));
 }
+// A part of a tensor of bytes as a tensor of its own: the small results of a call share one allocation.
+Tensor part_of(const Tensor& bytes, size_t& at, at::IntArrayRef shape, at::ScalarType type) {
+    Tensor part      = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(bytes.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(type));
+    const auto size  = c10::elementSize(type);
+    auto* const impl = part.unsafeGetTensorImpl();
+    impl->set_storage_offset(static_cast<int64_t>(at / size));
+    impl->set_sizes_contiguous(shape);
+    at += static_cast<size_t>(impl->numel()) * size;
+    return part;
+}
+
 template <typename T = void>
 T* pointer(const Tensor& x) {
     return static_cast<T*>(x.data_ptr());
@@ -173,10 +184,18 @@ PyObject* scores(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int64_t most = r.classes < VM_MAX_TOP ? r.classes : VM_MAX_TOP;
         if (top < 0 || top > most) refuse("top must be 0.." + std::to_string(most));
         const at::Device device = r.x.device();
-        const Tensor entropy = make({r.rows}, at::kFloat, device), log_sum = make({r.rows}, at::kFloat, device);
+        // the values of the rows are one allocation, the best classes another
+        const Tensor values  = make({r.rows * (r.labels ? 12 : 8)}, at::kByte, device);
+        size_t at            = 0;
+        const Tensor entropy = part_of(values, at, {r.rows}, at::kFloat), log_sum = part_of(values, at, {r.rows}, at::kFloat);
         Maybe log_prob, top_log_prob, top_index;
-        if (r.labels) log_prob = make({r.rows}, at::kFloat, device);
-        if (top > 0) top_log_prob = make({r.rows, top}, at::kFloat, device), top_index = make({r.rows, top}, at::kInt, device);
+        if (r.labels) log_prob = part_of(values, at, {r.rows}, at::kFloat);
+        if (top > 0) {
+            const Tensor best = make({r.rows * top * 8}, at::kByte, device);
+            at                = 0;
+            top_log_prob      = part_of(best, at, {r.rows, top}, at::kFloat);
+            top_index         = part_of(best, at, {r.rows, top}, at::kInt);
+        }
         check(vm_scores(device.index(), pointer(r.x), r.type, r.rows, static_cast<int32_t>(r.classes), r.stride, r.flags, pointer(r.labels), static_cast<int32_t>(top),
                         pointer<float>(log_prob), pointer<float>(entropy), pointer<float>(log_sum), pointer<float>(top_log_prob), pointer<int32_t>(top_index), stream_of(r.x)));
         return tuple_of({log_prob, entropy, log_sum, top_log_prob, top_index});

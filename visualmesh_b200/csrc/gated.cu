@@ -284,7 +284,6 @@ vm_status vm_gated_step(int device, int32_t type, int64_t rows, int64_t slots, i
         const auto q = static_cast<cudaStream_t>(stream);
         const StepArgs a{rows, slots, channels, state, state_stride, sequence(x), sequence(gate), sequence(y), index, static_cast<uint32_t*>(workspace)};
         if (needed > 0) {
-            VM_CUDA(cudaMemsetAsync(workspace, 0xFF, needed, q));
             launch_kernel(k_first_rows, dim3(blocks_of(rows)), STEP_BLOCK, 0, q, false, a);
         }
         const bool vectors = channels % 4 == 0 && takes(x, type, 4, sizes) && takes(gate, type, 4, sizes) && takes(y, type, 4, sizes) && aligned(state, 16) && state_stride % 4 == 0;
@@ -295,7 +294,7 @@ vm_status vm_gated_step(int device, int32_t type, int64_t rows, int64_t slots, i
                 const unsigned grid = blocks_of(rows * (channels / V));
                 if (index == nullptr) launch_kernel(k_gated_step<T, V, ROW_IS_SLOT>, dim3(grid), STEP_BLOCK, 0, q, false, a);
                 else if (needed == 0) launch_kernel(k_gated_step<T, V, LOOK_THROUGH>, dim3(grid), STEP_BLOCK, 0, q, false, a);
-                else launch_kernel(k_gated_step<T, V, TABLE>, dim3(grid), STEP_BLOCK, 0, q, false, a);
+                else launch_kernel(k_gated_step<T, V, TABLE>, dim3(grid), STEP_BLOCK, 0, q, true, a);
             };
             if (vectors) launch(std::integral_constant<int, 4>{});
             else launch(std::integral_constant<int, 1>{});

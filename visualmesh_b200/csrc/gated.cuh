@@ -717,64 +717,79 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
 // run in. With few rows every block looks through the index for itself; with many, a table with the first row of every slot is made before.
 constexpr int STEP_BLOCK = 256;
 
+// The table is not cleared before: what stands in it counts where it is a row that names the slot, which is true whoever wrote it and when.
 __global__ void __launch_bounds__(STEP_BLOCK) k_first_rows(const StepArgs a) {
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * STEP_BLOCK + threadIdx.x;
+    cudaTriggerProgrammaticLaunchCompletion();
+    const uint32_t row = blockIdx.x * STEP_BLOCK + threadIdx.x;
     if (row >= a.rows) return;
     const int32_t slot = a.index[row];
-    if (slot >= 0 && slot < a.slots) atomicMin(a.first + slot, static_cast<uint32_t>(row));
+    if (slot < 0 || slot >= a.slots) return;
+    uint32_t held = *static_cast<volatile uint32_t*>(a.first + slot);
+    while (!(held <= row && a.index[held] == slot)) {  // each round that fails found another row's entry, and those only fall
+        const uint32_t was = atomicCAS(a.first + slot, held, row);
+        if (was == held) break;
+        held = was;
+    }
 }
 
 enum Slots { ROW_IS_SLOT, LOOK_THROUGH, TABLE };
 
 template <typename T, int V, Slots SLOTS>
 __global__ void __launch_bounds__(STEP_BLOCK) k_gated_step(const StepArgs a) {
-    __shared__ int32_t slots[SLOTS == LOOK_THROUGH ? STEP_BLOCK : 1];  // of the block's rows
-    const int64_t each = a.channels / V, all = a.rows * each;          // V divides the channels
+    const int64_t each = a.channels / V, all = a.rows * each;  // V divides the channels
     const int64_t begin = static_cast<int64_t>(blockIdx.x) * STEP_BLOCK, at = begin + threadIdx.x;
     const auto row_at   = [&](int64_t i) -> int64_t { return all <= UINT32_MAX ? static_cast<uint32_t>(i) / static_cast<uint32_t>(each) : i / each; };
-    const int64_t row   = row_at(at < all ? at : all - 1);
+    const bool there    = at < all;
+    const int64_t row   = row_at(there ? at : all - 1), c = there ? (at - row * each) * V : 0;
+    int64_t slot        = SLOTS == ROW_IS_SLOT ? row : a.index[row];
+    if (slot < 0 || slot >= a.slots || !there) slot = -1;
+    // everything is on its way before it is known whether the row counts
+    Raw<T, V> rx{}, rg{};
+    float h[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) h[k] = 0.0f;
+    float* const state = a.state + (slot >= 0 ? slot * a.state_stride + c : 0);
+    if (slot >= 0) {
+        rx = *reinterpret_cast<const Raw<T, V>*>(static_cast<const T*>(a.x.data) + row * a.x.b + c * a.x.c);
+        rg = *reinterpret_cast<const Raw<T, V>*>(static_cast<const T*>(a.gate.data) + row * a.gate.b + c * a.gate.c);
+        load_floats<V>(state, h);
+    }
     if constexpr (SLOTS == LOOK_THROUGH) {
+        __shared__ int32_t slots[STEP_BLOCK], taken[STEP_BLOCK];  // of the block's rows
         const int low   = static_cast<int>(row_at(begin));
         const int count = static_cast<int>(row_at(begin + STEP_BLOCK < all ? begin + STEP_BLOCK - 1 : all - 1)) - low + 1;
-        __shared__ int32_t taken[STEP_BLOCK];
         if (threadIdx.x < count) {
             slots[threadIdx.x] = a.index[low + threadIdx.x];
             taken[threadIdx.x] = 0;
         }
         __syncthreads();
         for (int j = threadIdx.x; j < low + count - 1; j += STEP_BLOCK) {
-            const int32_t slot = a.index[j];
+            const int32_t earlier = a.index[j];
             for (int r = j < low ? 0 : j - low + 1; r < count; ++r)
-                if (slots[r] == slot) taken[r] = 1;
+                if (slots[r] == earlier) taken[r] = 1;
         }
         __syncthreads();
-        if (threadIdx.x < count && taken[threadIdx.x] != 0) slots[threadIdx.x] = -1;
-        __syncthreads();
+        if (taken[row - low] != 0) slot = -1;
     }
-    if (at >= all) return;
-    const int64_t c = (at - row * each) * V;
-    int64_t slot    = row;
-    if constexpr (SLOTS == LOOK_THROUGH) slot = slots[row - row_at(begin)];
-    if constexpr (SLOTS == TABLE) slot = a.index[row];
-    if (SLOTS != ROW_IS_SLOT && (slot < 0 || slot >= a.slots)) slot = -1;
     if constexpr (SLOTS == TABLE) {
+        cudaGridDependencySynchronize();
         if (slot >= 0 && a.first[slot] != row) slot = -1;
     }
-    float h[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) h[k] = 0.0f;
+    if (!there) return;
     if (slot >= 0) {
         float x[V], g[V];
-        float* state = a.state + slot * a.state_stride + c;
-        unpack<T, V>(*reinterpret_cast<const Raw<T, V>*>(static_cast<const T*>(a.x.data) + row * a.x.b + c * a.x.c), x);
-        unpack<T, V>(*reinterpret_cast<const Raw<T, V>*>(static_cast<const T*>(a.gate.data) + row * a.gate.b + c * a.gate.c), g);
-        load_floats<V>(state, h);
+        unpack<T, V>(rx, x);
+        unpack<T, V>(rg, g);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const Factors q = factors_of(g[k]);
             h[k]            = gated(q.f, h[k], gated(q.u, x[k]));
         }
         store_floats<V>(state, h);
+    }
+    else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) h[k] = 0.0f;
     }
     if (a.y.data != nullptr) *reinterpret_cast<Raw<T, V>*>(static_cast<T*>(a.y.data) + row * a.y.b + c * a.y.c) = pack<T, V>(h);
 }

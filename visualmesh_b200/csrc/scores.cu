@@ -77,6 +77,9 @@ int blocks_of_row(int64_t rows, int64_t classes, int32_t type) {
     return n;
 }
 
+// Rows from which on a block of half the threads takes one: what follows a row's last piece keeps fewer threads waiting.
+constexpr int64_t HALF_BLOCKS_FROM = 8 * SMS;
+
 template <typename Kernel>
 void launch_cluster(Kernel kernel, dim3 grid, int blocks, cudaStream_t q, const ScoresArgs& a) {
     cudaLaunchAttribute attribute{};
@@ -127,8 +130,9 @@ vm_status vm_scores(int device, const void* x, int32_t type, int64_t rows, int32
             const int blocks = blocks_of_row(rows, classes, type);
             const auto launch = [&](auto best) {
                 constexpr bool TOP = decltype(best)::value;
-                if (blocks > 1) launch_cluster(k_scores_stream<T, P, TOP, true>, grid_of(rows * blocks), blocks, q, a);
-                else launch_kernel(k_scores_stream<T, P, TOP, false>, grid_of(rows), STREAM_BLOCK, 0, q, false, a, 1);
+                if (blocks > 1) launch_cluster(k_scores_stream<T, P, TOP, STREAM_BLOCK, true>, grid_of(rows * blocks), blocks, q, a);
+                else if (rows < HALF_BLOCKS_FROM) launch_kernel(k_scores_stream<T, P, TOP, STREAM_BLOCK, false>, grid_of(rows), STREAM_BLOCK, 0, q, false, a, 1);
+                else launch_kernel(k_scores_stream<T, P, TOP, STREAM_BLOCK / 2, false>, grid_of(rows), STREAM_BLOCK / 2, 0, q, false, a, 1);
             };
             if (top > 0) launch(std::true_type{});
             else launch(std::false_type{});

@@ -104,9 +104,11 @@ __device__ __forceinline__ Row row_of(const Sums& q) {
     Row r{q.m, 0.0f, -INFINITY, 0.0f};
     if (!(q.s < INFINITY) || q.w != q.w) r.m = r.l = r.log_sum = r.entropy = NAN;
     else if (q.s > 0.0f) {
-        r.l       = logf(q.s);
-        r.log_sum = q.m + r.l;
-        r.entropy = r.l - __fdividef(q.w, PROBABILITIES ? SCALE * q.s : q.s);
+        // a softmax's sum is one but for roundings, d: the next term of the series is d^4 / 4
+        const float d = q.s - 1.0f;
+        r.l           = PROBABILITIES && fabsf(d) < 0.00390625f ? d * fmaf(d, fmaf(d, 0.333333333f, -0.5f), 1.0f) : logf(q.s);
+        r.log_sum     = q.m + r.l;
+        r.entropy     = r.l - __fdividef(q.w, PROBABILITIES ? SCALE * q.s : q.s);
     }
     return r;
 }
@@ -207,30 +209,32 @@ __global__ void __launch_bounds__(ROW_BLOCK) k_scores_own_row(const ScoresArgs a
         a.log_prob[row] = lp;
     }
     if (a.top > 0) {
-        uint32_t order[C];  // 0: taken
+        uint32_t order[C];
         if (PROBABILITIES && r.l == r.l) {
 #pragma unroll
-            for (int k = 0; k < C; ++k) order[k] = __float_as_uint(x[k] + 0.0f) + 1;  // no negative ones in a row that has a distribution
+            for (int k = 0; k < C; ++k) order[k] = __float_as_uint(x[k] + 0.0f);  // no negative ones in a row that has a distribution
         }
         else {
 #pragma unroll
             for (int k = 0; k < C; ++k) order[k] = order_of(x[k]);
         }
+        // every class writes itself where it stands in the order
         float* const values = a.top_log_prob + static_cast<int64_t>(row) * a.top;
         int32_t* const at   = a.top_index + static_cast<int64_t>(row) * a.top;
-        for (int n = 0; n < a.top; ++n) {
-            uint32_t best = order[0];
-            float lp      = v[0];
-            int index     = 0;
+        int place[C];
 #pragma unroll
-            for (int k = 1; k < C; ++k)
-                if (order[k] > best) best = order[k], lp = v[k], index = k;
+        for (int k = 0; k < C; ++k) place[k] = 0;
 #pragma unroll
-            for (int k = 0; k < C; ++k)
-                if (index == k) order[k] = 0;
-            values[n] = lp;
-            at[n]     = index;
+        for (int k = 0; k < C; ++k) {
+#pragma unroll
+            for (int j = k + 1; j < C; ++j) {
+                const bool behind = order[j] > order[k];
+                place[k] += behind, place[j] += !behind;
+            }
         }
+#pragma unroll
+        for (int k = 0; k < C; ++k)
+            if (place[k] < a.top) values[place[k]] = v[k], at[place[k]] = k;
     }
 }
 
@@ -407,7 +411,16 @@ __device__ __forceinline__ void largest_of_lanes(const uint64_t* keys, int n, in
     uint64_t held[K];
 #pragma unroll
     for (int i = 0; i < K; ++i) held[i] = i * WARP + lane < n ? keys[i * WARP + lane] : 0;
-    if constexpr (K > 1) {  // Batcher's merge sort of eight
+    if constexpr (K == 4) {  // Batcher's merge sort, of four and of eight
+        constexpr int PAIRS[5][2] = {{0, 1}, {2, 3}, {0, 2}, {1, 3}, {1, 2}};
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+            const uint64_t x = held[PAIRS[i][0]], y = held[PAIRS[i][1]];
+            held[PAIRS[i][0]] = x > y ? x : y;
+            held[PAIRS[i][1]] = x > y ? y : x;
+        }
+    }
+    else if constexpr (K > 1) {
         static_assert(K == 8, "the pairs below sort eight");
         constexpr int PAIRS[19][2] = {{0, 1}, {2, 3}, {4, 5}, {6, 7}, {0, 2}, {1, 3}, {4, 6}, {5, 7}, {1, 2}, {5, 6}, {0, 4}, {1, 5}, {2, 6}, {3, 7}, {2, 4}, {3, 5}, {1, 2}, {3, 4}, {5, 6}};
 #pragma unroll
@@ -419,9 +432,12 @@ __device__ __forceinline__ void largest_of_lanes(const uint64_t* keys, int n, in
     }
     for (int k = 0; k < top; ++k) {
         const uint32_t high = __reduce_max_sync(~0u, static_cast<uint32_t>(held[0] >> 32));
-        const bool equal    = static_cast<uint32_t>(held[0] >> 32) == high;
-        const uint32_t low  = __reduce_max_sync(~0u, equal ? static_cast<uint32_t>(held[0]) : 0);
-        if (equal && static_cast<uint32_t>(held[0]) == low) {
+        bool largest        = static_cast<uint32_t>(held[0] >> 32) == high;
+        if (__popc(__ballot_sync(~0u, largest)) > 1) {
+            const uint32_t low = __reduce_max_sync(~0u, largest ? static_cast<uint32_t>(held[0]) : 0);
+            largest            = largest && static_cast<uint32_t>(held[0]) == low;
+        }
+        if (largest) {
             into[k] = held[0];
 #pragma unroll
             for (int i = 0; i + 1 < K; ++i) held[i] = held[i + 1];
@@ -431,6 +447,7 @@ __device__ __forceinline__ void largest_of_lanes(const uint64_t* keys, int n, in
 }
 __device__ __forceinline__ void largest_keys(const uint64_t* keys, int n, int top, uint64_t* into) {
     if (n <= WARP) largest_of_lanes<1>(keys, n, top, into);
+    else if (n <= 4 * WARP) largest_of_lanes<4>(keys, n, top, into);
     else largest_of_lanes<CANDIDATES / WARP>(keys, n, top, into);
 }
 
@@ -503,8 +520,8 @@ __device__ __noinline__ Row row_again(const Pieces<T>& pieces) {
     return row_of<false>(joined_lanes<WARP>(q, [](const Sums& a, const Sums& b) { return Sums{a.m, a.s + b.s, a.w + b.w}; }));
 }
 
-template <typename T, bool PROBABILITIES, bool TOP, bool CLUSTER>
-__global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs a, int blocks) {
+template <typename T, bool PROBABILITIES, bool TOP, int BLOCK, bool CLUSTER>
+__global__ void __launch_bounds__(BLOCK) k_scores_stream(const ScoresArgs a, int blocks) {
     namespace cg = cooperative_groups;
     __shared__ StreamShared shared;
     const int rank    = CLUSTER ? blockIdx.x % blocks : 0;
@@ -516,18 +533,19 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs
     const int64_t share = CLUSTER ? (pieces.count + blocks - 1) / blocks : pieces.count;
     const int64_t begin = rank * share, end = begin + share < pieces.count ? begin + share : pieces.count;
     const T outside     = from_float<T>(PROBABILITIES ? 0.0f : -INFINITY);
+    if constexpr (CLUSTER) cg::this_cluster().barrier_arrive();  // this block runs: the others may write to it
 
     Sums q{PROBABILITIES ? 0.0f : Range<T>::START, 0.0f, 0.0f};
     float best = PROBABILITIES ? -1.0f : -INFINITY;
     int held   = static_cast<int>(begin) + threadIdx.x;  // the piece with the maximum
     float2 s2 = make_float2(0.0f, 0.0f), w2 = s2;
-    for (int64_t p = begin + threadIdx.x; p < end; p += STREAM_BLOCK * STREAM_AHEAD) {
+    for (int64_t p = begin + threadIdx.x; p < end; p += BLOCK * STREAM_AHEAD) {
         using P2 = Pair<T>;
         typename P2::type v[STREAM_AHEAD][N / 2];
 #pragma unroll
         for (int u = 0; u < STREAM_AHEAD; ++u) {
             uint4 raw;
-            if (p + u * STREAM_BLOCK < end) raw = pieces.load(p + u * STREAM_BLOCK, outside);
+            if (p + u * BLOCK < end) raw = pieces.load(p + u * BLOCK, outside);
             else {
                 T e[N];
 #pragma unroll
@@ -544,7 +562,7 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs
             for (int k = 1; k < N / 2; ++k) larger = P2::larger(larger, v[u][k]);
             const float2 f  = P2::floats(larger);
             const float top = fmaxf(f.x, f.y);
-            if (TOP && top > best) best = top, held = static_cast<int>(p) + u * STREAM_BLOCK;
+            if (TOP && top > best) best = top, held = static_cast<int>(p) + u * BLOCK;
             most = fmaxf(most, top);
         }
         if constexpr (PROBABILITIES) {
@@ -583,19 +601,19 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs
     if (lane == 0) shared.warps[warp] = q;
     bool search = __syncthreads_or(q.s != q.s || q.w != q.w);  // NaN, or an infinity: its maxima were no maxima
     if (!TOP && !CLUSTER && warp != 0) return;
-    q = joined_lanes<STREAM_BLOCK / WARP>(shared.warps[lane % (STREAM_BLOCK / WARP)], joined_stream<PROBABILITIES>);
+    q = joined_lanes<BLOCK / WARP>(shared.warps[lane % (BLOCK / WARP)], joined_stream<PROBABILITIES>);
 
     if constexpr (TOP) {
-        if (warp == 0) largest_keys(shared.keys, STREAM_BLOCK, a.top, shared.best);
+        if (warp == 0) largest_keys(shared.keys, BLOCK, a.top, shared.best);
         __syncthreads();
         const uint64_t least = shared.best[a.top - 1];
         if (!search) {
             const uint32_t least_order  = static_cast<uint32_t>(least >> 32);
             const int64_t least_piece   = 0xFFFFFFFFu - static_cast<uint32_t>(least);
-            for (int i = warp; i < a.top; i += STREAM_BLOCK / WARP) {
+            for (int i = warp; i < a.top; i += BLOCK / WARP) {
                 const int64_t piece = 0xFFFFFFFFu - static_cast<uint32_t>(shared.best[i]);
-                const int64_t first = begin + (piece - begin) % STREAM_BLOCK;
-                for (int64_t p = first + lane * STREAM_BLOCK; p < end; p += WARP * STREAM_BLOCK) {
+                const int64_t first = begin + (piece - begin) % BLOCK;
+                for (int64_t p = first + lane * BLOCK; p < end; p += WARP * BLOCK) {
                     float v[N];
                     values_of<T>(pieces.load(p, outside), v);
 #pragma unroll
@@ -616,7 +634,7 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs
             uint64_t below = ~0ull;
             for (int k = 0; k < a.top; ++k) {
                 uint64_t most = 0;
-                for (int64_t p = begin + threadIdx.x; p < end; p += STREAM_BLOCK) {
+                for (int64_t p = begin + threadIdx.x; p < end; p += BLOCK) {
                     float v[N];
                     values_of<T>(pieces.load(p, outside), v);
 #pragma unroll
@@ -634,7 +652,7 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs
                 if (lane == 0) shared.searched[warp] = most;
                 __syncthreads();
                 below = shared.searched[0];
-                for (int w = 1; w < STREAM_BLOCK / WARP; ++w) below = shared.searched[w] > below ? shared.searched[w] : below;
+                for (int w = 1; w < BLOCK / WARP; ++w) below = shared.searched[w] > below ? shared.searched[w] : below;
                 if (threadIdx.x == 0) shared.best[k] = below;
             }
         }
@@ -643,7 +661,7 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_stream(const ScoresArgs
 
     if constexpr (CLUSTER) {
         const cg::cluster_group cluster = cg::this_cluster();
-        cluster.sync();  // the first block runs
+        cluster.barrier_wait();
         StreamShared* first = cluster.map_shared_rank(&shared, 0);
         if (threadIdx.x == 0) first->sums[rank] = q;
         if (TOP && threadIdx.x < a.top) first->bests[rank * a.top + threadIdx.x] = shared.best[threadIdx.x];
