@@ -115,8 +115,10 @@ vm_status vm_scores(int device, const void* x, int32_t type, int64_t rows, int32
             using T = decltype(kind);
             constexpr bool P = decltype(probabilities)::value;
             if (classes <= MOST_OF_THREAD) {
+                const bool pairs = top == 2 && aligned(top_log_prob, 8) && aligned(top_index, 8);
                 with_classes(classes, [&](auto c) {
-                    launch_kernel(k_scores_own_row<T, P, decltype(c)::value>, grid_of((rows + ROW_BLOCK - 1) / ROW_BLOCK), ROW_BLOCK, 0, q, false, a, starts_on_row(x, row_stride, classes, type));
+                    launch_kernel(k_scores_own_row<T, P, decltype(c)::value>, grid_of((rows + ROW_BLOCK - 1) / ROW_BLOCK), ROW_BLOCK, 0, q, false, a,
+                                  starts_on_row(x, row_stride, classes, type), pairs);
                 });
                 return;
             }

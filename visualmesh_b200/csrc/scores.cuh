@@ -167,7 +167,7 @@ __device__ __forceinline__ void load_row(const T* x, bool wide, float (&to)[C]) 
 }
 
 template <typename T, bool PROBABILITIES, int C>
-__global__ void __launch_bounds__(ROW_BLOCK) k_scores_own_row(const ScoresArgs a, bool wide) {
+__global__ void __launch_bounds__(ROW_BLOCK) k_scores_own_row(const ScoresArgs a, bool wide, bool pairs) {
     const int row = blockIdx.x * ROW_BLOCK + threadIdx.x;  // rows < 2^31, and so are those of the last block
     if (row >= a.rows) return;
     float x[C], v[C];
@@ -218,9 +218,6 @@ __global__ void __launch_bounds__(ROW_BLOCK) k_scores_own_row(const ScoresArgs a
 #pragma unroll
             for (int k = 0; k < C; ++k) order[k] = order_of(x[k]);
         }
-        // every class writes itself where it stands in the order
-        float* const values = a.top_log_prob + static_cast<int64_t>(row) * a.top;
-        int32_t* const at   = a.top_index + static_cast<int64_t>(row) * a.top;
         int place[C];
 #pragma unroll
         for (int k = 0; k < C; ++k) place[k] = 0;
@@ -232,9 +229,27 @@ __global__ void __launch_bounds__(ROW_BLOCK) k_scores_own_row(const ScoresArgs a
                 place[k] += behind, place[j] += !behind;
             }
         }
+        const int64_t first = static_cast<int64_t>(row) * a.top;
+        if (a.top <= 2) {
+            float lp[2];
+            int index[2];
 #pragma unroll
-        for (int k = 0; k < C; ++k)
-            if (place[k] < a.top) values[place[k]] = v[k], at[place[k]] = k;
+            for (int k = 0; k < C; ++k) {
+                if (place[k] == 0) lp[0] = v[k], index[0] = k;
+                if (place[k] == 1) lp[1] = v[k], index[1] = k;
+            }
+            if (pairs) {  // two at once: half of the stores, which are what bounds rows of few classes
+                *reinterpret_cast<float2*>(a.top_log_prob + first) = make_float2(lp[0], lp[1]);
+                *reinterpret_cast<int2*>(a.top_index + first)      = make_int2(index[0], index[1]);
+                return;
+            }
+            for (int n = 0; n < a.top; ++n) a.top_log_prob[first + n] = lp[n], a.top_index[first + n] = index[n];
+        }
+        else {  // every class writes itself where it stands in the order
+#pragma unroll
+            for (int k = 0; k < C; ++k)
+                if (place[k] < a.top) a.top_log_prob[first + place[k]] = v[k], a.top_index[first + place[k]] = k;
+        }
     }
 }
 
@@ -432,12 +447,9 @@ __device__ __forceinline__ void largest_of_lanes(const uint64_t* keys, int n, in
     }
     for (int k = 0; k < top; ++k) {
         const uint32_t high = __reduce_max_sync(~0u, static_cast<uint32_t>(held[0] >> 32));
-        bool largest        = static_cast<uint32_t>(held[0] >> 32) == high;
-        if (__popc(__ballot_sync(~0u, largest)) > 1) {
-            const uint32_t low = __reduce_max_sync(~0u, largest ? static_cast<uint32_t>(held[0]) : 0);
-            largest            = largest && static_cast<uint32_t>(held[0]) == low;
-        }
-        if (largest) {
+        const bool equal    = static_cast<uint32_t>(held[0] >> 32) == high;
+        const uint32_t low  = __reduce_max_sync(~0u, equal ? static_cast<uint32_t>(held[0]) : 0);
+        if (equal && static_cast<uint32_t>(held[0]) == low) {
             into[k] = held[0];
 #pragma unroll
             for (int i = 0; i + 1 < K; ++i) held[i] = held[i + 1];
