@@ -94,17 +94,24 @@ struct Plan {
     int64_t blocks;  // along the channels
     int64_t run;     // steps of a part
     int64_t parts;
+    bool cluster;    // the parts are blocks of a cluster, which take every so manieth tile, instead
 };
 
-// `vector` elements and `length` steps a thread.
+// `vector` elements and `length` steps a thread; blocks that are on the card together.
 Plan plan_of(int64_t all, int64_t steps, int vector, int length) {
-    Plan p{(all + 31) / 32, steps, 1};
+    Plan p{(all + 31) / 32, steps, 1, false};
     const int64_t tile = THREADS / (32 / vector) * length, tiles = (steps + tile - 1) / tile;
-    if (p.blocks < SMS && tiles > 1) {
-        const int64_t wanted = std::min(tiles, (2 * SMS + p.blocks - 1) / p.blocks);
-        p.run                = (tiles + wanted - 1) / wanted * tile;
-        p.parts              = (steps + p.run - 1) / p.run;
+    if (p.blocks >= SMS || tiles <= 1) return p;
+    int64_t ranks = 2;
+    while (ranks < MOST_RANKS && ranks < tiles && p.blocks * ranks * 2 <= 3 * SMS) ranks *= 2;
+    if (p.blocks * ranks >= SMS || tiles <= 4 * ranks) {
+        p.parts   = ranks;
+        p.cluster = true;
+        return p;
     }
+    const int64_t wanted = std::min(tiles, (2 * SMS + p.blocks - 1) / p.blocks);
+    p.run                = (tiles + wanted - 1) / wanted * tile;
+    p.parts              = (steps + p.run - 1) / p.run;
     return p;
 }
 
@@ -127,20 +134,20 @@ void with_access(int32_t type, const Access& access, F f) {
         constexpr int SIZE = sizeof(kind);
         if (access.piece == 16) f(kind, integral_constant<int, 2>{}, integral_constant<int, 16>{});
         else if (access.vector == 2) f(kind, integral_constant<int, 2>{}, integral_constant<int, 2 * SIZE>{});
-        else f(kind, integral_constant<int, 1>{}, integral_constant<int, SIZE == 4 ? 4 : 0>{});
+        else f(kind, integral_constant<int, 1>{}, integral_constant<int, 0>{});
     });
 }
 // inputs are read through the ring in pieces, outputs are written by a thread's vectors
 Access access_of(int32_t type, int64_t channels, const int64_t (&sizes)[3], std::initializer_list<const vm_sequence*> inputs, std::initializer_list<const vm_sequence*> outputs, const float* states) {
     const int size = static_cast<int>(element_size(type)), wide = 16 / size;
     const auto all = [&](std::initializer_list<const vm_sequence*> list, int n) { return std::all_of(list.begin(), list.end(), [&](const vm_sequence* s) { return takes(s, type, n, sizes); }); };
-    if (channels % 2 != 0 || !all(inputs, 2) || !all(outputs, 2) || !aligned(states, 8)) return {1, size == 4 ? 4 : 0};
+    if (channels % 2 != 0 || !all(inputs, 2) || !all(outputs, 2) || !aligned(states, 8)) return {1, 0};
     return {2, channels % wide == 0 && all(inputs, wide) ? 16 : 2 * size};
 }
 
 // Launches one kernel, which is told once for a device that it may take more shared memory than every kernel may.
 template <auto KERNEL>
-void launch_tiles(dim3 grid, int shared, cudaStream_t q, const GatedArgs& a, const Split& s) {
+void launch_tiles(dim3 grid, int ranks, int shared, cudaStream_t q, const GatedArgs& a, const Split& s) {
     static LaunchPlans plans;
     if (shared > 0) {
         plans.get([&](int) {
@@ -148,7 +155,18 @@ void launch_tiles(dim3 grid, int shared, cudaStream_t q, const GatedArgs& a, con
             return LaunchPlan{};
         });
     }
-    launch_kernel(KERNEL, grid, THREADS, shared, q, false, a, s);
+    cudaLaunchAttribute attribute{};
+    attribute.id               = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = attribute.val.clusterDim.z = 1;
+    attribute.val.clusterDim.y = ranks;
+    cudaLaunchConfig_t config{};
+    config.gridDim          = grid;
+    config.blockDim         = dim3(THREADS);
+    config.dynamicSmemBytes = shared;
+    config.stream           = q;
+    config.attrs            = &attribute;
+    config.numAttrs         = ranks > 1 ? 1 : 0;
+    VM_CUDA(cudaLaunchKernelEx(&config, KERNEL, a, s));
 }
 
 Split split_of(const Plan& p, void* workspace) {
@@ -175,7 +193,10 @@ size_t vm_gated_workspace(int64_t batch, int64_t steps, int64_t channels) {
     const int64_t all = batch * channels;
     int64_t parts     = 1;
     for (const int vector : {1, 2})
-        for (const int length : {4, 8, 16}) parts = std::max(parts, plan_of(all, steps, vector, length).parts);
+        for (const int length : {4, 8, 16}) {
+            const Plan p = plan_of(all, steps, vector, length);
+            if (!p.cluster) parts = std::max(parts, p.parts);
+        }
     return parts > 1 ? static_cast<size_t>(parts * all) * sizeof(float2) : 0;
 }
 
@@ -192,6 +213,7 @@ vm_status vm_gated_scan(int device, int32_t type, int64_t batch, int64_t steps, 
         const OnDevice on(device);
         GatedArgs a{};
         a.batch = batch, a.steps = steps, a.channels = channels;
+        a.small = batch * channels <= UINT32_MAX;
         a.x = sequence(x), a.gate = sequence(gate), a.y = sequence(y);
         a.h0 = h0, a.lengths = lengths, a.last = last, a.states = states;
         const auto q       = static_cast<cudaStream_t>(stream);
@@ -207,8 +229,12 @@ vm_status vm_gated_scan(int device, int32_t type, int64_t batch, int64_t steps, 
         with_access(type, access, [&](auto kind, auto v, auto piece) {
             using T = decltype(kind);
             constexpr int V = decltype(v)::value, PIECE = decltype(piece)::value, L = forward_steps(V, sizeof(T) == 4), SHARED = Tiles<T, V, L, 2, PIECE, STAGES>::SHARED;
-            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, L, PIECE, STAGES, false>>(grid, SHARED, q, a, s);
-            launch_tiles<k_gated_scan<T, V, L, PIECE, STAGES>>(grid, SHARED, q, a, s);
+            if (p.cluster) {
+                launch_tiles<k_gated_scan<T, V, L, PIECE, STAGES, true>>(grid, static_cast<int>(p.parts), SHARED, q, a, s);
+                return;
+            }
+            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, L, PIECE, STAGES, false>>(grid, 1, SHARED, q, a, s);
+            launch_tiles<k_gated_scan<T, V, L, PIECE, STAGES, false>>(grid, 1, SHARED, q, a, s);
         });
     }
     catch (const std::string& refused) {
@@ -237,6 +263,7 @@ vm_status vm_gated_scan_backward(int device, int32_t type, int64_t batch, int64_
         const OnDevice on(device);
         GatedArgs a{};
         a.batch = batch, a.steps = steps, a.channels = channels;
+        a.small = batch * channels <= UINT32_MAX;
         a.x = sequence(x), a.gate = sequence(gate), a.y = sequence(dy);
         a.lengths = lengths, a.states = const_cast<float*>(states), a.d_last = d_last;
         a.dx = sequence(dx), a.d_gate = sequence(d_gate), a.d_h0 = d_h0;
@@ -248,8 +275,13 @@ vm_status vm_gated_scan_backward(int device, int32_t type, int64_t batch, int64_
         with_access(type, access, [&](auto kind, auto v, auto piece) {
             using T = decltype(kind);
             constexpr int V = decltype(v)::value, PIECE = decltype(piece)::value, L = backward_steps(V, sizeof(T) == 4);
-            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, L, PIECE, STAGES, true>>(grid, Tiles<T, V, L, 2, PIECE, STAGES>::SHARED, q, a, s);
-            launch_tiles<k_gated_scan_grad<T, V, L, PIECE, STAGES>>(grid, Tiles<T, V, L, 3, PIECE, STAGES>::SHARED, q, a, s);
+            constexpr int SHARED = Tiles<T, V, L, 3, PIECE, STAGES>::SHARED;
+            if (p.cluster) {
+                launch_tiles<k_gated_scan_grad<T, V, L, PIECE, STAGES, true>>(grid, static_cast<int>(p.parts), SHARED, q, a, s);
+                return;
+            }
+            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, L, PIECE, STAGES, true>>(grid, 1, Tiles<T, V, L, 2, PIECE, STAGES>::SHARED, q, a, s);
+            launch_tiles<k_gated_scan_grad<T, V, L, PIECE, STAGES, false>>(grid, 1, SHARED, q, a, s);
         });
     }
     catch (const std::string& refused) {

@@ -9,6 +9,8 @@
 // A factor of exactly 0 drops what it multiplies, NaN and infinities included.
 #pragma once
 
+#include <cooperative_groups.h>
+
 #include <cstdint>
 #include <cstring>
 #include <type_traits>
@@ -29,6 +31,7 @@ struct Sequence {
 
 struct GatedArgs {
     int64_t batch, steps, channels;
+    bool small;  // batch * channels < 2^32
     Sequence x, gate, y;  // backward: y is dy
     const float* h0;
     const int32_t* lengths;
@@ -70,6 +73,11 @@ constexpr float SMALLEST = 1.17549435e-38f;
 __device__ __forceinline__ float product(float a, float b) {
     const float r = a * b;
     return a == 0.0f || b == 0.0f ? 0.0f : r < SMALLEST ? SMALLEST : r;
+}
+
+// Of all sequences number `at`: its batch (a division in 32 bits is a quarter of one in 64).
+__device__ __forceinline__ int64_t batch_of(const GatedArgs& a, int64_t at) {
+    return a.small ? static_cast<uint32_t>(at) / static_cast<uint32_t>(a.channels) : at / a.channels;
 }
 
 __device__ __forceinline__ int64_t length_of(const GatedArgs& a, int64_t b) {
@@ -155,7 +163,7 @@ struct Place {
         ty    = warp * SEGMENTS + lane / TX;
         at    = (static_cast<int64_t>(blockIdx.x) * TX + tx) * V;
         there = at < a.batch * a.channels;
-        b     = there ? at / a.channels : 0;
+        b     = there ? batch_of(a, at) : 0;
         c     = there ? at - b * a.channels : 0;
     }
 };
@@ -270,11 +278,16 @@ __device__ __forceinline__ typename RawOf<PIECE>::type filled(bool gate) {
     return raw;
 }
 
+// How many of a thread's L steps from t on come before `stop`.
+template <int L>
+__device__ __forceinline__ int steps_before(int64_t stop, int64_t t) {
+    return stop - t >= L ? L : stop > t ? static_cast<int>(stop - t) : 0;
+}
 // The tiles of N sequences on their way through a ring in shared memory, a row of the block's 32 channels for a step. A thread copies
 // pieces of PIECE bytes (16 where the sequences' places allow it) for channels of its own, and after a barrier every thread reads what it works
 // on. Rows at and behind a sequence's stop are filled instead. A row of 16-bit elements is half as wide as the banks, so that the rows of
 // every other thread along time begin in their other half (a gap behind every L rows).
-// PIECE == 0: no ring, every thread reads its own elements when it needs them (single elements of 16 bits).
+// PIECE == 0: no ring, every thread reads its own (single) elements into registers, a tile ahead.
 template <typename T, int V, int L, int N, int PIECE, int STAGES>
 struct Tiles {
     static constexpr int CHANNELS = 32, TX = CHANNELS / V, TILE = THREADS / TX * L;
@@ -289,13 +302,13 @@ struct Tiles {
     int64_t stride[N];
     int64_t next, left;  // the step that the next tile begins with, and how many tiles are still to be asked for
     int put, at;
+    T held[N][PIECE > 0 ? 1 : L], coming[N][PIECE > 0 ? 1 : L];
 
     __device__ __forceinline__ static int offset(int row) {
         return row * ROW + row / L * GAP;
     }
     // by: steps from tile to tile
-    template <int BY>
-    __device__ __forceinline__ void ask(const int64_t (&stop)[N]) {
+    __device__ __forceinline__ void ask(int64_t by, const int64_t (&stop)[N]) {
         if (left-- > 0) {
             const int first = threadIdx.x / ACROSS;
 #pragma unroll
@@ -310,49 +323,65 @@ struct Tiles {
                     else *reinterpret_cast<typename RawOf<PIECE>::type*>(to + offset(row)) = filled<T, PIECE>(n == GATE);
                     p += ROWS * stride[n];
                 }
-                from[n] += BY * stride[n];
+                from[n] += by * stride[n];
             }
         }
-        next += BY;
+        next += by;
         put = put + 1 == STAGES ? 0 : put + 1;
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    // next: the thread's own step
+    __device__ __forceinline__ void read(int64_t by, const int64_t (&stop)[N], T (&to)[N][PIECE > 0 ? 1 : L]) {
+        if (left-- <= 0) return;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int there = steps_before<L>(stop[n], next);
+            const T* p      = from[n];
+#pragma unroll
+            for (int i = 0; i < L; ++i, p += stride[n]) {
+                to[n][i] = n == GATE ? kept_gate<T>() : from_float<T>(0.0f);
+                if (i < there) to[n][i] = *p;
+            }
+            from[n] += by * stride[n];
+        }
+        next += by;
+    }
     // The first tiles; `from` are the first elements of the first tile that the thread copies (PIECE == 0: that it works on, in that tile).
-    template <int BY>
-    __device__ __forceinline__ void begin(void* shared, int64_t first, int64_t tiles, const int64_t (&stop)[N]) {
+    __device__ __forceinline__ void begin(void* shared, int64_t by, int64_t first, int64_t tiles, const int64_t (&stop)[N]) {
         at = 0;
+        if constexpr (PIECE == 0) {
+            next = first + threadIdx.x / TX * L, left = tiles;
+            read(by, stop, held);
+        }
         if constexpr (PIECE > 0) {
             ring = static_cast<unsigned char*>(shared), next = first, left = tiles, put = 0;
 #pragma unroll
-            for (int s = 0; s + 1 < STAGES; ++s) ask<BY>(stop);
+            for (int s = 0; s + 1 < STAGES; ++s) ask(by, stop);
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         }
     }
     // In a tile, between two barriers that all threads come to with what they read of the tile before it: the tile behind it is there after
     // the second of them.
-    template <int BY>
-    __device__ __forceinline__ void ahead(const int64_t (&stop)[N]) {
+    __device__ __forceinline__ void ahead(int64_t by, const int64_t (&stop)[N]) {
         if constexpr (PIECE > 0) {
-            ask<BY>(stop);
+            ask(by, stop);
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         }
+        else read(by, stop, coming);
     }
-    template <int BY>
+    // Behind the last use of a tile.
     __device__ __forceinline__ void advance() {
         if constexpr (PIECE > 0) at = at + 1 == STAGES ? 0 : at + 1;
-        else {
-#pragma unroll
-            for (int n = 0; n < N; ++n) from[n] += BY * stride[n];
-        }
+        else memcpy(held, coming, sizeof(held));
     }
-    // step number i of the thread's (ty along time, tx along the channels) in sequence n, of which `there` come before its stop
-    __device__ __forceinline__ void get(int n, int i, int tx, int ty, int there, float (&to)[V]) const {
+    // step number i of the thread's (ty along time, tx along the channels) in sequence n
+    __device__ __forceinline__ void get(int n, int i, int tx, int ty, float (&to)[V]) const {
         T e[V];
         if constexpr (PIECE > 0) {
             const Raw<T, V> raw = *reinterpret_cast<const Raw<T, V>*>(ring + (at * N + n) * BYTES + offset(ty * L) + i * ROW + tx * V * sizeof(T));
             memcpy(e, &raw, sizeof(raw));
         }
-        else e[0] = i < there ? from[n][i * stride[n]] : n == GATE ? kept_gate<T>() : from_float<T>(0.0f);
+        else e[0] = held[n][i];
 #pragma unroll
         for (int k = 0; k < V; ++k) to[k] = to_float(e[k]);
     }
@@ -365,11 +394,21 @@ struct Split {
     float2* summary;  // [parts][batch * channels]: the map of every part
 };
 
-// How many of a thread's L steps from t on come before `stop`.
-template <int L>
-__device__ __forceinline__ int steps_before(int64_t stop, int64_t t) {
-    return stop - t >= L ? L : stop > t ? static_cast<int>(stop - t) : 0;
-}
+// The tiles of a block, in the order it takes them: a part of the sequence, or (CLUSTER) every so manieth tile of all of it.
+template <int TILE, bool CLUSTER, bool REVERSE>
+struct Walk {
+    int64_t first, by, tiles, end;  // the step that the first tile begins with (maybe behind the end), steps from tile to tile, how many, and the end of the steps
+    __device__ __forceinline__ Walk(const GatedArgs& a, const Split& s) {
+        const int64_t begin = CLUSTER ? 0 : blockIdx.y * s.run;
+        end                 = CLUSTER || begin + s.run > a.steps ? a.steps : begin + s.run;
+        const int64_t all   = (end - begin + TILE - 1) / TILE;
+        const int ranks     = CLUSTER ? gridDim.y : 1;  // a power of two
+        tiles               = (all + ranks - 1) >> (__ffs(ranks) - 1);
+        first               = begin + ((REVERSE && tiles > 0 ? tiles - 1 : 0) * ranks + (CLUSTER ? blockIdx.y : 0)) * TILE;
+        by                  = (REVERSE ? -TILE : TILE) * ranks;
+    }
+};
+
 // Sequence number n of a kernel, from step `first` on: where the thread's copies begin, and (returned) behind which step of first..end-1 there
 // is nothing. What a thread copies belongs to other channels than what it works on, maybe of another batch.
 template <typename T, int V, int L, int N, int PIECE, int STAGES>
@@ -379,7 +418,7 @@ __device__ __forceinline__ int64_t set_up(Tiles<T, V, L, N, PIECE, STAGES>& io, 
     io.stride[n]         = q.t;
     io.from[n]           = nullptr;
     if (copied >= a.batch * a.channels || q.data == nullptr) return 0;
-    const int64_t b = copied / a.channels, length = length_of(a, b);
+    const int64_t b = batch_of(a, copied), length = length_of(a, b);
     io.from[n] = static_cast<const T*>(q.data) + b * q.b + (copied - b * a.channels) * q.c + (first + (PIECE > 0 ? threadIdx.x / IO::ACROSS : at.ty * L)) * q.t;
     return end < length ? end : length;
 }
@@ -410,26 +449,58 @@ __device__ __forceinline__ void join_parts(const GatedArgs& a, const Split& s, c
     }
 }
 
+// Blocks of a cluster that share their channels, a tile of time each: maps of all their tiles, told to all of them.
+constexpr int MOST_RANKS = 8;
+template <int V, int TX, bool CLUSTER>
+struct Exchange {
+    float2 maps[CLUSTER ? 2 : 1][CLUSTER ? MOST_RANKS : 1][CLUSTER ? TX * V : 1];
+};
+// Between the two barriers of a tile, by all threads of a block: the map of its tile, which the thread of a channel makes of its warps', goes to every
+// block of the cluster, and comes back as the state in front of this block's tile (here) and the one behind the whole cluster's (carry).
+template <int V, int TX, bool REVERSE>
+__device__ __forceinline__ void tell_cluster(Exchange<V, TX, true>& shared, const Between<V, TX>& between, int window, int ranks, int channel, float& carry, float& here) {
+    namespace cg = cooperative_groups;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int rank                  = blockIdx.y;
+    float2(*maps)[TX * V]           = shared.maps[window & 1];
+    if (window == 0) cluster.barrier_wait();  // all blocks run
+    if (channel >= 0) {
+        float2 whole = make_float2(1.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < WARPS; ++i) {
+            const float2 q = between.totals[REVERSE ? WARPS - 1 - i : i][channel];
+            whole          = make_float2(product(q.x, whole.x), gated(q.x, whole.y, q.y));
+        }
+        for (int to = 0; to < ranks; ++to) *cluster.map_shared_rank(&maps[rank][channel], to) = whole;
+    }
+    cluster.sync();
+    if (channel >= 0) {
+        for (int i = 0; i < ranks; ++i) {
+            const int from = REVERSE ? ranks - 1 - i : i;
+            if (from == rank) here = carry;
+            const float2 q = maps[from][channel];
+            carry          = gated(q.x, carry, q.y);
+        }
+    }
+}
+
 // Maps of the parts of a split sequence, of the recurrence or (REVERSE) of its gradient.
 template <typename T, int V, int L, int PIECE, int STAGES, bool REVERSE>
 __global__ void __launch_bounds__(THREADS) k_gated_summary(const GatedArgs a, const Split s) {
     using IO = Tiles<T, V, L, 2, PIECE, STAGES>;
-    constexpr int TX = IO::TX, TILE = IO::TILE, BY = REVERSE ? -TILE : TILE;
+    constexpr int TX = IO::TX, TILE = IO::TILE;
     extern __shared__ uint4 ring[];
     __shared__ Between<V, TX> shared;
     const Place<V, TX> at(a);
-    const int64_t n     = at.there ? length_of(a, at.b) : 0;
-    const int64_t begin = blockIdx.y * s.run, end = begin + s.run < a.steps ? begin + s.run : a.steps;
-    const int64_t tiles = (end - begin + TILE - 1) / TILE, stop = end < n ? end : n, first = begin + (REVERSE ? tiles - 1 : 0) * TILE;
+    const Walk<TILE, false, REVERSE> walk(a, s);
+    const int64_t end = walk.end, tiles = walk.tiles, first = walk.first, by = walk.by;
     IO io;
     const int64_t stops[2] = {set_up(io, X, REVERSE ? a.y : a.x, a, at, first, end), set_up(io, GATE, a.gate, a, at, first, end)};
-    io.template begin<BY>(ring, first, tiles, stops);
+    io.begin(ring, by, first, tiles, stops);
     const int channel = threadIdx.x < at.CHANNELS ? threadIdx.x : -1;
     float carry = 0.0f, whole = 1.0f;
-    int64_t t = first + at.ty * L;
     __syncthreads();
-    for (int64_t tile = 0; tile < tiles; ++tile, t += BY) {
-        const int left = steps_before<L>(stop, t), in_left = REVERSE && a.y.data == nullptr ? 0 : left;
+    for (int64_t tile = 0; tile < tiles; ++tile) {
         float A[V], H[V];
         const auto pass = [&](auto careful) {
             constexpr bool CAREFUL = decltype(careful)::value;
@@ -438,8 +509,8 @@ __global__ void __launch_bounds__(THREADS) k_gated_summary(const GatedArgs a, co
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 float x[V], g[V];
-                io.get(X, i, at.tx, at.ty, in_left, x);
-                io.get(GATE, i, at.tx, at.ty, left, g);
+                io.get(X, i, at.tx, at.ty, x);
+                io.get(GATE, i, at.tx, at.ty, g);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     const Factors w = factors_of(g[k]);
@@ -454,32 +525,35 @@ __global__ void __launch_bounds__(THREADS) k_gated_summary(const GatedArgs a, co
         if (careful) pass(std::true_type{});
         scan_warp<V, TX, REVERSE>(at, A, H, careful, shared.totals);
         __syncthreads();
-        io.template ahead<BY>(stops);
+        io.ahead(by, stops);
         if (channel >= 0) {
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) whole = product(shared.totals[w][channel].x, whole);
             fold_warps<V, TX, REVERSE>(shared, channel, carry);
         }
         __syncthreads();
-        io.template advance<BY>();
+        io.advance();
     }
     const int64_t of_channel = static_cast<int64_t>(blockIdx.x) * at.CHANNELS + channel, all = a.batch * a.channels;
     if (channel >= 0 && of_channel < all) s.summary[blockIdx.y * all + of_channel] = make_float2(whole, carry);
 }
 
-template <typename T, int V, int L, int PIECE, int STAGES>
-__global__ void __launch_bounds__(THREADS, 2) k_gated_scan(const GatedArgs a, const Split s) {
+template <typename T, int V, int L, int PIECE, int STAGES, bool CLUSTER>
+__global__ void __launch_bounds__(THREADS, V == 1 ? 3 : 2) k_gated_scan(const GatedArgs a, const Split s) {
     using IO = Tiles<T, V, L, 2, PIECE, STAGES>;
     constexpr int TX = IO::TX, TILE = IO::TILE;
     extern __shared__ uint4 ring[];
     __shared__ Between<V, TX> shared;
+    __shared__ Exchange<V, TX, CLUSTER> exchange;
+    if constexpr (CLUSTER) cooperative_groups::this_cluster().barrier_arrive();
     const Place<V, TX> at(a);
     const int64_t n     = at.there ? length_of(a, at.b) : 0, kept = (a.steps + KEEP - 1) / KEEP;
-    const int64_t begin = blockIdx.y * s.run, end = begin + s.run < a.steps ? begin + s.run : a.steps;
-    const int64_t tiles = (end - begin + TILE - 1) / TILE, stop = end < n ? end : n;
+    const Walk<TILE, CLUSTER, false> walk(a, s);
+    const int64_t begin = walk.first, end = walk.end, tiles = walk.tiles, stop = end < n ? end : n;
+    const int64_t by    = walk.by;  // steps from tile to tile
     IO io;
     const int64_t stops[2] = {set_up(io, X, a.x, a, at, begin, end), set_up(io, GATE, a.gate, a, at, begin, end)};
-    io.template begin<TILE>(ring, begin, tiles, stops);
+    io.begin(ring, by, begin, tiles, stops);
     int64_t t         = begin + at.ty * L;
     T* y              = static_cast<T*>(a.y.data) + at.b * a.y.b + at.c * a.y.c + t * a.y.t;
     const bool writes = at.there && a.y.data != nullptr;
@@ -487,9 +561,9 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan(const GatedArgs a, co
     const int channel        = threadIdx.x < at.CHANNELS ? threadIdx.x : -1;
     const bool carries       = channel >= 0 && of_channel < a.batch * a.channels;
     float carry              = carries && a.h0 != nullptr ? a.h0[of_channel] : 0.0f;
-    if (s.parts > 1) join_parts<V, TX, false>(a, s, at, blockIdx.y, channel, carry, shared);
+    if (!CLUSTER && s.parts > 1) join_parts<V, TX, false>(a, s, at, blockIdx.y, channel, carry, shared);
     __syncthreads();
-    for (int64_t tile = 0; tile < tiles; ++tile, t += TILE, y += TILE * a.y.t) {
+    for (int64_t tile = 0; tile < tiles; ++tile, t += by, y += by * a.y.t) {
         const int left = steps_before<L>(stop, t), room = steps_before<L>(end, t);
         float f[L][V], v[L][V], A[V], H[V], h[V];
         const auto pass = [&](auto careful) {
@@ -498,8 +572,8 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan(const GatedArgs a, co
             for (int k = 0; k < V; ++k) A[k] = 1.0f, H[k] = 0.0f;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
-                io.get(X, i, at.tx, at.ty, left, v[i]);
-                io.get(GATE, i, at.tx, at.ty, left, f[i]);
+                io.get(X, i, at.tx, at.ty, v[i]);
+                io.get(GATE, i, at.tx, at.ty, f[i]);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     const Factors q = factors_of(f[i][k]);
@@ -515,10 +589,15 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan(const GatedArgs a, co
         if (careful) pass(std::true_type{});
         scan_warp<V, TX, false>(at, A, H, careful, shared.totals);
         __syncthreads();
-        io.template ahead<TILE>(stops);
-        if (channel >= 0) fold_warps<V, TX, false>(shared, channel, carry);
+        io.ahead(by, stops);
+        if constexpr (CLUSTER) {
+            float here = 0.0f;
+            tell_cluster<V, TX, false>(exchange, shared, static_cast<int>(tile), gridDim.y, channel, carry, here);
+            if (channel >= 0) fold_warps<V, TX, false>(shared, channel, here);
+        }
+        else if (channel >= 0) fold_warps<V, TX, false>(shared, channel, carry);
         __syncthreads();
-        io.template advance<TILE>();
+        io.advance();
         state_before<V, TX>(at, shared, A, H, h);
         if (a.states != nullptr && at.there && room > 0 && t % KEEP == 0) store_floats<V>(a.states + (at.b * kept + t / KEEP) * a.channels + at.c, h);
         if (careful || !finite<V>(h)) {
@@ -556,7 +635,7 @@ template <typename T>
 __global__ void __launch_bounds__(SERIAL_BLOCK) k_gated_serial(const GatedArgs a) {
     const int64_t at = static_cast<int64_t>(blockIdx.x) * SERIAL_BLOCK + threadIdx.x;
     if (at >= a.batch * a.channels) return;
-    const int64_t b = at / a.channels, c = at - b * a.channels;
+    const int64_t b = batch_of(a, at), c = at - b * a.channels;
     const int64_t n = length_of(a, b), kept = (a.steps + KEEP - 1) / KEEP;
     const T* x = static_cast<const T*>(a.x.data) + b * a.x.b + c * a.x.c;
     const T* g = static_cast<const T*>(a.gate.data) + b * a.gate.b + c * a.gate.c;
@@ -594,20 +673,22 @@ __global__ void __launch_bounds__(SERIAL_BLOCK) k_gated_serial(const GatedArgs a
 
 // The gradient's walk goes from the last tile to the first. Its own scan runs against time beside the recurrence's, which starts in every
 // tile from a kept state.
-template <typename T, int V, int L, int PIECE, int STAGES>
+template <typename T, int V, int L, int PIECE, int STAGES, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs a, const Split s) {
     using IO = Tiles<T, V, L, 3, PIECE, STAGES>;
     constexpr int TX = IO::TX, TILE = IO::TILE;
     extern __shared__ uint4 ring[];
     __shared__ Between<V, TX> shared, shared_back;
+    __shared__ Exchange<V, TX, CLUSTER> exchange;
+    if constexpr (CLUSTER) cooperative_groups::this_cluster().barrier_arrive();
     const Place<V, TX> at(a);
-    const int64_t n     = at.there ? length_of(a, at.b) : 0, kept = (a.steps + KEEP - 1) / KEEP;
-    const int64_t begin = blockIdx.y * s.run, end = begin + s.run < a.steps ? begin + s.run : a.steps;
-    const int64_t tiles = (end - begin + TILE - 1) / TILE, stop = end < n ? end : n;
-    int64_t t0 = begin + (tiles > 0 ? tiles - 1 : 0) * TILE, t = t0 + at.ty * L;
+    const int64_t kept = (a.steps + KEEP - 1) / KEEP;
+    const Walk<TILE, CLUSTER, true> walk(a, s);
+    const int64_t end = walk.end, tiles = walk.tiles, by = walk.by;
+    int64_t t0 = walk.first, t = t0 + at.ty * L;
     IO io;
     const int64_t stops[3] = {set_up(io, X, a.x, a, at, t0, end), set_up(io, GATE, a.gate, a, at, t0, end), set_up(io, DY, a.y, a, at, t0, end)};
-    io.template begin<-TILE>(ring, t0, tiles, stops);
+    io.begin(ring, by, t0, tiles, stops);
     T* dx = static_cast<T*>(a.dx.data) + at.b * a.dx.b + at.c * a.dx.c + t * a.dx.t;
     T* dg = static_cast<T*>(a.d_gate.data) + at.b * a.d_gate.b + at.c * a.d_gate.c + t * a.d_gate.t;
     const bool writes_x = at.there && a.dx.data != nullptr, writes_g = at.there && a.d_gate.data != nullptr;
@@ -617,15 +698,15 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
     const int64_t of_channel = static_cast<int64_t>(blockIdx.x) * at.CHANNELS + (channel >= 0 ? channel : channel_back), all = a.batch * a.channels;
     const bool carries = channel >= 0 && of_channel < all, carries_back = channel_back >= 0 && of_channel < all;
     const float* states = a.states;
-    if (carries) states += of_channel / a.channels * kept * a.channels + of_channel % a.channels;
-    float next = carries && tiles > 0 ? states[t0 / KEEP * a.channels] : 0.0f;  // the state in front of the tile to come
+    if (carries) states += of_channel + batch_of(a, of_channel) * (kept - 1) * a.channels;
+    float next = carries && tiles > 0 && t0 < a.steps ? states[t0 / KEEP * a.channels] : 0.0f;  // the state in front of the tile to come
     float back = carries_back && a.d_last != nullptr ? a.d_last[of_channel] : 0.0f;
-    if (s.parts > 1) join_parts<V, TX, true>(a, s, at, blockIdx.y, channel_back, back, shared_back);
+    if (!CLUSTER && s.parts > 1) join_parts<V, TX, true>(a, s, at, blockIdx.y, channel_back, back, shared_back);
     __syncthreads();
-    for (int64_t tile = 0; tile < tiles; ++tile, t0 -= TILE, t -= TILE, dx -= TILE * a.dx.t, dg -= TILE * a.d_gate.t) {
+    for (int64_t tile = 0; tile < tiles; ++tile, t0 += by, t += by, dx += by * a.dx.t, dg += by * a.d_gate.t) {
         float carry = next;
-        if (carries && tile + 1 < tiles) next = states[(t0 - TILE) / KEEP * a.channels];
-        const int left = steps_before<L>(stop, t), d_left = a.y.data == nullptr ? 0 : left, room = steps_before<L>(end, t);
+        if (carries && tile + 1 < tiles) next = states[(t0 + by) / KEEP * a.channels];
+        const int room = steps_before<L>(end, t);
         float f[L][V], u[L][V], w[L][V], A[V], H[V], AR[V], R[V], h[V], c[V];
         // x and dy are read from the ring twice, here and behind the scan, instead of being held
         const auto pass = [&](auto careful) {
@@ -635,9 +716,9 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 float x[V], d[V], g[V];
-                io.get(X, i, at.tx, at.ty, left, x);
-                io.get(GATE, i, at.tx, at.ty, left, g);
-                io.get(DY, i, at.tx, at.ty, d_left, d);
+                io.get(X, i, at.tx, at.ty, x);
+                io.get(GATE, i, at.tx, at.ty, g);
+                io.get(DY, i, at.tx, at.ty, d);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     const Factors q = factors_of(g[k]);
@@ -657,9 +738,14 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
         scan_warp<V, TX, false>(at, A, H, careful, shared.totals);
         scan_warp<V, TX, true>(at, AR, R, careful, shared_back.totals);
         __syncthreads();
-        io.template ahead<-TILE>(stops);
+        io.ahead(by, stops);
         if (channel >= 0) fold_warps<V, TX, false>(shared, channel, carry);
-        if (channel_back >= 0) fold_warps<V, TX, true>(shared_back, channel_back, back);
+        if constexpr (CLUSTER) {
+            float here = 0.0f;
+            tell_cluster<V, TX, true>(exchange, shared_back, static_cast<int>(tile), gridDim.y, channel_back, back, here);
+            if (channel_back >= 0) fold_warps<V, TX, true>(shared_back, channel_back, here);
+        }
+        else if (channel_back >= 0) fold_warps<V, TX, true>(shared_back, channel_back, back);
         __syncthreads();
         state_before<V, TX>(at, shared, A, H, h);
         state_before<V, TX>(at, shared_back, AR, R, c);
@@ -670,7 +756,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 float x[V];
-                io.get(X, i, at.tx, at.ty, left, x);
+                io.get(X, i, at.tx, at.ty, x);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     w[i][k] = h[k] - x[k];
@@ -680,7 +766,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
 #pragma unroll
             for (int i = L - 1; i >= 0; --i) {
                 float d[V];
-                io.get(DY, i, at.tx, at.ty, d_left, d);
+                io.get(DY, i, at.tx, at.ty, d);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     const float total = d[k] + c[k];
@@ -699,7 +785,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
         };
         if (careful) grads(std::true_type{});
         else grads(std::false_type{});
-        io.template advance<-TILE>();
+        io.advance();
         T* to_x = dx;
         T* to_g = dg;
 #pragma unroll

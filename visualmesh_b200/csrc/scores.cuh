@@ -243,7 +243,8 @@ __global__ void __launch_bounds__(ROW_BLOCK) k_scores_own_row(const ScoresArgs a
                 *reinterpret_cast<int2*>(a.top_index + first)      = make_int2(index[0], index[1]);
                 return;
             }
-            for (int n = 0; n < a.top; ++n) a.top_log_prob[first + n] = lp[n], a.top_index[first + n] = index[n];
+            a.top_log_prob[first] = lp[0], a.top_index[first] = index[0];
+            if (a.top == 2) a.top_log_prob[first + 1] = lp[1], a.top_index[first + 1] = index[1];
         }
         else {  // every class writes itself where it stands in the order
 #pragma unroll
