@@ -86,7 +86,6 @@ constexpr int forward_steps(int vector, bool wide_type) {
 constexpr int backward_steps(int vector, bool wide_type) {
     return vector == 2 && wide_type ? 4 : 8;
 }
-constexpr int STAGES = 3;
 // Sequences of single elements from which on each has a thread: two blocks an SM.
 constexpr int64_t SERIAL_FROM = 2 * SMS * SERIAL_BLOCK;
 
@@ -97,18 +96,16 @@ struct Plan {
     bool cluster;    // the parts are blocks of a cluster, which take every so manieth tile, instead
 };
 
-// `vector` elements and `length` steps a thread; blocks that are on the card together.
+// `vector` elements and `length` steps a thread.
 Plan plan_of(int64_t all, int64_t steps, int vector, int length) {
-    Plan p{(all + 31) / 32, steps, 1, false};
-    const int64_t tile = THREADS / (32 / vector) * length, tiles = (steps + tile - 1) / tile;
+    const auto blocks_of = [&](int channels) { return (all + channels - 1) / channels; };
+    const int64_t tile = 8 * vector * length, tiles = (steps + tile - 1) / tile;  // whatever the block: 32 W threads for 4 W / vector of them along the channels
+    Plan p{blocks_of(Shape<8>::CHANNELS), steps, 1, false};
     if (p.blocks >= SMS || tiles <= 1) return p;
-    int64_t ranks = 2;
-    while (ranks < MOST_RANKS && ranks < tiles && p.blocks * ranks * 2 <= 3 * SMS) ranks *= 2;
-    if (p.blocks * ranks >= SMS || tiles <= 4 * ranks) {
-        p.parts   = ranks;
-        p.cluster = true;
-        return p;
-    }
+    const int64_t narrow = blocks_of(Shape<4>::CHANNELS);
+    int64_t ranks        = 2;
+    while (ranks < MOST_RANKS && ranks < tiles && narrow * ranks * 2 <= 6 * SMS) ranks *= 2;
+    if (narrow * ranks >= 2 * SMS || tiles <= 4 * ranks) return Plan{narrow, steps, ranks, true};
     const int64_t wanted = std::min(tiles, (2 * SMS + p.blocks - 1) / p.blocks);
     p.run                = (tiles + wanted - 1) / wanted * tile;
     p.parts              = (steps + p.run - 1) / p.run;
@@ -147,7 +144,7 @@ Access access_of(int32_t type, int64_t channels, const int64_t (&sizes)[3], std:
 
 // Launches one kernel, which is told once for a device that it may take more shared memory than every kernel may.
 template <auto KERNEL>
-void launch_tiles(dim3 grid, int ranks, int shared, cudaStream_t q, const GatedArgs& a, const Split& s) {
+void launch_tiles(dim3 grid, int threads, int ranks, int shared, cudaStream_t q, const GatedArgs& a, const Split& s) {
     static LaunchPlans plans;
     if (shared > 0) {
         plans.get([&](int) {
@@ -161,7 +158,7 @@ void launch_tiles(dim3 grid, int ranks, int shared, cudaStream_t q, const GatedA
     attribute.val.clusterDim.y = ranks;
     cudaLaunchConfig_t config{};
     config.gridDim          = grid;
-    config.blockDim         = dim3(THREADS);
+    config.blockDim         = dim3(threads);
     config.dynamicSmemBytes = shared;
     config.stream           = q;
     config.attrs            = &attribute;
@@ -228,13 +225,13 @@ vm_status vm_gated_scan(int device, int32_t type, int64_t batch, int64_t steps, 
         const dim3 grid = grid_of(p);
         with_access(type, access, [&](auto kind, auto v, auto piece) {
             using T = decltype(kind);
-            constexpr int V = decltype(v)::value, PIECE = decltype(piece)::value, L = forward_steps(V, sizeof(T) == 4), SHARED = Tiles<T, V, L, 2, PIECE, STAGES>::SHARED;
+            constexpr int V = decltype(v)::value, PIECE = decltype(piece)::value, L = forward_steps(V, sizeof(T) == 4), SHARED = Tiles<T, V, L, 2, PIECE, 8>::SHARED;
             if (p.cluster) {
-                launch_tiles<k_gated_scan<T, V, L, PIECE, STAGES, true>>(grid, static_cast<int>(p.parts), SHARED, q, a, s);
+                launch_tiles<k_gated_scan<T, V, L, PIECE, true>>(grid, Shape<4>::THREADS, static_cast<int>(p.parts), Tiles<T, V, L, 2, PIECE, 4>::SHARED, q, a, s);
                 return;
             }
-            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, L, PIECE, STAGES, false>>(grid, 1, SHARED, q, a, s);
-            launch_tiles<k_gated_scan<T, V, L, PIECE, STAGES, false>>(grid, 1, SHARED, q, a, s);
+            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, L, PIECE, false>>(grid, Shape<8>::THREADS, 1, SHARED, q, a, s);
+            launch_tiles<k_gated_scan<T, V, L, PIECE, false>>(grid, Shape<8>::THREADS, 1, SHARED, q, a, s);
         });
     }
     catch (const std::string& refused) {
@@ -275,13 +272,12 @@ vm_status vm_gated_scan_backward(int device, int32_t type, int64_t batch, int64_
         with_access(type, access, [&](auto kind, auto v, auto piece) {
             using T = decltype(kind);
             constexpr int V = decltype(v)::value, PIECE = decltype(piece)::value, L = backward_steps(V, sizeof(T) == 4);
-            constexpr int SHARED = Tiles<T, V, L, 3, PIECE, STAGES>::SHARED;
             if (p.cluster) {
-                launch_tiles<k_gated_scan_grad<T, V, L, PIECE, STAGES, true>>(grid, static_cast<int>(p.parts), SHARED, q, a, s);
+                launch_tiles<k_gated_scan_grad<T, V, L, PIECE, true>>(grid, Shape<4>::THREADS, static_cast<int>(p.parts), Tiles<T, V, L, 3, PIECE, 4>::SHARED, q, a, s);
                 return;
             }
-            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, L, PIECE, STAGES, true>>(grid, 1, Tiles<T, V, L, 2, PIECE, STAGES>::SHARED, q, a, s);
-            launch_tiles<k_gated_scan_grad<T, V, L, PIECE, STAGES, false>>(grid, 1, SHARED, q, a, s);
+            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, L, PIECE, true>>(grid, Shape<8>::THREADS, 1, Tiles<T, V, L, 2, PIECE, 8>::SHARED, q, a, s);
+            launch_tiles<k_gated_scan_grad<T, V, L, PIECE, false>>(grid, Shape<8>::THREADS, 1, Tiles<T, V, L, 3, PIECE, 8>::SHARED, q, a, s);
         });
     }
     catch (const std::string& refused) {

@@ -96,8 +96,11 @@ __device__ __forceinline__ int64_t length_of(const GatedArgs& a, int64_t b) {
 //
 // Whether a factor of 0 meets an infinity or NaN is not asked step by step: a factor of 0 leaves A = 0, an infinity or NaN leaves H without
 // a finite value (0 times it is NaN), and only then the thread goes over its steps again, with the rule.
-constexpr int WARPS   = 8;
-constexpr int THREADS = 32 * WARPS;
+// W warps of a block, which has 4 W channels: eight where the walk over time is long, four (more blocks) where a cluster shares it.
+template <int W>
+struct Shape {
+    static constexpr int THREADS = 32 * W, CHANNELS = 4 * W;
+};
 
 template <int BYTES>
 struct RawOf;
@@ -149,10 +152,9 @@ __device__ __forceinline__ void store_floats(float* to, const float (&from)[V]) 
     *reinterpret_cast<Raw<float, V>*>(to) = raw;
 }
 
-template <int V, int TX>
+template <int V, int W>
 struct Place {
-    static constexpr int SEGMENTS = 32 / TX;  // of a warp
-    static constexpr int CHANNELS = TX * V;   // of the block
+    static constexpr int TX = Shape<W>::CHANNELS / V, SEGMENTS = 32 / TX;  // threads along the channels, along time in a warp
     int warp, lane, tx, ty;
     int64_t at, b, c;  // first of the thread's channels: of all, its batch, within that
     bool there;
@@ -169,19 +171,31 @@ struct Place {
 };
 
 // Maps of the warps of a block, and the states in front of them.
-template <int V, int TX>
+template <int V, int W>
 struct alignas(16) Between {
-    float before[WARPS][TX * V];
-    float2 totals[WARPS][TX * V];
+    static constexpr int CHANNELS = Shape<W>::CHANNELS;
+    float before[W][CHANNELS];
+    float2 totals[W][CHANNELS];
 };
 
-// Whether a run of steps met nothing that needs care: no factor of 0 (nor a product that came to it), no value that is not finite.
+// Whether a factor is 0, or came to it.
 template <int V>
-__device__ __forceinline__ bool plain(const float (&A)[V], const float (&H)[V]) {
-    bool ok = true;
+__device__ __forceinline__ bool has_zero(const float (&A)[V]) {
+    bool zero = false;
 #pragma unroll
-    for (int k = 0; k < V; ++k) ok = ok && A[k] > 0.0f && fabsf(H[k]) < INFINITY;
-    return ok;
+    for (int k = 0; k < V; ++k) zero = zero || A[k] == 0.0f;
+    return zero;
+}
+// The factor of L steps, 0 only where one of theirs is.
+template <int V, int L>
+__device__ __forceinline__ void products(const float (&f)[L][V], float (&A)[V]) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) A[k] = f[0][k];
+#pragma unroll
+    for (int i = 1; i < L; ++i) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) A[k] = product(f[i][k], A[k]);
+    }
 }
 template <int V>
 __device__ __forceinline__ bool finite(const float (&v)[V]) {
@@ -192,9 +206,10 @@ __device__ __forceinline__ bool finite(const float (&v)[V]) {
 }
 
 // Scan over the lanes along time, in their order or (REVERSE) against it. In: every thread's map (A, H). Out: the map of all threads
-// before it in its own warp, and that of the whole warp in `totals`. careful: in one of the lanes a factor is 0 or a value not finite.
-template <int V, int TX, bool REVERSE>
-__device__ __forceinline__ void scan_warp(const Place<V, TX>& at, float (&A)[V], float (&H)[V], bool careful, float2 (*totals)[TX * V]) {
+// before it in its own warp, and that of the whole warp in `shared`. careful: in one of the lanes a factor is 0 or a value not finite.
+template <int V, int W, bool REVERSE>
+__device__ __forceinline__ void scan_warp(const Place<V, W>& at, float (&A)[V], float (&H)[V], bool careful, Between<V, W>& shared) {
+    constexpr int TX = Place<V, W>::TX;
     const auto from = [](float v, int d) { return REVERSE ? __shfl_down_sync(~0u, v, d) : __shfl_up_sync(~0u, v, d); };
     const auto scan = [&](auto care) {
 #pragma unroll
@@ -220,7 +235,7 @@ __device__ __forceinline__ void scan_warp(const Place<V, TX>& at, float (&A)[V],
     else scan(std::false_type{});
     if (REVERSE ? at.lane < TX : at.lane >= 32 - TX) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) totals[at.warp][at.tx * V + k] = make_float2(A[k], H[k]);
+        for (int k = 0; k < V; ++k) shared.totals[at.warp][at.tx * V + k] = make_float2(A[k], H[k]);
     }
     const bool first = REVERSE ? at.lane >= 32 - TX : at.lane < TX;
 #pragma unroll
@@ -235,19 +250,19 @@ __device__ __forceinline__ void scan_warp(const Place<V, TX>& at, float (&A)[V],
 }
 // One thread for a channel, between two barriers: the states in front of every warp, from the one in front of the block (carry), which
 // becomes the one behind it.
-template <int V, int TX, bool REVERSE>
-__device__ __forceinline__ void fold_warps(Between<V, TX>& shared, int channel, float& carry) {
+template <int V, int W, bool REVERSE>
+__device__ __forceinline__ void fold_warps(Between<V, W>& shared, int channel, float& carry) {
 #pragma unroll
-    for (int i = 0; i < WARPS; ++i) {
-        const int w              = REVERSE ? WARPS - 1 - i : i;
+    for (int i = 0; i < W; ++i) {
+        const int w              = REVERSE ? W - 1 - i : i;
         const float2 q           = shared.totals[w][channel];
         shared.before[w][channel] = carry;
         carry                    = gated(q.x, carry, q.y);
     }
 }
 // The state in front of the thread's own steps.
-template <int V, int TX>
-__device__ __forceinline__ void state_before(const Place<V, TX>& at, const Between<V, TX>& shared, const float (&A)[V], const float (&H)[V], float (&h)[V]) {
+template <int V, int W>
+__device__ __forceinline__ void state_before(const Place<V, W>& at, const Between<V, W>& shared, const float (&A)[V], const float (&H)[V], float (&h)[V]) {
     float before[V];
     load_floats<V>(&shared.before[at.warp][at.tx * V], before);
 #pragma unroll
@@ -267,6 +282,7 @@ template <typename T>
 __device__ __forceinline__ T kept_gate() {
     return from_float<T>(INFINITY);
 }
+constexpr int STAGES = 3;  // tiles of the ring
 enum { X = 0, GATE = 1, DY = 2 };  // which of the sequences of a kernel
 template <typename T, int PIECE>
 __device__ __forceinline__ typename RawOf<PIECE>::type filled(bool gate) {
@@ -283,14 +299,14 @@ template <int L>
 __device__ __forceinline__ int steps_before(int64_t stop, int64_t t) {
     return stop - t >= L ? L : stop > t ? static_cast<int>(stop - t) : 0;
 }
-// The tiles of N sequences on their way through a ring in shared memory, a row of the block's 32 channels for a step. A thread copies
+// The tiles of N sequences on their way through a ring in shared memory, a row of the block's channels for a step. A thread copies
 // pieces of PIECE bytes (16 where the sequences' places allow it) for channels of its own, and after a barrier every thread reads what it works
 // on. Rows at and behind a sequence's stop are filled instead. A row of 16-bit elements is half as wide as the banks, so that the rows of
 // every other thread along time begin in their other half (a gap behind every L rows).
 // PIECE == 0: no ring, every thread reads its own (single) elements into registers, a tile ahead.
-template <typename T, int V, int L, int N, int PIECE, int STAGES>
+template <typename T, int V, int L, int N, int PIECE, int W>
 struct Tiles {
-    static constexpr int CHANNELS = 32, TX = CHANNELS / V, TILE = THREADS / TX * L;
+    static constexpr int THREADS = Shape<W>::THREADS, CHANNELS = Shape<W>::CHANNELS, TX = CHANNELS / V, TILE = THREADS / TX * L;
     static constexpr int ROW   = CHANNELS * sizeof(T), GAP = ROW < 128 ? ROW : 0;
     static constexpr int BYTES = TILE * ROW + TILE / L * GAP;  // of a tile of one sequence
     static constexpr int SHARED = PIECE > 0 ? STAGES * N * BYTES : 0;
@@ -313,7 +329,7 @@ struct Tiles {
             const int first = threadIdx.x / ACROSS;
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                const int64_t rows = stop[n] - next;  // of the tile that are there (or more)
+                const int rows     = steps_before<TILE>(stop[n], next);  // of the tile that are there
                 const T* p         = from[n];
                 unsigned char* to  = ring + (put * N + n) * BYTES + threadIdx.x % ACROSS * PIECE;
 #pragma unroll
@@ -411,9 +427,9 @@ struct Walk {
 
 // Sequence number n of a kernel, from step `first` on: where the thread's copies begin, and (returned) behind which step of first..end-1 there
 // is nothing. What a thread copies belongs to other channels than what it works on, maybe of another batch.
-template <typename T, int V, int L, int N, int PIECE, int STAGES>
-__device__ __forceinline__ int64_t set_up(Tiles<T, V, L, N, PIECE, STAGES>& io, int n, const Sequence& q, const GatedArgs& a, const Place<V, 32 / V>& at, int64_t first, int64_t end) {
-    using IO             = Tiles<T, V, L, N, PIECE, STAGES>;
+template <typename T, int V, int L, int N, int PIECE, int W>
+__device__ __forceinline__ int64_t set_up(Tiles<T, V, L, N, PIECE, W>& io, int n, const Sequence& q, const GatedArgs& a, const Place<V, W>& at, int64_t first, int64_t end) {
+    using IO             = Tiles<T, V, L, N, PIECE, W>;
     const int64_t copied = PIECE > 0 ? blockIdx.x * int64_t(IO::CHANNELS) + threadIdx.x % IO::ACROSS * (PIECE / int(sizeof(T))) : at.at;
     io.stride[n]         = q.t;
     io.from[n]           = nullptr;
@@ -425,9 +441,9 @@ __device__ __forceinline__ int64_t set_up(Tiles<T, V, L, N, PIECE, STAGES>& io, 
 
 // The state in front of part `part` of a split sequence (or, REVERSE, behind it), from the one at the sequence's end: a thread along
 // time for every part on that side. channel: the one whose state the thread carries, or -1.
-template <int V, int TX, bool REVERSE>
-__device__ __forceinline__ void join_parts(const GatedArgs& a, const Split& s, const Place<V, TX>& at, int part, int channel, float& carry, Between<V, TX>& shared) {
-    constexpr int TY  = THREADS / TX;
+template <int V, int W, bool REVERSE>
+__device__ __forceinline__ void join_parts(const GatedArgs& a, const Split& s, const Place<V, W>& at, int part, int channel, float& carry, Between<V, W>& shared) {
+    constexpr int TY  = W * Place<V, W>::SEGMENTS;
     const int64_t all = a.batch * a.channels;
     const int begin = REVERSE ? part + 1 : 0, end = REVERSE ? s.parts : part;
     const int rounds = (end - begin + TY - 1) / TY;
@@ -442,33 +458,33 @@ __device__ __forceinline__ void join_parts(const GatedArgs& a, const Split& s, c
                 A[k] = q.x, H[k] = q.y;
             }
         }
-        scan_warp<V, TX, REVERSE>(at, A, H, !plain<V>(A, H), shared.totals);
+        scan_warp<V, W, REVERSE>(at, A, H, !finite<V>(H) || has_zero<V>(A), shared);
         __syncthreads();
-        if (channel >= 0) fold_warps<V, TX, REVERSE>(shared, channel, carry);
+        if (channel >= 0) fold_warps<V, W, REVERSE>(shared, channel, carry);
         __syncthreads();
     }
 }
 
 // Blocks of a cluster that share their channels, a tile of time each: maps of all their tiles, told to all of them.
 constexpr int MOST_RANKS = 8;
-template <int V, int TX, bool CLUSTER>
+template <int W, bool CLUSTER>
 struct Exchange {
-    float2 maps[CLUSTER ? 2 : 1][CLUSTER ? MOST_RANKS : 1][CLUSTER ? TX * V : 1];
+    float2 maps[CLUSTER ? 2 : 1][CLUSTER ? MOST_RANKS : 1][CLUSTER ? Shape<W>::CHANNELS : 1];
 };
 // Between the two barriers of a tile, by all threads of a block: the map of its tile, which the thread of a channel makes of its warps', goes to every
 // block of the cluster, and comes back as the state in front of this block's tile (here) and the one behind the whole cluster's (carry).
-template <int V, int TX, bool REVERSE>
-__device__ __forceinline__ void tell_cluster(Exchange<V, TX, true>& shared, const Between<V, TX>& between, int window, int ranks, int channel, float& carry, float& here) {
+template <int V, int W, bool REVERSE>
+__device__ __forceinline__ void tell_cluster(Exchange<W, true>& shared, const Between<V, W>& between, int window, int ranks, int channel, float& carry, float& here) {
     namespace cg = cooperative_groups;
     const cg::cluster_group cluster = cg::this_cluster();
     const int rank                  = blockIdx.y;
-    float2(*maps)[TX * V]           = shared.maps[window & 1];
+    float2(*maps)[Shape<W>::CHANNELS] = shared.maps[window & 1];
     if (window == 0) cluster.barrier_wait();  // all blocks run
     if (channel >= 0) {
         float2 whole = make_float2(1.0f, 0.0f);
 #pragma unroll
-        for (int i = 0; i < WARPS; ++i) {
-            const float2 q = between.totals[REVERSE ? WARPS - 1 - i : i][channel];
+        for (int i = 0; i < W; ++i) {
+            const float2 q = between.totals[REVERSE ? W - 1 - i : i][channel];
             whole          = make_float2(product(q.x, whole.x), gated(q.x, whole.y, q.y));
         }
         for (int to = 0; to < ranks; ++to) *cluster.map_shared_rank(&maps[rank][channel], to) = whole;
@@ -485,19 +501,20 @@ __device__ __forceinline__ void tell_cluster(Exchange<V, TX, true>& shared, cons
 }
 
 // Maps of the parts of a split sequence, of the recurrence or (REVERSE) of its gradient.
-template <typename T, int V, int L, int PIECE, int STAGES, bool REVERSE>
-__global__ void __launch_bounds__(THREADS) k_gated_summary(const GatedArgs a, const Split s) {
-    using IO = Tiles<T, V, L, 2, PIECE, STAGES>;
-    constexpr int TX = IO::TX, TILE = IO::TILE;
+template <typename T, int V, int L, int PIECE, bool REVERSE>
+__global__ void __launch_bounds__(Shape<8>::THREADS) k_gated_summary(const GatedArgs a, const Split s) {
+    constexpr int W = 8;
+    using IO        = Tiles<T, V, L, 2, PIECE, W>;
+    constexpr int TILE = IO::TILE, CHANNELS = IO::CHANNELS;
     extern __shared__ uint4 ring[];
-    __shared__ Between<V, TX> shared;
-    const Place<V, TX> at(a);
+    __shared__ Between<V, W> shared;
+    const Place<V, W> at(a);
     const Walk<TILE, false, REVERSE> walk(a, s);
     const int64_t end = walk.end, tiles = walk.tiles, first = walk.first, by = walk.by;
     IO io;
     const int64_t stops[2] = {set_up(io, X, REVERSE ? a.y : a.x, a, at, first, end), set_up(io, GATE, a.gate, a, at, first, end)};
     io.begin(ring, by, first, tiles, stops);
-    const int channel = threadIdx.x < at.CHANNELS ? threadIdx.x : -1;
+    const int channel = threadIdx.x < CHANNELS ? threadIdx.x : -1;
     float carry = 0.0f, whole = 1.0f;
     __syncthreads();
     for (int64_t tile = 0; tile < tiles; ++tile) {
@@ -521,32 +538,33 @@ __global__ void __launch_bounds__(THREADS) k_gated_summary(const GatedArgs a, co
             }
         };
         pass(std::false_type{});
-        const bool careful = !plain<V>(A, H);
+        const bool careful = !finite<V>(H) || has_zero<V>(A);
         if (careful) pass(std::true_type{});
-        scan_warp<V, TX, REVERSE>(at, A, H, careful, shared.totals);
+        scan_warp<V, W, REVERSE>(at, A, H, careful, shared);
         __syncthreads();
         io.ahead(by, stops);
         if (channel >= 0) {
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) whole = product(shared.totals[w][channel].x, whole);
-            fold_warps<V, TX, REVERSE>(shared, channel, carry);
+            for (int w = 0; w < W; ++w) whole = product(shared.totals[w][channel].x, whole);
+            fold_warps<V, W, REVERSE>(shared, channel, carry);
         }
         __syncthreads();
         io.advance();
     }
-    const int64_t of_channel = static_cast<int64_t>(blockIdx.x) * at.CHANNELS + channel, all = a.batch * a.channels;
+    const int64_t of_channel = static_cast<int64_t>(blockIdx.x) * CHANNELS + channel, all = a.batch * a.channels;
     if (channel >= 0 && of_channel < all) s.summary[blockIdx.y * all + of_channel] = make_float2(whole, carry);
 }
 
-template <typename T, int V, int L, int PIECE, int STAGES, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS, V == 1 ? 3 : 2) k_gated_scan(const GatedArgs a, const Split s) {
-    using IO = Tiles<T, V, L, 2, PIECE, STAGES>;
-    constexpr int TX = IO::TX, TILE = IO::TILE;
+template <typename T, int V, int L, int PIECE, bool CLUSTER>
+__global__ void __launch_bounds__(CLUSTER ? 128 : 256, (V == 1 ? 3 : 2) * (CLUSTER ? 2 : 1)) k_gated_scan(const GatedArgs a, const Split s) {
+    constexpr int W = CLUSTER ? 4 : 8;
+    using IO        = Tiles<T, V, L, 2, PIECE, W>;
+    constexpr int TILE = IO::TILE, CHANNELS = IO::CHANNELS;
     extern __shared__ uint4 ring[];
-    __shared__ Between<V, TX> shared;
-    __shared__ Exchange<V, TX, CLUSTER> exchange;
+    __shared__ Between<V, W> shared;
+    __shared__ Exchange<W, CLUSTER> exchange;
     if constexpr (CLUSTER) cooperative_groups::this_cluster().barrier_arrive();
-    const Place<V, TX> at(a);
+    const Place<V, W> at(a);
     const int64_t n     = at.there ? length_of(a, at.b) : 0, kept = (a.steps + KEEP - 1) / KEEP;
     const Walk<TILE, CLUSTER, false> walk(a, s);
     const int64_t begin = walk.first, end = walk.end, tiles = walk.tiles, stop = end < n ? end : n;
@@ -557,11 +575,11 @@ __global__ void __launch_bounds__(THREADS, V == 1 ? 3 : 2) k_gated_scan(const Ga
     int64_t t         = begin + at.ty * L;
     T* y              = static_cast<T*>(a.y.data) + at.b * a.y.b + at.c * a.y.c + t * a.y.t;
     const bool writes = at.there && a.y.data != nullptr;
-    const int64_t of_channel = static_cast<int64_t>(blockIdx.x) * at.CHANNELS + threadIdx.x;
-    const int channel        = threadIdx.x < at.CHANNELS ? threadIdx.x : -1;
+    const int64_t of_channel = static_cast<int64_t>(blockIdx.x) * CHANNELS + threadIdx.x;
+    const int channel        = threadIdx.x < CHANNELS ? threadIdx.x : -1;
     const bool carries       = channel >= 0 && of_channel < a.batch * a.channels;
     float carry              = carries && a.h0 != nullptr ? a.h0[of_channel] : 0.0f;
-    if (!CLUSTER && s.parts > 1) join_parts<V, TX, false>(a, s, at, blockIdx.y, channel, carry, shared);
+    if (!CLUSTER && s.parts > 1) join_parts<V, W, false>(a, s, at, blockIdx.y, channel, carry, shared);
     __syncthreads();
     for (int64_t tile = 0; tile < tiles; ++tile, t += by, y += by * a.y.t) {
         const int left = steps_before<L>(stop, t), room = steps_before<L>(end, t);
@@ -585,20 +603,21 @@ __global__ void __launch_bounds__(THREADS, V == 1 ? 3 : 2) k_gated_scan(const Ga
             }
         };
         pass(std::false_type{});
-        bool careful = !plain<V>(A, H);
+        const bool careful = !finite<V>(H), zero = has_zero<V>(A);
         if (careful) pass(std::true_type{});
-        scan_warp<V, TX, false>(at, A, H, careful, shared.totals);
+        else if (zero) products<V, L>(f, A);
+        scan_warp<V, W, false>(at, A, H, careful || zero, shared);
         __syncthreads();
-        io.ahead(by, stops);
         if constexpr (CLUSTER) {
             float here = 0.0f;
-            tell_cluster<V, TX, false>(exchange, shared, static_cast<int>(tile), gridDim.y, channel, carry, here);
-            if (channel >= 0) fold_warps<V, TX, false>(shared, channel, here);
+            tell_cluster<V, W, false>(exchange, shared, static_cast<int>(tile), gridDim.y, channel, carry, here);
+            if (channel >= 0) fold_warps<V, W, false>(shared, channel, here);
         }
-        else if (channel >= 0) fold_warps<V, TX, false>(shared, channel, carry);
+        else if (channel >= 0) fold_warps<V, W, false>(shared, channel, carry);
+        io.ahead(by, stops);
         __syncthreads();
         io.advance();
-        state_before<V, TX>(at, shared, A, H, h);
+        state_before<V, W>(at, shared, A, H, h);
         if (a.states != nullptr && at.there && room > 0 && t % KEEP == 0) store_floats<V>(a.states + (at.b * kept + t / KEEP) * a.channels + at.c, h);
         if (careful || !finite<V>(h)) {
 #pragma unroll
@@ -673,15 +692,16 @@ __global__ void __launch_bounds__(SERIAL_BLOCK) k_gated_serial(const GatedArgs a
 
 // The gradient's walk goes from the last tile to the first. Its own scan runs against time beside the recurrence's, which starts in every
 // tile from a kept state.
-template <typename T, int V, int L, int PIECE, int STAGES, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs a, const Split s) {
-    using IO = Tiles<T, V, L, 3, PIECE, STAGES>;
-    constexpr int TX = IO::TX, TILE = IO::TILE;
+template <typename T, int V, int L, int PIECE, bool CLUSTER>
+__global__ void __launch_bounds__(CLUSTER ? 128 : 256, CLUSTER ? 4 : 2) k_gated_scan_grad(const GatedArgs a, const Split s) {
+    constexpr int W = CLUSTER ? 4 : 8;
+    using IO        = Tiles<T, V, L, 3, PIECE, W>;
+    constexpr int TILE = IO::TILE, CHANNELS = IO::CHANNELS, THREADS = IO::THREADS;
     extern __shared__ uint4 ring[];
-    __shared__ Between<V, TX> shared, shared_back;
-    __shared__ Exchange<V, TX, CLUSTER> exchange;
+    __shared__ Between<V, W> shared, shared_back;
+    __shared__ Exchange<W, CLUSTER> exchange;
     if constexpr (CLUSTER) cooperative_groups::this_cluster().barrier_arrive();
-    const Place<V, TX> at(a);
+    const Place<V, W> at(a);
     const int64_t kept = (a.steps + KEEP - 1) / KEEP;
     const Walk<TILE, CLUSTER, true> walk(a, s);
     const int64_t end = walk.end, tiles = walk.tiles, by = walk.by;
@@ -693,15 +713,15 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
     T* dg = static_cast<T*>(a.d_gate.data) + at.b * a.d_gate.b + at.c * a.d_gate.c + t * a.d_gate.t;
     const bool writes_x = at.there && a.dx.data != nullptr, writes_g = at.there && a.d_gate.data != nullptr;
     // the first threads carry the recurrence's states, the last ones the gradient's
-    static_assert(2 * Place<V, TX>::CHANNELS <= THREADS, "a thread carries one state");
-    const int channel = threadIdx.x < at.CHANNELS ? threadIdx.x : -1, channel_back = static_cast<int>(threadIdx.x) - (THREADS - at.CHANNELS);
-    const int64_t of_channel = static_cast<int64_t>(blockIdx.x) * at.CHANNELS + (channel >= 0 ? channel : channel_back), all = a.batch * a.channels;
+    static_assert(2 * CHANNELS <= THREADS, "a thread carries one state");
+    const int channel = threadIdx.x < CHANNELS ? threadIdx.x : -1, channel_back = static_cast<int>(threadIdx.x) - (THREADS - CHANNELS);
+    const int64_t of_channel = static_cast<int64_t>(blockIdx.x) * CHANNELS + (channel >= 0 ? channel : channel_back), all = a.batch * a.channels;
     const bool carries = channel >= 0 && of_channel < all, carries_back = channel_back >= 0 && of_channel < all;
     const float* states = a.states;
     if (carries) states += of_channel + batch_of(a, of_channel) * (kept - 1) * a.channels;
     float next = carries && tiles > 0 && t0 < a.steps ? states[t0 / KEEP * a.channels] : 0.0f;  // the state in front of the tile to come
     float back = carries_back && a.d_last != nullptr ? a.d_last[of_channel] : 0.0f;
-    if (!CLUSTER && s.parts > 1) join_parts<V, TX, true>(a, s, at, blockIdx.y, channel_back, back, shared_back);
+    if (!CLUSTER && s.parts > 1) join_parts<V, W, true>(a, s, at, blockIdx.y, channel_back, back, shared_back);
     __syncthreads();
     for (int64_t tile = 0; tile < tiles; ++tile, t0 += by, t += by, dx += by * a.dx.t, dg += by * a.d_gate.t) {
         float carry = next;
@@ -731,24 +751,26 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
             }
         };
         pass(std::false_type{});
-        bool careful = !plain<V>(A, H) || !finite<V>(R);
+        bool careful    = !finite<V>(H) || !finite<V>(R);
+        const bool zero = has_zero<V>(A);
         if (careful) pass(std::true_type{});
+        else if (zero) products<V, L>(f, A);
 #pragma unroll
         for (int k = 0; k < V; ++k) AR[k] = A[k];
-        scan_warp<V, TX, false>(at, A, H, careful, shared.totals);
-        scan_warp<V, TX, true>(at, AR, R, careful, shared_back.totals);
+        scan_warp<V, W, false>(at, A, H, careful || zero, shared);
+        scan_warp<V, W, true>(at, AR, R, careful || zero, shared_back);
         __syncthreads();
-        io.ahead(by, stops);
-        if (channel >= 0) fold_warps<V, TX, false>(shared, channel, carry);
+        if (channel >= 0) fold_warps<V, W, false>(shared, channel, carry);
         if constexpr (CLUSTER) {
             float here = 0.0f;
-            tell_cluster<V, TX, true>(exchange, shared_back, static_cast<int>(tile), gridDim.y, channel_back, back, here);
-            if (channel_back >= 0) fold_warps<V, TX, true>(shared_back, channel_back, here);
+            tell_cluster<V, W, true>(exchange, shared_back, static_cast<int>(tile), gridDim.y, channel_back, back, here);
+            if (channel_back >= 0) fold_warps<V, W, true>(shared_back, channel_back, here);
         }
-        else if (channel_back >= 0) fold_warps<V, TX, true>(shared_back, channel_back, back);
+        else if (channel_back >= 0) fold_warps<V, W, true>(shared_back, channel_back, back);
+        io.ahead(by, stops);
         __syncthreads();
-        state_before<V, TX>(at, shared, A, H, h);
-        state_before<V, TX>(at, shared_back, AR, R, c);
+        state_before<V, W>(at, shared, A, H, h);
+        state_before<V, W>(at, shared_back, AR, R, c);
         careful = careful || !finite<V>(h) || !finite<V>(c);
         // w: h_(t-1) - x, then the gradient of the gate; u: to the gradient of x
         const auto grads = [&](auto care) {
@@ -788,11 +810,19 @@ __global__ void __launch_bounds__(THREADS, 2) k_gated_scan_grad(const GatedArgs 
         io.advance();
         T* to_x = dx;
         T* to_g = dg;
+        if (writes_x && writes_g && room == L) {
 #pragma unroll
-        for (int i = 0; i < L; ++i) {
-            if (writes_x && i < room) *reinterpret_cast<Raw<T, V>*>(to_x) = pack<T, V>(u[i]);
-            if (writes_g && i < room) *reinterpret_cast<Raw<T, V>*>(to_g) = pack<T, V>(w[i]);
-            to_x += a.dx.t, to_g += a.d_gate.t;
+            for (int i = 0; i < L; ++i, to_x += a.dx.t, to_g += a.d_gate.t) {
+                *reinterpret_cast<Raw<T, V>*>(to_x) = pack<T, V>(u[i]);
+                *reinterpret_cast<Raw<T, V>*>(to_g) = pack<T, V>(w[i]);
+            }
+        }
+        else {
+#pragma unroll
+            for (int i = 0; i < L; ++i, to_x += a.dx.t, to_g += a.d_gate.t) {
+                if (writes_x && i < room) *reinterpret_cast<Raw<T, V>*>(to_x) = pack<T, V>(u[i]);
+                if (writes_g && i < room) *reinterpret_cast<Raw<T, V>*>(to_g) = pack<T, V>(w[i]);
+            }
         }
     }
     if (a.d_h0 != nullptr && carries_back && blockIdx.y == 0) a.d_h0[of_channel] = back;
