@@ -142,9 +142,9 @@ Access access_of(int32_t type, int64_t channels, const int64_t (&sizes)[3], std:
     return {2, channels % wide == 0 && all(inputs, wide) ? 16 : 2 * size};
 }
 
-// Launches one kernel, which is told once for a device that it may take more shared memory than every kernel may.
+// Launches one kernel (early: while the one in front of it runs, whose results it waits for itself), which is told once for a device that it may take more shared memory than every kernel may.
 template <auto KERNEL>
-void launch_tiles(dim3 grid, int threads, int ranks, int shared, cudaStream_t q, const GatedArgs& a, const Split& s) {
+void launch_tiles(dim3 grid, int threads, int ranks, bool early, int shared, cudaStream_t q, const GatedArgs& a, const Split& s) {
     static LaunchPlans plans;
     if (shared > 0) {
         plans.get([&](int) {
@@ -152,17 +152,26 @@ void launch_tiles(dim3 grid, int threads, int ranks, int shared, cudaStream_t q,
             return LaunchPlan{};
         });
     }
-    cudaLaunchAttribute attribute{};
-    attribute.id               = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = attribute.val.clusterDim.z = 1;
-    attribute.val.clusterDim.y = ranks;
+    cudaLaunchAttribute attributes[2]{};
+    int count = 0;
+    if (ranks > 1) {
+        cudaLaunchAttribute& cluster = attributes[count++];
+        cluster.id                   = cudaLaunchAttributeClusterDimension;
+        cluster.val.clusterDim.x = cluster.val.clusterDim.z = 1;
+        cluster.val.clusterDim.y = ranks;
+    }
+    if (early) {
+        cudaLaunchAttribute& programmatic                       = attributes[count++];
+        programmatic.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+        programmatic.val.programmaticStreamSerializationAllowed = 1;
+    }
     cudaLaunchConfig_t config{};
     config.gridDim          = grid;
     config.blockDim         = dim3(threads);
     config.dynamicSmemBytes = shared;
     config.stream           = q;
-    config.attrs            = &attribute;
-    config.numAttrs         = ranks > 1 ? 1 : 0;
+    config.attrs            = attributes;
+    config.numAttrs         = count;
     VM_CUDA(cudaLaunchKernelEx(&config, KERNEL, a, s));
 }
 
@@ -227,11 +236,11 @@ vm_status vm_gated_scan(int device, int32_t type, int64_t batch, int64_t steps, 
             using T = decltype(kind);
             constexpr int V = decltype(v)::value, PIECE = decltype(piece)::value, L = forward_steps(V, sizeof(T) == 4), SHARED = Tiles<T, V, L, 2, PIECE, 8>::SHARED;
             if (p.cluster) {
-                launch_tiles<k_gated_scan<T, V, L, PIECE, true>>(grid, Shape<4>::THREADS, static_cast<int>(p.parts), Tiles<T, V, L, 2, PIECE, 4>::SHARED, q, a, s);
+                launch_tiles<k_gated_scan<T, V, L, PIECE, true>>(grid, Shape<4>::THREADS, static_cast<int>(p.parts), false, Tiles<T, V, L, 2, PIECE, 4>::SHARED, q, a, s);
                 return;
             }
-            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, L, PIECE, false>>(grid, Shape<8>::THREADS, 1, SHARED, q, a, s);
-            launch_tiles<k_gated_scan<T, V, L, PIECE, false>>(grid, Shape<8>::THREADS, 1, SHARED, q, a, s);
+            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, L, PIECE, false>>(grid, Shape<8>::THREADS, 1, false, SHARED, q, a, s);
+            launch_tiles<k_gated_scan<T, V, L, PIECE, false>>(grid, Shape<8>::THREADS, 1, p.parts > 1, SHARED, q, a, s);
         });
     }
     catch (const std::string& refused) {
@@ -273,11 +282,11 @@ vm_status vm_gated_scan_backward(int device, int32_t type, int64_t batch, int64_
             using T = decltype(kind);
             constexpr int V = decltype(v)::value, PIECE = decltype(piece)::value, L = backward_steps(V, sizeof(T) == 4);
             if (p.cluster) {
-                launch_tiles<k_gated_scan_grad<T, V, L, PIECE, true>>(grid, Shape<4>::THREADS, static_cast<int>(p.parts), Tiles<T, V, L, 3, PIECE, 4>::SHARED, q, a, s);
+                launch_tiles<k_gated_scan_grad<T, V, L, PIECE, true>>(grid, Shape<4>::THREADS, static_cast<int>(p.parts), false, Tiles<T, V, L, 3, PIECE, 4>::SHARED, q, a, s);
                 return;
             }
-            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, L, PIECE, true>>(grid, Shape<8>::THREADS, 1, Tiles<T, V, L, 2, PIECE, 8>::SHARED, q, a, s);
-            launch_tiles<k_gated_scan_grad<T, V, L, PIECE, false>>(grid, Shape<8>::THREADS, 1, Tiles<T, V, L, 3, PIECE, 8>::SHARED, q, a, s);
+            if (p.parts > 1) launch_tiles<k_gated_summary<T, V, L, PIECE, true>>(grid, Shape<8>::THREADS, 1, false, Tiles<T, V, L, 2, PIECE, 8>::SHARED, q, a, s);
+            launch_tiles<k_gated_scan_grad<T, V, L, PIECE, false>>(grid, Shape<8>::THREADS, 1, p.parts > 1, Tiles<T, V, L, 3, PIECE, 8>::SHARED, q, a, s);
         });
     }
     catch (const std::string& refused) {

@@ -445,6 +445,7 @@ template <int V, int W, bool REVERSE>
 __device__ __forceinline__ void join_parts(const GatedArgs& a, const Split& s, const Place<V, W>& at, int part, int channel, float& carry, Between<V, W>& shared) {
     constexpr int TY  = W * Place<V, W>::SEGMENTS;
     const int64_t all = a.batch * a.channels;
+    cudaGridDependencySynchronize();  // the summaries are there
     const int begin = REVERSE ? part + 1 : 0, end = REVERSE ? s.parts : part;
     const int rounds = (end - begin + TY - 1) / TY;
     for (int r = 0; r < rounds; ++r) {
@@ -508,6 +509,7 @@ __global__ void __launch_bounds__(Shape<8>::THREADS) k_gated_summary(const Gated
     constexpr int TILE = IO::TILE, CHANNELS = IO::CHANNELS;
     extern __shared__ uint4 ring[];
     __shared__ Between<V, W> shared;
+    cudaTriggerProgrammaticLaunchCompletion();  // the kernel behind this one reads its first tiles meanwhile
     const Place<V, W> at(a);
     const Walk<TILE, false, REVERSE> walk(a, s);
     const int64_t end = walk.end, tiles = walk.tiles, first = walk.first, by = walk.by;
