@@ -42,9 +42,10 @@ void with_classes(int classes, F f) {
 template <typename F>
 void with_lanes(int classes, F f) {
     using std::integral_constant;
-    if (classes <= 16) f(integral_constant<int, 4>{}, integral_constant<int, 4>{});
-    else if (classes <= 32) f(integral_constant<int, 8>{}, integral_constant<int, 4>{});
-    else if (classes <= 128) f(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+    if (classes <= 16) f(integral_constant<int, 2>{}, integral_constant<int, 8>{});
+    else if (classes <= 32) f(integral_constant<int, 4>{}, integral_constant<int, 8>{});
+    else if (classes <= 64) f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+    else if (classes <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
     else if (classes <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
     else if (classes <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
     else f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
