@@ -1,4 +1,5 @@
 // vm_scores and vm_scores_backward: checks and launches of the kernels in scores.cuh.
+#include <algorithm>
 #include <type_traits>
 
 #include "device_call.hpp"
@@ -126,7 +127,11 @@ vm_status vm_scores(int device, const void* x, int32_t type, int64_t rows, int32
             if (classes <= MOST_IN_ROWS) {
                 with_lanes(classes, [&](auto lanes, auto values) {
                     constexpr int G = decltype(lanes)::value, E = decltype(values)::value;
-                    launch_kernel(k_scores_rows<T, P, G, E>, grid_of((rows * G + ROW_BLOCK - 1) / ROW_BLOCK), ROW_BLOCK, 0, q, false, a, starts_on_16(x, row_stride, type));
+                    // as many rows for the same lanes as leave every SM two warps a scheduler
+                    const int64_t each  = std::clamp<int64_t>(rows * G / (WARP * 8 * SMS), 1, G);
+                    const int64_t block = ROWS_BLOCK / G * each;
+                    launch_kernel(k_scores_rows<T, P, G, E>, grid_of((rows + block - 1) / block), ROWS_BLOCK, ROWS_BLOCK * top * sizeof(uint2), q, false, a,
+                                  starts_on_16(x, row_stride, type), static_cast<int>(each));
                 });
                 return;
             }
@@ -135,6 +140,7 @@ vm_status vm_scores(int device, const void* x, int32_t type, int64_t rows, int32
                 constexpr bool TOP = decltype(best)::value;
                 if (blocks > 1) launch_cluster(k_scores_stream<T, P, TOP, STREAM_BLOCK, true>, grid_of(rows * blocks), blocks, q, a);
                 else if (rows < HALF_BLOCKS_FROM) launch_kernel(k_scores_stream<T, P, TOP, STREAM_BLOCK, false>, grid_of(rows), STREAM_BLOCK, 0, q, false, a, 1);
+                else if (classes * sizeof(T) / 16 < 1024) launch_kernel(k_scores_stream<T, P, TOP, WARP, false>, grid_of(rows), WARP, 0, q, false, a, 1);
                 else launch_kernel(k_scores_stream<T, P, TOP, STREAM_BLOCK / 2, false>, grid_of(rows), STREAM_BLOCK / 2, 0, q, false, a, 1);
             };
             if (top > 0) launch(std::true_type{});

@@ -10,6 +10,7 @@
 
 #include <cstdint>
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/vmcuda.h"
 #include "element.cuh"
@@ -134,7 +135,7 @@ __device__ __forceinline__ void write_top(const ScoresArgs& a, int64_t row, int 
     a.top_log_prob[row * a.top + k] = log_prob_of(value_of<PROBABILITIES>(value_of_order(order)), r);
 }
 
-constexpr int ROW_BLOCK = 256;
+constexpr int ROW_BLOCK = 256, ROWS_BLOCK = 128;
 
 // ---- up to 8 classes: a thread per row -----------------------------------------------------------------------------------------
 // C values in registers, every loop over them unrolled. Bound by instructions rather than bytes (48 bytes a row of three classes with
@@ -295,78 +296,135 @@ __device__ __forceinline__ void over_lanes(F f) {
     for (int d = G / 2; d > 0; d /= 2) f(d);
 }
 
+// The order of a 16-bit element's values in 16 bits, as order_of; never 0. And back.
+template <typename T>
+__device__ __forceinline__ uint32_t short_order_of(float x) {
+    const T e = from_float<T>(x + 0.0f);
+    uint16_t bits;
+    memcpy(&bits, &e, 2);
+    return x != x ? 0xFFFEu : (bits & 0x8000u) ? 0xFFFFu & ~static_cast<uint32_t>(bits) : bits | 0x8000u;
+}
+template <typename T>
+__device__ __forceinline__ float value_of_short_order(uint32_t order) {
+    const uint16_t bits = static_cast<uint16_t>((order & 0x8000u) ? order ^ 0x8000u : ~order);
+    T e;
+    memcpy(&e, &bits, 2);
+    return order == 0xFFFEu ? NAN : to_float(e);
+}
+
+// The lanes of a row take `each` rows one after another (G of them: a warp has 32 neighbouring rows; few rows: 1), and every lane keeps the sums
+// of one: what follows the sums (logarithms, labels, results) is then done once for all of them by all lanes, and the results lie side by
+// side. The next rows are read meanwhile.
+// The best classes are taken one by one, the largest of the lanes' (value, index) each time; of 16-bit values both are one number of 32 bits.
 template <typename T, bool PROBABILITIES, int G, int E>
-__global__ void __launch_bounds__(ROW_BLOCK) k_scores_rows(const ScoresArgs a, bool wide) {
-    const int64_t row = (static_cast<int64_t>(blockIdx.x) * ROW_BLOCK + threadIdx.x) / G;
-    const int lane    = threadIdx.x % G;
-    const bool there  = row < a.rows;
-    const int classes = there ? a.classes : 0;
-    const T* x        = static_cast<const T*>(a.x) + (there ? row : 0) * a.row_stride;
-    using Load        = RowLoad<T, G, E>;
+__global__ void __launch_bounds__(ROWS_BLOCK) k_scores_rows(const ScoresArgs a, bool wide, int each) {
+    extern __shared__ uint2 tops[];  // [warps][32][top]: order and index
+    const int64_t warp = static_cast<int64_t>(blockIdx.x) * (ROWS_BLOCK / WARP) + threadIdx.x / WARP;
+    const int lane = threadIdx.x % WARP, l = lane % G;
+    const int64_t first = (warp * (WARP / G) + lane / G) * each;  // of the rows of these lanes
+    uint2* const warp_tops = tops + threadIdx.x / WARP * WARP * a.top;
+    using Load             = RowLoad<T, G, E>;
+    const auto load        = [&](int i, float (&to)[E]) {
+        const int64_t row = first + i;
+        Load::load(static_cast<const T*>(a.x) + (row < a.rows ? row : 0) * a.row_stride, row < a.rows ? a.classes : 0, wide, l, to);
+    };
+    Sums mine{0.0f, 0.0f, 0.0f};
     float v[E];
-    Load::load(x, classes, wide, lane, v);
-
-    Sums q{0.0f, 0.0f, 0.0f};
-    if constexpr (PROBABILITIES) {
+    load(0, v);
+    for (int i = 0; i < each; ++i) {
+        float next[E];
+        if (i + 1 < each) load(i + 1, next);
+        Sums q{0.0f, 0.0f, 0.0f};
+        if constexpr (PROBABILITIES) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            if (Load::index(wide, lane, i) < classes) {
-                q.s += v[i];
-                q.w += times_log(v[i]);
+            for (int j = 0; j < E; ++j) {
+                if (Load::index(wide, l, j) < a.classes) {
+                    q.s += v[j];
+                    q.w += times_log(v[j]);
+                }
             }
         }
-    }
-    else {
-        q.m = -INFINITY;
+        else {
+            q.m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-            if (Load::index(wide, lane, i) < classes) q.m = fmaxf(q.m, v[i]);
-        over_lanes<G>([&](int d) { q.m = fmaxf(q.m, __shfl_xor_sync(~0u, q.m, d)); });
-        if (q.m == -INFINITY) q.m = 0.0f;  // then nothing is left, or only NaN
+            for (int j = 0; j < E; ++j)
+                if (Load::index(wide, l, j) < a.classes) q.m = fmaxf(q.m, v[j]);
+            over_lanes<G>([&](int d) { q.m = fmaxf(q.m, __shfl_xor_sync(~0u, q.m, d)); });
+            if (q.m == -INFINITY) q.m = 0.0f;  // then nothing is left, or only NaN
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            if (Load::index(wide, lane, i) < classes) {
-                const float t = v[i] - q.m, e = exp_of(t);
-                q.s += e;
-                q.w = fmaf(e, bounded(t), q.w);
+            for (int j = 0; j < E; ++j) {
+                if (Load::index(wide, l, j) < a.classes) {
+                    const float t = v[j] - q.m, e = exp_of(t);
+                    q.s += e;
+                    q.w = fmaf(e, bounded(t), q.w);
+                }
             }
         }
-    }
-    over_lanes<G>([&](int d) {
-        q.s += __shfl_xor_sync(~0u, q.s, d);
-        q.w += __shfl_xor_sync(~0u, q.w, d);
-    });
-    const Row r = row_of<PROBABILITIES>(q);
-    if (there && lane == 0) write_row<T, PROBABILITIES>(a, row, x, r);
+        over_lanes<G>([&](int d) {
+            q.s += __shfl_xor_sync(~0u, q.s, d);
+            q.w += __shfl_xor_sync(~0u, q.w, d);
+        });
+        if (l == i) mine = q;
 
-    if (a.top > 0) {
-        uint32_t order[E];  // 0: not there, or taken
+        if (a.top > 0) {
+            uint2* const to = warp_tops + (lane / G * G + i) * a.top;
+            uint32_t key[E];  // 0: not there, or taken
+            if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) order[i] = Load::index(wide, lane, i) < classes ? order_of(v[i]) : 0;
-        for (int k = 0; k < a.top; ++k) {
-            uint32_t best = 0;
-            int at        = 0;
+                for (int j = 0; j < E; ++j) {
+                    const int at = Load::index(wide, l, j);
+                    key[j]       = at < a.classes ? short_order_of<T>(v[j]) << 16 | (0xFFFFu - static_cast<uint32_t>(at)) : 0;
+                }
+                for (int k = 0; k < a.top; ++k) {
+                    uint32_t best = key[0];
 #pragma unroll
-            for (int i = 0; i < E; ++i) {  // a lane's indices rise with i: the first of equals stays
-                if (order[i] > best) best = order[i], at = Load::index(wide, lane, i);
-            }
-            const uint32_t mine = best;
-            const int mine_at   = at;
-            if constexpr (G == 32) {
-                best = __reduce_max_sync(~0u, mine);
-                at   = __reduce_min_sync(~0u, mine == best ? mine_at : INT32_MAX);
+                    for (int j = 1; j < E; ++j) best = max(best, key[j]);
+                    if constexpr (G == WARP) best = __reduce_max_sync(~0u, best);
+                    else over_lanes<G>([&](int d) { best = max(best, __shfl_xor_sync(~0u, best, d)); });
+#pragma unroll
+                    for (int j = 0; j < E; ++j)
+                        if (key[j] == best) key[j] = 0;
+                    if (l == 0) to[k] = make_uint2(best >> 16, 0xFFFFu - (best & 0xFFFFu));
+                }
             }
             else {
-                over_lanes<G>([&](int d) {
-                    const uint32_t o = __shfl_xor_sync(~0u, best, d);
-                    const int o_at   = __shfl_xor_sync(~0u, at, d);
-                    if (o > best || (o == best && o_at < at)) best = o, at = o_at;
-                });
-            }
 #pragma unroll
-            for (int i = 0; i < E; ++i)
-                if (Load::index(wide, lane, i) == at) order[i] = 0;
-            if (there && lane == 0) write_top<PROBABILITIES>(a, row, k, best, at, r);
+                for (int j = 0; j < E; ++j) key[j] = Load::index(wide, l, j) < a.classes ? order_of(v[j]) : 0;
+                for (int k = 0; k < a.top; ++k) {
+                    uint32_t best = key[0];
+#pragma unroll
+                    for (int j = 1; j < E; ++j) best = max(best, key[j]);
+                    if constexpr (G == WARP) best = __reduce_max_sync(~0u, best);
+                    else over_lanes<G>([&](int d) { best = max(best, __shfl_xor_sync(~0u, best, d)); });
+                    int at = INT32_MAX;
+#pragma unroll
+                    for (int j = E - 1; j >= 0; --j)  // a lane's indices rise with j: the first of equals stays
+                        if (key[j] == best) at = Load::index(wide, l, j);
+                    if constexpr (G == WARP) at = __reduce_min_sync(~0u, at);
+                    else over_lanes<G>([&](int d) { at = min(at, __shfl_xor_sync(~0u, at, d)); });
+#pragma unroll
+                    for (int j = 0; j < E; ++j)
+                        if (Load::index(wide, l, j) == at) key[j] = 0;
+                    if (l == 0) to[k] = make_uint2(best, at);
+                }
+            }
+        }
+        if (i + 1 < each) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) v[j] = next[j];
+        }
+    }
+    __syncwarp();
+    const int64_t row = first + l;
+    if (l >= each || row >= a.rows) return;
+    const Row r = row_of<PROBABILITIES>(mine);
+    write_row<T, PROBABILITIES>(a, row, static_cast<const T*>(a.x) + row * a.row_stride, r);
+    if (a.top > 0) {
+        for (int k = 0; k < a.top; ++k) {
+            const uint2 q   = warp_tops[lane * a.top + k];
+            const float x   = sizeof(T) == 2 ? value_of_short_order<std::conditional_t<sizeof(T) == 2, T, __half>>(q.x) : value_of_order(q.x);
+            a.top_index[row * a.top + k]    = static_cast<int32_t>(q.y);
+            a.top_log_prob[row * a.top + k] = log_prob_of(value_of<PROBABILITIES>(x), r);
         }
     }
 }
