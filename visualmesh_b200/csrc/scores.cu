@@ -22,7 +22,8 @@ vm_status check_rows(const void* x, int32_t type, int64_t rows, int32_t classes,
 
 constexpr int SMS          = 148;
 constexpr int MOST_OF_THREAD = 8;     // classes that a thread holds in registers
-constexpr int MOST_IN_ROWS   = 1024;  // and several lanes of a warp
+constexpr int MOST_OF_LANES  = 256;   // and several lanes of a warp
+constexpr int MOST_OF_WARP   = 1024;  // and a warp, for gradients
 
 // f(classes), as a constant
 template <typename F>
@@ -47,7 +48,12 @@ void with_lanes(int classes, F f) {
     else if (classes <= 32) f(integral_constant<int, 4>{}, integral_constant<int, 8>{});
     else if (classes <= 64) f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
     else if (classes <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
-    else if (classes <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+    else f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+}
+template <typename F>
+void with_lanes_of_gradient(int classes, F f) {
+    using std::integral_constant;
+    if (classes <= 256) with_lanes(classes, f);
     else if (classes <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
     else f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
 }
@@ -79,8 +85,9 @@ int blocks_of_row(int64_t rows, int64_t classes, int32_t type) {
     return n;
 }
 
-// Rows from which on a block of half the threads takes one: what follows a row's last piece keeps fewer threads waiting.
-constexpr int64_t HALF_BLOCKS_FROM = 8 * SMS;
+// Rows from which on a block of half the threads takes one, and pieces of 16 bytes up to which a warp alone does: what follows a row's last
+// piece keeps fewer threads waiting.
+constexpr int64_t HALF_BLOCKS_FROM = 8 * SMS, WARP_UP_TO = 1024;
 
 template <typename Kernel>
 void launch_cluster(Kernel kernel, dim3 grid, int blocks, cudaStream_t q, const ScoresArgs& a) {
@@ -124,23 +131,25 @@ vm_status vm_scores(int device, const void* x, int32_t type, int64_t rows, int32
                 });
                 return;
             }
-            if (classes <= MOST_IN_ROWS) {
+            if (classes <= MOST_OF_LANES) {
                 with_lanes(classes, [&](auto lanes, auto values) {
                     constexpr int G = decltype(lanes)::value, E = decltype(values)::value;
                     // as many rows for the same lanes as leave every SM two warps a scheduler
                     const int64_t each  = std::clamp<int64_t>(rows * G / (WARP * 8 * SMS), 1, G);
                     const int64_t block = ROWS_BLOCK / G * each;
-                    launch_kernel(k_scores_rows<T, P, G, E>, grid_of((rows + block - 1) / block), ROWS_BLOCK, ROWS_BLOCK * top * sizeof(uint2), q, false, a,
-                                  starts_on_16(x, row_stride, type), static_cast<int>(each));
+                    const auto kernel   = top > 0 ? k_scores_rows<T, P, true, G, E> : k_scores_rows<T, P, false, G, E>;
+                    launch_kernel(kernel, grid_of((rows + block - 1) / block), ROWS_BLOCK, ROWS_BLOCK * top * sizeof(uint2), q, false, a, starts_on_16(x, row_stride, type),
+                                  static_cast<int>(each));
                 });
                 return;
             }
-            const int blocks = blocks_of_row(rows, classes, type);
+            const int blocks     = blocks_of_row(rows, classes, type);
+            const int64_t pieces = classes * static_cast<int64_t>(sizeof(T)) / 16;
             const auto launch = [&](auto best) {
                 constexpr bool TOP = decltype(best)::value;
                 if (blocks > 1) launch_cluster(k_scores_stream<T, P, TOP, STREAM_BLOCK, true>, grid_of(rows * blocks), blocks, q, a);
+                else if (pieces <= STREAM_BLOCK || (pieces <= WARP_UP_TO && rows >= HALF_BLOCKS_FROM)) launch_kernel(k_scores_stream<T, P, TOP, WARP, false>, grid_of(rows), WARP, 0, q, false, a, 1);
                 else if (rows < HALF_BLOCKS_FROM) launch_kernel(k_scores_stream<T, P, TOP, STREAM_BLOCK, false>, grid_of(rows), STREAM_BLOCK, 0, q, false, a, 1);
-                else if (classes * sizeof(T) / 16 < 1024) launch_kernel(k_scores_stream<T, P, TOP, WARP, false>, grid_of(rows), WARP, 0, q, false, a, 1);
                 else launch_kernel(k_scores_stream<T, P, TOP, STREAM_BLOCK / 2, false>, grid_of(rows), STREAM_BLOCK / 2, 0, q, false, a, 1);
             };
             if (top > 0) launch(std::true_type{});
@@ -182,9 +191,9 @@ vm_status vm_scores_backward(int device, const void* x, int32_t type, int64_t ro
                 });
                 return;
             }
-            if (classes <= MOST_IN_ROWS) {
+            if (classes <= MOST_OF_WARP) {
                 const bool wide = starts_on_16(x, row_stride, type) && starts_on_16(dx, dx_row_stride, type);
-                with_lanes(classes, [&](auto lanes, auto values) {
+                with_lanes_of_gradient(classes, [&](auto lanes, auto values) {
                     constexpr int G = decltype(lanes)::value, E = decltype(values)::value;
                     launch_kernel(k_scores_grad_rows<T, P, G, E>, grid_of((rows * G + ROW_BLOCK - 1) / ROW_BLOCK), ROW_BLOCK, 0, q, false, a, wide);
                 });

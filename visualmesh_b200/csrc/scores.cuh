@@ -66,14 +66,14 @@ __device__ __forceinline__ float times_log(float x) {
     return x == 0.0f ? 0.0f : SCALE * x * __logf(x);
 }
 
-// An order of all floats in which larger values have larger keys, equal ones (0 and -0 too) the lower index the larger key, and NaN
-// the largest: 32 bits of value above 32 bits of index. No key is 0 or has all bits set.
+// An order of all floats in which larger values have larger numbers, 0 and -0 the same, and NaN the largest (adding 0 makes one zero of both
+// and one NaN, 0x7FFFFFFF, of all). No value has 0. With the index below it, the lower the larger: an order of a row's classes.
 __device__ __forceinline__ uint32_t order_of(float x) {
     const uint32_t bits = __float_as_uint(x + 0.0f);
-    return x != x ? 0xFFFFFFFEu : (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
+    return bits ^ (static_cast<uint32_t>(static_cast<int32_t>(bits) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float value_of_order(uint32_t order) {
-    return order == 0xFFFFFFFEu ? NAN : __uint_as_float((order & 0x80000000u) ? order ^ 0x80000000u : ~order);
+    return __uint_as_float(order ^ (~static_cast<uint32_t>(static_cast<int32_t>(order) >> 31) | 0x80000000u));
 }
 __device__ __forceinline__ uint64_t key_of(float x, int32_t index) {
     return static_cast<uint64_t>(order_of(x)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(index));
@@ -169,93 +169,102 @@ __device__ __forceinline__ void load_row(const T* x, bool wide, float (&to)[C]) 
 
 template <typename T, bool PROBABILITIES, int C>
 __global__ void __launch_bounds__(ROW_BLOCK) k_scores_own_row(const ScoresArgs a, bool wide, bool pairs) {
-    const int row = blockIdx.x * ROW_BLOCK + threadIdx.x;  // rows < 2^31, and so are those of the last block
-    if (row >= a.rows) return;
-    float x[C], v[C];
-    load_row<T, C>(static_cast<const T*>(a.x) + row * a.row_stride, wide, x);
-    const int64_t label = a.log_prob != nullptr ? label_of(a.labels, a.labels_64, row) : -1;
-    const int labelled  = label >= 0 && label < C ? static_cast<int>(label) : label == -1 ? -1 : -2;
+    __shared__ uint2 tops[C > 2 ? ROW_BLOCK * C : 1];
+    const int first_row = blockIdx.x * ROW_BLOCK, row = first_row + threadIdx.x;  // rows < 2^31, and so are those of the last block
+    const int rows      = static_cast<int>(a.rows - first_row < ROW_BLOCK ? a.rows - first_row : ROW_BLOCK);
+    if (row < a.rows) {
+        float x[C], v[C];
+        load_row<T, C>(static_cast<const T*>(a.x) + row * a.row_stride, wide, x);
+        const int64_t label = a.log_prob != nullptr ? label_of(a.labels, a.labels_64, row) : -1;
+        const int labelled  = label >= 0 && label < C ? static_cast<int>(label) : label == -1 ? -1 : -2;
 
-    Sums q{0.0f, 0.0f, 0.0f};
-    if constexpr (PROBABILITIES) {
-#pragma unroll
-        for (int k = 0; k < C; ++k) {
-            v[k] = logf(x[k]);
-            q.s += x[k];
-            q.w = fmaf(SCALE * x[k], bounded_or_nan(v[k]), q.w);
-        }
-    }
-    else {
-        q.m = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < C; ++k) v[k] = x[k], q.m = fmaxf(q.m, v[k]);
-        if (q.m == -INFINITY) q.m = 0.0f;  // then nothing is left, or only NaN
-#pragma unroll
-        for (int k = 0; k < C; ++k) {
-            const float t = v[k] - q.m, e = exp_of(t);
-            q.s += e;
-            q.w = fmaf(e, bounded(t), q.w);
-        }
-    }
-    const Row r = row_of<PROBABILITIES>(q);
-    if (a.log_sum != nullptr) a.log_sum[row] = r.log_sum;
-    if (a.entropy != nullptr) a.entropy[row] = r.entropy;
-#pragma unroll
-    for (int k = 0; k < C; ++k) v[k] = log_prob_of(v[k], r);
-    if (a.log_prob != nullptr) {
-        float lp = labelled == -1 ? 0.0f : NAN;
-#pragma unroll
-        for (int k = 0; k < C; ++k)
-            if (labelled == k) lp = v[k];
-        a.log_prob[row] = lp;
-    }
-    if (a.top > 0) {
-        uint32_t order[C];
-        if (PROBABILITIES && r.l == r.l) {
-#pragma unroll
-            for (int k = 0; k < C; ++k) order[k] = __float_as_uint(x[k] + 0.0f);  // no negative ones in a row that has a distribution
-        }
-        else {
-#pragma unroll
-            for (int k = 0; k < C; ++k) order[k] = order_of(x[k]);
-        }
-        int place[C];
-#pragma unroll
-        for (int k = 0; k < C; ++k) place[k] = 0;
-#pragma unroll
-        for (int k = 0; k < C; ++k) {
-#pragma unroll
-            for (int j = k + 1; j < C; ++j) {
-                const bool behind = order[j] > order[k];
-                place[k] += behind, place[j] += !behind;
-            }
-        }
-        const int64_t first = static_cast<int64_t>(row) * a.top;
-        if (a.top <= 2) {
-            float lp[2];
-            int index[2];
+        Sums q{0.0f, 0.0f, 0.0f};
+        if constexpr (PROBABILITIES) {
 #pragma unroll
             for (int k = 0; k < C; ++k) {
-                if (place[k] == 0) lp[0] = v[k], index[0] = k;
-                if (place[k] == 1) lp[1] = v[k], index[1] = k;
+                v[k] = logf(x[k]);
+                q.s += x[k];
+                q.w = fmaf(SCALE * x[k], bounded_or_nan(v[k]), q.w);
             }
-            if (pairs) {  // two at once: half of the stores, which are what bounds rows of few classes
-                *reinterpret_cast<float2*>(a.top_log_prob + first) = make_float2(lp[0], lp[1]);
-                *reinterpret_cast<int2*>(a.top_index + first)      = make_int2(index[0], index[1]);
-                return;
-            }
-            a.top_log_prob[first] = lp[0], a.top_index[first] = index[0];
-            if (a.top == 2) a.top_log_prob[first + 1] = lp[1], a.top_index[first + 1] = index[1];
         }
-        else {  // every class writes itself where it stands in the order
+        else {
+            q.m = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < C; ++k) v[k] = x[k], q.m = fmaxf(q.m, v[k]);
+            if (q.m == -INFINITY) q.m = 0.0f;  // then nothing is left, or only NaN
+#pragma unroll
+            for (int k = 0; k < C; ++k) {
+                const float t = v[k] - q.m, e = exp_of(t);
+                q.s += e;
+                q.w = fmaf(e, bounded(t), q.w);
+            }
+        }
+        const Row r = row_of<PROBABILITIES>(q);
+        if (a.log_sum != nullptr) a.log_sum[row] = r.log_sum;
+        if (a.entropy != nullptr) a.entropy[row] = r.entropy;
+#pragma unroll
+        for (int k = 0; k < C; ++k) v[k] = log_prob_of(v[k], r);
+        if (a.log_prob != nullptr) {
+            float lp = labelled == -1 ? 0.0f : NAN;
 #pragma unroll
             for (int k = 0; k < C; ++k)
-                if (place[k] < a.top) a.top_log_prob[first + place[k]] = v[k], a.top_index[first + place[k]] = k;
+                if (labelled == k) lp = v[k];
+            a.log_prob[row] = lp;
         }
+        if (a.top > 0) {
+            uint32_t order[C];
+            if (PROBABILITIES && r.l == r.l) {
+#pragma unroll
+                for (int k = 0; k < C; ++k) order[k] = __float_as_uint(x[k] + 0.0f);  // no negative ones in a row that has a distribution
+            }
+            else {
+#pragma unroll
+                for (int k = 0; k < C; ++k) order[k] = order_of(x[k]);
+            }
+            int place[C];
+#pragma unroll
+            for (int k = 0; k < C; ++k) place[k] = 0;
+#pragma unroll
+            for (int k = 0; k < C; ++k) {
+#pragma unroll
+                for (int j = k + 1; j < C; ++j) {
+                    const bool behind = order[j] > order[k];
+                    place[k] += behind, place[j] += !behind;
+                }
+            }
+            const int64_t first = static_cast<int64_t>(row) * a.top;
+            if (a.top <= 2) {
+                float lp[2];
+                int index[2];
+#pragma unroll
+                for (int k = 0; k < C; ++k) {
+                    if (place[k] == 0) lp[0] = v[k], index[0] = k;
+                    if (place[k] == 1) lp[1] = v[k], index[1] = k;
+                }
+                if (pairs) {  // two at once: half of the stores, which are what bounds rows of few classes
+                    *reinterpret_cast<float2*>(a.top_log_prob + first) = make_float2(lp[0], lp[1]);
+                    *reinterpret_cast<int2*>(a.top_index + first)      = make_int2(index[0], index[1]);
+                }
+                else {
+                    a.top_log_prob[first] = lp[0], a.top_index[first] = index[0];
+                    if (a.top == 2) a.top_log_prob[first + 1] = lp[1], a.top_index[first + 1] = index[1];
+                }
+            }
+            else if constexpr (C > 2) {  // every class puts itself where it stands in the order
+#pragma unroll
+                for (int k = 0; k < C; ++k)
+                    if (place[k] < a.top) tops[threadIdx.x * a.top + place[k]] = make_uint2(__float_as_uint(v[k]), k);
+            }
+        }
+    }
+    if (C > 2 && a.top > 2) {  // the rows of a block lie side by side, and so do their best classes
+        __syncthreads();
+        const int64_t first = static_cast<int64_t>(first_row) * a.top;
+        for (int i = threadIdx.x; i < rows * a.top; i += ROW_BLOCK) a.top_log_prob[first + i] = __uint_as_float(tops[i].x), a.top_index[first + i] = static_cast<int32_t>(tops[i].y);
     }
 }
 
-// ---- up to 1024 classes: G lanes per row, E values a lane in registers ---------------------------------------------------------
+// ---- up to 256 classes (gradients 1024): G lanes per row, E values a lane in registers ---------------------------------------------------------
 // Lane l of a row has the values l, l + G, l + 2 G, ..., or (WIDE, G = 32, rows that begin on 16 bytes) the same with pieces of 16 bytes.
 template <typename T, int G, int E>
 struct RowLoad {
@@ -296,27 +305,20 @@ __device__ __forceinline__ void over_lanes(F f) {
     for (int d = G / 2; d > 0; d /= 2) f(d);
 }
 
-// The order of a 16-bit element's values in 16 bits, as order_of; never 0. And back.
-template <typename T>
-__device__ __forceinline__ uint32_t short_order_of(float x) {
-    const T e = from_float<T>(x + 0.0f);
-    uint16_t bits;
-    memcpy(&bits, &e, 2);
-    return x != x ? 0xFFFEu : (bits & 0x8000u) ? 0xFFFFu & ~static_cast<uint32_t>(bits) : bits | 0x8000u;
+// Order and index of up to 256 values of a 16-bit type in one number: such a value has no more than the upper 19 bits of a float. Never 0.
+__device__ __forceinline__ uint32_t short_key_of(float x, int index) {
+    return ((order_of(x) >> 5) & 0x07FFFF00u) | (255u - static_cast<uint32_t>(index));
 }
-template <typename T>
-__device__ __forceinline__ float value_of_short_order(uint32_t order) {
-    const uint16_t bits = static_cast<uint16_t>((order & 0x8000u) ? order ^ 0x8000u : ~order);
-    T e;
-    memcpy(&e, &bits, 2);
-    return order == 0xFFFEu ? NAN : to_float(e);
+__device__ __forceinline__ uint32_t order_of_short_key(uint32_t key) {
+    const uint32_t upper = (key & 0x07FFFF00u) << 5;
+    return (upper & 0x80000000u) ? upper : upper | 0x1FFFu;  // those of negative values are inverted, with ones below
 }
 
 // The lanes of a row take `each` rows one after another (G of them: a warp has 32 neighbouring rows; few rows: 1), and every lane keeps the sums
 // of one: what follows the sums (logarithms, labels, results) is then done once for all of them by all lanes, and the results lie side by
 // side. The next rows are read meanwhile.
 // The best classes are taken one by one, the largest of the lanes' (value, index) each time; of 16-bit values both are one number of 32 bits.
-template <typename T, bool PROBABILITIES, int G, int E>
+template <typename T, bool PROBABILITIES, bool TOP, int G, int E>
 __global__ void __launch_bounds__(ROWS_BLOCK) k_scores_rows(const ScoresArgs a, bool wide, int each) {
     extern __shared__ uint2 tops[];  // [warps][32][top]: order and index
     const int64_t warp = static_cast<int64_t>(blockIdx.x) * (ROWS_BLOCK / WARP) + threadIdx.x / WARP;
@@ -366,46 +368,52 @@ __global__ void __launch_bounds__(ROWS_BLOCK) k_scores_rows(const ScoresArgs a, 
         });
         if (l == i) mine = q;
 
-        if (a.top > 0) {
-            uint2* const to = warp_tops + (lane / G * G + i) * a.top;
-            uint32_t key[E];  // 0: not there, or taken
-            if constexpr (sizeof(T) == 2) {
+        if constexpr (TOP) {
+            uint2* const to = warp_tops + (lane / G * each + i) * a.top;
+            // the first is a value that equals the maximum (but in a row with NaN, which the maximum does not show)
+            int k = 0;
+            if (!PROBABILITIES && sizeof(T) == 4 && a.top == 1 && !__any_sync(~0u, q.s != q.s)) {
+                const float m = q.s > 0.0f ? q.m : -INFINITY;
+                int at        = INT32_MAX;
+#pragma unroll
+                for (int j = E - 1; j >= 0; --j)
+                    if (v[j] == m && Load::index(wide, l, j) < a.classes) at = Load::index(wide, l, j);
+                if constexpr (G == WARP) at = __reduce_min_sync(~0u, at);
+                else over_lanes<G>([&](int d) { at = min(at, __shfl_xor_sync(~0u, at, d)); });
+                if (l == 0) to[0] = make_uint2(order_of(m), at);
+                k = 1;
+            }
+            if (k < a.top) {
+                uint32_t key[E];  // 0: not there, or taken
 #pragma unroll
                 for (int j = 0; j < E; ++j) {
                     const int at = Load::index(wide, l, j);
-                    key[j]       = at < a.classes ? short_order_of<T>(v[j]) << 16 | (0xFFFFu - static_cast<uint32_t>(at)) : 0;
+                    key[j]       = at >= a.classes ? 0 : sizeof(T) == 2 ? short_key_of(v[j], at) : order_of(v[j]);
                 }
-                for (int k = 0; k < a.top; ++k) {
+                for (; k < a.top; ++k) {
                     uint32_t best = key[0];
 #pragma unroll
                     for (int j = 1; j < E; ++j) best = max(best, key[j]);
                     if constexpr (G == WARP) best = __reduce_max_sync(~0u, best);
                     else over_lanes<G>([&](int d) { best = max(best, __shfl_xor_sync(~0u, best, d)); });
+                    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-                    for (int j = 0; j < E; ++j)
-                        if (key[j] == best) key[j] = 0;
-                    if (l == 0) to[k] = make_uint2(best >> 16, 0xFFFFu - (best & 0xFFFFu));
-                }
-            }
-            else {
+                        for (int j = 0; j < E; ++j)
+                            if (key[j] == best) key[j] = 0;
+                        if (l == 0) to[k] = make_uint2(order_of_short_key(best), 255u - (best & 255u));
+                    }
+                    else {
+                        int at = INT32_MAX;
 #pragma unroll
-                for (int j = 0; j < E; ++j) key[j] = Load::index(wide, l, j) < a.classes ? order_of(v[j]) : 0;
-                for (int k = 0; k < a.top; ++k) {
-                    uint32_t best = key[0];
+                        for (int j = E - 1; j >= 0; --j)  // a lane's indices rise with j: the first of equals stays
+                            if (key[j] == best) at = Load::index(wide, l, j);
+                        if constexpr (G == WARP) at = __reduce_min_sync(~0u, at);
+                        else over_lanes<G>([&](int d) { at = min(at, __shfl_xor_sync(~0u, at, d)); });
 #pragma unroll
-                    for (int j = 1; j < E; ++j) best = max(best, key[j]);
-                    if constexpr (G == WARP) best = __reduce_max_sync(~0u, best);
-                    else over_lanes<G>([&](int d) { best = max(best, __shfl_xor_sync(~0u, best, d)); });
-                    int at = INT32_MAX;
-#pragma unroll
-                    for (int j = E - 1; j >= 0; --j)  // a lane's indices rise with j: the first of equals stays
-                        if (key[j] == best) at = Load::index(wide, l, j);
-                    if constexpr (G == WARP) at = __reduce_min_sync(~0u, at);
-                    else over_lanes<G>([&](int d) { at = min(at, __shfl_xor_sync(~0u, at, d)); });
-#pragma unroll
-                    for (int j = 0; j < E; ++j)
-                        if (Load::index(wide, l, j) == at) key[j] = 0;
-                    if (l == 0) to[k] = make_uint2(best, at);
+                        for (int j = 0; j < E; ++j)
+                            if (Load::index(wide, l, j) == at) key[j] = 0;
+                        if (l == 0) to[k] = make_uint2(best, at);
+                    }
                 }
             }
         }
@@ -416,15 +424,18 @@ __global__ void __launch_bounds__(ROWS_BLOCK) k_scores_rows(const ScoresArgs a, 
     }
     __syncwarp();
     const int64_t row = first + l;
-    if (l >= each || row >= a.rows) return;
-    const Row r = row_of<PROBABILITIES>(mine);
-    write_row<T, PROBABILITIES>(a, row, static_cast<const T*>(a.x) + row * a.row_stride, r);
-    if (a.top > 0) {
-        for (int k = 0; k < a.top; ++k) {
-            const uint2 q   = warp_tops[lane * a.top + k];
-            const float x   = sizeof(T) == 2 ? value_of_short_order<std::conditional_t<sizeof(T) == 2, T, __half>>(q.x) : value_of_order(q.x);
-            a.top_index[row * a.top + k]    = static_cast<int32_t>(q.y);
-            a.top_log_prob[row * a.top + k] = log_prob_of(value_of<PROBABILITIES>(x), r);
+    if (l < each && row < a.rows) {
+        const Row r = row_of<PROBABILITIES>(mine);
+        write_row<T, PROBABILITIES>(a, row, static_cast<const T*>(a.x) + row * a.row_stride, r);
+        uint2* const own = warp_tops + (lane / G * each + l) * a.top;
+        for (int k = 0; TOP && k < a.top; ++k) own[k].x = __float_as_uint(log_prob_of(value_of<PROBABILITIES>(value_of_order(own[k].x)), r));
+    }
+    if constexpr (TOP) {  // the rows of a warp lie side by side, and so do their best classes
+        __syncwarp();
+        const int64_t begin = warp * (WARP / G) * each, rows = min(static_cast<int64_t>(WARP / G * each), a.rows - begin);
+        for (int i = lane; i < rows * a.top; i += WARP) {
+            a.top_log_prob[begin * a.top + i] = __uint_as_float(warp_tops[i].x);
+            a.top_index[begin * a.top + i]    = static_cast<int32_t>(warp_tops[i].y);
         }
     }
 }
@@ -433,7 +444,7 @@ __global__ void __launch_bounds__(ROWS_BLOCK) k_scores_rows(const ScoresArgs a, 
 // One pass over the row in pieces of 16 bytes (the row's first and last may be shorter): a thread keeps its running maximum with the sums
 // below it, and which of its pieces held the maximum. The `top` largest then need no second pass: with the threads' maxima in order (by
 // value, then by place), every one of the row's `top` largest values lies in a thread whose maximum is among the first `top`, and is at
-// least the last of those. So `top` threads' pieces are read again (by a warp each, from the cache), what is that large is
+// least the last of those. So `top` threads' pieces are read again (from the cache), what is that large is
 // collected and the largest of it taken. Where that is more than there is room for (many of the largest in one thread's pieces) or the row holds
 // NaN, the row is searched `top` times instead.
 // Few rows: a cluster of blocks shares a row, and the first of them joins their results through its shared memory.
@@ -681,20 +692,27 @@ __global__ void __launch_bounds__(BLOCK) k_scores_stream(const ScoresArgs a, int
         if (!search) {
             const uint32_t least_order  = static_cast<uint32_t>(least >> 32);
             const int64_t least_piece   = 0xFFFFFFFFu - static_cast<uint32_t>(least);
-            for (int i = warp; i < a.top; i += BLOCK / WARP) {
-                const int64_t piece = 0xFFFFFFFFu - static_cast<uint32_t>(shared.best[i]);
-                const int64_t first = begin + (piece - begin) % BLOCK;
-                for (int64_t p = first + lane * BLOCK; p < end; p += WARP * BLOCK) {
-                    float v[N];
-                    values_of<T>(pieces.load(p, outside), v);
+            const auto collect = [&](int64_t p) {
+                float v[N];
+                values_of<T>(pieces.load(p, outside), v);
 #pragma unroll
-                    for (int k = 0; k < N; ++k) {
-                        const int64_t j      = pieces.first(p) + k;
-                        const uint32_t order = order_of(v[k]);
-                        if (j < 0 || j >= a.classes || order < least_order || (order == least_order && p > least_piece)) continue;
-                        const int at = atomicAdd(&shared.found, 1);
-                        if (at < CANDIDATES) shared.keys[at] = key_of(v[k], static_cast<int32_t>(j));
-                    }
+                for (int k = 0; k < N; ++k) {
+                    const int64_t j      = pieces.first(p) + k;
+                    const uint32_t order = order_of(v[k]);
+                    if (j < 0 || j >= a.classes || order < least_order || (order == least_order && p > least_piece)) continue;
+                    const int at = atomicAdd(&shared.found, 1);
+                    if (at < CANDIDATES) shared.keys[at] = key_of(v[k], static_cast<int32_t>(j));
+                }
+            };
+            if ((end - begin + BLOCK - 1) / BLOCK * (BLOCK / WARP) <= a.top) {  // few pieces a thread: every one of those threads reads its own
+                const uint64_t own = static_cast<uint64_t>(order_of(best)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(held));
+                for (int64_t p = begin + threadIdx.x; p < end && own >= least; p += BLOCK) collect(p);
+            }
+            else {
+                for (int i = warp; i < a.top; i += BLOCK / WARP) {
+                    const int64_t piece = 0xFFFFFFFFu - static_cast<uint32_t>(shared.best[i]);
+                    const int64_t first = begin + (piece - begin) % BLOCK;
+                    for (int64_t p = first + lane * BLOCK; p < end; p += WARP * BLOCK) collect(p);
                 }
             }
             __syncthreads();
@@ -702,7 +720,7 @@ __global__ void __launch_bounds__(BLOCK) k_scores_stream(const ScoresArgs a, int
             if (!search && warp == 0) largest_keys(shared.keys, shared.found, a.top, shared.best);
         }
         if (search) {
-            uint64_t below = ~0ull;
+            uint64_t below = 0;
             for (int k = 0; k < a.top; ++k) {
                 uint64_t most = 0;
                 for (int64_t p = begin + threadIdx.x; p < end; p += BLOCK) {
@@ -712,7 +730,7 @@ __global__ void __launch_bounds__(BLOCK) k_scores_stream(const ScoresArgs a, int
                     for (int i = 0; i < N; ++i) {
                         const int64_t j    = pieces.first(p) + i;
                         const uint64_t key = j >= 0 && j < a.classes ? key_of(v[i], static_cast<int32_t>(j)) : 0;
-                        if (key < below && key > most) most = key;
+                        if ((k == 0 || key < below) && key > most) most = key;
                     }
                 }
                 over_lanes<WARP>([&](int d) {
