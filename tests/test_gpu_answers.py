@@ -430,7 +430,18 @@ def test_scan_of_long_sequences(answers, batch, steps, channels, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("steps,channels", [(50, 8), (200, 3), (3000, 24)])
+@pytest.mark.parametrize("batch,steps,channels", [(1, 70, 76001), (30000, 67, 3), (2, 66, 40002)])
+def test_scan_of_many_sequences(answers, batch, steps, channels, dtype):
+    """Enough for a thread each, where they are single elements; states are kept twice."""
+    x, g, h0, dy, d_last = sequences(batch, steps, channels, dtype, 3)
+    g[:, 5] = -math.inf
+    lengths = torch.randint(0, steps + 1, (batch,), device="cuda", generator=generator(batch)).to(torch.int32)
+    check_scan(answers, x, g, h0, None, dy, d_last)
+    check_scan(answers, x, g, None, lengths, dy, None)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("steps,channels", [(50, 8), (200, 3), (3000, 24), (9000, 6), (60, 80001)])
 def test_scan_gates_that_drop(answers, steps, channels, dtype):
     """-inf drops the past, +inf the present, whatever is there; a gate of NaN drops nothing."""
     x, g, h0, dy, d_last = sequences(1, steps, channels, dtype, steps)
@@ -655,24 +666,31 @@ def test_refusals_of_tensors(answers):
         answers.scores(x.clone().requires_grad_())
 
 
-def everything(answers, x, labels, s, g, table, index):
-    got = answers.scores(x, labels, 3)
-    dx = answers.scores_backward(x, got, labels, got.log_prob, got.entropy)
-    scan = answers.gated_scan(s, g, keep=True)
-    grads = answers.gated_scan_backward(s, g, scan.states, scan.y, scan.last)
-    y = answers.gated_step(table, s[:, -1], g[:, -1], index)
-    return list(got) + [dx] + list(scan) + list(grads) + [y, table]
+def everything(answers, x, labels, s, g, long, table, index, few):
+    """Every operator, in launches of every kind: rows of lanes, blocks and clusters, sequences whole, in clusters and in parts, both kinds of steps."""
+    out = []
+    for rows, n in ((x, 300), (x[:, :77], 300), (x[:3], 3)):
+        got = answers.scores(rows, labels[:n], 3)
+        out += list(got) + [answers.scores_backward(rows, got, labels[:n], got.log_prob, got.entropy)]
+    for a, b in ((s, g), (long, long)):
+        scan = answers.gated_scan(a, b, keep=True)
+        out += list(scan) + list(answers.gated_scan_backward(a, b, scan.states, scan.y, scan.last))
+    rows = s.view(-1, 8)[:1800]
+    out += [answers.gated_step(table, rows, rows, index), answers.gated_step(table, rows[:40], rows[:40], few), table]
+    return out
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_graphs_streams_and_devices(answers, dtype):
     """A captured run replayed on new inputs, two graphs at once, and calls on a stream of their own give what a plain call gives."""
     def inputs(seed):
-        x, labels, _ = answers_of(300, 4099, dtype, seed)
+        x, labels, _ = answers_of(300, 16411, dtype, seed)
+        labels = labels % 77
         s, g, _, _, _ = sequences(2, 3000, 24, dtype, seed)
-        table = torch.ones((2000, 24), device="cuda")
-        index = torch.tensor([5, 7], dtype=torch.int32, device="cuda")
-        return [x, labels, s, g, table, index]
+        long = sequences(1, 9100, 16, dtype, seed)[0]
+        table = torch.ones((2000, 8), device="cuda")
+        index = torch.randint(-1, 2000, (1800,), device="cuda", generator=generator(seed)).int()
+        return [x, labels, s, g, long, table, index, index[:40].clone()]
 
     plain = {seed: [v.clone() for v in everything(answers, *inputs(seed))] for seed in (1, 2)}
     graphs = []

@@ -226,7 +226,7 @@ class BatchResult:
         def tensor(pointer, shape, kind, dtype):
             if 0 in shape:
                 return torch.empty(shape, dtype=dtype, device="cuda")
-            return torch.as_tensor(_DeviceArray(pointer, shape, kind), device="cuda")
+            return torch.as_tensor(_DeviceArray(pointer, shape, kind))  # on the device that the memory is on
 
         return {"pixel_coordinates": tensor(self.raw.pixel_coordinates, (points, 2), "<f4", torch.float32),
                 "global_indices": tensor(self.raw.global_indices, (points,), "<i4", torch.int32),
