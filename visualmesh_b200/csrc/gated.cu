@@ -86,6 +86,11 @@ constexpr int forward_steps(int vector, bool wide_type) {
 constexpr int backward_steps(int vector, bool wide_type) {
     return vector == 2 && wide_type ? 4 : 8;
 }
+// Blocks of 16 channels that an SM's registers hold.
+constexpr int forward_resident(int vector) {
+    return vector == 2 ? 4 : 6;
+}
+constexpr int BACKWARD_RESIDENT = 4;
 // Sequences of single elements from which on each has a thread: two blocks an SM.
 constexpr int64_t SERIAL_FROM = 2 * SMS * SERIAL_BLOCK;
 
@@ -96,15 +101,23 @@ struct Plan {
     bool cluster;    // the parts are blocks of a cluster, which take every so manieth tile, instead
 };
 
-// `vector` elements and `length` steps a thread.
-Plan plan_of(int64_t all, int64_t steps, int vector, int length) {
+// `vector` elements and `length` steps a thread, `resident` blocks of a cluster's kind on an SM at a time.
+//
+// Blocks of 32 channels that fill the SMs take their sequences whole. Fewer share each: with clusters of blocks of 16 channels, which read
+// everything once, or, where clusters of 8 would still leave SMs without a block and each block more than 4 tiles, as parts, which are read
+// twice. A cluster grows while all of the call's blocks run together: its blocks wait for each other's tiles, and a second round of
+// clusters costs as much as the first. Forward / backward on B200, us:
+//   3 x 1021 x 515 (97 blocks of 16, float): clusters of 4  13 / 15, of 8  10 / 20 (of which 6 and 4 blocks fit an SM)
+//   3 x 4096 x 1024 (192): clusters of 2  41 / 76, of 4  44 / 88, whole  42 / 77
+//   1 x 65537 x 64 (4): 8 parts in a cluster 40, 74 parts 18.6
+Plan plan_of(int64_t all, int64_t steps, int vector, int length, int resident) {
     const auto blocks_of = [&](int channels) { return (all + channels - 1) / channels; };
     const int64_t tile = 8 * vector * length, tiles = (steps + tile - 1) / tile;  // whatever the block: 32 W threads for 4 W / vector of them along the channels
     Plan p{blocks_of(Shape<8>::CHANNELS), steps, 1, false};
     if (p.blocks >= SMS || tiles <= 1) return p;
     const int64_t narrow = blocks_of(Shape<4>::CHANNELS);
     int64_t ranks        = 2;
-    while (ranks < MOST_RANKS && ranks < tiles && narrow * ranks * 2 <= 6 * SMS) ranks *= 2;
+    while (ranks < MOST_RANKS && ranks < tiles && narrow * ranks * 2 <= resident * SMS) ranks *= 2;
     if (narrow * ranks >= 2 * SMS || tiles <= 4 * ranks) return Plan{narrow, steps, ranks, true};
     const int64_t wanted = std::min(tiles, (2 * SMS + p.blocks - 1) / p.blocks);
     p.run                = (tiles + wanted - 1) / wanted * tile;
@@ -199,10 +212,11 @@ size_t vm_gated_workspace(int64_t batch, int64_t steps, int64_t channels) {
     const int64_t all = batch * channels;
     int64_t parts     = 1;
     for (const int vector : {1, 2})
-        for (const int length : {4, 8, 16}) {
-            const Plan p = plan_of(all, steps, vector, length);
-            if (!p.cluster) parts = std::max(parts, p.parts);
-        }
+        for (const int length : {4, 8, 16})
+            for (const int resident : {forward_resident(vector), BACKWARD_RESIDENT}) {
+                const Plan p = plan_of(all, steps, vector, length, resident);
+                if (!p.cluster) parts = std::max(parts, p.parts);
+            }
     return parts > 1 ? static_cast<size_t>(parts * all) * sizeof(float2) : 0;
 }
 
@@ -229,7 +243,7 @@ vm_status vm_gated_scan(int device, int32_t type, int64_t batch, int64_t steps, 
             with_type(type, [&](auto kind) { launch_kernel(k_gated_serial<decltype(kind)>, grid, SERIAL_BLOCK, 0, q, false, a); });
             return VM_OK;
         }
-        const Plan p    = plan_of(batch * channels, steps, access.vector, forward_steps(access.vector, type == VM_F32));
+        const Plan p    = plan_of(batch * channels, steps, access.vector, forward_steps(access.vector, type == VM_F32), forward_resident(access.vector));
         const Split s   = split_of(p, workspace);
         const dim3 grid = grid_of(p);
         with_access(type, access, [&](auto kind, auto v, auto piece) {
@@ -275,7 +289,7 @@ vm_status vm_gated_scan_backward(int device, int32_t type, int64_t batch, int64_
         a.dx = sequence(dx), a.d_gate = sequence(d_gate), a.d_h0 = d_h0;
         const auto q     = static_cast<cudaStream_t>(stream);
         const Access access = access_of(type, channels, sizes, {x, gate, dy}, {dx, d_gate}, nullptr);
-        const Plan p     = plan_of(batch * channels, steps, access.vector, backward_steps(access.vector, type == VM_F32));
+        const Plan p     = plan_of(batch * channels, steps, access.vector, backward_steps(access.vector, type == VM_F32), BACKWARD_RESIDENT);
         const Split s    = split_of(p, workspace);
         const dim3 grid  = grid_of(p);
         with_access(type, access, [&](auto kind, auto v, auto piece) {
