@@ -295,7 +295,8 @@ enum {
  * Label -1: none, log_prob is 0. Any other label outside 0..classes-1: log_prob is NaN.
  * v_j = -infinity (a probability of 0) masks a class: it adds nothing to sum and entropy and its log probability is -infinity. A row
  * with nothing else has log_sum -infinity and entropy 0. A row with NaN or +infinity (or a negative probability, or a sum of
- * probabilities beyond 2^96) has no distribution: its log_sum, entropy and log probabilities are NaN; in the order of the top values NaN comes before +infinity. */
+ * probabilities beyond 2^96) has no distribution: its log_sum, entropy and log probabilities are NaN; in the order of the top values
+ * NaN comes before +infinity. */
 VM_API vm_status vm_scores(int device,
                            const void* x,
                            int32_t type,

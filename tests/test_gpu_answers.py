@@ -40,12 +40,15 @@ def half_step(v, dtype):
 
 
 def near(got, want, tolerance):
-    """Equal where want is not finite, else within tolerance. What 32 bits cannot hold is infinite there."""
+    """Equal where want is not finite, else within tolerance. What rounds beyond got's largest number (half a step, eps / 4 of it) is infinite there."""
+    kind = torch.finfo(got.dtype)
+    limit, sign = kind.max * (1 + kind.eps / 4), torch.sign(want)
     got = got.double()
-    largest = torch.finfo(torch.float32).max
-    want = torch.where(want > largest, math.inf, torch.where(want < -largest, -math.inf, want))
+    beyond = want.abs() > limit
+    beyond |= (want.abs() + tolerance > limit) & (got == sign * math.inf)  # either is right
+    want = torch.where(beyond, sign * math.inf, want)
     fine = torch.isfinite(want)
-    same = (got == want) | (torch.isnan(got) & torch.isnan(want))
+    same = (got == want) | (torch.isnan(got) & torch.isnan(want)) | (beyond & (got.abs() + tolerance > limit) & (torch.sign(got) == sign))
     off = torch.where(fine, (got - want).abs() - tolerance, torch.zeros_like(want))
     assert bool((same | fine).all()), "values that are not finite differ"
     assert bool((off <= 0).all()), f"off by {float(((got - want).abs())[fine].max()):.3g}, {float(off[fine].max()):.3g} more than allowed"
@@ -180,6 +183,19 @@ def test_scores_of_probabilities(answers, rows, classes, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,classes", [(80001, 9), (60007, 16), (30001, 21), (20003, 50), (9001, 100), (4001, 200), (1300, 300), (1500, 2055), (400, 9000), (1200, 8300)])
+def test_scores_of_many_rows(answers, rows, classes, dtype):
+    """Rows one after another for the same lanes, and blocks of every size."""
+    x, labels, grads = answers_of(rows, classes, dtype, rows)
+    for top in (0, 1, 5):
+        got = check_scores(answers, x, labels, top)
+    check_scores_grad(answers, x, labels, got, *grads)
+    p = torch.softmax(x.float(), 1).to(dtype)
+    got = check_scores(answers, p, labels, 3, True)
+    check_scores_grad(answers, p, labels, got, *grads, True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("classes", [2, 3, 7, 32, 40, 500, 9001, 70001])
 def test_scores_masks_and_special_values(answers, classes, dtype):
     x, labels, grads = answers_of(24, classes, dtype, classes)
@@ -228,6 +244,9 @@ def test_scores_of_probabilities_that_are_none(answers, classes):
     x[7] = 2.0**-140                      # below the normal numbers
     labels[:8] = 0
     got = check_scores(answers, x, labels, 2, True)
+    large = answers.scores(torch.tensor([[2.0**90] * classes, [2.0**97] + [1.0] * (classes - 1)], device="cuda"), labels[:2], 2, True)
+    near(large.entropy[:1], torch.tensor([math.log(classes) if classes <= 64 else math.nan], dtype=torch.float64, device="cuda"), sum_error(classes) * (3 + 2 * math.log(classes)) + 2 * U * math.log(2.0**90 * classes))
+    assert bool(torch.isnan(large.entropy[1])) and bool(torch.isnan(large.log_sum[1])) and bool(torch.isnan(large.log_prob[1])) and large.top_index[1].tolist() == [0, 1]
     # gradients of rows with a distribution; 2^-140 has an inverse that 32 bits cannot hold
     keep = torch.tensor([0, 1, 2, 6, 8, 9, 10, 11], device="cuda")
     part = answers.Scores(None, got.entropy[keep].contiguous(), got.log_sum[keep].contiguous(), None, None)

@@ -103,7 +103,8 @@ struct Row {
 template <bool PROBABILITIES>
 __device__ __forceinline__ Row row_of(const Sums& q) {
     Row r{q.m, 0.0f, -INFINITY, 0.0f};
-    if (!(q.s < INFINITY) || q.w != q.w) r.m = r.l = r.log_sum = r.entropy = NAN;
+    // a sum of probabilities that leaves room for SCALE and for a logarithm
+    if (!(q.s <= (PROBABILITIES ? 7.92281625e28f : 3.402823466e38f)) || q.w != q.w) r.m = r.l = r.log_sum = r.entropy = NAN;
     else if (q.s > 0.0f) {
         // a softmax's sum is one but for roundings, d: the next term of the series is d^4 / 4
         const float d = q.s - 1.0f;
