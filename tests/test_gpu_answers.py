@@ -449,18 +449,20 @@ def test_scan_of_long_sequences(answers, batch, steps, channels, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("batch,steps,channels", [(1, 70, 76001), (30000, 67, 3), (2, 66, 40002)])
+@pytest.mark.parametrize("batch,steps,channels", [(1, 70, 76001), (30000, 67, 3), (2, 66, 40002), (1, 64, 20003), (9000, 17, 4), (2, 33, 9002), (3, 1, 8000), (5, 8, 16384)])
 def test_scan_of_many_sequences(answers, batch, steps, channels, dtype):
     """Enough for a thread each, where they are single elements; states are kept twice."""
     x, g, h0, dy, d_last = sequences(batch, steps, channels, dtype, 3)
-    g[:, 5] = -math.inf
+    g[:, steps // 5] = -math.inf
     lengths = torch.randint(0, steps + 1, (batch,), device="cuda", generator=generator(batch)).to(torch.int32)
     check_scan(answers, x, g, h0, None, dy, d_last)
     check_scan(answers, x, g, None, lengths, dy, None)
+    beside = [torch.empty(batch * channels + 1, device="cuda")[1:].view(batch, channels).copy_(v) for v in (h0, d_last)]  # no vector load fits them
+    check_scan(answers, x, g, beside[0], lengths, None, beside[1])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("steps,channels", [(50, 8), (200, 3), (3000, 24), (9000, 6), (60, 80001)])
+@pytest.mark.parametrize("steps,channels", [(50, 8), (200, 3), (3000, 24), (9000, 6), (60, 80001), (50, 20002), (300, 76000)])
 def test_scan_gates_that_drop(answers, steps, channels, dtype):
     """-inf drops the past, +inf the present, whatever is there; a gate of NaN drops nothing."""
     x, g, h0, dy, d_last = sequences(1, steps, channels, dtype, steps)

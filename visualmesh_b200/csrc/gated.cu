@@ -63,9 +63,8 @@ Sequence sequence(const vm_sequence* s) {
 // Rows of a step among which every block looks for those that name a slot before it does.
 constexpr int64_t MOST_LOOKED_THROUGH = 1024;
 
-static_assert(STEP_BLOCK == SERIAL_BLOCK, "blocks_of counts blocks of either");
-unsigned blocks_of(int64_t threads) {
-    const int64_t n = (threads + STEP_BLOCK - 1) / STEP_BLOCK;
+unsigned blocks_of(int64_t threads, int block) {
+    const int64_t n = (threads + block - 1) / block;
     if (n > INT32_MAX) throw std::string("too many elements for one call");
     return static_cast<unsigned>(n);
 }
@@ -91,8 +90,14 @@ constexpr int forward_resident(int vector) {
     return vector == 2 ? 4 : 6;
 }
 constexpr int BACKWARD_RESIDENT = 4;
-// Sequences of single elements from which on each has a thread: two blocks an SM.
-constexpr int64_t SERIAL_FROM = 2 * SMS * SERIAL_BLOCK;
+// Whether every sequence gets a thread of its own, which walks along time alone: many short ones, of which a tile over time would be mostly
+// empty. Tiles / a thread each, us: forward 64 x 204304 bf16 95 / 24, float 76 / 33; 512 x 100000 81 / 84 and 111 / 114;
+// 200 x 40000 23 / 27. Backward 64 x 204304 107 / 58 and 97 / 77, 128 x 80000 49 / 58 and 58 / 67. 64 steps of 40000 sequences forward
+// 21 / 11, backward 23 / 17; of 10000 10 / 8 and 11 / 13.
+bool serial(int64_t all, int64_t steps, bool backward) {
+    constexpr int64_t FEW = 16384, MANY = 75776, LONG = 512;
+    return (steps <= KEEP && all >= FEW) || (!backward && steps <= LONG && all >= MANY);
+}
 
 struct Plan {
     int64_t blocks;  // along the channels
@@ -141,18 +146,27 @@ template <typename F>
 void with_access(int32_t type, const Access& access, F f) {
     using std::integral_constant;
     with_type(type, [&](auto kind) {
-        constexpr int SIZE = sizeof(kind);
         if (access.piece == 16) f(kind, integral_constant<int, 2>{}, integral_constant<int, 16>{});
-        else if (access.vector == 2) f(kind, integral_constant<int, 2>{}, integral_constant<int, 2 * SIZE>{});
+        else if constexpr (sizeof(kind) == 2) {
+            if (access.vector == 2) f(kind, integral_constant<int, 2>{}, integral_constant<int, 4>{});
+            else f(kind, integral_constant<int, 1>{}, integral_constant<int, 0>{});
+        }
         else f(kind, integral_constant<int, 1>{}, integral_constant<int, 0>{});
     });
 }
-// inputs are read through the ring in pieces, outputs are written by a thread's vectors
+bool in_pairs(int32_t type, int64_t channels, const int64_t (&sizes)[3], std::initializer_list<const vm_sequence*> sequences) {
+    return channels % 2 == 0 && std::all_of(sequences.begin(), sequences.end(), [&](const vm_sequence* s) { return takes(s, type, 2, sizes); });
+}
+// Inputs are read through the ring in pieces, outputs are written by a thread's vectors. Where no piece of 16 bytes fits, single elements go
+// through registers, but pairs of 16 bits through the ring where blocks are few. Forward / backward by pairs and by single elements, us:
+// bf16 8 x 40462 x 74 117 / 165 and 155 / 201, 1 x 65536 x 66 32 / 42 and 36 / 38, but 6 x 3216 x 1710 130 / 181 and 87 / 163; float
+// 3 x 4096 x 1022 58 / 141 and 50 / 93, 1 x 16384 x 514 56 / 90 and 47 / 58.
 Access access_of(int32_t type, int64_t channels, const int64_t (&sizes)[3], std::initializer_list<const vm_sequence*> inputs, std::initializer_list<const vm_sequence*> outputs, const float* states) {
-    const int size = static_cast<int>(element_size(type)), wide = 16 / size;
-    const auto all = [&](std::initializer_list<const vm_sequence*> list, int n) { return std::all_of(list.begin(), list.end(), [&](const vm_sequence* s) { return takes(s, type, n, sizes); }); };
-    if (channels % 2 != 0 || !all(inputs, 2) || !all(outputs, 2) || !aligned(states, 8)) return {1, 0};
-    return {2, channels % wide == 0 && all(inputs, wide) ? 16 : 2 * size};
+    const int wide = 16 / static_cast<int>(element_size(type));
+    if (!in_pairs(type, channels, sizes, inputs) || !in_pairs(type, channels, sizes, outputs) || !aligned(states, 8)) return {1, 0};
+    if (channels % wide == 0 && std::all_of(inputs.begin(), inputs.end(), [&](const vm_sequence* s) { return takes(s, type, wide, sizes); })) return {2, 16};
+    if (type != VM_F32 && sizes[0] * channels < SMS * Shape<8>::CHANNELS) return {2, 4};
+    return {1, 0};
 }
 
 // Launches one kernel (early: while the one in front of it runs, whose results it waits for itself), which is told once for a device that it may take more shared memory than every kernel may.
@@ -237,12 +251,18 @@ vm_status vm_gated_scan(int device, int32_t type, int64_t batch, int64_t steps, 
         a.x = sequence(x), a.gate = sequence(gate), a.y = sequence(y);
         a.h0 = h0, a.lengths = lengths, a.last = last, a.states = states;
         const auto q       = static_cast<cudaStream_t>(stream);
-        const Access access = access_of(type, channels, sizes, {x, gate}, {y}, states);
-        if (access.vector == 1 && batch * channels >= SERIAL_FROM) {
-            const dim3 grid(blocks_of(batch * channels));
-            with_type(type, [&](auto kind) { launch_kernel(k_gated_serial<decltype(kind)>, grid, SERIAL_BLOCK, 0, q, false, a); });
+        if (serial(batch * channels, steps, false)) {
+            const auto launch = [&](auto kind, auto v) {
+                constexpr int V = decltype(v)::value;
+                launch_kernel(k_gated_serial<decltype(kind), V>, dim3(blocks_of(batch * channels / V, SERIAL_BLOCK)), SERIAL_BLOCK, 0, q, false, a);
+            };
+            with_type(type, [&](auto kind) {
+                if (in_pairs(type, channels, sizes, {x, gate, y}) && aligned(h0, 8) && aligned(last, 8) && aligned(states, 8)) launch(kind, std::integral_constant<int, 2>{});
+                else launch(kind, std::integral_constant<int, 1>{});
+            });
             return VM_OK;
         }
+        const Access access = access_of(type, channels, sizes, {x, gate}, {y}, states);
         const Plan p    = plan_of(batch * channels, steps, access.vector, forward_steps(access.vector, type == VM_F32), forward_resident(access.vector));
         const Split s   = split_of(p, workspace);
         const dim3 grid = grid_of(p);
@@ -287,7 +307,12 @@ vm_status vm_gated_scan_backward(int device, int32_t type, int64_t batch, int64_
         a.x = sequence(x), a.gate = sequence(gate), a.y = sequence(dy);
         a.lengths = lengths, a.states = const_cast<float*>(states), a.d_last = d_last;
         a.dx = sequence(dx), a.d_gate = sequence(d_gate), a.d_h0 = d_h0;
-        const auto q     = static_cast<cudaStream_t>(stream);
+        const auto q = static_cast<cudaStream_t>(stream);
+        if (serial(batch * channels, steps, true)) {
+            const dim3 grid(blocks_of(batch * channels, SERIAL_GRAD_BLOCK));
+            with_type(type, [&](auto kind) { launch_kernel(k_gated_serial_grad<decltype(kind)>, grid, SERIAL_GRAD_BLOCK, serial_shared(steps, element_size(type)), q, false, a); });
+            return VM_OK;
+        }
         const Access access = access_of(type, channels, sizes, {x, gate, dy}, {dx, d_gate}, nullptr);
         const Plan p     = plan_of(batch * channels, steps, access.vector, backward_steps(access.vector, type == VM_F32), BACKWARD_RESIDENT);
         const Split s    = split_of(p, workspace);
@@ -335,14 +360,14 @@ vm_status vm_gated_step(int device, int32_t type, int64_t rows, int64_t slots, i
         const auto q = static_cast<cudaStream_t>(stream);
         const StepArgs a{rows, slots, channels, state, state_stride, sequence(x), sequence(gate), sequence(y), index, static_cast<uint32_t*>(workspace)};
         if (needed > 0) {
-            launch_kernel(k_first_rows, dim3(blocks_of(rows)), STEP_BLOCK, 0, q, false, a);
+            launch_kernel(k_first_rows, dim3(blocks_of(rows, STEP_BLOCK)), STEP_BLOCK, 0, q, false, a);
         }
         const bool vectors = channels % 4 == 0 && takes(x, type, 4, sizes) && takes(gate, type, 4, sizes) && takes(y, type, 4, sizes) && aligned(state, 16) && state_stride % 4 == 0;
         with_type(type, [&](auto kind) {
             using T = decltype(kind);
             const auto launch = [&](auto v) {
                 constexpr int V     = decltype(v)::value;
-                const unsigned grid = blocks_of(rows * (channels / V));
+                const unsigned grid = blocks_of(rows * (channels / V), STEP_BLOCK);
                 if (index == nullptr) launch_kernel(k_gated_step<T, V, ROW_IS_SLOT>, dim3(grid), STEP_BLOCK, 0, q, false, a);
                 else if (needed == 0) launch_kernel(k_gated_step<T, V, LOOK_THROUGH>, dim3(grid), STEP_BLOCK, 0, q, false, a);
                 else launch_kernel(k_gated_step<T, V, TABLE>, dim3(grid), STEP_BLOCK, 0, q, true, a);

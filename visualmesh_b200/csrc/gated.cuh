@@ -649,47 +649,141 @@ __global__ void __launch_bounds__(CLUSTER ? 128 : 256, (V == 1 ? 3 : 2) * (CLUST
     if (a.last != nullptr && carries && blockIdx.y + 1 == gridDim.y) a.last[of_channel] = carry;
 }
 
-// Many sequences of single elements: a thread for each walks along time alone, AHEAD steps' loads in front of itself.
-constexpr int SERIAL_BLOCK = 256, AHEAD = 8;
+// Many short sequences, or single elements: a thread walks along time alone, AHEAD steps' loads in front of itself.
+constexpr int SERIAL_BLOCK = 128, AHEAD = 8;
 
-template <typename T>
+template <int BLOCK, int V>
+struct Serial {
+    int64_t at, b, c, n, kept;
+    __device__ __forceinline__ explicit Serial(const GatedArgs& a) : at((static_cast<int64_t>(blockIdx.x) * BLOCK + threadIdx.x) * V), b(0), c(0), n(0), kept((a.steps + KEEP - 1) / KEEP) {
+        if (at < a.batch * a.channels) b = batch_of(a, at), c = at - b * a.channels, n = length_of(a, b);
+    }
+    template <typename T>
+    __device__ __forceinline__ T* of(const Sequence& s, int64_t t = 0) const {
+        return static_cast<T*>(s.data) + b * s.b + c * s.c + t * s.t;
+    }
+};
+
+template <typename T, int V>
 __global__ void __launch_bounds__(SERIAL_BLOCK) k_gated_serial(const GatedArgs a) {
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * SERIAL_BLOCK + threadIdx.x;
-    if (at >= a.batch * a.channels) return;
-    const int64_t b = batch_of(a, at), c = at - b * a.channels;
-    const int64_t n = length_of(a, b), kept = (a.steps + KEEP - 1) / KEEP;
-    const T* x = static_cast<const T*>(a.x.data) + b * a.x.b + c * a.x.c;
-    const T* g = static_cast<const T*>(a.gate.data) + b * a.gate.b + c * a.gate.c;
-    T* y       = static_cast<T*>(a.y.data) + b * a.y.b + c * a.y.c;
-    T rx[AHEAD], rg[AHEAD];
+    const Serial<SERIAL_BLOCK, V> q(a);
+    if (q.at >= a.batch * a.channels) return;
+    const T* x = q.template of<const T>(a.x);
+    const T* g = q.template of<const T>(a.gate);
+    T* y       = q.template of<T>(a.y);
+    Raw<T, V> rx[AHEAD], rg[AHEAD];
     const auto load = [&](int64_t t) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            if (t + i < n) rx[i] = *x, rg[i] = *g;
+            if (t + i < q.n) rx[i] = *reinterpret_cast<const Raw<T, V>*>(x), rg[i] = *reinterpret_cast<const Raw<T, V>*>(g);
             x += a.x.t, g += a.gate.t;
         }
     };
-    float h = a.h0 != nullptr ? a.h0[at] : 0.0f;
+    float h[V] = {};
+    if (a.h0 != nullptr) load_floats<V>(a.h0 + q.at, h);
     load(0);
     for (int64_t t = 0; t < a.steps; t += AHEAD) {
-        float f[AHEAD], v[AHEAD];
+        float f[AHEAD][V], v[AHEAD][V];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const bool on   = t + i < n;
-            const Factors q = factors_of(on ? to_float(rg[i]) : 0.0f);
-            f[i] = on ? q.f : 1.0f;
-            v[i] = on ? gated(q.u, to_float(rx[i])) : 0.0f;
+            float xs[V], gs[V];
+            unpack<T, V>(rx[i], xs);
+            unpack<T, V>(rg[i], gs);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const bool on   = t + i < q.n;
+                const Factors w = factors_of(on ? gs[k] : 0.0f);
+                f[i][k] = on ? w.f : 1.0f;
+                v[i][k] = on ? gated(w.u, xs[k]) : 0.0f;
+            }
         }
         load(t + AHEAD);
-        if (a.states != nullptr && t % KEEP == 0) a.states[(b * kept + t / KEEP) * a.channels + c] = h;
+        if (a.states != nullptr && t % KEEP == 0) store_floats<V>(a.states + (q.b * q.kept + t / KEEP) * a.channels + q.c, h);
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            h = gated(f[i], h, v[i]);
-            if (a.y.data != nullptr && t + i < a.steps) *y = from_float<T>(t + i < n ? h : 0.0f);
+#pragma unroll
+            for (int k = 0; k < V; ++k) h[k] = gated(f[i][k], h[k], v[i][k]);
+            if (a.y.data != nullptr && t + i < a.steps) *reinterpret_cast<Raw<T, V>*>(y) = t + i < q.n ? pack<T, V>(h) : Raw<T, V>{};
             y += a.y.t;
         }
     }
-    if (a.last != nullptr) a.last[at] = h;
+    if (a.last != nullptr) store_floats<V>(a.last + q.at, h);
+}
+
+// The gradient of few steps: forward through them from the kept state, with h_(t-1) - x_t and the gates left in shared memory (every thread
+// has its own column), then backward.
+constexpr int SERIAL_GRAD_BLOCK = 64;
+inline size_t serial_shared(int64_t steps, size_t element) {
+    return static_cast<size_t>(steps) * SERIAL_GRAD_BLOCK * (sizeof(float) + element);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(SERIAL_GRAD_BLOCK) k_gated_serial_grad(const GatedArgs a) {
+    extern __shared__ uint4 columns[];
+    const int steps    = static_cast<int>(a.steps);  // KEEP at most
+    float* const apart = reinterpret_cast<float*>(columns) + threadIdx.x;
+    T* const gates     = reinterpret_cast<T*>(reinterpret_cast<float*>(columns) + steps * SERIAL_GRAD_BLOCK) + threadIdx.x;
+    const Serial<SERIAL_GRAD_BLOCK, 1> q(a);
+    if (q.at >= a.batch * a.channels) return;
+    const int n = static_cast<int>(q.n);
+    {
+        const T* x = q.template of<const T>(a.x);
+        const T* g = q.template of<const T>(a.gate);
+        T rx[AHEAD], rg[AHEAD], nx[AHEAD], ng[AHEAD];
+        const auto load = [&](int t) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i, x += a.x.t, g += a.gate.t)
+                if (t + i < n) nx[i] = *x, ng[i] = *g;
+        };
+        float h = n > 0 ? a.states[q.at] : 0.0f;
+        load(0);
+        for (int t = 0; t < n; t += AHEAD) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) rx[i] = nx[i], rg[i] = ng[i];
+            load(t + AHEAD);
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                if (t + i >= n) break;
+                const Factors w = factors_of(to_float(rg[i]));
+                const float xt  = to_float(rx[i]);
+                apart[(t + i) * SERIAL_GRAD_BLOCK] = h - xt;
+                gates[(t + i) * SERIAL_GRAD_BLOCK] = rg[i];
+                h = gated(w.f, h, gated(w.u, xt));
+            }
+        }
+    }
+    T* dx = q.template of<T>(a.dx, steps - 1);
+    T* dg = q.template of<T>(a.d_gate, steps - 1);
+    for (int t = steps - 1; t >= n; --t, dx -= a.dx.t, dg -= a.d_gate.t) {
+        if (a.dx.data != nullptr) *dx = from_float<T>(0.0f);
+        if (a.d_gate.data != nullptr) *dg = from_float<T>(0.0f);
+    }
+    const T* dy = q.template of<const T>(a.y, n - 1);
+    T rd[AHEAD], nd[AHEAD];
+    const auto load = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i, dy -= a.y.t) {
+            nd[i] = from_float<T>(0.0f);
+            if (a.y.data != nullptr && t - i >= 0) nd[i] = *dy;
+        }
+    };
+    float c = a.d_last != nullptr ? a.d_last[q.at] : 0.0f;
+    load(n - 1);
+    for (int t = n - 1; t >= 0; t -= AHEAD) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) rd[i] = nd[i];
+        load(t - AHEAD);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i, dx -= a.dx.t, dg -= a.d_gate.t) {
+            if (t - i < 0) break;
+            const Factors w   = factors_of(to_float(gates[(t - i) * SERIAL_GRAD_BLOCK]));
+            const float total = to_float(rd[i]) + c;
+            if (a.dx.data != nullptr) *dx = from_float<T>(gated(w.u, total));
+            if (a.d_gate.data != nullptr) *dg = from_float<T>(gated(w.f * w.u, apart[(t - i) * SERIAL_GRAD_BLOCK] * total));
+            c = gated(w.f, total);
+        }
+    }
+    if (a.d_h0 != nullptr) a.d_h0[q.at] = c;
 }
 
 // The gradient's walk goes from the last tile to the first. Its own scan runs against time beside the recurrence's, which starts in every
