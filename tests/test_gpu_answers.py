@@ -183,7 +183,7 @@ def test_scores_of_probabilities(answers, rows, classes, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,classes", [(80001, 9), (60007, 16), (30001, 21), (20003, 50), (9001, 100), (4001, 200), (1300, 300), (1500, 2055), (400, 9000), (1200, 8300)])
+@pytest.mark.parametrize("rows,classes", [(80001, 9), (60007, 16), (30001, 21), (20003, 50), (9001, 100), (4001, 200), (1300, 300), (5003, 300), (2501, 512), (320, 2400), (40, 33000), (1500, 2055), (400, 9000), (1200, 8300)])
 def test_scores_of_many_rows(answers, rows, classes, dtype):
     """Rows one after another for the same lanes, and blocks of every size."""
     x, labels, grads = answers_of(rows, classes, dtype, rows)
@@ -603,7 +603,7 @@ def check_step(answers, state, x, g, index):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,slots,channels", [(1, 1, 1), (1, 9, 4096), (3, 3, 7), (64, 100, 64), (65, 70, 33), (300, 1000, 3), (1500, 1501, 2), (2500, 9000, 5), (5, 6, 20000)])
+@pytest.mark.parametrize("rows,slots,channels", [(1, 1, 1), (1, 9, 4096), (3, 3, 7), (64, 100, 64), (65, 70, 33), (300, 1000, 3), (250, 1000, 5), (900, 1000, 96), (1500, 1501, 2), (2500, 9000, 5), (5, 6, 20000)])
 def test_step(answers, rows, slots, channels, dtype):
     q = generator(rows)
     state = torch.randn((slots, channels), device="cuda", generator=q)
@@ -619,15 +619,18 @@ def test_step(answers, rows, slots, channels, dtype):
     check_step(answers, state, x, g, index)
 
 
-@pytest.mark.parametrize("rows", [2, 40, 1025, 3000])
-def test_step_of_a_slot_named_twice(answers, rows):
+@pytest.mark.parametrize("channels", [6, 64])
+@pytest.mark.parametrize("rows", [2, 40, 256, 257, 700, 1025, 3000])
+def test_step_of_a_slot_named_twice(answers, rows, channels):
     """The first row that names a slot advances it, each time the same."""
     q = generator(rows)
-    x, g = (torch.randn((rows, 6), device="cuda", generator=q) for _ in range(2))
+    x, g = (torch.randn((rows, channels), device="cuda", generator=q) for _ in range(2))
     index = torch.randint(0, 1 + rows // 3, (rows,), device="cuda", generator=q).int()
     for _ in range(3):
-        check_step(answers, torch.ones((rows, 6), device="cuda"), x, g, index)
-    check_step(answers, torch.ones((rows, 6), device="cuda"), x, g, torch.full_like(index, rows - 1))
+        check_step(answers, torch.ones((rows, channels), device="cuda"), x, g, index)
+    check_step(answers, torch.ones((rows, channels), device="cuda"), x, g, torch.full_like(index, rows - 1))
+    none = torch.empty((0, channels), device="cuda")
+    assert not bool(answers.gated_step(none, x, g, index).any())
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -60,8 +60,13 @@ Sequence sequence(const vm_sequence* s) {
     return Sequence{s->data, s->batch_stride, s->step_stride, s->channel_stride};
 }
 
-// Rows of a step among which every block looks for those that name a slot before it does.
-constexpr int64_t MOST_LOOKED_THROUGH = 1024;
+// Whether every block looks for earlier rows of its slots in the index itself: few rows, or rows of so many channels that a block has few of
+// them. By blocks / with a table of first rows, us: 256 rows of 3 channels 6.3 / 7.1, 512 10.4 / 6.9; 1024 of 64 6.5 / 7.0, of 512 6.2 / 7.1;
+// 2048 of 512 8.4 / 7.0.
+constexpr int64_t MOST_LOOKED_THROUGH = 256;
+bool looks_through(int64_t rows, int64_t channels) {
+    return rows <= MOST_LOOKED_THROUGH || (rows <= 4 * MOST_LOOKED_THROUGH && channels >= 64);
+}
 
 unsigned blocks_of(int64_t threads, int block) {
     const int64_t n = (threads + block - 1) / block;
@@ -359,7 +364,8 @@ vm_status vm_gated_step(int device, int32_t type, int64_t rows, int64_t slots, i
         const OnDevice on(device);
         const auto q = static_cast<cudaStream_t>(stream);
         const StepArgs a{rows, slots, channels, state, state_stride, sequence(x), sequence(gate), sequence(y), index, static_cast<uint32_t*>(workspace)};
-        if (needed > 0) {
+        const bool table = needed > 0 && !looks_through(rows, channels);
+        if (table) {
             launch_kernel(k_first_rows, dim3(blocks_of(rows, STEP_BLOCK)), STEP_BLOCK, 0, q, false, a);
         }
         const bool vectors = channels % 4 == 0 && takes(x, type, 4, sizes) && takes(gate, type, 4, sizes) && takes(y, type, 4, sizes) && aligned(state, 16) && state_stride % 4 == 0;
@@ -368,8 +374,8 @@ vm_status vm_gated_step(int device, int32_t type, int64_t rows, int64_t slots, i
             const auto launch = [&](auto v) {
                 constexpr int V     = decltype(v)::value;
                 const unsigned grid = blocks_of(rows * (channels / V), STEP_BLOCK);
-                if (index == nullptr) launch_kernel(k_gated_step<T, V, ROW_IS_SLOT>, dim3(grid), STEP_BLOCK, 0, q, false, a);
-                else if (needed == 0) launch_kernel(k_gated_step<T, V, LOOK_THROUGH>, dim3(grid), STEP_BLOCK, 0, q, false, a);
+                if (index == nullptr || slots == 0) launch_kernel(k_gated_step<T, V, ROW_IS_SLOT>, dim3(grid), STEP_BLOCK, 0, q, false, a);
+                else if (!table) launch_kernel(k_gated_step<T, V, LOOK_THROUGH>, dim3(grid), STEP_BLOCK, 0, q, false, a);
                 else launch_kernel(k_gated_step<T, V, TABLE>, dim3(grid), STEP_BLOCK, 0, q, true, a);
             };
             if (vectors) launch(std::integral_constant<int, 4>{});

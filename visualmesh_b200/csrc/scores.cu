@@ -20,10 +20,13 @@ vm_status check_rows(const void* x, int32_t type, int64_t rows, int32_t classes,
     return VM_OK;
 }
 
-constexpr int SMS          = 148;
-constexpr int MOST_OF_THREAD = 8;     // classes that a thread holds in registers
-constexpr int MOST_OF_LANES  = 256;   // and several lanes of a warp
-constexpr int MOST_OF_WARP   = 1024;  // and a warp, for gradients
+constexpr int SMS = 148;
+// Classes that a thread holds in its registers. 1,000,000 rows of 8 floats, with the two best / their gradient: 19 / 19 us, by two lanes a row
+// 35 / 23; of 3 floats 11 / 11 and 36 / 16.
+constexpr int MOST_OF_THREAD = 8;
+// Classes that lanes of a warp share with the best of them, without, and for gradients; beyond that a warp at least streams through its row.
+// 100,000 rows of 256 floats with five best 91 us and 117; 60,000 of 512 bf16 without 33 and 44, of 1024 69 and 50; the gradient of 1024 64 and 194.
+constexpr int MOST_OF_LANES_TOP = 256, MOST_OF_LANES = 512, MOST_OF_LANES_GRADIENT = 1024;
 
 // f(classes), as a constant
 template <typename F>
@@ -40,22 +43,19 @@ void with_classes(int classes, F f) {
         default: return f(integral_constant<int, 8>{});
     }
 }
-// f(lanes of a row, values of a lane), as constants
-template <typename F>
+// f(lanes of a row, values of a lane), as constants, for up to MOST classes
+template <int MOST, typename F>
 void with_lanes(int classes, F f) {
     using std::integral_constant;
     if (classes <= 16) f(integral_constant<int, 2>{}, integral_constant<int, 8>{});
     else if (classes <= 32) f(integral_constant<int, 4>{}, integral_constant<int, 8>{});
     else if (classes <= 64) f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
     else if (classes <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
-    else f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
-}
-template <typename F>
-void with_lanes_of_gradient(int classes, F f) {
-    using std::integral_constant;
-    if (classes <= 256) with_lanes(classes, f);
-    else if (classes <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
-    else f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+    else if (MOST <= 256 || classes <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+    else if constexpr (MOST > 256) {
+        if (MOST <= 512 || classes <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+        else if constexpr (MOST > 512) f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+    }
 }
 template <typename F>
 void with_values(int32_t type, uint32_t flags, F f) {
@@ -78,16 +78,19 @@ bool starts_on_row(const void* x, int64_t stride, int classes, int32_t type) {
     return aligned(x, to) && stride * size % to == 0;
 }
 
-// Blocks of a cluster for one row: as many as keep the SMs busy with all rows' blocks, each with at least two pieces of 16 bytes a thread.
+// Blocks of a cluster for one row, where rows are so few that SMs would have none, each with at least two pieces of 16 bytes a thread: the
+// cluster's barrier and the joining cost 2 to 4 us. 4 x 131072 bf16 with five best: one block 18.9 us, 2 14.8, 4 10.9, 8 10.7; 32 x 65536
+// 13.0, 2 10.9; but 64 x 32768 9.9, 2 10.7 and 290 x 60000 15.3, 2 18.3.
 int blocks_of_row(int64_t rows, int64_t classes, int32_t type) {
     int n = 1;
-    while (n < MOST_BLOCKS && rows * n * 2 <= 4 * SMS && classes * static_cast<int64_t>(element_size(type)) / 16 / (n * 2) >= 2 * STREAM_BLOCK) n *= 2;
+    while (n < MOST_BLOCKS && rows * n * 2 <= SMS * 2 / 3 && classes * static_cast<int64_t>(element_size(type)) / 16 / (n * 2) >= 2 * STREAM_BLOCK) n *= 2;
     return n;
 }
 
 // Rows from which on a block of half the threads takes one, and pieces of 16 bytes up to which a warp alone does: what follows a row's last
-// piece keeps fewer threads waiting.
-constexpr int64_t HALF_BLOCKS_FROM = 8 * SMS, WARP_UP_TO = 1024;
+// piece keeps fewer threads waiting. bf16 with five best by 32, 128 and 256 threads, us: 300 x 2048 8.9, 7.4, 8.9; 1024 x 9000 17.0, 13.1,
+// 16.9; 1024 x 60000 91, 37.5, 39.7; 8000 x 2048 25, 40, 68; 4000 x 8192 25, 29, 40; 4000 x 12000 37.5, 35.3, 49.7; 600 x 3000 10.0, 8.9, 11.1.
+constexpr int64_t HALF_BLOCKS_FROM = 2 * SMS, WARPS_FROM = 8 * SMS, WARP_UP_TO = 1024;
 
 template <typename Kernel>
 void launch_cluster(Kernel kernel, dim3 grid, int blocks, cudaStream_t q, const ScoresArgs& a) {
@@ -131,24 +134,22 @@ vm_status vm_scores(int device, const void* x, int32_t type, int64_t rows, int32
                 });
                 return;
             }
-            if (classes <= MOST_OF_LANES) {
-                with_lanes(classes, [&](auto lanes, auto values) {
-                    constexpr int G = decltype(lanes)::value, E = decltype(values)::value;
-                    // as many rows for the same lanes as leave every SM two warps a scheduler
-                    const int64_t each  = std::clamp<int64_t>(rows * G / (WARP * 8 * SMS), 1, G);
-                    const int64_t block = ROWS_BLOCK / G * each;
-                    const auto kernel   = top > 0 ? k_scores_rows<T, P, true, G, E> : k_scores_rows<T, P, false, G, E>;
-                    launch_kernel(kernel, grid_of((rows + block - 1) / block), ROWS_BLOCK, ROWS_BLOCK * top * sizeof(uint2), q, false, a, starts_on_16(x, row_stride, type),
-                                  static_cast<int>(each));
-                });
-                return;
-            }
+            const auto launch_rows = [&](auto best, auto lanes, auto values) {
+                constexpr int G = decltype(lanes)::value, E = decltype(values)::value;
+                // as many rows for the same lanes as leave every SM two warps a scheduler
+                const int64_t each  = std::clamp<int64_t>(rows * G / (WARP * 8 * SMS), 1, G);
+                const int64_t block = ROWS_BLOCK / G * each;
+                launch_kernel(k_scores_rows<T, P, decltype(best)::value, G, E>, grid_of((rows + block - 1) / block), ROWS_BLOCK, ROWS_BLOCK * top * sizeof(uint2), q, false, a,
+                              starts_on_16(x, row_stride, type), static_cast<int>(each));
+            };
+            if (top > 0 && classes <= MOST_OF_LANES_TOP) return with_lanes<MOST_OF_LANES_TOP>(classes, [&](auto lanes, auto values) { launch_rows(std::true_type{}, lanes, values); });
+            if (top == 0 && classes <= MOST_OF_LANES) return with_lanes<MOST_OF_LANES>(classes, [&](auto lanes, auto values) { launch_rows(std::false_type{}, lanes, values); });
             const int blocks     = blocks_of_row(rows, classes, type);
             const int64_t pieces = classes * static_cast<int64_t>(sizeof(T)) / 16;
             const auto launch = [&](auto best) {
                 constexpr bool TOP = decltype(best)::value;
                 if (blocks > 1) launch_cluster(k_scores_stream<T, P, TOP, STREAM_BLOCK, true>, grid_of(rows * blocks), blocks, q, a);
-                else if (pieces <= STREAM_BLOCK || (pieces <= WARP_UP_TO && rows >= HALF_BLOCKS_FROM)) launch_kernel(k_scores_stream<T, P, TOP, WARP, false>, grid_of(rows), WARP, 0, q, false, a, 1);
+                else if (pieces <= STREAM_BLOCK || (pieces <= WARP_UP_TO && rows >= WARPS_FROM)) launch_kernel(k_scores_stream<T, P, TOP, WARP, false>, grid_of(rows), WARP, 0, q, false, a, 1);
                 else if (rows < HALF_BLOCKS_FROM) launch_kernel(k_scores_stream<T, P, TOP, STREAM_BLOCK, false>, grid_of(rows), STREAM_BLOCK, 0, q, false, a, 1);
                 else launch_kernel(k_scores_stream<T, P, TOP, STREAM_BLOCK / 2, false>, grid_of(rows), STREAM_BLOCK / 2, 0, q, false, a, 1);
             };
@@ -191,9 +192,9 @@ vm_status vm_scores_backward(int device, const void* x, int32_t type, int64_t ro
                 });
                 return;
             }
-            if (classes <= MOST_OF_WARP) {
+            if (classes <= MOST_OF_LANES_GRADIENT) {
                 const bool wide = starts_on_16(x, row_stride, type) && starts_on_16(dx, dx_row_stride, type);
-                with_lanes_of_gradient(classes, [&](auto lanes, auto values) {
+                with_lanes<MOST_OF_LANES_GRADIENT>(classes, [&](auto lanes, auto values) {
                     constexpr int G = decltype(lanes)::value, E = decltype(values)::value;
                     launch_kernel(k_scores_grad_rows<T, P, G, E>, grid_of((rows * G + ROW_BLOCK - 1) / ROW_BLOCK), ROW_BLOCK, 0, q, false, a, wide);
                 });
