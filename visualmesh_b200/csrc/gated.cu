@@ -83,7 +83,7 @@ void check_sizes(int32_t type, int64_t batch, int64_t steps, int64_t channels) {
 constexpr int SMS = 148;
 
 // A thread takes pairs of channels where they lie side by side, else single ones; a block 32 channels either way. Steps of a thread in the
-// forward and in the backward pass: what its registers hold, with 24 to 34 KB for a tile of the ring, of which there are three.
+// forward and in the backward pass: what its registers hold (128 each without a spill) and a block's shared memory, of which two fit an SM.
 constexpr int forward_steps(int vector, bool wide_type) {
     return vector == 2 && !wide_type ? 16 : 8;
 }
@@ -174,7 +174,8 @@ Access access_of(int32_t type, int64_t channels, const int64_t (&sizes)[3], std:
     return {1, 0};
 }
 
-// Launches one kernel (early: while the one in front of it runs, whose results it waits for itself), which is told once for a device that it may take more shared memory than every kernel may.
+// Launches one kernel (early: while the one in front of it runs, whose results it waits for itself), which is told once for a device that it
+// may take more shared memory than every kernel may.
 template <auto KERNEL>
 void launch_tiles(dim3 grid, int threads, int ranks, bool early, int shared, cudaStream_t q, const GatedArgs& a, const Split& s) {
     static LaunchPlans plans;

@@ -87,16 +87,24 @@ __device__ __forceinline__ int64_t length_of(const GatedArgs& a, int64_t b) {
 }
 
 // ---- tiles -------------------------------------------------------------------------------------------------------------------
-// A block owns TX * V neighbouring channels and walks over time, a tile of WARPS * 32 / TX * L steps at a time: a thread holds V channels of
-// L consecutive steps, TX threads lie along the channels, the others along time. A step h -> f h + v is an affine map, and so is every run
-// of steps (A, H): h -> A h + H. A tile is three things: the maps of the threads' own steps, a scan of the maps over the threads along time
-// (shuffles inside a warp, shared memory between the warps, one barrier), and the states of the own steps from the one that the scan gives.
-// Every element is read once and written once. Vectors come through a ring of tiles in shared memory, where every thread has its
-// own places, filled by asynchronous copies a few tiles ahead: they hold no registers and need no barrier.
+// A block of W warps owns CHANNELS = 4 W neighbouring channels and walks over time in tiles: a thread holds V channels of L consecutive
+// steps, CHANNELS / V threads lie along the channels, the others along time. A step h -> f h + v is an affine map, and so is every run of
+// steps (A, H): h -> A h + H. A tile is three things: the maps of the threads' own steps, a scan of the maps over the threads along time
+// (shuffles inside a warp, shared memory between the warps), and the states of the own steps from the one that the scan gives. Every element
+// is read once and written once.
 //
-// Whether a factor of 0 meets an infinity or NaN is not asked step by step: a factor of 0 leaves A = 0, an infinity or NaN leaves H without
-// a finite value (0 times it is NaN), and only then the thread goes over its steps again, with the rule.
-// W warps of a block, which has 4 W channels: eight where the walk over time is long, four (more blocks) where a cluster shares it.
+// Whether a factor of 0 meets an infinity or NaN is not asked step by step: an infinity or NaN leaves H without a finite value (0 times it is
+// NaN), and only then the thread goes over its steps again, with the rule.
+//
+// Two barriers a tile: behind the first the warps' maps lie in shared memory and one thread for every channel folds them, from the state that
+// it carries; behind the second the states in front of every warp are there, and the ring's next tile.
+//
+// W is 8 where a block walks alone (the more threads along time, the fewer tiles), 4 where a cluster shares a sequence: narrower blocks are
+// more of them, and a cluster need not be as large (3 x 1021 x 515 floats, forward and backward: 33 us and 29).
+// Bound by the instructions: 30 for an element forward and 60 backward (an exponential, a reciprocal, conversions, one map or two, the scan's
+// share), which take 60 % of the issue slots with 16 warps an SM (128 registers), the rest being barriers and the ring's wait. 4 x 4096 x 2048
+// forward / backward: bf16 53 / 97 us (31 / 51 at the memory's rate), float 67 / 118 (61 / 102). Clusters were slower wherever blocks fill the
+// SMs (the same in clusters of 2: 66 / 123), as were pairs of floats in one instruction (moves into even registers cost what they save).
 template <int W>
 struct Shape {
     static constexpr int THREADS = 32 * W, CHANNELS = 4 * W;
@@ -299,11 +307,13 @@ template <int L>
 __device__ __forceinline__ int steps_before(int64_t stop, int64_t t) {
     return stop - t >= L ? L : stop > t ? static_cast<int>(stop - t) : 0;
 }
-// The tiles of N sequences on their way through a ring in shared memory, a row of the block's channels for a step. A thread copies
-// pieces of PIECE bytes (16 where the sequences' places allow it) for channels of its own, and after a barrier every thread reads what it works
-// on. Rows at and behind a sequence's stop are filled instead. A row of 16-bit elements is half as wide as the banks, so that the rows of
-// every other thread along time begin in their other half (a gap behind every L rows).
-// PIECE == 0: no ring, every thread reads its own (single) elements into registers, a tile ahead.
+// The tiles of N sequences on their way through a ring in shared memory (asynchronous copies hold no registers while they are under way), a
+// row of the block's channels for a step. A thread copies pieces of PIECE bytes (16 where the sequences' places allow it) for channels of its
+// own, and after a barrier every thread reads what it works on. Rows at and behind a sequence's stop are filled instead. A row of 16-bit
+// elements is half as wide as the banks, so that the rows of every other thread along time begin in their other half (a gap behind every L
+// rows). Copies by the whole block in pieces of 16 bytes instead of every thread's own pairs: 4 x 4096 x 2048 bf16 forward and backward
+// 222 -> 150 us.
+// PIECE == 0: no ring, every thread reads its own (single) elements into registers, a tile ahead: an asynchronous copy has 4 bytes at least.
 template <typename T, int V, int L, int N, int PIECE, int W>
 struct Tiles {
     static constexpr int THREADS = Shape<W>::THREADS, CHANNELS = Shape<W>::CHANNELS, TX = CHANNELS / V, TILE = THREADS / TX * L;
@@ -501,7 +511,9 @@ __device__ __forceinline__ void tell_cluster(Exchange<W, true>& shared, const Be
     }
 }
 
-// Maps of the parts of a split sequence, of the recurrence or (REVERSE) of its gradient.
+// Maps of the parts of a split sequence, of the recurrence or (REVERSE) of its gradient. The pass behind it reads the inputs once more, mostly from
+// the cache; it starts while this one ends. 65537 x 64 bf16 (74 parts): 18.6 us for both, 20.5 one after the other, 3.8 at the memory's rate
+// and 6 for two empty launches.
 template <typename T, int V, int L, int PIECE, bool REVERSE>
 __global__ void __launch_bounds__(Shape<8>::THREADS) k_gated_summary(const GatedArgs a, const Split s) {
     constexpr int W = 8;
@@ -557,6 +569,7 @@ __global__ void __launch_bounds__(Shape<8>::THREADS) k_gated_summary(const Gated
     if (channel >= 0 && of_channel < all) s.summary[blockIdx.y * all + of_channel] = make_float2(whole, carry);
 }
 
+// y, the last state and the kept ones. Bounds of registers: 16 warps an SM for pairs (16 steps of 16-bit ones a thread), 24 for single elements.
 template <typename T, int V, int L, int PIECE, bool CLUSTER>
 __global__ void __launch_bounds__(CLUSTER ? 128 : 256, (V == 1 ? 3 : 2) * (CLUSTER ? 2 : 1)) k_gated_scan(const GatedArgs a, const Split s) {
     constexpr int W = CLUSTER ? 4 : 8;
@@ -649,7 +662,8 @@ __global__ void __launch_bounds__(CLUSTER ? 128 : 256, (V == 1 ? 3 : 2) * (CLUST
     if (a.last != nullptr && carries && blockIdx.y + 1 == gridDim.y) a.last[of_channel] = carry;
 }
 
-// Many short sequences, or single elements: a thread walks along time alone, AHEAD steps' loads in front of itself.
+// Many short sequences: a thread walks along time alone, AHEAD steps' loads in front of itself. Bound by the memory: 64 x 204303 floats 33 us,
+// 24 at the memory's rate; 64 x 204304 bf16 in pairs 24 (by single elements 28), 12 at the memory's rate.
 constexpr int SERIAL_BLOCK = 128, AHEAD = 8;
 
 template <int BLOCK, int V>
@@ -711,7 +725,8 @@ __global__ void __launch_bounds__(SERIAL_BLOCK) k_gated_serial(const GatedArgs a
 }
 
 // The gradient of few steps: forward through them from the kept state, with h_(t-1) - x_t and the gates left in shared memory (every thread
-// has its own column), then backward.
+// has its own column: no two of a warp share a bank, nothing waits), then backward. Bound by latency: shared memory holds 7 blocks of 64
+// threads an SM. 64 x 204304: bf16 58 us (20 at the memory's rate), floats 77 (40); 16 x 204304 17 and 15. Pairs were no faster (58 and 101).
 constexpr int SERIAL_GRAD_BLOCK = 64;
 inline size_t serial_shared(int64_t steps, size_t element) {
     return static_cast<size_t>(steps) * SERIAL_GRAD_BLOCK * (sizeof(float) + element);
@@ -787,7 +802,8 @@ __global__ void __launch_bounds__(SERIAL_GRAD_BLOCK) k_gated_serial_grad(const G
 }
 
 // The gradient's walk goes from the last tile to the first. Its own scan runs against time beside the recurrence's, which starts in every
-// tile from a kept state.
+// tile from a kept state. x and dy are read from the ring twice: 8 steps of all that a thread has to hold would spill at 128 registers (260 us
+// instead of 222 for 4 x 4096 x 2048 forward and backward, before the copies by the whole block).
 template <typename T, int V, int L, int PIECE, bool CLUSTER>
 __global__ void __launch_bounds__(CLUSTER ? 128 : 256, CLUSTER ? 4 : 2) k_gated_scan_grad(const GatedArgs a, const Split s) {
     constexpr int W = CLUSTER ? 4 : 8;
@@ -927,6 +943,8 @@ __global__ void __launch_bounds__(CLUSTER ? 128 : 256, CLUSTER ? 4 : 2) k_gated_
 // ---- single steps ------------------------------------------------------------------------------------------------------------
 // A thread has V channels of a row. Of the rows that name a slot the first is the one that counts: a slot is one row's, whatever order they
 // run in. With few rows every block looks through the index for itself; with many, a table with the first row of every slot is made before.
+// Bound by launches: 64 rows of 2048 bf16 channels 4.7 us and 68100 of 3 floats, with the table, 7.3, where an empty call takes 4; 0.3 and 0.7
+// at the memory's rate.
 constexpr int STEP_BLOCK = 256;
 
 // The table is not cleared before: what stands in it counts where it is a row that names the slot, which is true whoever wrote it and when.

@@ -141,7 +141,8 @@ constexpr int ROW_BLOCK = 256, ROWS_BLOCK = 128;
 // ---- up to 8 classes: a thread per row -----------------------------------------------------------------------------------------
 // C values in registers, every loop over them unrolled. Bound by instructions rather than bytes (48 bytes a row of three classes with
 // their two best are 2.1 cycles of an SM's share of the memory, 270 instructions of its lanes), so each logarithm is taken once, for the sum, the
-// label and the best classes alike.
+// label and the best classes alike, and a class's place in the order is counted (C (C - 1) / 2 comparisons) instead of searched for.
+// 4,480,064 rows of three floats with two best: 46 us, 33 at the memory's rate.
 template <typename T, int C>
 __device__ __forceinline__ void load_row(const T* x, bool wide, float (&to)[C]) {
     T e[C];
@@ -319,6 +320,8 @@ __device__ __forceinline__ uint32_t order_of_short_key(uint32_t key) {
 // of one: what follows the sums (logarithms, labels, results) is then done once for all of them by all lanes, and the results lie side by
 // side. The next rows are read meanwhile.
 // The best classes are taken one by one, the largest of the lanes' (value, index) each time; of 16-bit values both are one number of 32 bits.
+// Bound by instructions: 100,000 rows of 128 floats 15 us (8 at the memory's rate), with five best 50. `each` rows instead of one: 300,000 rows of
+// 60 floats 27 -> 19 us, with two best 54 -> 38.
 template <typename T, bool PROBABILITIES, bool TOP, int G, int E>
 __global__ void __launch_bounds__(ROWS_BLOCK) k_scores_rows(const ScoresArgs a, bool wide, int each) {
     extern __shared__ uint2 tops[];  // [warps][32][top]: order and index
@@ -449,6 +452,9 @@ __global__ void __launch_bounds__(ROWS_BLOCK) k_scores_rows(const ScoresArgs a, 
 // collected and the largest of it taken. Where that is more than there is room for (many of the largest in one thread's pieces) or the row holds
 // NaN, the row is searched `top` times instead.
 // Few rows: a cluster of blocks shares a row, and the first of them joins their results through its shared memory.
+// 4099 rows of 32771 bf16: 60 us, with five best 73, 41 at the memory's rate; a plain sum over the same rows takes 59. Two thirds of the issue
+// slots and of the exponentials' pipe are taken; loads a step ahead in registers moved it by -4 to +2 % (fewer blocks fit). 4 x 131072 fp16 with
+// 20 best: 12.3 us, of which 4 are a launch and 4 the cluster's two barriers and the joining.
 constexpr int STREAM_BLOCK = 256;
 constexpr int STREAM_AHEAD = 4;    // pieces that a thread has under way
 constexpr int CANDIDATES   = 256;  // top * (values of a piece) at least: that many can tie
@@ -771,7 +777,8 @@ __global__ void __launch_bounds__(BLOCK) k_scores_stream(const ScoresArgs a, int
 }
 
 // ---- gradients -----------------------------------------------------------------------------------------------------------------
-// One pass over the elements once the row's sums are known.
+// One pass over the elements once the row's sums are known. 16 x 68101 rows of five floats, forward and backward: 26.6 us (two launches, 15 at the
+// memory's rate for both passes); 2048 x 50021 bf16: 130, of which this is 80 (its 410 MB at 5.1 TB/s; 63 at the memory's rate).
 template <bool PROBABILITIES>
 struct RowGrad {
     float log_sum, d_label, d_entropy, offset, one_over_sum;
