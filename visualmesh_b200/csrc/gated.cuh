@@ -512,7 +512,7 @@ __device__ __forceinline__ void tell_cluster(Exchange<W, true>& shared, const Be
 }
 
 // Maps of the parts of a split sequence, of the recurrence or (REVERSE) of its gradient. The pass behind it reads the inputs once more, mostly from
-// the cache; it starts while this one ends. 65537 x 64 bf16 (74 parts): 18.6 us for both, 20.5 one after the other, 3.8 at the memory's rate
+// the cache; it starts while this one ends. 65537 x 64 bf16 (129 parts): 18.6 us for both, 20.5 one after the other, 3.8 at the memory's rate
 // and 6 for two empty launches.
 template <typename T, int V, int L, int PIECE, bool REVERSE>
 __global__ void __launch_bounds__(Shape<8>::THREADS) k_gated_summary(const GatedArgs a, const Split s) {
