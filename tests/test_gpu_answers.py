@@ -183,7 +183,7 @@ def test_scores_of_probabilities(answers, rows, classes, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows,classes", [(80001, 9), (60007, 16), (30001, 21), (20003, 50), (9001, 100), (4001, 200), (1300, 300), (5003, 300), (2501, 512), (320, 2400), (40, 33000), (1500, 2055), (400, 9000), (1200, 8300)])
+@pytest.mark.parametrize("rows,classes", [(80001, 9), (60007, 16), (30001, 21), (30001, 32), (20003, 50), (20003, 64), (9001, 100), (5003, 128), (9001, 24), (4001, 200), (1300, 300), (5003, 300), (2501, 512), (320, 2400), (40, 33000), (1500, 2055), (400, 9000), (1200, 8300)])
 def test_scores_of_many_rows(answers, rows, classes, dtype):
     """Rows one after another for the same lanes, and blocks of every size."""
     x, labels, grads = answers_of(rows, classes, dtype, rows)

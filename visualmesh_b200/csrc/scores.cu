@@ -72,6 +72,13 @@ dim3 grid_of(int64_t blocks) {
 bool starts_on_16(const void* p, int64_t stride, int32_t type) {
     return aligned(p, 16) && stride * static_cast<int64_t>(element_size(type)) % 16 == 0;
 }
+// Whether lanes of a row take pieces of 16 bytes where its rows begin on them: all of a warp, two, or four that a row fills; else single elements,
+// which are spread better. 1,000,000 rows, scores / gradient by elements and by pieces, us: 16 floats 36 / 48 and 19 / 28, 12 19 / 36 and
+// 19 / 24, 32 40 / 70 and 35 / 50, 48 55 / 82 and 60 / 87, 96 97 / 151 and 111 / 166; bf16 16 21 / 40 and 19 / 21, 24 29 / 44 and 33 / 48, 32
+// 39 / 53 and 29 / 45.
+bool in_pieces(int lanes, int classes) {
+    return lanes == 2 || lanes == WARP || (lanes == 4 && classes == 32);
+}
 // whether loads of 8 or 16 bytes fit every row of a few classes
 bool starts_on_row(const void* x, int64_t stride, int classes, int32_t type) {
     const int64_t size = static_cast<int64_t>(element_size(type)), to = classes * size == 8 ? 8 : 16;
@@ -140,7 +147,7 @@ vm_status vm_scores(int device, const void* x, int32_t type, int64_t rows, int32
                 const int64_t each  = std::clamp<int64_t>(rows * G / (WARP * 8 * SMS), 1, G);
                 const int64_t block = ROWS_BLOCK / G * each;
                 launch_kernel(k_scores_rows<T, P, decltype(best)::value, G, E>, grid_of((rows + block - 1) / block), ROWS_BLOCK, ROWS_BLOCK * top * sizeof(uint2), q, false, a,
-                              starts_on_16(x, row_stride, type), static_cast<int>(each));
+                              in_pieces(G, classes) && starts_on_16(x, row_stride, type), static_cast<int>(each));
             };
             if (top > 0 && classes <= MOST_OF_LANES_TOP) return with_lanes<MOST_OF_LANES_TOP>(classes, [&](auto lanes, auto values) { launch_rows(std::true_type{}, lanes, values); });
             if (top == 0 && classes <= MOST_OF_LANES) return with_lanes<MOST_OF_LANES>(classes, [&](auto lanes, auto values) { launch_rows(std::false_type{}, lanes, values); });
@@ -196,7 +203,7 @@ vm_status vm_scores_backward(int device, const void* x, int32_t type, int64_t ro
                 const bool wide = starts_on_16(x, row_stride, type) && starts_on_16(dx, dx_row_stride, type);
                 with_lanes<MOST_OF_LANES_GRADIENT>(classes, [&](auto lanes, auto values) {
                     constexpr int G = decltype(lanes)::value, E = decltype(values)::value;
-                    launch_kernel(k_scores_grad_rows<T, P, G, E>, grid_of((rows * G + ROW_BLOCK - 1) / ROW_BLOCK), ROW_BLOCK, 0, q, false, a, wide);
+                    launch_kernel(k_scores_grad_rows<T, P, G, E>, grid_of((rows * G + ROW_BLOCK - 1) / ROW_BLOCK), ROW_BLOCK, 0, q, false, a, wide && in_pieces(G, classes));
                 });
                 return;
             }

@@ -267,11 +267,12 @@ __global__ void __launch_bounds__(ROW_BLOCK) k_scores_own_row(const ScoresArgs a
 }
 
 // ---- up to 256 classes (gradients 1024): G lanes per row, E values a lane in registers ---------------------------------------------------------
-// Lane l of a row has the values l, l + G, l + 2 G, ..., or (WIDE, G = 32, rows that begin on 16 bytes) the same with pieces of 16 bytes.
+// Lane l of a row has the values l, l + G, l + 2 G, ..., or (wide, rows that begin on 16 bytes) the same with pieces of 16 bytes. 8 and 16 lanes
+// never do: their code for both would hold more registers (64 floats with two best 111 -> 125 us), and they gain 10 % at most.
 template <typename T, int G, int E>
 struct RowLoad {
     static constexpr int PIECE = 16 / sizeof(T);
-    static constexpr bool MAY  = G == 32 && E % PIECE == 0;
+    static constexpr bool MAY  = G <= 4 || G == WARP;
     __device__ static __forceinline__ int index(bool wide, int lane, int i) {
         return MAY && wide ? (i / PIECE * G + lane) * PIECE + i % PIECE : i * G + lane;
     }
