@@ -83,7 +83,7 @@ void check_sizes(int32_t type, int64_t batch, int64_t steps, int64_t channels) {
 constexpr int SMS = 148;
 
 // A thread takes pairs of channels where they lie side by side, else single ones; a block 32 channels either way. Steps of a thread in the
-// forward and in the backward pass: what its registers hold (128 each without a spill) and a block's shared memory, of which two fit an SM.
+// forward and in the backward pass: what its 128 registers hold (but for a few outside of the loops) and a block's shared memory, of which two fit an SM.
 constexpr int forward_steps(int vector, bool wide_type) {
     return vector == 2 && !wide_type ? 16 : 8;
 }
@@ -119,7 +119,7 @@ struct Plan {
 // clusters costs as much as the first. Forward / backward on B200, us:
 //   3 x 1021 x 515 (97 blocks of 16, float): clusters of 4  13 / 15, of 8  10 / 20 (of which 6 and 4 blocks fit an SM)
 //   3 x 4096 x 1024 (192): clusters of 2  41 / 76, of 4  44 / 88, whole  42 / 77
-//   1 x 65537 x 64 (4): 8 parts in a cluster 40, 129 parts 18.6
+//   1 x 65537 x 64 (4): 8 parts in a cluster 40, 129 parts 16.4
 Plan plan_of(int64_t all, int64_t steps, int vector, int length, int resident) {
     const auto blocks_of = [&](int channels) { return (all + channels - 1) / channels; };
     const int64_t tile = 8 * vector * length, tiles = (steps + tile - 1) / tile;  // whatever the block: 32 W threads for 4 W / vector of them along the channels
