@@ -449,11 +449,11 @@ def test_scan_of_long_sequences(answers, batch, steps, channels, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("batch,steps,channels", [(1, 70, 76001), (30000, 67, 3), (2, 66, 40002), (1, 64, 20003), (9000, 17, 4), (2, 33, 9002), (3, 1, 8000), (5, 8, 16384)])
+@pytest.mark.parametrize("batch,steps,channels", [(1, 70, 76001), (30000, 67, 3), (2, 66, 40002), (1, 64, 20003), (9000, 17, 4), (2, 33, 9002), (3, 1, 8000), (5, 8, 16384), (1, 0, 20000)])
 def test_scan_of_many_sequences(answers, batch, steps, channels, dtype):
     """Enough for a thread each, where they are single elements; states are kept twice."""
     x, g, h0, dy, d_last = sequences(batch, steps, channels, dtype, 3)
-    g[:, steps // 5] = -math.inf
+    g[:, steps // 5:steps // 5 + 1] = -math.inf
     lengths = torch.randint(0, steps + 1, (batch,), device="cuda", generator=generator(batch)).to(torch.int32)
     check_scan(answers, x, g, h0, None, dy, d_last)
     check_scan(answers, x, g, None, lengths, dy, None)

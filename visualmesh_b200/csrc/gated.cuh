@@ -451,7 +451,7 @@ __device__ __forceinline__ int64_t set_up(Tiles<T, V, L, N, PIECE, W>& io, int n
 
 // The state in front of part `part` of a split sequence (or, REVERSE, behind it), from the one at the sequence's end: a thread along
 // time takes its share of the parts on that side one after another, several loads at a time, and the threads are joined as in a tile: 129 parts
-// in as many rounds of joined threads as it takes cost 3 us more, 180 parts of 12381 x 2 floats 7.
+// in as many rounds of joined threads as it takes cost 3 us more, 194 parts of 12381 x 2 floats 7.
 // channel: the one whose state the thread carries, or -1.
 template <int V, int W, bool REVERSE>
 __device__ __forceinline__ void join_parts(const GatedArgs& a, const Split& s, const Place<V, W>& at, int part, int channel, float& carry, Between<V, W>& shared) {
