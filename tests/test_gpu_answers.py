@@ -833,3 +833,26 @@ def test_a_stream_of_frames_is_filtered_scored_and_learned_from(answers):
             with pytest.raises(VisualMeshError):
                 moved.filtered(gate)
     engine.close()
+
+
+def test_tensors_of_a_batch_hold_on_to_its_engine(answers):
+    import gc
+
+    import golden_io as G
+    from visualmesh_b200.engine import Engine, FrameInput, Mesh
+
+    case = G.Case("ring6_equisolid_rgba")
+    mesh = Mesh.from_arrays(case.rays, case.nbrs, case.bsp)
+    fr = case.frames[0]
+
+    def held():
+        engine = Engine(case.network, device=0)
+        frames = [FrameInput(mesh, fr["Hoc"], case.lens, fr["image"], case.format)] * 2
+        want = engine.run_batch(frames).frame(1).classifications
+        return want, engine.run_batch(frames, results_on_device=True).tensors()["classifications"]
+
+    want, x = held()
+    gc.collect()
+    assert bool((x[want.shape[0]:].cpu() == torch.from_numpy(want)).all())
+    got = answers.scores(x, probabilities=True)
+    assert bool(torch.isfinite(got.entropy).all())

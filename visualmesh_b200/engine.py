@@ -176,9 +176,10 @@ class FrameInput:
 
 
 class _DeviceArray:
-    """Device memory of the engine, for torch.as_tensor."""
+    """Device memory of the engine, for torch.as_tensor; a tensor holds on to this, and with it to the engine."""
 
-    def __init__(self, pointer, shape, kind):
+    def __init__(self, pointer, shape, kind, engine):
+        self.engine = engine
         self.__cuda_array_interface__ = {"data": (C.cast(pointer, C.c_void_p).value, False), "shape": shape, "typestr": kind, "version": 3}
 
 
@@ -186,8 +187,9 @@ class BatchResult:
     """Results of Engine.run_batch: per-frame views into the engine's pinned buffers (valid until its next call),
     or device pointers when the batch was run with results_on_device."""
 
-    def __init__(self, raw: abi.vm_batch_result):
+    def __init__(self, raw: abi.vm_batch_result, engine=None):
         self.raw = raw
+        self.engine = engine  # whose memory this is
         self.n_frames = raw.n_frames
         self.n_neighbours = raw.n_neighbours
         self.n_classes = raw.n_classes
@@ -223,14 +225,16 @@ class BatchResult:
             raise VisualMeshError(abi.VM_ERR_INVALID_ARGUMENT, "results were copied to the host")
         points, rows = self.total_points, self.total_points + self.n_frames
 
-        def tensor(pointer, shape, kind, dtype):
+        def tensor(pointer, shape, kind, dtype, device="cuda"):
             if 0 in shape:
-                return torch.empty(shape, dtype=dtype, device="cuda")
-            return torch.as_tensor(_DeviceArray(pointer, shape, kind))  # on the device that the memory is on
+                return torch.empty(shape, dtype=dtype, device=device)
+            return torch.as_tensor(_DeviceArray(pointer, shape, kind, self.engine))  # on the device that the memory is on
 
-        return {"pixel_coordinates": tensor(self.raw.pixel_coordinates, (points, 2), "<f4", torch.float32),
-                "global_indices": tensor(self.raw.global_indices, (points,), "<i4", torch.int32),
-                "neighbourhood": tensor(self.raw.neighbourhood, (rows, self.n_neighbours), "<i4", torch.int32),
+        neighbourhood = tensor(self.raw.neighbourhood, (rows, self.n_neighbours), "<i4", torch.int32)  # has a row for every frame
+        device = neighbourhood.device
+        return {"pixel_coordinates": tensor(self.raw.pixel_coordinates, (points, 2), "<f4", torch.float32, device),
+                "global_indices": tensor(self.raw.global_indices, (points,), "<i4", torch.int32, device),
+                "neighbourhood": neighbourhood,
                 "classifications": tensor(self.raw.classifications, (rows, self.n_classes), "<f4", torch.float32) if self.n_classes else None}
 
     def _classifications(self):
@@ -358,7 +362,7 @@ class Engine:
         flags = (abi.VM_RESULTS_ON_DEVICE if results_on_device else 0) | (abi.VM_TIME_STAGES if time_stages else 0)
         res = abi.vm_batch_result()
         abi.check(self._lib.vm_run_batch(self._ptr, arr, n, flags, C.byref(res)))
-        return res if raw else BatchResult(res)
+        return res if raw else BatchResult(res, self)
 
     def run_batch(self, frames: Sequence[FrameInput], results_on_device=False, time_stages=False) -> BatchResult:
         return self.run_prepared(self.prepare_batch(frames), results_on_device, time_stages)
