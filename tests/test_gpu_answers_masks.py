@@ -132,3 +132,31 @@ def test_scores_of_rows_far_from_zero(answers, classes, dtype):
     for rows, chosen in ((x, labels), (x[:2], labels[:2]), (x.repeat(6, 1), labels.repeat(6))):
         for top in (0, min(5, classes)):
             check(answers, rows, chosen, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("classes", [5, 300, 1000, 1025, 2055, 9001, 70001])
+def test_gradient_of_rows_with_a_clear_maximum_far_from_zero(answers, classes, dtype):
+    """One class is all of the distribution (the others are masked, or some thousands below): log_sum is that logit, p is 1 there and 0 elsewhere, and
+    the entropy 0 but for 4u."""
+    values = [1e3, -1e3, 6e4, -6e4] + ([] if dtype == torch.float16 else [3e5, -3e5, 1e6, -1e6, 2e10, -2e10, 1e20, -1e20, 1e36, -1e36])
+    rows = 2 * len(values)
+    x = torch.tensor(values, dtype=torch.float64, device="cuda").repeat(2)[:, None].expand(rows, classes).clone()
+    x[:len(values)] -= x[:len(values)].abs() * 0.25 + 300
+    x[len(values):] = -math.inf
+    winner = (torch.arange(rows, device="cuda") * 37 + classes // 2) % classes
+    x.scatter_(1, winner[:, None], torch.tensor(values, dtype=torch.float64, device="cuda").repeat(2)[:, None])
+    x = torch.where(x == -math.inf, x, x.clamp(min=torch.finfo(dtype).min)).to(dtype)
+    q = generator(classes)
+    d_l, d_e, d_s = (torch.randn(rows, device="cuda", generator=q) for _ in range(3))
+    labels = (winner + torch.arange(rows, device="cuda") % 2) % classes  # every other label is another class
+    got = answers.scores(x, labels)
+    assert torch.equal(got.log_sum, x.gather(1, winner[:, None])[:, 0].float()) and bool((got.entropy.abs() <= 4 * U).all())
+    dx = answers.scores_backward(x, got, labels, d_l, d_e, d_s)
+    want = torch.zeros((rows, classes), dtype=torch.float64, device="cuda")
+    want.scatter_add_(1, winner[:, None], (d_s - d_l).double()[:, None])
+    there = torch.isfinite(x.gather(1, labels[:, None])[:, 0].float())  # a masked label's gradient is 0
+    want.scatter_add_(1, labels[:, None], torch.where(there, d_l, torch.zeros_like(d_l)).double()[:, None])
+    step = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    size = (d_s.abs() + d_l.abs() + d_e.abs()).double()[:, None]
+    near(dx, want, want.abs() * step + torch.where(want != 0, 8 * U * size, torch.zeros_like(want)))

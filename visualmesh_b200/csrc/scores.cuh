@@ -922,10 +922,11 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_grad_stream(const Score
     for (int u = 0; u < STREAM_AHEAD; ++u)
         if (begin + u * STREAM_BLOCK < pieces.count) raw[u] = pieces.load(begin + u * STREAM_BLOCK, outside);
     const RowGrad<PROBABILITIES> grad(a, row);
-    // Logits, in powers of two and by pairs as above: with t = x L - S, S = log_sum L and rho = log_sum L - S, p = 2^(t + rho), so that the factor 2^rho
-    // joins those of the row. Values are not let below log_sum - 1000 (p is 0 there), which has to be a number of the type.
-    const float S = grad.log_sum * LOG2_E, back = exp2_of(-fmaf(grad.log_sum, LOG2_E, -S));
-    const float slope = -grad.d_entropy * LOG_2 * back, level = grad.offset * back;
+    // Logits, in powers of two and by pairs as above: with S = log_sum L rounded, t = x L - S and rho = log_sum L - S, log p = (t - rho) log 2
+    // and p = 2^(t - rho), so that rho joins the factors of the row. Values are not let below log_sum - 1000, where p is 0: rounded to the type that stays 700 below log_sum
+    // within the range of the sums, but beyond 2^18 it would be log_sum itself in bfloat16, and every class as likely as the best.
+    const float S = grad.log_sum * LOG2_E, rho = fmaf(grad.log_sum, LOG2_E, -S), back = exp2_of(-rho);
+    const float slope = -grad.d_entropy * LOG_2 * back, level = fmaf(grad.d_entropy * LOG_2, rho, grad.offset) * back;
     const bool quick  = !PROBABILITIES && grad.log_sum > Range<T>::ABOVE + 2000.0f && grad.log_sum < Range<T>::BELOW && fabsf(grad.offset) < INFINITY;
     const auto low    = Pair<T>::both(grad.log_sum - 1000.0f);
 #pragma unroll
