@@ -9,6 +9,8 @@ Tolerances, with u = 2^-24 (half a step of 32 bits), n classes and t_j = v_j - m
   entropy = log s - E t: S (3 + 2 ln n) + 4u, whatever the maximum.
   gradient: p from log p = v - log_sum is off by what log_sum was rounded by, u |log_sum|, as long as |log_sum| is below FAR (64, and 1024
     for 16 bits: a sixteenth of their half step); beyond that it is computed again from the row, so that min(|log_sum|, FAR) u counts.
+    p below 2^-126 counts as 0 (exp_of has no numbers below the normal ones), and a result there is rounded to them: 2^-125 (1 + |bracket|), the
+    bracket being what multiplies p.
   results of 16 bits: half a step more.
 """
 import math
@@ -160,3 +162,45 @@ def test_gradient_of_rows_with_a_clear_maximum_far_from_zero(answers, classes, d
     step = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
     size = (d_s.abs() + d_l.abs() + d_e.abs()).double()[:, None]
     near(dx, want, want.abs() * step + torch.where(want != 0, 8 * U * size, torch.zeros_like(want)))
+
+
+def check_gradient(answers, x, labels, grads):
+    d_l, d_e, d_s = (d.double()[:, None] for d in grads)
+    classes, dtype = x.shape[1], x.dtype
+    got = answers.scores(x, labels)
+    dx = answers.scores_backward(x, got, labels, *grads)
+    log_p, p, _, entropy, log_sum, _ = reference(x, labels, 0)
+    lp = torch.where(p > 0, log_p, torch.zeros_like(log_p))
+    at = torch.zeros_like(p).scatter_(1, labels[:, None], 1.0)
+    bracket = d_s - d_l - d_e * (lp + entropy[:, None])
+    want = p * bracket + at * d_l
+    base = sum_error(classes) + 2 * U * (1 + math.log(classes)) + U * log_sum.abs().clamp(max=FAR[dtype])[:, None]
+    of_entropy = sum_error(classes) * (3 + 2 * math.log(classes)) + 4 * U
+    error = p * (bracket.abs() * (base + 2.4 * U * lp.abs() + 8 * U) + d_e.abs() * (base + of_entropy + 2 * U * lp.abs()) + 4 * U * (d_s.abs() + d_l.abs() + d_e.abs() * (lp.abs() + entropy[:, None])))
+    error += at * d_l.abs() * 2 * U
+    if dtype != torch.float32:
+        error += want.abs().clamp(min=torch.finfo(dtype).tiny) * torch.finfo(dtype).eps / 2
+    near(dx, want, error + 2.0**-125 * (1 + bracket.abs()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("classes", [3, 5, 8, 16, 33, 100, 300, 700, 1024, 1025, 2055, 9001, 70001])
+def test_gradient_of_rows_far_from_zero(answers, classes, dtype):
+    """Wherever a row lies, its gradient is that of its distribution: a row of the type's lowest value has 1 / n for every class."""
+    x = filled_rows(classes, dtype)
+    labels = torch.arange(x.shape[0], device="cuda") % classes
+    grads = [torch.randn(x.shape[0], device="cuda", generator=generator(classes + k)) for k in range(3)]
+    check_gradient(answers, x, labels, grads)
+    check_gradient(answers, x.repeat(7, 1), labels.repeat(7), [d.repeat(7) for d in grads])
+    wide = torch.full((x.shape[0], classes + 3), math.nan, dtype=dtype, device="cuda")
+    wide[:, 1:classes + 1] = x
+    check_gradient(answers, wide[:, 1:classes + 1], labels, grads)  # rows that begin inside a piece
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("classes", [5, 33, 300, 1000, 2055, 9001, 70001])
+def test_gradient_of_classes_masked_by_finite_numbers(answers, classes, dtype):
+    for value in values_of(dtype):
+        x, labels = masked_rows(21, classes, dtype, value, classes)
+        grads = [torch.randn(x.shape[0], device="cuda", generator=generator(classes + k)) for k in range(3)]
+        check_gradient(answers, x, labels, grads)

@@ -603,6 +603,7 @@ __device__ __noinline__ Row row_again(const Pieces<T>& pieces, Sums* warps) {
     };
     const auto joined = [&](Sums q, auto join) {
         q = joined_lanes<WARP>(q, join);
+        if (BLOCK == WARP) return q;
         __syncthreads();  // what stood there is read
         if (threadIdx.x % WARP == 0) warps[threadIdx.x / WARP] = q;
         __syncthreads();
@@ -698,11 +699,17 @@ __global__ void __launch_bounds__(BLOCK) k_scores_stream(const ScoresArgs a, int
     if (TOP && threadIdx.x == 0) shared.found = 0;
     if (TOP) shared.keys[threadIdx.x] = begin + threadIdx.x < end ? static_cast<uint64_t>(order_of(best)) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(held)) : 0;
     q = joined_lanes<WARP>(q, joined_stream<PROBABILITIES>);
-    if (lane == 0) shared.warps[warp] = q;
-    bool search = __syncthreads_or(q.s != q.s || q.w != q.w);  // NaN, or an infinity: its maxima were no maxima
-    q = joined_lanes<BLOCK / WARP>(shared.warps[lane % (BLOCK / WARP)], joined_stream<PROBABILITIES>);
+    if (BLOCK > WARP && lane == 0) shared.warps[warp] = q;
     const auto out_of_range = [&] { return !PROBABILITIES && !(q.m > Range<T>::ABOVE && q.m < Range<T>::BELOW); };
-    if (!TOP && !CLUSTER && warp != 0 && !out_of_range()) return;
+    bool search = false;
+    if (TOP || CLUSTER) search = __syncthreads_or(q.s != q.s || q.w != q.w);  // NaN, or an infinity: its maxima were no maxima
+    else {
+        // The warps behind the first stay only for a row that is summed again: the largest of the warps' maxima is beyond BELOW where one of them is,
+        // and above ABOVE where one of them is.
+        const int ways = __syncthreads_count(!PROBABILITIES && (q.m >= Range<T>::BELOW || (q.m > Range<T>::ABOVE && lane == 0)));
+        if (warp != 0 && (PROBABILITIES || (ways > 0 && ways < WARP))) return;
+    }
+    if (BLOCK > WARP) q = joined_lanes<BLOCK / WARP>(shared.warps[lane % (BLOCK / WARP)], joined_stream<PROBABILITIES>);
 
     if constexpr (TOP) {
         if (warp == 0) largest_keys(shared.keys, BLOCK, a.top, shared.best);
@@ -792,6 +799,39 @@ __global__ void __launch_bounds__(BLOCK) k_scores_stream(const ScoresArgs a, int
 // ---- gradients -----------------------------------------------------------------------------------------------------------------
 // One pass over the elements once the row's sums are known. 16 x 68101 rows of five floats, forward and backward: 26.6 us (two launches, 15 at the
 // memory's rate for both passes); 2048 x 50021 bf16: 130, of which this is 80 (its 410 MB at 5.1 TB/s; 63 at the memory's rate).
+//
+// The probabilities come from log p = v - log_sum, off by what log_sum was rounded by when it was written: half a step of it. Beyond FAR that is
+// more than a result should lose (2^-19 of p; with 16 bits 2^-15, a sixteenth of their half step), and a row of the type's lowest value would
+// have p = 1 for every class. There the row's maximum m and log sum e^(v - m) are computed again, and v - m stands for v. That is done
+// behind what is done for every row, and written over it: a branch in front cost the other rows 5 to 14 % of their time, this costs up to 5
+// (4096 x 2000 floats 14.0 us, with every fourth row far 20.7; 4099 x 32771 bf16 101 and 218).
+template <typename T>
+constexpr float FAR = sizeof(T) == 4 ? 64.0f : 1024.0f;
+template <typename T>
+__device__ __forceinline__ bool is_far(float log_sum) {
+    return fabsf(log_sum) >= FAR<T> && fabsf(log_sum) < INFINITY;
+}
+template <int G>
+__device__ __forceinline__ unsigned lanes_of_row() {
+    return G == WARP ? ~0u : ((1u << G % WARP) - 1) << (threadIdx.x % WARP / G * G);
+}
+// Maximum and log sum of a row, by its G lanes.
+template <typename T, int G>
+__device__ __forceinline__ float2 near_row(const T* x, int classes, int lane) {
+    const unsigned lanes = lanes_of_row<G>();
+    float m = -INFINITY, s = 0.0f;
+#pragma unroll 1
+    for (int j = lane; j < classes; j += G) m = fmaxf(m, to_float(x[j]));
+    over_lanes<G>([&](int d) { m = fmaxf(m, __shfl_xor_sync(lanes, m, d)); });
+#pragma unroll 1
+    for (int j = lane; j < classes; j += G) s += exp_of(to_float(x[j]) - m);
+    over_lanes<G>([&](int d) { s += __shfl_xor_sync(lanes, s, d); });
+    return make_float2(m, logf(s));
+}
+// v - m, -infinity for a masked class alone
+__device__ __forceinline__ float less(float v, float m) {
+    return v == -INFINITY ? v : fmaxf(v - m, -3.402823466e38f);
+}
 template <bool PROBABILITIES>
 struct RowGrad {
     float log_sum, d_label, d_entropy, offset, one_over_sum;
@@ -832,19 +872,49 @@ struct RowGrad {
     }
 };
 
+// Every `step`-th element from `begin` on of a row that is far from 0, of which grad holds the log sum of what is less its maximum m.
+template <typename T>
+__device__ __forceinline__ void far_elements(const RowGrad<false>& grad, const T* x, float m, int64_t begin, int64_t end, int step, T* dx) {
+#pragma unroll 1
+    for (int64_t j = begin; j < end; j += step) {
+        const float v[1] = {less(to_float(x[j]), m)};
+        float d[1];
+        grad.of(v, j, d);
+        dx[j] = from_float<T>(d[0]);
+    }
+}
+
+// A row that is far from 0, by its G lanes (staged: where the block's rows are gathered, or NULL). A function that is called and looks everything up
+// for itself: what it needs would otherwise be held in registers for all rows.
+template <typename T, int G>
+__device__ __noinline__ void far_row(const ScoresGradArgs& a, T* staged) {
+    const int64_t row = (static_cast<int64_t>(blockIdx.x) * ROW_BLOCK + threadIdx.x) / G;
+    const int lane    = threadIdx.x % G;
+    const T* x        = static_cast<const T*>(a.x) + row * a.row_stride;
+    const float2 r    = near_row<T, G>(x, a.classes, lane);
+    RowGrad<false> grad(a, row);
+    grad.log_sum = r.y;
+    __syncwarp(lanes_of_row<G>());  // what the row's lanes wrote before comes before what they write now
+    far_elements<T>(grad, x, r.x, lane, a.classes, G, staged != nullptr ? staged + threadIdx.x * a.classes : static_cast<T*>(a.dx) + row * a.dx_row_stride);
+}
+
 // Up to 8 classes: a thread per row. The results go through shared memory, so that a block writes its rows, which lie side by side (dense),
 // in one piece.
 template <typename T, bool PROBABILITIES, int C>
-__global__ void __launch_bounds__(ROW_BLOCK) k_scores_grad_own_row(const ScoresGradArgs a, bool wide, bool dense) {
+__global__ void __launch_bounds__(ROW_BLOCK) k_scores_grad_own_row(const __grid_constant__ ScoresGradArgs a, bool wide, bool dense) {
     __shared__ alignas(16) T staged[ROW_BLOCK * C];
     const int first = blockIdx.x * ROW_BLOCK, row = first + threadIdx.x;
     if (row < a.rows) {
         float x[C], d[C];
         load_row<T, C>(static_cast<const T*>(a.x) + row * a.row_stride, wide, x);
-        RowGrad<PROBABILITIES>(a, row).of(x, 0, d);
+        const RowGrad<PROBABILITIES> grad(a, row);
         T* const dx = dense ? staged + threadIdx.x * C : static_cast<T*>(a.dx) + row * a.dx_row_stride;
+            grad.of(x, 0, d);
 #pragma unroll
         for (int k = 0; k < C; ++k) dx[k] = from_float<T>(d[k]);
+        if constexpr (!PROBABILITIES) {
+            if (is_far<T>(grad.log_sum)) far_row<T, 1>(a, dense ? staged : nullptr);
+        }
     }
     if (dense) {
         __syncthreads();
@@ -858,7 +928,7 @@ __global__ void __launch_bounds__(ROW_BLOCK) k_scores_grad_own_row(const ScoresG
 
 // Up to 1024 classes, G lanes per row as above.
 template <typename T, bool PROBABILITIES, int G, int E>
-__global__ void __launch_bounds__(ROW_BLOCK) k_scores_grad_rows(const ScoresGradArgs a, bool wide) {
+__global__ void __launch_bounds__(ROW_BLOCK) k_scores_grad_rows(const __grid_constant__ ScoresGradArgs a, bool wide) {
     const int64_t row = (static_cast<int64_t>(blockIdx.x) * ROW_BLOCK + threadIdx.x) / G;
     const int lane    = threadIdx.x % G;
     if (row >= a.rows) return;
@@ -890,25 +960,66 @@ __global__ void __launch_bounds__(ROW_BLOCK) k_scores_grad_rows(const ScoresGrad
                         if (j + k < a.classes) dx[j + k] = e[k];
                 }
             }
-            return;
         }
     }
+    if (!(Load::MAY && wide)) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const int j = i * G + lane;
-        if (j < a.classes) {
-            const float x[1] = {v[i]};
-            float d[1];
-            grad.of(x, j, d);
-            dx[j] = from_float<T>(d[0]);
+        for (int i = 0; i < E; ++i) {
+            const int j = i * G + lane;
+            if (j < a.classes) {
+                const float x[1] = {v[i]};
+                float d[1];
+                grad.of(x, j, d);
+                dx[j] = from_float<T>(d[0]);
+            }
         }
     }
+    if constexpr (!PROBABILITIES) {
+        if (is_far<T>(grad.log_sum)) far_row<T, G>(a, nullptr);
+    }
+}
+
+// The same for a block of a long row, whose blocks each go over the whole row for themselves. Its barriers come between the two results.
+template <typename T>
+__device__ __noinline__ void far_block(const ScoresGradArgs& a, int blocks) {
+    __shared__ float warps[2][STREAM_BLOCK / WARP];
+    const int64_t row = a.rows - 1 - blockIdx.x / blocks;
+    const T* x        = static_cast<const T*>(a.x) + row * a.row_stride;
+    const Pieces<T> pieces(x, a.classes);
+    constexpr int N = Pieces<T>::N;
+    const int lane = threadIdx.x % WARP, warp = threadIdx.x / WARP;
+    const auto over = [&](auto f) {
+        for (int64_t p = threadIdx.x; p < pieces.count; p += STREAM_BLOCK) {
+            float v[N];
+            values_of<T>(pieces.load(p, from_float<T>(-INFINITY)), v);
+            for (int k = 0; k < N; ++k) f(v[k]);
+        }
+    };
+    float m = -INFINITY, s = 0.0f;
+    over([&](float v) { m = fmaxf(m, v); });
+    over_lanes<WARP>([&](int d) { m = fmaxf(m, __shfl_xor_sync(~0u, m, d)); });
+    if (lane == 0) warps[0][warp] = m;
+    __syncthreads();
+    m = warps[0][lane % (STREAM_BLOCK / WARP)];
+    over_lanes<STREAM_BLOCK / WARP>([&](int d) { m = fmaxf(m, __shfl_xor_sync(~0u, m, d)); });
+    over([&](float v) { s += exp_of(v - m); });
+    over_lanes<WARP>([&](int d) { s += __shfl_xor_sync(~0u, s, d); });
+    if (lane == 0) warps[1][warp] = s;
+    __syncthreads();
+    s = warps[1][lane % (STREAM_BLOCK / WARP)];
+    over_lanes<STREAM_BLOCK / WARP>([&](int d) { s += __shfl_xor_sync(~0u, s, d); });
+    RowGrad<false> grad(a, row);
+    grad.log_sum = logf(s);
+    const int64_t first = pieces.first(static_cast<int64_t>(blockIdx.x % blocks) * (STREAM_BLOCK * STREAM_AHEAD)), end = first + STREAM_BLOCK * STREAM_AHEAD * N;
+    far_elements<T>(grad, x, m, (first < 0 ? 0 : first) + threadIdx.x, end < a.classes ? end : a.classes, STREAM_BLOCK, static_cast<T*>(a.dx) + row * a.dx_row_stride);
 }
 
 // Longer rows: a block for STREAM_BLOCK * STREAM_AHEAD pieces of a row. The last rows come first: they are what the cache still holds of
 // the pass that made the sums.
+// The bound holds the 16-bit kernels of logits to the 48 registers of five blocks an SM: with 57 they took 79 and 85 us instead of 75 and 73 (2048 x
+// 50021 bf16, 20000 x 2055 fp16).
 template <typename T, bool PROBABILITIES>
-__global__ void __launch_bounds__(STREAM_BLOCK) k_scores_grad_stream(const ScoresGradArgs a, int blocks) {
+__global__ void __launch_bounds__(STREAM_BLOCK, !PROBABILITIES && sizeof(T) == 2 ? 5 : 0) k_scores_grad_stream(const __grid_constant__ ScoresGradArgs a, int blocks) {
     const int64_t row = a.rows - 1 - blockIdx.x / blocks;
     const T* x        = static_cast<const T*>(a.x) + row * a.row_stride;
     T* dx             = static_cast<T*>(a.dx) + row * a.dx_row_stride;
@@ -923,11 +1034,11 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_grad_stream(const Score
         if (begin + u * STREAM_BLOCK < pieces.count) raw[u] = pieces.load(begin + u * STREAM_BLOCK, outside);
     const RowGrad<PROBABILITIES> grad(a, row);
     // Logits, in powers of two and by pairs as above: with S = log_sum L rounded, t = x L - S and rho = log_sum L - S, log p = (t - rho) log 2
-    // and p = 2^(t - rho), so that rho joins the factors of the row. Values are not let below log_sum - 1000, where p is 0: rounded to the type that stays 700 below log_sum
-    // within the range of the sums, but beyond 2^18 it would be log_sum itself in bfloat16, and every class as likely as the best.
+    // and p = 2^(t - rho), so that rho joins the factors of the row. Values are not let below
+    // log_sum - 1000, where p is 0: of a row that is not far from 0 that is below log_sum in every type.
     const float S = grad.log_sum * LOG2_E, rho = fmaf(grad.log_sum, LOG2_E, -S), back = exp2_of(-rho);
     const float slope = -grad.d_entropy * LOG_2 * back, level = fmaf(grad.d_entropy * LOG_2, rho, grad.offset) * back;
-    const bool quick  = !PROBABILITIES && grad.log_sum > Range<T>::ABOVE + 2000.0f && grad.log_sum < Range<T>::BELOW && fabsf(grad.offset) < INFINITY;
+    const bool quick  = !PROBABILITIES && fabsf(grad.log_sum) < INFINITY && fabsf(grad.offset) < INFINITY;
     const auto low    = Pair<T>::both(grad.log_sum - 1000.0f);
 #pragma unroll
     for (int u = 0; u < STREAM_AHEAD; ++u) {
@@ -969,6 +1080,9 @@ __global__ void __launch_bounds__(STREAM_BLOCK) k_scores_grad_stream(const Score
             for (int k = 0; k < N; ++k)
                 if (j + k >= 0 && j + k < a.classes) dx[j + k] = e[k];
         }
+    }
+    if constexpr (!PROBABILITIES) {
+        if (is_far<T>(grad.log_sum)) far_block<T>(a, blocks);
     }
 }
 
