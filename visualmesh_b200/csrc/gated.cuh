@@ -67,9 +67,13 @@ __device__ __forceinline__ float gated(float a, float b) {
 __device__ __forceinline__ float gated(float a, float b, float c) {
     return a == 0.0f ? c : fmaf(a, b, c);
 }
-// The factor of two runs of steps. It is 0 only where a step's is: what 32 bits cannot hold becomes their smallest normal number, so that an
-// infinity or NaN goes on through a long run as it does step by step.
-constexpr float SMALLEST = 1.17549435e-38f;
+// a * b * c, where a of 0 drops the others, and a large b does not leave the range before a small a has met it
+__device__ __forceinline__ float gated_gradient(float a, float b, float c) {
+    return a == 0.0f ? 0.0f : a * b * c;
+}
+// The factor of two runs of steps. It is 0 only where a step's is: what 32 bits cannot hold becomes their smallest number, so that an infinity or NaN
+// goes on through a long run as it does step by step, and of a state at the end of the range 5e-7 stay.
+constexpr float SMALLEST = 1.40129846e-45f;
 __device__ __forceinline__ float product(float a, float b) {
     const float r = a * b;
     return a == 0.0f || b == 0.0f ? 0.0f : r < SMALLEST ? SMALLEST : r;
@@ -807,7 +811,7 @@ __global__ void __launch_bounds__(SERIAL_GRAD_BLOCK) k_gated_serial_grad(const G
             const Factors w   = factors_of(to_float(gates[(t - i) * SERIAL_GRAD_BLOCK]));
             const float total = to_float(rd[i]) + c;
             if (a.dx.data != nullptr) *dx = from_float<T>(gated(w.u, total));
-            if (a.d_gate.data != nullptr) *dg = from_float<T>(gated(w.f * w.u, apart[(t - i) * SERIAL_GRAD_BLOCK] * total));
+            if (a.d_gate.data != nullptr) *dg = from_float<T>(gated_gradient(w.f * w.u, apart[(t - i) * SERIAL_GRAD_BLOCK], total));
             c = gated(w.f, total);
         }
     }
@@ -918,13 +922,13 @@ __global__ void __launch_bounds__(CLUSTER ? 128 : 256, CLUSTER ? 4 : 2) k_gated_
                 for (int k = 0; k < V; ++k) {
                     const float total = d[k] + c[k];
                     if constexpr (CAREFUL) {
-                        w[i][k] = gated(f[i][k] * u[i][k], w[i][k] * total);
+                        w[i][k] = gated_gradient(f[i][k] * u[i][k], w[i][k], total);
                         c[k]    = gated(f[i][k], total);
                         u[i][k] = gated(u[i][k], total);
                     }
                     else {
                         c[k]    = f[i][k] * total;
-                        w[i][k] = u[i][k] * (w[i][k] * c[k]);
+                        w[i][k] = u[i][k] * w[i][k] * c[k];  // in this order large states do not leave the range
                         u[i][k] = u[i][k] * total;
                     }
                 }
