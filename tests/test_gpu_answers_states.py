@@ -151,3 +151,41 @@ def test_large_states_are_forgotten(answers, batch, steps, channels, dtype):
     g = torch.full_like(g, -6.0)
     x[:] = 0
     check(answers, x, g, h0, dy, d_last)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch,steps,channels", SIZES)
+def test_factors_below_the_normal_numbers(answers, batch, steps, channels, dtype):
+    """A gate between -104 and 104 drops nothing: its factors are numbers of 32 bits, and an infinity goes on."""
+    x, g, h0, dy, d_last = sequences(batch, steps, channels, dtype, steps + 2)
+    gates = torch.tensor([-86.0, -88.0, -90.0, -95.0, -100.0, -103.0], device="cuda")
+    at = torch.arange(4, min(steps - 2, 40), 5, device="cuda")
+    g[:, at] = gates[at % 6][None, :, None].to(dtype).expand(batch, -1, channels)
+    g[:, at + 1] = -gates[at % 6][None, :, None].to(dtype).expand(batch, -1, channels)
+    if dtype != torch.float16:
+        x[:, at + 1, 1] = 3e38  # masked by a gate that lets a little of it through
+        x[:, at - 1, 2] = 1e38
+    h0[:, 0] = math.inf
+    x[:, 2, 1] = -math.inf
+    check(answers, x, g, h0)
+    h0[:, 0], x[:, 2, 1] = 3e38, 0.5
+    check(answers, x, g, h0, dy, d_last)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,channels", [(5, 7), (40, 64), (700, 3)])
+def test_steps_with_factors_below_the_normal_numbers(answers, rows, channels, dtype):
+    q = generator(rows)
+    state = torch.randn((rows, channels), device="cuda", generator=q) * 1e38
+    x = torch.randn((rows, channels), device="cuda", generator=q).to(dtype)
+    g = torch.linspace(-103.5, 103.5, rows * channels, device="cuda").view(rows, channels).to(dtype)
+    state[0, 0] = math.inf
+    for index in (None, torch.randperm(rows, device="cuda", generator=q).int()):
+        table = state.clone()
+        rows_of = torch.arange(rows, device="cuda") if index is None else index.long()
+        f, u = factors(g.double())
+        want = times(f, state.double()[rows_of]) + times(u, x.double())
+        error = 2 * (10 + 1.2 * g.double().abs()) * U * (times(f, state.double()[rows_of].abs()) + times(u, x.double().abs())) + 2.0**-148 * state.double()[rows_of].abs()
+        y = answers.gated_step(table, x, g, index)
+        near(y, want, error.nan_to_num(0, 0, 0) + rounding(want, dtype) + 1e-37)
+        near(table[rows_of], want, error.nan_to_num(0, 0, 0) + 1e-37)
