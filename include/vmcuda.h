@@ -226,6 +226,12 @@ VM_API vm_status vm_project_static(vm_engine* engine,
                                    int32_t* d_n_points,
                                    int32_t* n_points);
 
+/* Results that were left on the device are the engine's memory, and its own streams do not wait for others. After this call the
+ * engine's calls write there only once everything that `stream` (a cudaStream_t of the engine's device, NULL: the default stream) holds
+ * now is done; the host does not wait here, and streams add up. While `stream` is being captured the call does nothing: make it again behind
+ * every launch of the graph. */
+VM_API vm_status vm_wait_for(vm_engine* engine, void* stream);
+
 /* Stand-alone stages on caller-provided HOST arrays, for testing a stage against the reference function it
  * replaces with identical inputs.
  * vm_sample: cpu::interpolate (cpp/visualmesh/engine/cpu/pixel.hpp:116-144) at n pixel coordinates -> n x 4 floats.
@@ -276,7 +282,7 @@ VM_API void vm_host_free(void* ptr);
  * current is current again when the call returns). The calls enqueue their kernels on `stream` (a cudaStream_t, NULL: the default
  * stream) and return: they neither wait, allocate nor keep anything, so they may be captured into a CUDA graph, from any number of
  * threads. Outputs overlap neither inputs nor one another. What an engine left on the device (VM_RESULTS_ON_DEVICE) is complete when
- * its call returns; let `stream` finish before the engine's next call writes there again.
+ * its call returns; before the engine's next call writes there again, `stream` has to be done with it: see vm_wait_for.
  * ------------------------------------------------------------------------------------------------------------------ */
 
 /* element types; sums, logarithms and states are 32-bit floats whatever the type */

@@ -265,6 +265,10 @@ struct vm_engine {
     vm::DeviceArray<int32_t> d_nb;
     vm::DeviceArray<float> d_cls;
     std::unique_ptr<vm::Results> host;  // ... and where they arrive on the host
+    // what still reads results that were left on the device (vm_wait_for): a stream that waits for all of it, an event behind it
+    cudaStream_t readers   = nullptr;
+    cudaEvent_t ev_reading = nullptr, ev_readers = nullptr;
+    bool being_read        = false;
     std::shared_ptr<vm::ResultPool> pool = std::make_shared<vm::ResultPool>();
     int32_t* flags = nullptr;  // abort flags, pinned host memory that the kernels raise them in
     std::vector<vm_mesh*> meshes;
@@ -301,6 +305,11 @@ struct vm_engine {
 };
 
 namespace vm {
+
+// Before anything is written to the results: what a lane enqueues from here on waits for their readers. (A reallocation waits by itself.)
+static void await_readers(vm_engine* e, Lane& lane) {
+    if (e->being_read) VM_CUDA(cudaStreamWaitEvent(lane.stream, e->ev_readers, 0));
+}
 
 // Device buffers and staging blocks of the batch path: a reallocation makes the recorded graphs stale.
 template <typename Array>
@@ -1171,6 +1180,7 @@ static vm_status run_batch(vm_engine* e, const vm_frame* frames, int32_t n_frame
                 VM_CUDA(cudaEventSynchronize(lane.ev_done));
                 lane.busy = false;
             }
+            await_readers(e, lane);
             if (classify) {
                 images = plan_images(frames, f0, f1);
                 upload.reset();
@@ -1192,6 +1202,7 @@ static vm_status run_batch(vm_engine* e, const vm_frame* frames, int32_t n_frame
             if (lane.busy) VM_CUDA(cudaEventSynchronize(lane.ev_done));
             lane.busy = false;
         }
+        e->being_read = false;  // every lane that ran waited for them
         // read once, after the last kernel of EVERY lane
         if (e->flags[ABORT_TC_TIMEOUT]) return fail(VM_ERR_DEVICE_ABORT, "a tensor-core kernel gave up waiting on an mbarrier");
         if (e->flags[ABORT_BSP_DEPTH]) return fail(VM_ERR_DEVICE_ABORT, "a kernel gave up on a bounded loop (BSP deeper than 128 levels)");
@@ -1465,6 +1476,9 @@ void vm_engine_destroy(vm_engine* e) {
             if (ev) cudaEventDestroy(ev);
     }
     if (e->copy_stream) cudaStreamDestroy(e->copy_stream);
+    if (e->readers) cudaStreamDestroy(e->readers);
+    for (cudaEvent_t ev : {e->ev_reading, e->ev_readers})
+        if (ev) cudaEventDestroy(ev);
     e->d_offsets.release();
     e->d_px.release();
     e->d_gi.release();
@@ -1644,6 +1658,28 @@ void vm_results_release(vm_results* kept) {
     if (!k->pool->closed) k->pool->free.push_back(std::move(k->results));
 }
 
+vm_status vm_wait_for(vm_engine* e, void* stream) {
+    if (e == nullptr) return fail(VM_ERR_INVALID_ARGUMENT, "null engine");
+    try {
+        const OnDevice on(e->device);
+        const auto s                 = static_cast<cudaStream_t>(stream);
+        cudaStreamCaptureStatus taken = cudaStreamCaptureStatusNone;
+        VM_CUDA(cudaStreamIsCapturing(s, &taken));
+        if (taken != cudaStreamCaptureStatusNone) return VM_OK;
+        for (cudaEvent_t* ev : {&e->ev_reading, &e->ev_readers})
+            if (*ev == nullptr) VM_CUDA(cudaEventCreateWithFlags(ev, cudaEventDisableTiming));
+        if (e->readers == nullptr) VM_CUDA(cudaStreamCreateWithFlags(&e->readers, cudaStreamNonBlocking));
+        VM_CUDA(cudaEventRecord(e->ev_reading, s));
+        VM_CUDA(cudaStreamWaitEvent(e->readers, e->ev_reading, 0));
+        VM_CUDA(cudaEventRecord(e->ev_readers, e->readers));
+        e->being_read = true;
+    }
+    catch (...) {
+        return status_of_exception();
+    }
+    return VM_OK;
+}
+
 vm_status vm_sample(vm_engine* e, const float* px, int32_t n, const void* image, int32_t width, int32_t height, uint32_t format, float* out) {
     if (e == nullptr || px == nullptr || image == nullptr || out == nullptr || n < 0 || width <= 0 || height <= 0) {
         return fail(VM_ERR_INVALID_ARGUMENT, "null argument");
@@ -1701,6 +1737,7 @@ vm_status vm_network(vm_engine* e, const float* input, const int32_t* neighbourh
         need(e, lane.d_feat[0], rows * e->max_width);
         need(e, lane.d_feat[1], rows * e->max_width);
         const int32_t offsets[2] = {0, n_rows - 1};
+        await_readers(e, lane);
         VM_CUDA(cudaMemcpyAsync(e->d_offsets.p, offsets, sizeof(offsets), cudaMemcpyHostToDevice, lane.stream));
         VM_CUDA(cudaMemcpyAsync(e->d_nb.p, neighbourhood, sizeof(int32_t) * rows * n_neighbours, cudaMemcpyHostToDevice, lane.stream));
         e->timing = false;
@@ -1719,6 +1756,7 @@ vm_status vm_network(vm_engine* e, const float* input, const int32_t* neighbourh
             run_network(e, lane, with_plan, e->d_offsets.p, e->d_nb.p, n_neighbours, 0, 1, n_rows, e->d_cls.p, true, n_rows);
             VM_CUDA(cudaMemcpyAsync(out, e->d_cls.p, sizeof(float) * rows * e->n_classes, cudaMemcpyDeviceToHost, lane.stream));
             VM_CUDA(cudaStreamSynchronize(lane.stream));
+            e->being_read = false;
             if (e->flags[ABORT_TC_TIMEOUT]) return fail(VM_ERR_DEVICE_ABORT, "a kernel gave up on a bounded wait");
             if (e->flags[ABORT_TC_RANGE] && e->use_tc) {
                 e->use_tc = false;  // a value beyond the fp16 split's range: recompute with the FFMA kernels

@@ -12,6 +12,7 @@ coordinates and global indices, n + 1 neighbourhood and classification rows (the
 Errors the reference throws as exceptions are raised as VisualMeshError. Nothing here computes: every call goes to
 libvmcuda.so, and a missing library or GPU is an error, not a fallback.
 """
+import contextlib
 import ctypes as C
 import math
 from dataclasses import dataclass
@@ -219,7 +220,7 @@ class BatchResult:
         """The arrays of results that were left on the device as torch tensors, frames one after another: pixel_coordinates [points, 2],
         global_indices [points], neighbourhood and classifications [points + n_frames, ...] (each frame's last row is its off-screen
         row; classifications is None after a projection). They are the engine's memory: valid until its next call, which does not wait
-        for what other streams still read there."""
+        for what other streams still read there unless Engine.wait_for was called behind it (scores, advance and filtered do)."""
         import torch
         if not self.on_device:
             raise VisualMeshError(abi.VM_ERR_INVALID_ARGUMENT, "results were copied to the host")
@@ -237,6 +238,16 @@ class BatchResult:
                 "neighbourhood": neighbourhood,
                 "classifications": tensor(self.raw.classifications, (rows, self.n_classes), "<f4", torch.float32) if self.n_classes else None}
 
+    @contextlib.contextmanager
+    def _read(self, x):
+        """Around calls that read x, memory of the engine: its next call waits for them."""
+        import torch
+        try:
+            yield
+        finally:
+            if self.engine is not None:
+                self.engine.wait_for(torch.cuda.current_stream(x.device))
+
     def _classifications(self):
         got = self.tensors()
         if got["classifications"] is None:
@@ -247,7 +258,9 @@ class BatchResult:
         """answers.scores of the classifications of a network that ends in a softmax: how probable its label ([points + n_frames], -1: none)
         is for every row, its entropy, and its best classes."""
         from . import answers
-        return answers.scores(self._classifications()[0], labels, top, probabilities=True)
+        x = self._classifications()[0]
+        with self._read(x):
+            return answers.scores(x, labels, top, probabilities=True)
 
     def advance(self, state, gate):
         """Filters the classifications over time, node by node: answers.gated_step for frame after frame, with the state of every node of
@@ -258,10 +271,11 @@ class BatchResult:
         from . import answers
         x, nodes = self._classifications()
         gate, y = gate.expand(x.shape), torch.zeros_like(x)
-        for f in range(self.n_frames):
-            p0, p1 = int(self.offsets[f]), int(self.offsets[f + 1])
-            at = slice(p0 + f, p1 + f)
-            answers.gated_step(state, x[at], gate[at], nodes[p0:p1], out=y[at])
+        with self._read(x):
+            for f in range(self.n_frames):
+                p0, p1 = int(self.offsets[f]), int(self.offsets[f + 1])
+                at = slice(p0 + f, p1 + f)
+                answers.gated_step(state, x[at], gate[at], nodes[p0:p1], out=y[at])
         return y
 
     def filtered(self, gate, h0=None, keep=False):
@@ -274,7 +288,8 @@ class BatchResult:
         if any(int(self.offsets[f]) != f * n for f in range(self.n_frames + 1)) or not bool((nodes.view(self.n_frames, n) == nodes[:n]).all()):
             raise VisualMeshError(abi.VM_ERR_INVALID_ARGUMENT, "the frames show different nodes")
         gate = gate.expand(self.n_frames, n + 1, self.n_classes).reshape(1, self.n_frames, -1)
-        return answers.gated_scan(x.view(gate.shape), gate, None if h0 is None else h0.reshape(1, -1), keep=keep)
+        with self._read(x):
+            return answers.gated_scan(x.view(gate.shape), gate, None if h0 is None else h0.reshape(1, -1), keep=keep)
 
 
 def _mesh_at(mesh, Hoc) -> Mesh:
@@ -417,6 +432,12 @@ class Engine:
         """Polls one bounded wait of the tensor-core kernels makes before the kernel gives up and the call fails with
         VM_ERR_DEVICE_ABORT (vm_set_wait_limit); 0 makes every such wait give up at once."""
         abi.check(self._lib.vm_set_wait_limit(self._ptr, int(polls)))
+
+    def wait_for(self, stream=None):
+        """The engine's next calls write to results that were left on the device only once everything that `stream` (a torch stream of the
+        engine's device; None: the current one) holds now is done (vm_wait_for). The host does not wait."""
+        import torch
+        abi.check(self._lib.vm_wait_for(self._ptr, (stream or torch.cuda.current_stream()).cuda_stream))
 
     def launch_count(self) -> int:
         return int(self._lib.vm_launch_count(self._ptr))
