@@ -4,7 +4,7 @@ import torch
 
 import golden_io as G
 from visualmesh_b200 import workloads as W
-from visualmesh_b200.engine import Engine, FrameInput, Mesh
+from visualmesh_b200.engine import Engine, FrameInput, Mesh, VisualMeshError
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +97,19 @@ def test_reads_of_results_are_captured(setup):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_results_of_an_earlier_call_cannot_be_had(setup):
+    engine, mesh, first, second = setup
+    old = engine.run_prepared(first, results_on_device=True)
+    new = engine.run_prepared(second, results_on_device=True)
+    new.scores()
+    with pytest.raises(VisualMeshError):
+        old.scores()
+    case = G.Case("ring6_equisolid_rgba")
+    fr = case.frames[0]
+    other = Engine(case.network, device=0)
+    result = other.run_batch([FrameInput(mesh, fr["Hoc"], case.lens, fr["image"], case.format)], results_on_device=True)
+    other.close()
+    with pytest.raises(VisualMeshError):
+        result.tensors()

@@ -191,6 +191,7 @@ class BatchResult:
     def __init__(self, raw: abi.vm_batch_result, engine=None):
         self.raw = raw
         self.engine = engine  # whose memory this is
+        self._call = engine.calls if engine is not None else None  # of the engine's calls the one that wrote it
         self.n_frames = raw.n_frames
         self.n_neighbours = raw.n_neighbours
         self.n_classes = raw.n_classes
@@ -219,11 +220,14 @@ class BatchResult:
     def tensors(self):
         """The arrays of results that were left on the device as torch tensors, frames one after another: pixel_coordinates [points, 2],
         global_indices [points], neighbourhood and classifications [points + n_frames, ...] (each frame's last row is its off-screen
-        row; classifications is None after a projection). They are the engine's memory: valid until its next call, which does not wait
-        for what other streams still read there unless Engine.wait_for was called behind it (scores, advance and filtered do)."""
+        row; classifications is None after a projection). They are the engine's memory: valid until its next call or until it is closed
+        (behind either they cannot be had any more). The next call does not wait for what other streams still read there unless
+        Engine.wait_for was called behind it; scores, advance and filtered do that."""
         import torch
         if not self.on_device:
             raise VisualMeshError(abi.VM_ERR_INVALID_ARGUMENT, "results were copied to the host")
+        if self.engine is not None and (self.engine.closed or self.engine.calls != self._call):
+            raise VisualMeshError(abi.VM_ERR_INVALID_ARGUMENT, "the engine was closed, or called again since: these results are gone")
         points, rows = self.total_points, self.total_points + self.n_frames
 
         def tensor(pointer, shape, kind, dtype, device="cuda"):
@@ -306,6 +310,7 @@ class Engine:
         self._lib = abi.load()
         self._max_cached_meshes = max_cached_meshes
         self._ptr = None
+        self.calls = 0  # that wrote, or tried to write, results
         structure = structure or []
         flat = [layer for group in structure for layer in group]
         layers = (abi.vm_layer * max(len(flat), 1))()
@@ -325,6 +330,10 @@ class Engine:
         self._ptr = ptr
         self._meshes = {}  # id(mesh) -> (mesh, device handle): the cache the OpenCL engine keeps per &mesh
         self.n_classes = flat[-1].biases.shape[0] if flat else 0
+
+    @property
+    def closed(self) -> bool:
+        return not self._ptr
 
     def close(self):
         if self._ptr:
@@ -376,6 +385,7 @@ class Engine:
         arr, n, _ = prepared
         flags = (abi.VM_RESULTS_ON_DEVICE if results_on_device else 0) | (abi.VM_TIME_STAGES if time_stages else 0)
         res = abi.vm_batch_result()
+        self.calls += 1
         abi.check(self._lib.vm_run_batch(self._ptr, arr, n, flags, C.byref(res)))
         return res if raw else BatchResult(res, self)
 
@@ -403,6 +413,7 @@ class Engine:
             ranges = None
         if image is not None and self.n_classes == 0:
             raise VisualMeshError(abi.VM_ERR_NETWORK_SHAPE, "this engine was created without a network")
+        self.calls += 1
         out = abi.native().call(self._ptr.value, self._device_mesh(m).value, host or 0, ranges, Hoc, lens, image, format or 0)
         if isinstance(out, int):
             abi.check(out)
@@ -455,6 +466,7 @@ class Engine:
         x = np.ascontiguousarray(inputs, dtype=np.float32).reshape(-1, 4)
         nb = np.ascontiguousarray(neighbourhood, dtype=np.int32)
         out = np.empty((x.shape[0], self.n_classes), dtype=np.float32)
+        self.calls += 1
         abi.check(self._lib.vm_network(self._ptr, x.ctypes.data, nb.ctypes.data, x.shape[0], nb.shape[1],
                                        out.ctypes.data))
         return out
