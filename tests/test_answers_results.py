@@ -25,3 +25,14 @@ def test_results_that_are_gone_cannot_be_had(change):
     for read in (result.tensors, result.scores, lambda: result.advance(None, None), lambda: result.filtered(None)):
         with pytest.raises(VisualMeshError, match="gone"):
             read()
+
+
+def test_scores_need_probabilities(monkeypatch):
+    engine = FakeEngine()
+    engine.gives_probabilities = False
+    raw = abi.vm_batch_result()
+    raw.on_device = 1
+    result = BatchResult(raw, engine)
+    monkeypatch.setattr(result, "_classifications", lambda: (None, None))
+    with pytest.raises(VisualMeshError, match="probabilities"):
+        result.scores()

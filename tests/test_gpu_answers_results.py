@@ -1,4 +1,6 @@
 """Results that an engine left on the device, read by torch's streams while the engine goes on."""
+import dataclasses
+
 import pytest
 import torch
 
@@ -113,3 +115,21 @@ def test_results_of_an_earlier_call_cannot_be_had(setup):
     other.close()
     with pytest.raises(VisualMeshError):
         result.tensors()
+
+
+@pytest.mark.parametrize("activation", [W.SELU, W.RELU, W.SOFTMAX, W.TANH])
+def test_scores_of_answers_that_are_no_probabilities_are_refused(activation):
+    from visualmesh_b200 import answers
+    case = G.Case("ring6_equisolid_rgba")
+    network = [list(group) for group in case.network]
+    network[-1][-1] = dataclasses.replace(network[-1][-1], activation=activation)
+    mesh, fr = Mesh.from_arrays(case.rays, case.nbrs, case.bsp), case.frames[0]
+    engine = Engine(network, device=0)
+    result = engine.run_batch([FrameInput(mesh, fr["Hoc"], case.lens, fr["image"], case.format)], results_on_device=True)
+    if activation == W.SOFTMAX:
+        assert bool(torch.isfinite(result.scores().entropy).all())
+    else:
+        with pytest.raises(VisualMeshError, match="probabilities"):
+            result.scores()
+        answers.scores(result.tensors()["classifications"])
+    engine.close()

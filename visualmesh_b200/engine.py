@@ -22,7 +22,7 @@ import numpy as np
 
 from . import abi
 from .abi import VisualMeshError  # noqa: F401  (re-export)
-from .workloads import Lens
+from .workloads import SOFTMAX, Lens
 
 
 def _c_lens(lens) -> abi.vm_lens:
@@ -259,10 +259,13 @@ class BatchResult:
         return got["classifications"], got["global_indices"]
 
     def scores(self, labels=None, top=1):
-        """answers.scores of the classifications of a network that ends in a softmax: how probable its label ([points + n_frames], -1: none)
-        is for every row, its entropy, and its best classes."""
+        """answers.scores of the classifications of a network that ends in a softmax (of another's they would be no probabilities, and are refused;
+        answers.scores takes its tensor as logits): how probable its label ([points + n_frames], -1: none) is for every row, its entropy, and
+        its best classes."""
         from . import answers
         x = self._classifications()[0]
+        if self.engine is not None and not self.engine.gives_probabilities:
+            raise VisualMeshError(abi.VM_ERR_NETWORK_SHAPE, "this network does not end in a softmax: its answers are no probabilities")
         with self._read(x):
             return answers.scores(x, labels, top, probabilities=True)
 
@@ -330,6 +333,7 @@ class Engine:
         self._ptr = ptr
         self._meshes = {}  # id(mesh) -> (mesh, device handle): the cache the OpenCL engine keeps per &mesh
         self.n_classes = flat[-1].biases.shape[0] if flat else 0
+        self.gives_probabilities = bool(flat) and int(flat[-1].activation) == SOFTMAX
 
     @property
     def closed(self) -> bool:
