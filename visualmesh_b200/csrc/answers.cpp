@@ -83,6 +83,11 @@ Maybe like(PyObject* o, const char* name, at::IntArrayRef shape, at::ScalarType 
     return x;
 }
 
+// x is written in place: autograd's record of what it saved of x is no longer of x. (Tensors of inference mode have no such record.)
+void written(const Tensor& x) {
+    if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor make(at::IntArrayRef shape, at::ScalarType type, const at::Device& device) {
     return at::empty(shape, at::TensorOptions().dtype(type).device(device));
 }
@@ -299,6 +304,8 @@ PyObject* gated_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const size_t size = index ? vm_gated_step_workspace(rows, slots) : 0;
         const Maybe workspace = workspace_of(size, device);
         const vm_sequence vx = row_sequence(x), vg = row_sequence(gate), vy = row_sequence(y);
+        written(state);
+        if (out) written(*out);
         check(vm_gated_step(device.index(), type, rows, slots, channels, pointer<float>(state), state.stride(0), &vx, &vg, pointer<int32_t>(index), &vy, pointer(workspace), size,
                             stream_of(x)));
         return wrap(y);
