@@ -6,6 +6,7 @@
 
 #include <ATen/Functions.h>
 #include <ATen/core/Tensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -50,14 +51,19 @@ const Tensor& tensor_of(PyObject* o, const char* name) {
     if (!THPVariable_Check(o)) refuse(std::string(name) + " must be a tensor on the GPU (there is no CPU fallback)");
     return THPVariable_Unpack(o);
 }
-void check_grad(const Tensor& x, const char* name) {
-    if (x.requires_grad() && c10::GradMode::is_enabled()) refuse(std::string(name) + " requires a gradient, which autograd would not get: detach it and call the backward function");
+// No gradient, forward or backward, would be lost, and x holds its own values.
+void check_plain(const Tensor& x, const char* name) {
+    if (x.unsafeGetTensorImpl()->autograd_meta() != nullptr) {  // plain tensors have none
+        if (x.requires_grad() && c10::GradMode::is_enabled()) refuse(std::string(name) + " requires a gradient, which autograd would not get: detach it and call the backward function");
+        if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && x._fw_grad(0).defined()) refuse(std::string(name) + " has a tangent, which forward differentiation would lose: unpack it first");
+    }
+    if (x.key_set().has_any(c10::DispatchKeySet({c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor}))) refuse(std::string(name) + " is a view that holds no values of its own: call resolve_neg() or clone()");
 }
 // x is on the GPU, has so many dimensions and one of the three types, which is returned
 int32_t type_of(const Tensor& x, const char* name, int64_t dimensions) {
     if (!x.is_cuda() || x.layout() != at::kStrided) refuse(std::string(name) + " must be a tensor on the GPU (there is no CPU fallback)");
     if (x.dim() != dimensions) refuse(std::string(name) + " must have " + std::to_string(dimensions) + " dimensions");
-    check_grad(x, name);
+    check_plain(x, name);
     switch (x.scalar_type()) {
         case at::kFloat: return VM_F32;
         case at::kHalf: return VM_F16;
@@ -73,7 +79,7 @@ void check_like(const Tensor& x, const char* name, at::IntArrayRef shape, at::Sc
         for (const int64_t n : shape) wanted += std::to_string(n) + ", ";
         refuse(wanted + ")");
     }
-    check_grad(x, name);
+    check_plain(x, name);
     if (layout == DENSE && !x.is_contiguous()) refuse(std::string(name) + " must be contiguous");
 }
 Maybe like(PyObject* o, const char* name, at::IntArrayRef shape, at::ScalarType type, const at::Device& device, Layout layout) {
