@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/vmcuda.h"
@@ -44,6 +45,13 @@ inline bool known_type(int32_t type) {
 }
 inline bool aligned(const void* p, size_t to) {
     return reinterpret_cast<uintptr_t>(p) % to == 0;
+}
+
+// whether all of these begin on their 32-bit elements (NULL: absent)
+inline bool words_aligned(std::initializer_list<const void*> pointers) {
+    for (const void* p : pointers)
+        if (!aligned(p, 4)) return false;
+    return true;
 }
 
 // f(a value of the element type) for one of the three types

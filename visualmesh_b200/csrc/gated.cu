@@ -250,6 +250,7 @@ vm_status vm_gated_scan(int device, int32_t type, int64_t batch, int64_t steps, 
         check_sequence(x, "x", type, sizes, steps > 0, false);
         check_sequence(gate, "gate", type, sizes, steps > 0, false);
         check_sequence(y, "y", type, sizes, false, true);
+        if (!words_aligned({h0, lengths, last, states})) throw std::string("h0, lengths, last or states are not aligned to their elements");
         check_workspace(batch, steps, channels, workspace, workspace_bytes);
         const OnDevice on(device);
         GatedArgs a{};
@@ -306,6 +307,7 @@ vm_status vm_gated_scan_backward(int device, int32_t type, int64_t batch, int64_
         check_sequence(dx, "dx", type, sizes, false, true);
         check_sequence(d_gate, "d_gate", type, sizes, false, true);
         if (steps > 0 && states == nullptr) throw std::string("null states");
+        if (!words_aligned({states, lengths, d_last, d_h0})) throw std::string("states, lengths, d_last or d_h0 are not aligned to their elements");
         check_workspace(batch, steps, channels, workspace, workspace_bytes);
         const OnDevice on(device);
         GatedArgs a{};
@@ -360,6 +362,7 @@ vm_status vm_gated_step(int device, int32_t type, int64_t rows, int64_t slots, i
         check_sequence(gate, "gate", type, sizes, true, false);
         check_sequence(y, "y", type, sizes, false, true);
         if (slots > 0 && state == nullptr) throw std::string("null state");
+        if (!words_aligned({state, index})) throw std::string("state or index are not aligned to their elements");
         if (state_stride < (slots > 1 ? channels : 0) || state_stride > MOST / (slots > 0 ? slots : 1)) throw std::string("the states of slots overlap");
         const size_t needed = index != nullptr ? vm_gated_step_workspace(rows, slots) : 0;
         if (workspace_bytes < needed || (needed > 0 && (workspace == nullptr || !aligned(workspace, 16)))) throw std::string("the workspace is too small, null or not aligned");

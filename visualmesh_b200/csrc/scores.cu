@@ -126,6 +126,7 @@ vm_status vm_scores(int device, const void* x, int32_t type, int64_t rows, int32
         if (top < 0 || top > VM_MAX_TOP || top > classes) return fail(VM_ERR_INVALID_ARGUMENT, "top must be 0..min(classes, VM_MAX_TOP)");
         if (rows == 0) return VM_OK;
         if (top > 0 && (top_log_prob == nullptr || top_index == nullptr)) return fail(VM_ERR_INVALID_ARGUMENT, "top without its outputs");
+        if (!words_aligned({log_prob, entropy, log_sum, top_log_prob, top_index})) return fail(VM_ERR_INVALID_ARGUMENT, "an output is not aligned to its elements");
         if (log_prob != nullptr && labels == nullptr) return fail(VM_ERR_INVALID_ARGUMENT, "log_prob without labels");
         const OnDevice on(device);
         const ScoresArgs a{x, rows, classes, row_stride, labels, (flags & VM_LABELS_64) != 0, top, log_prob, entropy, log_sum, top_log_prob, top_index};
@@ -183,6 +184,7 @@ vm_status vm_scores_backward(int device, const void* x, int32_t type, int64_t ro
         if (rows == 0) return VM_OK;
         if (dx == nullptr || log_sum == nullptr) return fail(VM_ERR_INVALID_ARGUMENT, "null dx or log_sum");
         if (!aligned(dx, element_size(type))) return fail(VM_ERR_INVALID_ARGUMENT, "dx is not aligned to its elements");
+        if (!words_aligned({entropy, log_sum, d_log_prob, d_entropy, d_log_sum})) return fail(VM_ERR_INVALID_ARGUMENT, "an input is not aligned to its elements");
         if (d_log_prob != nullptr && labels == nullptr) return fail(VM_ERR_INVALID_ARGUMENT, "d_log_prob without labels");
         if (d_entropy != nullptr && entropy == nullptr) return fail(VM_ERR_INVALID_ARGUMENT, "d_entropy without entropy");
         const OnDevice on(device);
