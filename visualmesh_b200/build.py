@@ -9,6 +9,7 @@ library; a unit is recompiled when it or one of the headers it includes is newer
 -fmad=false and -ffp-contract=off are part of the contract: the projection arithmetic must round every operation
 the way the reference CPU engine does. The graph-convolution kernels call fmaf() explicitly.
 """
+import importlib.util
 import os
 import subprocess
 import sys
@@ -64,7 +65,12 @@ def _stale(unit):
 
 def needs_build():
     """The library is missing or older than one of its sources (object files may be absent: they do not travel)."""
-    return _library_stale() or any(_module_stale(m) for m in MODULES)
+    return _library_stale() or any(_module_stale(m) for m in MODULES if m != ANSWERS or _has_torch())
+
+
+def _has_torch():
+    """_answers is torch's tensors for the operators on answers; everything else is built and runs without torch."""
+    return importlib.util.find_spec("torch") is not None
 
 
 def _library_stale():
@@ -93,7 +99,9 @@ def build(force=False, verbose=False):
     if force or _module_stale(NATIVE):
         import numpy
         _build_module(NATIVE, ["-I", numpy.get_include()])
-    if force or _module_stale(ANSWERS):
+    if not _has_torch():
+        sys.stderr.write("torch is not installed: visualmesh_b200._answers is not built\n")
+    elif force or _module_stale(ANSWERS):
         from torch.utils import cpp_extension  # torch's own libraries are loaded before the module is
         _build_module(ANSWERS, [f"-isystem{p}" for p in cpp_extension.include_paths("cuda")] + [f"-L{cpp_extension.library_paths()[0]}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
                                                                                                 "-ltorch", "-ltorch_python"])
