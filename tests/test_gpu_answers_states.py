@@ -189,3 +189,16 @@ def test_steps_with_factors_below_the_normal_numbers(answers, rows, channels, dt
         y = answers.gated_step(table, x, g, index)
         near(y, want, error.nan_to_num(0, 0, 0) + rounding(want, dtype) + 1e-37)
         near(table[rows_of], want, error.nan_to_num(0, 0, 0) + 1e-37)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("batch,steps,channels", SIZES)
+def test_lowest_values_that_are_masked_beside_large_states(answers, batch, steps, channels, dtype):
+    """What a gate of infinity drops has no part in a gradient, though its difference to the state is beyond the range."""
+    x, g, h0, dy, d_last = sequences(batch, steps, channels, dtype, steps + 3)
+    h0 = h0.abs() * 1e37 + 1e37
+    at = torch.arange(2, 12, 3, device="cuda")
+    g[:, at] = math.inf
+    x[:, at] = torch.finfo(dtype).min
+    g[:, 12] = -math.inf
+    check(answers, x, g, h0, dy * 0.5, d_last)

@@ -212,13 +212,16 @@ __device__ __forceinline__ void products(const float (&f)[L][V], float (&A)[V]) 
         for (int k = 0; k < V; ++k) A[k] = product(f[i][k], A[k]);
     }
 }
+// Whether all are below `limit` (and numbers).
 template <int V>
-__device__ __forceinline__ bool finite(const float (&v)[V]) {
+__device__ __forceinline__ bool finite(const float (&v)[V], float limit = INFINITY) {
     bool ok = true;
 #pragma unroll
-    for (int k = 0; k < V; ++k) ok = ok && fabsf(v[k]) < INFINITY;
+    for (int k = 0; k < V; ++k) ok = ok && fabsf(v[k]) < limit;
     return ok;
 }
+// States from which on h - x leaves the range where x is the lowest value (half a step of it), which a factor of 0 has to drop where it is masked.
+constexpr float LARGE = 1e31f;
 
 // Scan over the lanes along time, in their order or (REVERSE) against it. In: every thread's map (A, H). Out: the map of all threads
 // before it in its own warp, and that of the whole warp in `shared`. careful: in one of the lanes a factor is 0 or a value not finite.
@@ -883,7 +886,7 @@ __global__ void __launch_bounds__(CLUSTER ? 128 : 256, CLUSTER ? 4 : 2) k_gated_
             }
         };
         pass(std::false_type{});
-        bool careful    = !finite<V>(H) || !finite<V>(R);
+        bool careful    = !finite<V>(H, LARGE) || !finite<V>(R);
         const bool zero = has_zero<V>(A);
         if (careful) pass(std::true_type{});
         else if (zero) products<V, L>(f, A);
@@ -903,7 +906,7 @@ __global__ void __launch_bounds__(CLUSTER ? 128 : 256, CLUSTER ? 4 : 2) k_gated_
         __syncthreads();
         state_before<V, W>(at, shared, A, H, h);
         state_before<V, W>(at, shared_back, AR, R, c);
-        careful = careful || !finite<V>(h) || !finite<V>(c);
+        careful = careful || !finite<V>(h, LARGE) || !finite<V>(c);
         // w: h_(t-1) - x, then the gradient of the gate; u: to the gradient of x
         const auto grads = [&](auto care) {
             constexpr bool CAREFUL = decltype(care)::value;
