@@ -281,8 +281,9 @@ VM_API void vm_host_free(void* ptr);
  * sequence of frames adds. All pointers are DEVICE pointers of the caller, on `device` (< 0: the current device; the device that was
  * current is current again when the call returns). The calls enqueue their kernels on `stream` (a cudaStream_t, NULL: the default
  * stream) and return: they neither wait, allocate nor keep anything, so they may be captured into a CUDA graph, from any number of
- * threads. Pointers are aligned to their elements; outputs overlap neither inputs nor one another. What an engine left on the device (VM_RESULTS_ON_DEVICE) is complete when
- * its call returns; before the engine's next call writes there again, `stream` has to be done with it: see vm_wait_for.
+ * threads. Pointers are aligned to their elements; outputs overlap neither inputs nor one another. What an engine left on the device
+ * (VM_RESULTS_ON_DEVICE) is complete when its call returns; before the engine's next call writes there again, `stream` has to be done
+ * with it: see vm_wait_for.
  * ------------------------------------------------------------------------------------------------------------------ */
 
 /* element types; sums, logarithms and states are 32-bit floats whatever the type */

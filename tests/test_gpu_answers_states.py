@@ -1,8 +1,10 @@
 """The gated recurrence with states and values of any size: what a factor of 32 bits can hold of them, and nothing more, is lost.
 
-Tolerances, with u = 2^-24: a factor (ex2 of half the rounded product, squared, and a reciprocal) is off by (8 + 1.2 |g|) u of itself as long as
-it is a normal number, and by 2^-149 more below. |g| counts up to 104, where the factor is 0 in 32 bits. With e_t = 2 (10 + 1.2 |g_t|) u for a
-step (its factor, product and sum, and as much again for the joining of runs of steps) the error E_t of h_t obeys
+Tolerances, with u = 2^-24: the half of a gate times log2 e is off by |g| u in the exponent (its product and its constant), ex2.approx by 2^-22.5
+of its result, both doubled by the square; with the square's own rounding, the sum, the reciprocal (2u) and the product behind it a factor is off by
+(11 + 2 |g|) u of itself as long as it is a normal number, and by 2^-149 more below. |g| counts up to 104, where the factor is 0 in 32 bits. A step's
+product and sum round by 2u, and of the joining of runs of steps it has less than 3u (a tile of 64 steps and more is joined in some thirteen
+products). With e_t = (20 + 2.4 |g_t|) u for a step the error E_t of h_t obeys
 E_t = f_t E_(t-1) + e_t M_t with the majorant M_t = f_t M_(t-1) + u_t |x_t|, and the gradient's the same backwards. The factor of a run of steps
 may be a number below the normal ones, off by 2^-149 for each of 64 products (the steps of a thread, the threads of a block, the tiles):
 2^-143 of the largest state or sum of gradients in all.

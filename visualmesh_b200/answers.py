@@ -9,8 +9,9 @@
 What each computes, masks, lengths and special values included, is written beside its entry point in include/vmcuda.h. The calls
 enqueue on torch's current stream of the tensors' device and return without waiting; they may be captured into a CUDA graph. Results and
 workspaces are new tensors of every call. Tensors have float32, float16 or bfloat16 elements with any strides that are not negative,
-where nothing else is said. Autograd does not see these calls: the gradients are functions of their own, and a tensor that requires a
-gradient is refused where gradients are recorded. Refused calls raise VisualMeshError.
+where nothing else is said. Autograd does not see these calls: the gradients are functions of their own, a tensor that requires a
+gradient is refused where gradients are recorded, and so is one with a tangent of forward differentiation. What gated_step writes in place
+counts as written. Refused calls raise VisualMeshError.
 """
 from typing import NamedTuple, Optional
 

@@ -1,6 +1,6 @@
-// Elements of 32 or 16 bits read as 32-bit floats and written with one rounding to nearest; e^t and 1 / d for arguments that stay away
+// Elements of 32 or 16 bits read as 32-bit floats and written with one rounding to nearest; e^t, 2^t and 1 / d for arguments that stay away
 // from the ends of the range: one instruction each beside a product, with numbers below the normal ones taken for 0 (the general forms spend
-// three to four more on those). Both are off by two units in the last place at most, e^t by 1.2 |t| more for the product's rounding.
+// three to four more on those). All are off by two units in the last place at most, e^t by 1.2 |t| more for the product's rounding.
 #pragma once
 
 #include <cuda_bf16.h>

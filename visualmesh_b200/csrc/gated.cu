@@ -80,7 +80,7 @@ void check_sizes(int32_t type, int64_t batch, int64_t steps, int64_t channels) {
 }
 
 // ---- how a scan is laid out ----------------------------------------------------------------------------------------------
-constexpr int SMS = 148;
+constexpr int SMS = 148;  // of a B200; which launch is taken depends on it, no result
 
 // A thread takes pairs of channels where they lie side by side, else single ones; a block 32 channels either way. Steps of a thread in the
 // forward and in the backward pass: what its 128 registers hold (but for a few outside of the loops), with two blocks an SM. Half the steps in 80

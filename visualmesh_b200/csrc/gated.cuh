@@ -108,9 +108,9 @@ __device__ __forceinline__ int64_t length_of(const GatedArgs& a, int64_t b) {
 //
 // W is 8 where a block walks alone (the more threads along time, the fewer tiles), 4 where a cluster shares a sequence: narrower blocks are
 // more of them, and a cluster need not be as large (3 x 1021 x 515 floats, forward and backward: 33 us and 29).
-// Bound by the instructions: 30 for an element forward and 60 backward (an exponential, a reciprocal, conversions, one map or two, the scan's
-// share), which take 60 % of the issue slots with 16 warps an SM (128 registers), the rest being barriers and the ring's wait. 4 x 4096 x 2048
-// forward / backward: bf16 53 / 97 us (31 / 51 at the memory's rate), float 67 / 118 (61 / 102). Clusters were slower wherever blocks fill the
+// Bound by the instructions: 32 for an element forward and 64 backward (an exponential, a reciprocal, conversions, one map or two, the scan's
+// share), which take 66 to 71 % of the active issue slots with 16 warps an SM (128 registers), the rest being barriers and the ring's wait. 4 x 4096 x
+// 2048 forward / backward: bf16 51 / 95 us (31 / 51 at the memory's rate), float 66 / 115 (61 / 102). Clusters were slower wherever blocks fill the
 // SMs (the same in clusters of 2: 66 / 123), as were pairs of floats in one instruction (moves into even registers cost what they save).
 template <int W>
 struct Shape {
@@ -289,10 +289,10 @@ __device__ __forceinline__ void state_before(const Place<V, W>& at, const Betwee
 
 template <int BYTES>
 __device__ __forceinline__ void copy_async(void* to, const void* from) {
-    static_assert(BYTES == 4 || BYTES == 8 || BYTES == 16, "sizes of an asynchronous copy");
+    static_assert(BYTES == 4 || BYTES == 16, "pieces of the ring");
     const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
     if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(at), "l"(from) : "memory");
 }
 
 // A gate that keeps the state: what stands for steps that are not there (with a value of 0).
@@ -685,8 +685,8 @@ __global__ void __launch_bounds__(CLUSTER ? 128 : 256, (V == 1 ? 3 : 2) * (CLUST
     if (a.last != nullptr && carries && blockIdx.y + 1 == gridDim.y) a.last[of_channel] = carry;
 }
 
-// Many short sequences: a thread walks along time alone, AHEAD steps' loads in front of itself. Bound by the memory: 64 x 204303 floats 33 us,
-// 24 at the memory's rate; 64 x 204304 bf16 in pairs 24 (by single elements 28), 12 at the memory's rate.
+// Many short sequences: a thread walks along time alone, AHEAD steps' loads in front of itself. Bound by the loads' latency: 64 x 204303 floats 33
+// us, 24 at the memory's rate; 64 x 204304 bf16 in pairs 23 (by single elements 28), 12 at the memory's rate.
 constexpr int SERIAL_BLOCK = 128, AHEAD = 8;
 
 template <int BLOCK, int V>
@@ -749,7 +749,7 @@ __global__ void __launch_bounds__(SERIAL_BLOCK) k_gated_serial(const GatedArgs a
 
 // The gradient of few steps: forward through them from the kept state, with h_(t-1) - x_t and the gates left in shared memory (every thread
 // has its own column: no two of a warp share a bank, nothing waits), then backward. Bound by latency: shared memory holds 7 blocks of 64
-// threads an SM. 64 x 204304: bf16 58 us (20 at the memory's rate), floats 77 (40); 16 x 204304 17 and 15. Pairs were no faster (58 and 101).
+// threads an SM. 64 x 204304: bf16 56 us (20 at the memory's rate), floats 76 (40); 16 x 204304 17 and 15. Pairs were no faster (58 and 101).
 constexpr int SERIAL_GRAD_BLOCK = 64;
 inline size_t serial_shared(int64_t steps, size_t element) {
     return static_cast<size_t>(steps) * SERIAL_GRAD_BLOCK * (sizeof(float) + element);

@@ -20,7 +20,7 @@ vm_status check_rows(const void* x, int32_t type, int64_t rows, int32_t classes,
     return VM_OK;
 }
 
-constexpr int SMS = 148;
+constexpr int SMS = 148;  // of a B200; which launch is taken depends on it, no result
 // Classes that a thread holds in its registers. 1,000,000 rows of 8 floats, with the two best / their gradient: 19 / 19 us, by two lanes a row
 // 35 / 23; of 3 floats 11 / 11 and 36 / 16.
 constexpr int MOST_OF_THREAD = 8;

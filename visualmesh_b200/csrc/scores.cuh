@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(ROWS_BLOCK) k_scores_rows(const ScoresArgs a, 
 // collected and the largest of it taken. Where that is more than there is room for (many of the largest in one thread's pieces) or the row holds
 // NaN, the row is searched `top` times instead.
 // Few rows: a cluster of blocks shares a row, and the first of them joins their results through its shared memory.
-// 4099 rows of 32771 bf16: 60 us, with five best 73, 41 at the memory's rate; a plain sum over the same rows takes 59. Two thirds of the issue
+// 4099 rows of 32771 bf16: 62 us, with five best 72, 41 at the memory's rate; a plain sum over the same rows takes 59. Two thirds of the issue
 // slots and of the exponentials' pipe are taken; loads a step ahead in registers moved it by -4 to +2 % (fewer blocks fit). 4 x 131072 fp16 with
 // 20 best: 12.3 us, of which 4 are a launch and 4 the cluster's two barriers and the joining.
 constexpr int STREAM_BLOCK = 256;
@@ -704,8 +704,8 @@ __global__ void __launch_bounds__(BLOCK) k_scores_stream(const ScoresArgs a, int
     bool search = false;
     if (TOP || CLUSTER) search = __syncthreads_or(q.s != q.s || q.w != q.w);  // NaN, or an infinity: its maxima were no maxima
     else {
-        // The warps behind the first stay only for a row that is summed again: the largest of the warps' maxima is beyond BELOW where one of them is,
-        // and above ABOVE where one of them is.
+        // The warps behind the first stay only for a row that is summed again: where one of the warps' maxima is beyond BELOW (all lanes count), or
+        // none is above ABOVE (one lane each). To have them all join the sums for that took 3 to 6 % more.
         const int ways = __syncthreads_count(!PROBABILITIES && (q.m >= Range<T>::BELOW || (q.m > Range<T>::ABOVE && lane == 0)));
         if (warp != 0 && (PROBABILITIES || (ways > 0 && ways < WARP))) return;
     }
@@ -798,7 +798,7 @@ __global__ void __launch_bounds__(BLOCK) k_scores_stream(const ScoresArgs a, int
 
 // ---- gradients -----------------------------------------------------------------------------------------------------------------
 // One pass over the elements once the row's sums are known. 16 x 68101 rows of five floats, forward and backward: 26.6 us (two launches, 15 at the
-// memory's rate for both passes); 2048 x 50021 bf16: 130, of which this is 80 (its 410 MB at 5.1 TB/s; 63 at the memory's rate).
+// memory's rate for both passes); 2048 x 50021 bf16: 128, of which this is 79 (its 410 MB at 5.2 TB/s; 63 at the memory's rate).
 //
 // The probabilities come from log p = v - log_sum, off by what log_sum was rounded by when it was written: half a step of it. Beyond FAR that is
 // more than a result should lose (2^-19 of p; with 16 bits 2^-15, a sixteenth of their half step), and a row of the type's lowest value would
@@ -1034,8 +1034,8 @@ __global__ void __launch_bounds__(STREAM_BLOCK, !PROBABILITIES && sizeof(T) == 2
         if (begin + u * STREAM_BLOCK < pieces.count) raw[u] = pieces.load(begin + u * STREAM_BLOCK, outside);
     const RowGrad<PROBABILITIES> grad(a, row);
     // Logits, in powers of two and by pairs as above: with S = log_sum L rounded, t = x L - S and rho = log_sum L - S, log p = (t - rho) log 2
-    // and p = 2^(t - rho), so that rho joins the factors of the row. Values are not let below
-    // log_sum - 1000, where p is 0: of a row that is not far from 0 that is below log_sum in every type.
+    // and p = 2^(t - rho), so that rho joins the factors of the row. Values are not let below log_sum - 1000, where p is 0; of a row that is not
+    // far from 0 that is well below log_sum in every type.
     const float S = grad.log_sum * LOG2_E, rho = fmaf(grad.log_sum, LOG2_E, -S), back = exp2_of(-rho);
     const float slope = -grad.d_entropy * LOG_2 * back, level = fmaf(grad.d_entropy * LOG_2, rho, grad.offset) * back;
     const bool quick  = !PROBABILITIES && fabsf(grad.log_sum) < INFINITY && fabsf(grad.offset) < INFINITY;

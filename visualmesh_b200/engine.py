@@ -287,8 +287,9 @@ class BatchResult:
 
     def filtered(self, gate, h0=None, keep=False):
         """answers.gated_scan over the frames of a camera that stands still over one mesh: every frame shows the same nodes (anything else is
-        refused), so that row r of all frames is one sequence. gate: what broadcasts to [n_frames, rows, n_classes] float32; h0: [rows,
-        n_classes]. y, last and states have the rows' classes side by side."""
+        refused; the host waits for the comparison, so that this call cannot be captured), so that row r of all frames is one sequence. gate:
+        what broadcasts to [n_frames, rows, n_classes] float32 (written out in full where it is smaller); h0: [rows, n_classes]. y, last and states
+        have the rows' classes side by side."""
         from . import answers
         x, nodes = self._classifications()
         n = self.total_points // max(self.n_frames, 1)
