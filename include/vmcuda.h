@@ -358,8 +358,9 @@ typedef struct vm_sequence {
 /* A gated linear recurrence over `steps` of batch x channels sequences: with f = 1 / (1 + exp(-gate)),
  *   h_t = f_t h_(t-1) + (1 - f_t) x_t,   y_t = h_t,   h_(-1) = h0 (NULL: zero),   last = h after the last step.
  * gate = -infinity drops what was before (the sequence begins anew), +infinity drops x_t (nothing was seen), whatever they hold, NaN
- * and infinities included; so do gates beyond -104 and 104, whose factor is 0 in 32 bits. lengths (NULL: all `steps`): sequence b has lengths[b] steps (clamped to 0..steps); y is 0 behind them and
- * last is h after the last of them. x, gate and y have `type`; h0, last and states are 32-bit, batch x channels without gaps.
+ * and infinities included; so do gates beyond -104 and 104, whose factor is 0 in 32 bits. lengths (NULL: all `steps`): sequence b has
+ * lengths[b] steps (clamped to 0..steps); y is 0 behind them and last is h after the last of them. x, gate and y have `type`; h0, last and
+ * states are 32-bit, batch x channels without gaps.
  * states (may be NULL): batch x ceil(steps / VM_GATED_KEEP) x channels, h before steps 0, 64, 128, ...: what the backward pass starts from.
  * y and last may be NULL. workspace: at least vm_gated_workspace(batch, steps, channels) bytes, aligned to 16, that no other call uses
  * until this one's kernels are done (NULL when that is 0). steps, batch or channels may be 0. */
