@@ -204,3 +204,18 @@ def test_lowest_values_that_are_masked_beside_large_states(answers, batch, steps
     x[:, at] = torch.finfo(dtype).min
     g[:, 12] = -math.inf
     check(answers, x, g, h0, dy * 0.5, d_last)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("batch,steps,channels", SIZES)
+def test_values_at_both_ends_of_the_range(answers, batch, steps, channels, dtype):
+    """States and values whose difference is beyond the range, inside a thread's steps too: what a factor of 0 drops is dropped, and a small one comes first."""
+    x, g, h0, dy, d_last = sequences(batch, steps, channels, dtype, steps + 4)
+    lowest = torch.finfo(dtype).min
+    for at in (2, 9, 19, 27):
+        x[:, at], g[:, at] = 3e37, 1.0                  # large for a while,
+        x[:, at + 1], g[:, at + 1] = lowest, math.inf   # beside what is masked,
+        x[:, at + 2], g[:, at + 2] = lowest, -math.inf  # until a new beginning with the lowest value,
+        x[:, at + 3], g[:, at + 3] = 2e37, -20.0        # which is forgotten at once
+        g[:, at + 4] = -math.inf
+    check(answers, x, g, h0, dy * 0.1, d_last)

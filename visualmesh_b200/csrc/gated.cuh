@@ -70,10 +70,6 @@ __device__ __forceinline__ float gated(float a, float b) {
 __device__ __forceinline__ float gated(float a, float b, float c) {
     return a == 0.0f ? c : fmaf(a, b, c);
 }
-// a * b * c, where a of 0 drops the others, and a large b does not leave the range before a small a has met it
-__device__ __forceinline__ float gated_gradient(float a, float b, float c) {
-    return a == 0.0f ? 0.0f : a * b * c;
-}
 // The factor of two runs of steps. It is 0 only where a step's is: what 32 bits cannot hold becomes their smallest number, so that an infinity or NaN
 // goes on through a long run as it does step by step, and of a state at the end of the range 5e-7 stay.
 constexpr float SMALLEST = 1.40129846e-45f;
@@ -212,16 +208,13 @@ __device__ __forceinline__ void products(const float (&f)[L][V], float (&A)[V]) 
         for (int k = 0; k < V; ++k) A[k] = product(f[i][k], A[k]);
     }
 }
-// Whether all are below `limit` (and numbers).
 template <int V>
-__device__ __forceinline__ bool finite(const float (&v)[V], float limit = INFINITY) {
+__device__ __forceinline__ bool finite(const float (&v)[V]) {
     bool ok = true;
 #pragma unroll
-    for (int k = 0; k < V; ++k) ok = ok && fabsf(v[k]) < limit;
+    for (int k = 0; k < V; ++k) ok = ok && fabsf(v[k]) < INFINITY;
     return ok;
 }
-// States from which on h - x leaves the range where x is the lowest value (half a step of it), which a factor of 0 has to drop where it is masked.
-constexpr float LARGE = 1e31f;
 
 // Scan over the lanes along time, in their order or (REVERSE) against it. In: every thread's map (A, H). Out: the map of all threads
 // before it in its own warp, and that of the whole warp in `shared`. careful: in one of the lanes a factor is 0 or a value not finite.
@@ -747,7 +740,7 @@ __global__ void __launch_bounds__(SERIAL_BLOCK) k_gated_serial(const GatedArgs a
     if (a.last != nullptr) store_floats<V>(a.last + q.at, h);
 }
 
-// The gradient of few steps: forward through them from the kept state, with h_(t-1) - x_t and the gates left in shared memory (every thread
+// The gradient of few steps: forward through them from the kept state, with half of h_(t-1) - x_t and the gates left in shared memory (every thread
 // has its own column: no two of a warp share a bank, nothing waits), then backward. Bound by latency: shared memory holds 7 blocks of 64
 // threads an SM. 64 x 204304: bf16 56 us (20 at the memory's rate), floats 76 (40); 16 x 204304 17 and 15. Pairs were no faster (58 and 101).
 constexpr int SERIAL_GRAD_BLOCK = 64;
@@ -784,7 +777,7 @@ __global__ void __launch_bounds__(SERIAL_GRAD_BLOCK) k_gated_serial_grad(const G
                 if (t + i >= n) break;
                 const Factors w = factors_of(to_float(rg[i]));
                 const float xt  = to_float(rx[i]);
-                apart[(t + i) * SERIAL_GRAD_BLOCK] = h - xt;
+                apart[(t + i) * SERIAL_GRAD_BLOCK] = fmaf(0.5f, h, -0.5f * xt);
                 gates[(t + i) * SERIAL_GRAD_BLOCK] = rg[i];
                 h = gated(w.f, h, gated(w.u, xt));
             }
@@ -817,7 +810,7 @@ __global__ void __launch_bounds__(SERIAL_GRAD_BLOCK) k_gated_serial_grad(const G
             const Factors w   = factors_of(to_float(gates[(t - i) * SERIAL_GRAD_BLOCK]));
             const float total = to_float(rd[i]) + c;
             if (a.dx.data != nullptr) *dx = from_float<T>(gated(w.u, total));
-            if (a.d_gate.data != nullptr) *dg = from_float<T>(gated_gradient(w.f * w.u, apart[(t - i) * SERIAL_GRAD_BLOCK], total));
+            if (a.d_gate.data != nullptr) *dg = from_float<T>(gated(w.f * w.u, apart[(t - i) * SERIAL_GRAD_BLOCK]) * (total + total));
             c = gated(w.f, total);
         }
     }
@@ -886,7 +879,7 @@ __global__ void __launch_bounds__(CLUSTER ? 128 : 256, CLUSTER ? 4 : 2) k_gated_
             }
         };
         pass(std::false_type{});
-        bool careful    = !finite<V>(H, LARGE) || !finite<V>(R);
+        bool careful    = !finite<V>(H) || !finite<V>(R);
         const bool zero = has_zero<V>(A);
         if (careful) pass(std::true_type{});
         else if (zero) products<V, L>(f, A);
@@ -906,8 +899,8 @@ __global__ void __launch_bounds__(CLUSTER ? 128 : 256, CLUSTER ? 4 : 2) k_gated_
         __syncthreads();
         state_before<V, W>(at, shared, A, H, h);
         state_before<V, W>(at, shared_back, AR, R, c);
-        careful = careful || !finite<V>(h, LARGE) || !finite<V>(c);
-        // w: h_(t-1) - x, then the gradient of the gate; u: to the gradient of x
+        careful = careful || !finite<V>(h) || !finite<V>(c);
+        // w: f u (h_(t-1) - x), then the gradient of the gate; u: to the gradient of x
         const auto grads = [&](auto care) {
             constexpr bool CAREFUL = decltype(care)::value;
 #pragma unroll
@@ -916,8 +909,10 @@ __global__ void __launch_bounds__(CLUSTER ? 128 : 256, CLUSTER ? 4 : 2) k_gated_
                 io.get(X, i, at.tx, at.ty, x);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
-                    w[i][k] = h[k] - x[k];
-                    h[k]    = CAREFUL ? gated(f[i][k], h[k], gated(u[i][k], x[k])) : fmaf(f[i][k], h[k], u[i][k] * x[k]);
+                    const float fu = f[i][k] * u[i][k];  // a quarter at most: h and x beside it stay in the range, and a factor of 0 drops them
+                    if constexpr (CAREFUL) w[i][k] = gated(fu, h[k]) - gated(fu, x[k]);
+                    else w[i][k] = fmaf(fu, h[k], -(fu * x[k]));
+                    h[k] = CAREFUL ? gated(f[i][k], h[k], gated(u[i][k], x[k])) : fmaf(f[i][k], h[k], u[i][k] * x[k]);
                 }
             }
 #pragma unroll
@@ -927,16 +922,9 @@ __global__ void __launch_bounds__(CLUSTER ? 128 : 256, CLUSTER ? 4 : 2) k_gated_
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     const float total = d[k] + c[k];
-                    if constexpr (CAREFUL) {
-                        w[i][k] = gated_gradient(f[i][k] * u[i][k], w[i][k], total);
-                        c[k]    = gated(f[i][k], total);
-                        u[i][k] = gated(u[i][k], total);
-                    }
-                    else {
-                        c[k]    = f[i][k] * total;
-                        w[i][k] = u[i][k] * w[i][k] * c[k];  // in this order large states do not leave the range
-                        u[i][k] = u[i][k] * total;
-                    }
+                    w[i][k] = CAREFUL && f[i][k] * u[i][k] == 0.0f ? 0.0f : w[i][k] * total;
+                    c[k]    = CAREFUL ? gated(f[i][k], total) : f[i][k] * total;
+                    u[i][k] = CAREFUL ? gated(u[i][k], total) : u[i][k] * total;
                 }
             }
         };
