@@ -104,9 +104,9 @@ __device__ __forceinline__ int64_t length_of(const GatedArgs& a, int64_t b) {
 //
 // W is 8 where a block walks alone (the more threads along time, the fewer tiles), 4 where a cluster shares a sequence: narrower blocks are
 // more of them, and a cluster need not be as large (3 x 1021 x 515 floats, forward and backward: 33 us and 29).
-// Bound by the instructions: 32 for an element forward and 64 backward (an exponential, a reciprocal, conversions, one map or two, the scan's
+// Bound by the instructions: 32 for an element forward and 65 backward (an exponential, a reciprocal, conversions, one map or two, the scan's
 // share), which take 66 to 71 % of the active issue slots with 16 warps an SM (128 registers), the rest being barriers and the ring's wait. 4 x 4096 x
-// 2048 forward / backward: bf16 51 / 95 us (31 / 51 at the memory's rate), float 66 / 115 (61 / 102). Clusters were slower wherever blocks fill the
+// 2048 forward / backward: bf16 51 / 96 us (31 / 51 at the memory's rate), float 66 / 115 (61 / 102). Clusters were slower wherever blocks fill the
 // SMs (the same in clusters of 2: 66 / 123), as were pairs of floats in one instruction (moves into even registers cost what they save).
 template <int W>
 struct Shape {
@@ -742,7 +742,7 @@ __global__ void __launch_bounds__(SERIAL_BLOCK) k_gated_serial(const GatedArgs a
 
 // The gradient of few steps: forward through them from the kept state, with half of h_(t-1) - x_t and the gates left in shared memory (every thread
 // has its own column: no two of a warp share a bank, nothing waits), then backward. Bound by latency: shared memory holds 7 blocks of 64
-// threads an SM. 64 x 204304: bf16 56 us (20 at the memory's rate), floats 76 (40); 16 x 204304 17 and 15. Pairs were no faster (58 and 101).
+// threads an SM. 64 x 204304: bf16 57 us (20 at the memory's rate), floats 75 (40); 16 x 204304 17 and 15. Pairs were no faster (58 and 101).
 constexpr int SERIAL_GRAD_BLOCK = 64;
 inline size_t serial_shared(int64_t steps, size_t element) {
     return static_cast<size_t>(steps) * SERIAL_GRAD_BLOCK * (sizeof(float) + element);
